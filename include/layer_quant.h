@@ -281,6 +281,85 @@ int lq_int4_prefill_attention(const lq_tensor* q, const lq_tensor* k_packed,
                               int num_key_value_groups, int group_size, void* stream);
 
 /*
+ * Workspace bytes that lq_int4_shared_decode_attention needs for this shape (0 if none): split
+ * partials, in no particular state before or after a call.
+ */
+size_t lq_int4_shared_decode_attention_workspace(int64_t prompts, int64_t members,
+                                                 int64_t n_q_heads, int64_t n_kv_heads,
+                                                 int64_t head_dim, int64_t prefix_len,
+                                                 int64_t seq_len, int group_size);
+
+/*
+ * q_len = 1 GQA attention of rows that share their prompt's cache. Row b = prompt * N + member of q
+ * (N = B / P members for each of the P prompts) attends to rows [0, prefix_len) of its prompt's
+ * cache and then to rows [0, seq_len - prefix_len) of its own: the attention of
+ * lq_int4_decode_attention over the two in sequence, with each prompt's rows read once for all its
+ * members. With k_new and v_new [B, Hkv, 1, D] (both or neither NULL) the step's token is first
+ * packed into own row seq_len - prefix_len - 1, as lq_int4_decode_attention_pack does.
+ *   q         [B, Hq, 1, D] or [B, Hq, D]   f32/f16/bf16
+ *   prefix_*  the prompts' cache, k_packed/v_packed [P, Hkv, cap, D/2] u8 and scales [P, Hkv, cap,
+ *             D/g] f32;  k_packed .. v_scale the rows' own cache, the same with B rows and a
+ *             capacity of its own
+ *   mask      NULL, [B, 1, 1, Lm] f32 (added to the scores in exp2 units, as in
+ *             lq_int4_decode_attention; only batch and key strides are used) or a keep-mask [B, Lm]
+ *             i64 (0 masks the key). Its key j is prefix row j, or own row j - prefix_len; keys at or
+ *             beyond Lm are masked. A masked key's cache row may hold any bytes where no row that
+ *             shares it attends to it; a row without a key gives NaN.
+ *   out       [B, Hq, D]   f32/f16/bf16
+ * prefix_len may be 0, and seq_len equal to prefix_len (no own rows; then without k_new).
+ * No counterpart in the reference, whose caches are one per row.
+ */
+int lq_int4_shared_decode_attention(
+    const lq_tensor* q, const lq_tensor* k_new, const lq_tensor* v_new,
+    const lq_tensor* prefix_k_packed, const lq_tensor* prefix_v_packed,
+    const lq_tensor* prefix_k_scale, const lq_tensor* prefix_v_scale, const lq_tensor* k_packed,
+    const lq_tensor* v_packed, const lq_tensor* k_scale, const lq_tensor* v_scale,
+    const lq_tensor* mask, const lq_tensor* out, int64_t prefix_len, int64_t seq_len,
+    int num_key_value_groups, int group_size, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/*
+ * Beam selection: for each of P prompts the `num` best continuations of its N beams, num the extent
+ * of the outputs' second dim. The total of beam n and token t is scores[n] + logits[n][t] - lse[n],
+ * lse[n] the log-sum-exp of the beam's logits; totals are compared in 64 bits, equal ones by the
+ * lower n * V + t. A finished beam has one continuation, pad_token at its own score, and its logits
+ * are not read. Continuations of a beam whose score or log-sum-exp is not finite (a NaN or +inf
+ * logit, no logit above -inf) count as -inf, and so do the other tokens of a finished beam.
+ *   logits    [P, N, V]  f32/f16/bf16, any strides
+ *   scores    [P, N]     f32
+ *   finished  NULL or [P, N] u8 (0: not finished)
+ *   out_scores [P, num] f32 (the totals), out_beams [P, num] i64 (n), out_tokens [P, num] i64 (t)
+ * The outputs are in descending order, or with keep_slots (num == N) by place: the best selected
+ * continuation of a beam stands at that beam's place, the others at the places of the beams without
+ * one, in order, so that lq_reorder_beams moves no state of a beam that goes on.
+ * num <= N * V. No counterpart in the reference, which scores given text.
+ */
+#define LQ_BEAM_SELECT_MAX_BEAMS 64
+#define LQ_BEAM_SELECT_MAX_NUM 64
+#define LQ_BEAM_SELECT_MAX_VOCAB (1 << 24)
+size_t lq_beam_select_workspace(int64_t prompts, int64_t beams, int64_t vocab, int num);
+int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores, const lq_tensor* finished,
+                   const lq_tensor* out_scores, const lq_tensor* out_beams,
+                   const lq_tensor* out_tokens, int64_t pad_token, int keep_slots, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
+ * The states of P prompts x N beams follow the selected beams, in place: for each of `count` tensors
+ * (an array of descriptors, any dtype, 1 to 4 dims, P * N rows, any strides without a broadcast
+ * dimension) row p*N + n takes the contents that row p*N + beams[p][n] had before the call. Rows with
+ * beams[p][n] == n stay as they are, and so do rows whose entry is outside [0, N).
+ *   rows   NULL, or for each tensor how many entries of dim 2 are moved (the live rows of a cache
+ *          [B, Hkv, cap, .]; what lies behind them stays), -1 for the whole tensor
+ *   beams  [P, N] i64
+ * The tensors must not overlap (one listed twice is refused). One launch for up to 256 tensors of up
+ * to 16 row shapes. No counterpart in the reference.
+ */
+#define LQ_REORDER_MAX_BEAMS 64
+#define LQ_REORDER_MAX_TENSORS 512
+int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, int count,
+                     const lq_tensor* beams, void* stream);
+
+/*
  * MX state layouts. Every MX entry point takes either layout and tells them apart by the shapes
  * of q_state and micro_exp (N = 16 * shared_exp.shape[3]):
  *   reference layout (hybrid_quant/mamba_state_8b_kernel.py:11-25, 575-598):

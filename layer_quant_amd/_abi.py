@@ -79,6 +79,11 @@ EXPORTED_SYMBOLS = (
     "lq_selective_state_update",
     "lq_max_position",
     "lq_keep_mask_bias",
+    "lq_int4_shared_decode_attention_workspace",
+    "lq_int4_shared_decode_attention",
+    "lq_beam_select_workspace",
+    "lq_beam_select",
+    "lq_reorder_beams",
 )
 
 
@@ -158,6 +163,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.lq_max_position.argtypes = [_P, ctypes.c_void_p, ctypes.c_void_p]
     lib.lq_keep_mask_bias.restype = ctypes.c_int
     lib.lq_keep_mask_bias.argtypes = [_P, _P, ctypes.c_void_p]
+    lib.lq_int4_shared_decode_attention_workspace.restype = ctypes.c_size_t
+    lib.lq_int4_shared_decode_attention_workspace.argtypes = [ctypes.c_int64] * 7 + [ctypes.c_int]
+    lib.lq_int4_shared_decode_attention.restype = ctypes.c_int
+    lib.lq_int4_shared_decode_attention.argtypes = [_P] * 13 + [
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_size_t, ctypes.c_void_p]
+    lib.lq_beam_select_workspace.restype = ctypes.c_size_t
+    lib.lq_beam_select_workspace.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int]
+    lib.lq_beam_select.restype = ctypes.c_int
+    lib.lq_beam_select.argtypes = [_P] * 6 + [ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                              ctypes.c_size_t, ctypes.c_void_p]
+    lib.lq_reorder_beams.restype = ctypes.c_int
+    lib.lq_reorder_beams.argtypes = [_P, ctypes.POINTER(ctypes.c_int64), ctypes.c_int, _P,
+                                     ctypes.c_void_p]
 
 
 def lib() -> ctypes.CDLL:
@@ -185,6 +204,8 @@ _HOST_ENTRIES = (
     "lq_int4_decode_attention_keep", "lq_int4_prefill_attention",
     "lq_mx_encode", "lq_mx_state_update", "lq_mx_state_update_device_step",
     "lq_selective_state_update", "lq_max_position", "lq_keep_mask_bias",
+    "lq_int4_shared_decode_attention_workspace", "lq_int4_shared_decode_attention",
+    "lq_beam_select_workspace", "lq_beam_select", "lq_reorder_beams",
 )
 
 
@@ -432,6 +453,31 @@ class _Workspace:
 _workspace = _Workspace()
 
 
+class _Scratch:
+    """Scratch of the calls that need no particular contents: per (device, stream), grown on demand.
+    A call that is being captured gets a buffer of the graph's own memory instead, so that graphs
+    captured on one stream do not share it and an eager call that grows the buffer leaves theirs."""
+
+    def __init__(self):
+        self._bufs: dict[tuple[int, int], torch.Tensor] = {}
+        self._lock = threading.Lock()
+
+    def get(self, index: int, stream: int, nbytes: int) -> torch.Tensor:
+        device = torch.device("cuda", index)
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        key = (index, stream)
+        with self._lock:
+            buf = self._bufs.get(key)
+            if buf is None or buf.numel() < nbytes:
+                buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+                self._bufs[key] = buf
+            return buf
+
+
+_scratch = _Scratch()
+
+
 def int4_decode_attention_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
                                     seq_len: int, group_size: int) -> int:
     return int(lib().lq_int4_decode_attention_workspace(batch, n_q_heads, n_kv_heads, head_dim,
@@ -631,3 +677,74 @@ def selective_state_update(state, x, dt, dt_bias, A, B, C, D, z, out,
         desc(z), desc(out), 1 if dt_softplus else 0, _stream(dev))
     check(rc, "lq_selective_state_update")
     return out
+
+
+def int4_shared_decode_attention(q: torch.Tensor, k_new: torch.Tensor | None,
+                                 v_new: torch.Tensor | None, prefix, own,
+                                 mask: torch.Tensor | None, out: torch.Tensor, prefix_len: int,
+                                 seq_len: int, num_key_value_groups: int,
+                                 group_size: int) -> torch.Tensor:
+    """q_len=1 attention of q [P*N, Hq, 1, D] over keys [0, prefix_len) of its prompt's cache and
+    then its own keys -> out; `prefix` and `own` are the caches' (k_packed, v_packed, k_scale,
+    v_scale). With k_new and v_new [P*N, Hkv, 1, D] the token is packed into the last own row first.
+    mask: None, an additive fp32 bias [P*N, 1, 1, Lm] or an int64 keep-mask [P*N, Lm]."""
+    host = _host or host_binding()
+    if host:
+        rc = host.int4_shared_decode_attention(q, k_new, v_new, *prefix, *own, mask, out, prefix_len,
+                                               seq_len, num_key_value_groups, group_size,
+                                               _scratch.get)
+        if rc is not None:
+            check(rc, "lq_int4_shared_decode_attention")
+            return out
+    dev = _require_gpu(q, k_new, v_new, *prefix, *own, mask, out)
+    stream = _stream(dev)
+    prompts = prefix[0].shape[0]
+    need = int(lib().lq_int4_shared_decode_attention_workspace(
+        prompts, q.shape[0] // max(prompts, 1), q.shape[1], prefix[0].shape[1], q.shape[-1],
+        int(prefix_len), int(seq_len), int(group_size)))
+    ws = _scratch.get(dev.index, stream, need) if need else None
+    rc = lib().lq_int4_shared_decode_attention(
+        desc(q), desc(k_new), desc(v_new), *map(desc, prefix), *map(desc, own), desc(mask),
+        desc(out), int(prefix_len), int(seq_len), int(num_key_value_groups), int(group_size),
+        None if ws is None else ws.data_ptr(), need, stream)
+    check(rc, "lq_int4_shared_decode_attention")
+    return out
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None,
+                out_scores: torch.Tensor, out_beams: torch.Tensor, out_tokens: torch.Tensor,
+                pad_token: int, keep_slots: bool) -> None:
+    """The best continuations of logits [P, N, V] and scores [P, N] (finished: uint8 [P, N] or None)
+    into the outputs [P, num]."""
+    host = _host or host_binding()
+    if host:
+        rc = host.beam_select(logits, scores, finished, out_scores, out_beams, out_tokens, pad_token,
+                              keep_slots, _scratch.get)
+        if rc is not None:
+            return check(rc, "lq_beam_select")
+    dev = _require_gpu(logits, scores, finished, out_scores, out_beams, out_tokens)
+    stream = _stream(dev)
+    need = int(lib().lq_beam_select_workspace(*logits.shape, out_scores.shape[1]))
+    ws = _scratch.get(dev.index, stream, need) if need else None
+    rc = lib().lq_beam_select(desc(logits), desc(scores), desc(finished), desc(out_scores),
+                              desc(out_beams), desc(out_tokens), int(pad_token),
+                              1 if keep_slots else 0, None if ws is None else ws.data_ptr(), need,
+                              stream)
+    check(rc, "lq_beam_select")
+
+
+def reorder_beams(tensors, rows, beams: torch.Tensor) -> None:
+    """Row p*N + n of every tensor takes the contents of row p*N + beams[p, n], in place; rows[i]:
+    entries of dim 2 that are moved (None or -1: all). `rows` may be None."""
+    host = _host or host_binding()
+    if host:
+        rc = host.reorder_beams(tensors, rows, beams)
+        if rc is not None:
+            return check(rc, "lq_reorder_beams")
+    dev = _require_gpu(beams, *tensors)
+    table = (LQTensor * max(len(tensors), 1))(*(desc(t).contents for t in tensors))
+    live = None
+    if rows is not None:
+        live = (ctypes.c_int64 * max(len(tensors), 1))(*(-1 if r is None else int(r) for r in rows))
+    rc = lib().lq_reorder_beams(table, live, len(tensors), desc(beams), _stream(dev))
+    check(rc, "lq_reorder_beams")

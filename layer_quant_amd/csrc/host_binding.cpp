@@ -30,6 +30,11 @@ struct Entries {
   decltype(&lq_selective_state_update) ssm;
   decltype(&lq_max_position) max_position;
   decltype(&lq_keep_mask_bias) keep_mask;
+  decltype(&lq_int4_shared_decode_attention_workspace) shared_workspace;
+  decltype(&lq_int4_shared_decode_attention) shared;
+  decltype(&lq_beam_select_workspace) select_workspace;
+  decltype(&lq_beam_select) select;
+  decltype(&lq_reorder_beams) reorder;
 } entries;
 constexpr int kEntries = sizeof(Entries) / sizeof(void*);
 
@@ -301,6 +306,105 @@ PyObject* py_keep_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return launch(t.device, [&](void* s) { return entries.keep_mask(t.ptr[0], t.ptr[1], s); });
 }
 
+// Scratch of `need` bytes from get(device index, stream handle, bytes) -> uint8 tensor, held by *buf
+// until the launch; false with a Python error set.
+bool scratch_of(PyObject* get, int device, PyObject* handle, size_t need, PyObject*& buf, void*& ws) {
+  buf = nullptr;
+  ws = nullptr;
+  if (need == 0) return true;
+  buf = PyObject_CallFunction(get, "iOn", device, handle, (Py_ssize_t)need);
+  if (buf == nullptr || !THPVariable_Check(buf)) {
+    Py_XDECREF(buf);
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "the workspace must be a tensor");
+    return false;
+  }
+  ws = THPVariable_Unpack(buf).data_ptr();
+  return true;
+}
+
+// Runs `call(workspace, bytes, stream)` without the interpreter lock and returns its code.
+template <class F>
+PyObject* launch_with(int device, PyObject* get, size_t need, F&& call) {
+  PyObject *handle, *buf;
+  void *stream, *ws;
+  if (!stream_of(device, handle, stream)) return nullptr;
+  const bool ok = scratch_of(get, device, handle, need, buf, ws);
+  Py_DECREF(handle);
+  if (!ok) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = call(ws, need, stream);
+  Py_END_ALLOW_THREADS
+  Py_XDECREF(buf);
+  return PyLong_FromLong(rc);
+}
+
+// q, k_new, v_new, the prefix's four cache tensors, the own ones, mask, out, prefix length, sequence
+// length, groups, group size, scratch getter
+PyObject* py_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!has_args(n, 18)) return nullptr;
+  Tensors<13> t;
+  int64_t prefix_len, seq_len;
+  int nrep, g;
+  LQ_NOT_PLAIN(!t.add_all(a) || !to_int64(a[13], prefix_len) || !to_int64(a[14], seq_len) ||
+               !to_int(a[15], nrep) || !to_int(a[16], g));
+  const lq_tensor* const* p = t.ptr;
+  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim < 2 || p[3] == nullptr || p[3]->ndim < 2 ||
+               p[3]->shape[0] < 1);
+  const size_t need = entries.shared_workspace(p[3]->shape[0], p[0]->shape[0] / p[3]->shape[0],
+                                               p[0]->shape[1], p[3]->shape[1],
+                                               p[0]->shape[p[0]->ndim - 1], prefix_len, seq_len, g);
+  return launch_with(t.device, a[17], need, [&](void* ws, size_t bytes, void* s) {
+    return entries.shared(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], p[11],
+                          p[12], prefix_len, seq_len, nrep, g, ws, bytes, s);
+  });
+}
+
+// logits, scores, finished, the three outputs, pad token, keep slots, scratch getter
+PyObject* py_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!has_args(n, 9)) return nullptr;
+  Tensors<6> t;
+  int64_t pad;
+  LQ_NOT_PLAIN(!t.add_all(a) || !to_int64(a[6], pad));
+  const int slots = PyObject_IsTrue(a[7]);
+  if (slots < 0) return nullptr;
+  const lq_tensor* const* p = t.ptr;
+  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim != 3 || p[3] == nullptr || p[3]->ndim != 2 ||
+               p[3]->shape[1] > INT32_MAX);
+  const size_t need = entries.select_workspace(p[0]->shape[0], p[0]->shape[1], p[0]->shape[2],
+                                               (int)p[3]->shape[1]);
+  return launch_with(t.device, a[8], need, [&](void* ws, size_t bytes, void* s) {
+    return entries.select(p[0], p[1], p[2], p[3], p[4], p[5], pad, slots, ws, bytes, s);
+  });
+}
+
+// list or tuple of tensors, list or tuple of row counts (None or -1: all) or None, beams
+PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!has_args(n, 3)) return nullptr;
+  LQ_NOT_PLAIN(!PyList_CheckExact(a[0]) && !PyTuple_CheckExact(a[0]));
+  LQ_NOT_PLAIN(a[1] != Py_None && !PyList_CheckExact(a[1]) && !PyTuple_CheckExact(a[1]));
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(a[0]);
+  LQ_NOT_PLAIN(count > LQ_REORDER_MAX_TENSORS);
+  LQ_NOT_PLAIN(a[1] != Py_None && PySequence_Fast_GET_SIZE(a[1]) != count);
+  lq_tensor list[LQ_REORDER_MAX_TENSORS];
+  int64_t rows[LQ_REORDER_MAX_TENSORS];
+  Tensors<1> one, beams;
+  LQ_NOT_PLAIN(!beams.add_all(a + 2));
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* item = PySequence_Fast_GET_ITEM(a[0], i);
+    one.device = beams.device;
+    LQ_NOT_PLAIN(item == Py_None || !one.add(0, item));
+    list[i] = one.desc[0];
+    rows[i] = -1;
+    if (a[1] == Py_None) continue;
+    PyObject* live = PySequence_Fast_GET_ITEM(a[1], i);
+    LQ_NOT_PLAIN(live != Py_None && !to_int64(live, rows[i]));
+  }
+  return launch(beams.device, [&](void* s) {
+    return entries.reorder(list, rows, (int)count, beams.ptr[0], s);
+  });
+}
+
 // bind(current raw stream function, addresses of the entry points in the order of Entries)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!has_args(n, 1 + kEntries)) return nullptr;
@@ -347,6 +451,9 @@ PyMethodDef methods[] = {LQ_METHOD("bind", py_bind),
                          LQ_METHOD("selective_state_update", py_ssm),
                          LQ_METHOD("max_position", py_max_position),
                          LQ_METHOD("keep_mask_bias", py_keep_mask),
+                         LQ_METHOD("int4_shared_decode_attention", py_shared),
+                         LQ_METHOD("beam_select", py_select),
+                         LQ_METHOD("reorder_beams", py_reorder),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lq_host", nullptr, -1, methods,

@@ -72,4 +72,8 @@ bool fast_path_ok(const AttnParams& p);
 SplitPlan plan_fast(int64_t B, int64_t Hkv, int64_t S);
 int launch_fast(const AttnParams& p, hipStream_t stream);
 
+// Merges the split partials (ws_m, ws_l, ws_acc: nsplit slots per (batch, query head)) into p.out
+// (int4_attention.hip); uses B, Hq, D, nsplit, out and the partials of p.
+void launch_merge(const AttnParams& p, hipStream_t stream);
+
 }  // namespace lq

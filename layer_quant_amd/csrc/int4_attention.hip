@@ -299,7 +299,7 @@ __global__ __launch_bounds__(1024) void attn_merge_few_kernel(const float* __res
   store_float(out.data, out.dtype, b * out.s[0] + qh * out.s[1] + d * out.s[2], acc / L);
 }
 
-static void launch_merge(const AttnParams& p, hipStream_t st) {
+void launch_merge(const AttnParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.Hq));
   const int groups = (p.nsplit + MERGE_PER_GROUP - 1) / MERGE_PER_GROUP;
   if (p.D > 256 || groups > MERGE_GROUPS) {

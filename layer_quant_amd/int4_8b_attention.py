@@ -26,13 +26,18 @@ from . import _abi
 @dataclass
 class Int4KVLayerCache:
     """Packed per-layer cache (ia.py:12-18): nibbles [B, Hkv, cap, D/2] uint8, fp32 group
-    scales [B, Hkv, cap, D/g], and the number of valid rows."""
+    scales [B, Hkv, cap, D/g], and the number of valid rows.
+
+    With `prefix` (no reference counterpart) the rows go on from a cache of B / N prompts that each
+    N consecutive rows share: row b's keys are prefix rows [0, prefix.length) of prompt b // N, then
+    its own rows (shared_prefix_decode_attention)."""
 
     k_packed: torch.Tensor
     v_packed: torch.Tensor
     k_scale: torch.Tensor
     v_scale: torch.Tensor
     length: int = 0
+    prefix: Int4KVLayerCache | None = None
 
 
 def int4_quant_dequant(x: torch.Tensor, group_size: int = 64) -> torch.Tensor:
@@ -111,6 +116,7 @@ def _ensure_layer_cache(past_key_value, layer_idx: int, batch: int, kv_heads: in
     for name in ("k_packed", "v_packed", "k_scale", "v_scale"):
         getattr(grown, name)[:, :, :old_cap].copy_(getattr(current, name))
     grown.length = current.length
+    grown.prefix = current.prefix
     caches[layer_idx] = grown
     return grown
 
@@ -228,6 +234,41 @@ def _pack_and_decode_attention(query_states: torch.Tensor, key_states: torch.Ten
     return out
 
 
+def shared_prefix_decode_attention(query_states: torch.Tensor, cache: Int4KVLayerCache,
+                                   seq_len: int, num_key_value_groups: int, group_size: int,
+                                   attention_mask: torch.Tensor | None = None,
+                                   key_states: torch.Tensor | None = None,
+                                   value_states: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q [P*N, Hq, 1, D] over a cache with a shared prefix -> [P*N, Hq, D] in q's dtype
+    (no reference counterpart): row p*N + n attends to prefix rows [0, prefix.length) of prompt p and
+    then to its own rows, seq_len keys in all. Each prompt's rows are read once for its N members.
+
+    With key_states and value_states [P*N, Hkv, 1, D] the step's token is first packed into own row
+    seq_len - prefix.length - 1, and cache.length follows. The mask is that of _decode_attention over
+    the seq_len keys. A row whose keys are all masked gives NaN, as there."""
+    batch, n_heads, q_len, head_dim = query_states.shape
+    if q_len != 1:
+        raise ValueError(f"Fused INT4 decode attention expects q_len=1, got {q_len}")
+    prefix = cache.prefix
+    if prefix is None:
+        raise ValueError("the cache has no shared prefix")
+    if (key_states is None) != (value_states is None):
+        raise ValueError("key_states and value_states: both or neither")
+    out = torch.empty((batch, n_heads, head_dim), device=query_states.device,
+                      dtype=query_states.dtype)
+    mask = _keep_rows(attention_mask, batch, seq_len, query_states.device)
+    if mask is None:
+        mask = _decode_attention_mask(attention_mask, batch, seq_len, query_states.device)
+    _abi.int4_shared_decode_attention(
+        query_states, key_states, value_states,
+        (prefix.k_packed, prefix.v_packed, prefix.k_scale, prefix.v_scale),
+        (cache.k_packed, cache.v_packed, cache.k_scale, cache.v_scale), mask, out, prefix.length,
+        seq_len, num_key_value_groups, group_size)
+    if key_states is not None:
+        cache.length = max(cache.length, seq_len - prefix.length)
+    return out
+
+
 def _prefill_attention(query_states: torch.Tensor, cache: Int4KVLayerCache,
                        num_key_value_groups: int, group_size: int) -> torch.Tensor:
     """Causal attention of q [B, Hq, L, D] over cache rows [0, L): position t attends to rows
@@ -244,7 +285,8 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
                            past_key_value=None, output_attentions=False, use_cache=False,
                            cache_position=None):
     """Patched attention forward (ia.py:628-714): pack this step's K/V into the INT4 cache;
-    decode (q_len == 1) attends over the cache, prefill runs SDPA on the unquantized K/V."""
+    decode (q_len == 1) attends over the cache, prefill runs SDPA on the unquantized K/V. Over a cache
+    with a shared prefix (beam_decode.share_prompt) only decode steps behind the prefix are defined."""
     if output_attentions or hidden_states.device.type != "cuda" or past_key_value is None:
         return self._int4_kv_original_forward(
             hidden_states=hidden_states, attention_mask=attention_mask,
@@ -278,9 +320,19 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
     finally:
         last = None if pending is None else pending.wait()
     required_len = (int(positions.max().item()) if last is None else last) + 1
+    current = _cache_dict(past_key_value).get(self.layer_idx)
+    shared_len = 0 if current is None or current.prefix is None else current.prefix.length
+    if shared_len and (q_len != 1 or required_len <= shared_len):
+        raise ValueError(f"a cache behind {shared_len} shared rows takes one later token at a time, "
+                         f"got {q_len} up to position {required_len - 1}")
     layer_cache = _ensure_layer_cache(past_key_value, self.layer_idx, bsz,
-                                      self.num_key_value_heads, required_len, self.head_dim,
-                                      group_size, hidden_states.device)
+                                      self.num_key_value_heads, required_len - shared_len,
+                                      self.head_dim, group_size, hidden_states.device)
+    if shared_len:
+        attn = shared_prefix_decode_attention(query_states, layer_cache, required_len,
+                                              self.num_key_value_groups, group_size, attention_mask,
+                                              key_states, value_states)
+        return self.o_proj(attn.reshape(bsz, q_len, self.hidden_size)), None, past_key_value
     if q_len == 1:
         # the token's row is required_len - 1 (positions holds that one value)
         attn = _pack_and_decode_attention(query_states, key_states, value_states, layer_cache,
