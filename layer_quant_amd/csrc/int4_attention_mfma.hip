@@ -44,6 +44,7 @@
 
 #include "int4_attention.h"
 #include "int4_quant.h"
+#include "lds_loads.h"
 
 namespace lq {
 
@@ -59,7 +60,6 @@ constexpr int WAVES = 4;             // waves per workgroup, each on its own key
 constexpr int THREADS = 64 * WAVES;
 constexpr float LAZY_LOG2 = 8.0f;    // running-max slack of the lazy softmax rescale
 constexpr uint32_t NIB2 = 0x000F000Fu;
-constexpr int BUF_DWORD3 = 0x00020000;  // raw 32-bit buffer, gfx9 family
 // The tile loads carry the non-temporal (nt) policy: each byte is read once per call, and at
 // B=64, ctx 16384 the 1.34 GB stream measured 248 us with the default policy and 237 us with nt
 // (a read-only probe of the same volume: 7.2 TB/s with nt, 5.4-6.3 without).
@@ -132,60 +132,6 @@ struct alignas(16) TileLds {
 // the form that a serving loop has in hand: read here it costs 8 bytes per key where its bias costs
 // a launch and 4 (batch 8, 4001 keys: 16.9 us a step, 18.6 with the bias kernel before it).
 enum { MASK_NONE = 0, MASK_BIAS = 1, MASK_KEEP = 2 };
-
-typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
-
-// Raw buffer descriptor (base, stride 0, num_records = bytes, gfx9 dword 3) for wave-uniform
-// arguments, so that it lives in 4 SGPRs.
-__device__ __forceinline__ i32x4_t make_desc(const void* base, int bytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)base;
-  i32x4_t d;
-  d[0] = (int32_t)(uint32_t)a;
-  d[1] = (int32_t)((uint32_t)(a >> 32) & 0xffffu);
-  d[2] = bytes;
-  d[3] = BUF_DWORD3;
-  return d;
-}
-
-// One 16-byte-per-lane buffer load that writes LDS directly: lane l's 16 bytes (at byte offset
-// voff of the buffer; zero past num_records) land at LDS byte address lds + 16 l. Written as
-// inline assembly with its own M0 set-up: the compiler's wait insertion for the builtin form did
-// not track which LDS buffer each such load targets (it emitted no wait before the reads of one
-// buffer and a full wait before the other's), so the waits are explicit (wait_loads) instead.
-// M0 is declared clobbered; no other code of this kernel uses M0 (the compiler warns that a
-// reserved register in a clobber list is not saved for it).
-__device__ __forceinline__ void load_to_lds(i32x4_t desc, const void* lds, int voff) {
-  const uint32_t addr =
-      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
-      :
-      : "s"(addr), "v"(voff), "s"(desc)
-      : "memory", "m0");
-}
-
-// The same with 4 bytes per lane (lane l's dword lands at lds + 4 l; each dword is range-checked
-// on its own).
-__device__ __forceinline__ void load_to_lds_b32(i32x4_t desc, const void* lds, int voff) {
-  const uint32_t addr =
-      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dword %1, %2, 0 offen nt lds"
-      :
-      : "s"(addr), "v"(voff), "s"(desc)
-      : "memory", "m0");
-}
-
-// Wait until at most N vector-memory loads of this wave are outstanding (loads complete in issue
-// order, so every load older than the newest N has landed).
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
 
 // Per-wave bases of this (batch, KV head) block; rows are contiguous (64 packed bytes, G scale
 // words). Each tile builds buffer descriptors whose base is the tile's first key and whose size
