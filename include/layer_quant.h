@@ -295,7 +295,8 @@ size_t lq_int4_shared_decode_attention_workspace(int64_t prompts, int64_t member
  * cache and then to rows [0, seq_len - prefix_len) of its own: the attention of
  * lq_int4_decode_attention over the two in sequence, with each prompt's rows read once for all its
  * members. With k_new and v_new [B, Hkv, 1, D] (both or neither NULL) the step's token is first
- * packed into own row seq_len - prefix_len - 1, as lq_int4_decode_attention_pack does.
+ * packed into own row seq_len - prefix_len - 1, with scale = max(absmax * fl(1/7), 1e-8) (within one
+ * unit in the last place of lq_int4_pack_kv's quotient) and the levels of lq_int4_pack_kv under it.
  *   q         [B, Hq, 1, D] or [B, Hq, D]   f32/f16/bf16
  *   prefix_*  the prompts' cache, k_packed/v_packed [P, Hkv, cap, D/2] u8 and scales [P, Hkv, cap,
  *             D/g] f32;  k_packed .. v_scale the rows' own cache, the same with B rows and a
@@ -304,7 +305,8 @@ size_t lq_int4_shared_decode_attention_workspace(int64_t prompts, int64_t member
  *             lq_int4_decode_attention; only batch and key strides are used) or a keep-mask [B, Lm]
  *             i64 (0 masks the key). Its key j is prefix row j, or own row j - prefix_len; keys at or
  *             beyond Lm are masked. A masked key's cache row may hold any bytes where no row that
- *             shares it attends to it; a row without a key gives NaN.
+ *             shares it attends to it; a row without a key gives NaN. Value scales above 2^100 may
+ *             give infinities.
  *   out       [B, Hq, D]   f32/f16/bf16
  * prefix_len may be 0, and seq_len equal to prefix_len (no own rows; then without k_new).
  * No counterpart in the reference, whose caches are one per row.

@@ -41,6 +41,7 @@ COMMON_FLAGS = [
 # (for the rarely taken softmax rescale), 36 extra instructions per tile.
 SOURCE_FLAGS = {
     "int4_attention_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "int4_shared_attention_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -32,6 +32,48 @@ struct SharedParams {
   int nsp, nso;               // splits of the prefix and of the own rows
   int64_t chunk_p, chunk_o;   // keys per split
   float scale_sm;             // log2(e) / sqrt(D)
+  // the new token's K and V rows [B, Hkv, D] (strides of b, h, d), packed into own row own_len - 1
+  View knew, vnew;
+  int pack;
+  // MFMA path
+  int q_rows;               // query rows contiguous and 16-byte aligned
+  int col_tiles;            // 16-row column tiles of a prefix unit's wave
+  int rb_prefix, rb_own;    // row blocks of a prefix and of an own unit
+  uint32_t prefix_blocks;   // workgroups of the prefix units
 };
+
+// Splits of the two key ranges.
+struct SharedPlan {
+  SplitPlan prefix, own;
+};
+
+// `len` keys in about `want` splits of whole `step`s.
+inline SplitPlan split_of(int64_t len, int64_t want, int64_t step) {
+  SplitPlan s{0, step};
+  if (len == 0) return s;
+  want = std::max<int64_t>(1, std::min(want, (len + step - 1) / step));
+  s.chunk = ((len + want - 1) / want + step - 1) / step * step;
+  s.nsplit = (int)((len + s.chunk - 1) / s.chunk);
+  return s;
+}
+
+// The new token's scale: absmax * fl(1/7), the product rounded once, at least 1e-8. It is within one
+// unit in the last place of int4_quantize_pair's quotient and equal to what int4_quant_dequant's
+// division by 7 gives on the GPU.
+__device__ __forceinline__ float token_scale(float amax) {
+  return fmaxf(amax * (1.0f / 7.0f), 1.0e-8f);
+}
+
+// Level of x under that scale, as 4 bits: IEEE quotient, round half to even, [-8, 7].
+__device__ __forceinline__ uint32_t token_level(float x, float scale) {
+  return (uint32_t)min(max((int)rintf(x / scale), -8), 7) & 15u;
+}
+
+// MFMA path (int4_shared_attention_mfma.hip)
+bool shared_fast_shape_ok(int64_t head_dim, int group_size);
+bool shared_fast_ok(const SharedParams& p);
+SharedPlan plan_shared_fast(int64_t P, int64_t N, int64_t Hkv, int64_t nrep, int64_t prefix_len,
+                            int64_t own_len);
+int launch_shared_fast(SharedParams p, hipStream_t stream);
 
 }  // namespace lq

@@ -7,8 +7,10 @@
 // prefix and the own rows are split over workgroups; every split leaves (m, l, acc[D]) of each of its
 // query rows in the workspace and the decode attention's merge joins them.
 //
-// shared_generic_kernel: any even group dividing any head_dim <= 512, any query type; one wave per
-// (row, query head, split), fp32 VALU throughout.
+//   * shared_mfma_kernel (int4_shared_attention_mfma.hip): head_dim 128, group 32/64/128, 16-bit
+//     queries; packs the new token itself.
+//   * shared_generic_kernel: any even group dividing any head_dim <= 512, any query type; one wave per
+//     (row, query head, split), fp32 VALU throughout, behind shared_pack_kernel.
 #include <math.h>
 
 #include "int4_quant.h"
@@ -138,18 +140,33 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedParams p) {
   }
 }
 
-// Splits of the two key ranges.
-struct SharedPlan {
-  SplitPlan prefix, own;
-};
-
-SplitPlan split_of(int64_t len, int64_t want, int64_t step) {
-  SplitPlan s{0, step};
-  if (len == 0) return s;
-  want = std::max<int64_t>(1, std::min(want, (len + step - 1) / step));
-  s.chunk = ((len + want - 1) / want + step - 1) / step * step;
-  s.nsplit = (int)((len + s.chunk - 1) / s.chunk);
-  return s;
+// The new token's K and V rows into own row own_len - 1: one wave per (row, KV head, K or V, group).
+__global__ __launch_bounds__(64) void shared_pack_kernel(SharedParams p) {
+  const int lane = threadIdx.x;
+  const int kvh = blockIdx.x % p.Hkv;
+  const int b = blockIdx.x / p.Hkv;
+  const int gi = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const View& x = is_v ? p.vnew : p.knew;
+  const int64_t at = b * x.s[0] + kvh * x.s[1];
+  const int64_t row = p.own_len - 1;
+  float amax = 0.0f;
+  for (int d = gi * p.g + lane; d < (gi + 1) * p.g; d += 64) {
+    amax = fmaxf(amax, fabsf(load_float(x.data, x.dtype, at + d * x.s[2])));
+  }
+  const float scale = token_scale(group_max<64>(amax));
+  const int64_t* ps = is_v ? p.own.vps : p.own.kps;
+  const int64_t* ss = is_v ? p.own.vss : p.own.kss;
+  uint8_t* packed = const_cast<uint8_t*>(is_v ? p.own.vp : p.own.kp) + b * ps[0] + kvh * ps[1] + row * ps[2];
+  for (int j = lane; j < p.g / 2; j += 64) {
+    const int d = gi * p.g + 2 * j;
+    const float x0 = load_float(x.data, x.dtype, at + d * x.s[2]);
+    const float x1 = load_float(x.data, x.dtype, at + (d + 1) * x.s[2]);
+    packed[(d >> 1) * ps[3]] = (uint8_t)(token_level(x0, scale) | token_level(x1, scale) << 4);
+  }
+  if (lane == 0) {
+    const_cast<float*>(is_v ? p.own.vs : p.own.ks)[b * ss[0] + kvh * ss[1] + row * ss[2] + gi * ss[3]] = scale;
+  }
 }
 
 // About 2048 waves in flight, at least 64 keys per split, the splits shared out by length.
@@ -220,8 +237,15 @@ extern "C" size_t lq_int4_shared_decode_attention_workspace(int64_t prompts, int
     return 0;
   }
   const int64_t B = prompts * members;
-  return partial_bytes(B, n_q_heads, head_dim,
-                       plan_generic(B, n_q_heads, prefix_len, seq_len - prefix_len));
+  size_t need = partial_bytes(B, n_q_heads, head_dim,
+                              plan_generic(B, n_q_heads, prefix_len, seq_len - prefix_len));
+  if (shared_fast_shape_ok(head_dim, group_size) && n_q_heads % n_kv_heads == 0) {
+    need = std::max(need, partial_bytes(B, n_q_heads, head_dim,
+                                        plan_shared_fast(prompts, members, n_kv_heads,
+                                                         n_q_heads / n_kv_heads, prefix_len,
+                                                         seq_len - prefix_len)));
+  }
+  return need;
 }
 
 extern "C" int lq_int4_shared_decode_attention(
@@ -344,7 +368,18 @@ extern "C" int lq_int4_shared_decode_attention(
   p.own_len = own_len;
   p.scale_sm = (float)(1.4426950408889634 / sqrt((double)D));
 
-  const SharedPlan plan = plan_generic(B, Hq, prefix_len, own_len);
+  const bool fast = shared_fast_ok(p);
+  if (!fast && diag(LQ_DIAG_ATTN_REQUIRE_FAST)) {  // tests: the call must take the MFMA kernel
+    return fail(LQ_ERR_INVALID_ARG,
+                "LQ_ATTN_REQUIRE_FAST is set and this call takes the generic kernel");
+  }
+  if (k_new != nullptr) {
+    p.knew = row_view(k_new, 3);
+    p.vnew = row_view(v_new, 3);
+    p.pack = 1;
+  }
+  const SharedPlan plan = fast ? plan_shared_fast(P, B / P, Hkv, num_key_value_groups, prefix_len, own_len)
+                               : plan_generic(B, Hq, prefix_len, own_len);
   p.nsp = plan.prefix.nsplit;
   p.nso = plan.own.nsplit;
   p.chunk_p = plan.prefix.chunk;
@@ -365,15 +400,17 @@ extern "C" int lq_int4_shared_decode_attention(
     p.ws_acc = (float*)((char*)workspace + 2 * align256(slots * 4));
   }
   const hipStream_t st = (hipStream_t)stream;
-  if (k_new != nullptr) {
-    if ((rc = pack_pair_at(k_new, v_new, k_packed, v_packed, k_scale, v_scale, own_len - 1,
-                           group_size, true, st,
-                           "lq_int4_shared_decode_attention (pack)")) != LQ_OK) {
-      return rc;
+  if (fast) {
+    if ((rc = launch_shared_fast(p, st)) != LQ_OK) return rc;
+  } else {
+    if (p.pack) {
+      hipLaunchKernelGGL(shared_pack_kernel, dim3((unsigned)(B * Hkv), (unsigned)(D / group_size), 2),
+                         dim3(64), 0, st, p);
+      if ((rc = check_launch("lq_int4_shared_decode_attention (pack)")) != LQ_OK) return rc;
     }
+    hipLaunchKernelGGL(shared_generic_kernel, dim3((unsigned)(B * Hq), (unsigned)ns), dim3(64), 0, st, p);
+    if ((rc = check_launch("lq_int4_shared_decode_attention")) != LQ_OK) return rc;
   }
-  hipLaunchKernelGGL(shared_generic_kernel, dim3((unsigned)(B * Hq), (unsigned)ns), dim3(64), 0, st, p);
-  if ((rc = check_launch("lq_int4_shared_decode_attention")) != LQ_OK) return rc;
   if (ns > 1) {
     AttnParams a{};
     a.ws_m = p.ws_m;

@@ -1,0 +1,702 @@
+// MFMA path of the shared-prefix decode attention (head_dim 128, group 32/64/128, bf16 or fp16
+// queries, contiguous cache rows).
+//
+// One workgroup = 4 waves on one unit and key split. A prefix unit is (prompt, KV head, block of 16 QT
+// query rows), its query rows the prompt's members x the heads of the KV head; an own unit is (row, KV
+// head), its query rows the heads alone. Each wave takes every fourth 32-key tile of the split, on its
+// own: a ring of 3 tiles in LDS filled by loads that write LDS directly, no barrier in the key loop.
+// At the end the 4 partial softmax states are joined through LDS, and the split's (m, l, acc) goes to
+// the workspace (or, where it is the only split, out).
+//
+// Products use v_mfma_f32_16x16x32_f16, D[16x16] += A[16x32] * B[32x16] (lane l holds A row l%16 and B
+// column l%16, each with K slots 8*(l/16) .. +7, and D rows 4*(l/16) .. +3 of column l%16):
+//   S^T[key][query] per group m: A = K rows as exact fp16 integers, B = Q^T scaled by a power of two
+//     per query row so that its largest value lies in [2^14, 2^15) (16-bit queries are then exact in
+//     fp16, products exact, sums fp32); the groups' partial sums are scaled by the fp32 key scales and
+//     added in fp32.
+//   O^T[dim][query]: A = V^T as exact fp16 integers, B = P'_m[key][query] = 2^(s - M) * vscale[key][m],
+//     formed in fp32 and rounded to fp16 (bf16 outputs; relative 2^-11, less than the output's own
+//     rounding of 2^-8) or split into fp16 hi + lo (other outputs; about 22 bits).
+// M is the lazily moved running maximum of the row's scores plus an offset of the wave that follows the
+// largest value scale seen, so that P' stays below 2^15 and is exact to 2^-24 of 2^7 at the largest
+// score and scale: fp16 has no exponent range to spare for both.
+#include <math.h>
+
+#include "int4_f16.h"
+#include "int4_shared_attention.h"
+#include "lds_loads.h"
+
+namespace lq {
+namespace {
+
+constexpr int SD = 128;     // head_dim
+constexpr int TILE = 32;    // keys per wave step
+constexpr int WAVES = 4;
+constexpr int THREADS = 64 * WAVES;
+constexpr int SEG = 16;     // tiles of a wave whose keep-mask words are made together
+constexpr int OROW = SD + 4;  // floats per row of a wave's partial output (rows 4 banks apart)
+constexpr float LAZY = 8.0f;  // running-max slack of the lazy rescale
+constexpr int P_TOP = 7;      // P' of the largest score and value scale is about 2^P_TOP
+
+enum { MASK_NONE = 0, MASK_BIAS = 1, MASK_KEEP = 2 };
+
+// One wave's copy of a 32-key tile. K rows: 16-byte unit u of row r (r = key & 15 of the half) sits in
+// slot 4 r + (u ^ ((r >> 2) & 3)), so that the 64 dwords that one QK operand read takes lie in 64
+// different banks. V rows and the scales keep their order ([key][64 bytes], [key][group]).
+struct alignas(16) SharedTile {
+  u32x4_t k[2][64];
+  u32x4_t v[2][64];
+  float ks[TILE * 4];
+  float vs[TILE * 4];
+};
+
+// A wave's partial result: o [row][dim], then m and l per row.
+template <int QT>
+struct alignas(16) WavePartial {
+  float o[16 * QT][OROW];
+  float m[16 * QT], l[16 * QT];
+};
+
+template <int QT>
+union SharedLds {
+  SharedTile tiles[3][WAVES];
+  WavePartial<QT> part[WAVES];
+};
+
+struct MaskWords {
+  uint32_t w[SEG][33];  // keep bits of a tile's 32 keys per member of the row block; [32]: any member
+};
+
+// A unit of work: one stretch of one cache, and the query rows that attend to it.
+struct Unit {
+  const CacheView* c;
+  int64_t crow;      // the cache's row
+  int kvh;
+  int t0, t1, S;     // the split's keys, the cache's live keys
+  int64_t key0;      // the mask's key of cache row 0
+  int row0, rows;    // first query row of the block, query rows of the unit
+  int64_t b0;        // row of member 0 in q
+  int split;         // partial slot
+  bool pack;         // the token goes into cache row S - 1
+};
+
+template <int G>
+__device__ __forceinline__ void issue_tile(const uint8_t* kb, const uint8_t* vb, const float* ksb,
+                                           const float* vsb, int kvo, int tb, int S, SharedTile& B,
+                                           int lane) {
+  tb = __builtin_amdgcn_readfirstlane(tb);
+  const int rem = S - tb;  // > 0: keys past S read as 0
+  const i32x4_t rk = make_desc(kb + (int64_t)tb * 64, rem * 64);
+  const i32x4_t rv = make_desc(vb + (int64_t)tb * 64, rem * 64);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    load_to_lds(rk, &B.k[h][0], kvo + 1024 * h);
+    load_to_lds(rv, &B.v[h][0], 16 * lane + 1024 * h);
+  }
+  const i32x4_t rks = make_desc(ksb + (int64_t)tb * G, rem * G * 4);
+  const i32x4_t rvs = make_desc(vsb + (int64_t)tb * G, rem * G * 4);
+  // (lane 0 always issues these two, so that every tile counts 6 loads in the waits)
+  if constexpr (G == 4) {
+    if (lane < 32) {
+      load_to_lds(rks, &B.ks[0], 16 * lane);
+      load_to_lds(rvs, &B.vs[0], 16 * lane);
+    }
+  } else {
+    if (lane < 32 * G) {
+      load_to_lds_b32(rks, &B.ks[0], 4 * lane);
+      load_to_lds_b32(rvs, &B.vs[0], 4 * lane);
+    }
+  }
+}
+constexpr int LPT = 6;  // loads per tile
+
+// The scales of the lane's 8 keys q4 + 4e, all groups.
+template <int G>
+__device__ __forceinline__ void read_scales(const float* s, int q4, float (&out)[8][G]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float* at = s + (q4 + 4 * e) * G;
+    if constexpr (G == 4) {
+      const f32x4_t v = *(const f32x4_t*)at;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) out[e][m] = v[m];
+    } else {
+#pragma unroll
+      for (int m = 0; m < G; ++m) out[e][m] = at[m];
+    }
+  }
+}
+
+// Power of two at or above v as its exponent, kept between -60 and MAX_E: weights 2^(s - M) of 2^(8 - e)
+// at most still add up below 2^127, and those of 2^-e are normal 2^-20 times over.
+constexpr int MAX_E = 100;
+__device__ __forceinline__ int exponent_above(float v) {
+  const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
+  const int e = (int)(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0 ? 1 : 0);
+  return min(max(e, -60), MAX_E);
+}
+
+template <int QT, int G, int MASK, bool EXACT>
+__device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, SharedTile* ring,
+                                         MaskWords* words, WavePartial<QT>* part) {
+  constexpr int CPG = 4 / G;  // 32-dim chunks per group
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int q4 = lane >> 4;
+  const int c16 = lane & 15;
+  const CacheView& c = *u.c;
+  const uint8_t* kb = c.kp + u.crow * c.kps[0] + u.kvh * c.kps[1];
+  const uint8_t* vb = c.vp + u.crow * c.vps[0] + u.kvh * c.vps[1];
+  const float* ksb = c.ks + u.crow * c.kss[0] + u.kvh * c.kss[1];
+  const float* vsb = c.vs + u.crow * c.vss[0] + u.kvh * c.vss[1];
+  const int ntile = (u.t1 - u.t0 + TILE - 1) / TILE;
+  const int nw = ntile > wave ? (ntile - wave + WAVES - 1) / WAVES : 0;
+  auto tile_key = [&](const int i) { return u.t0 + (wave + WAVES * i) * TILE; };
+  // K slot l of a half holds row l >> 2, unit (l & 3) ^ ((l >> 4) & 3)
+  const int kvo = (lane >> 2) * 64 + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+  SharedTile& tile0 = ring[0 * WAVES + wave];
+  SharedTile& tile1 = ring[1 * WAVES + wave];
+  SharedTile& tile2 = ring[2 * WAVES + wave];
+  if (nw > 0) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(0), u.S, tile0, lane);
+  if (nw > 1) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(1), u.S, tile1, lane);
+
+  // Query operands: lane (q4, c16) of column tile qt holds query row row0 + 16 qt + c16, dims
+  // 32c + 8 q4 + (0,4,1,5,2,6,3,7) for chunk c, as fp16 q * 2^-e; cs turns its raw scores into exp2
+  // units. Rows past the unit's count hold 0.
+  u32x4_t qop[QT][4];
+  float cs[QT];
+  int member[QT];  // the row's member, relative to the row block's first
+  const int first_member = u.row0 / p.nrep;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int row = u.row0 + 16 * qt + c16;
+    const bool ok = row < u.rows;
+    const int r = ok ? row : u.rows - 1;
+    const int n = r / p.nrep;
+    member[qt] = n - first_member;
+    const int64_t base = (u.b0 + n) * p.q.s[0] + (int64_t)(u.kvh * p.nrep + r - n * p.nrep) * p.q.s[1];
+    uint32_t w[4][4];
+    const uint16_t* at = (const uint16_t*)p.q.data + base;
+    if (p.q_rows) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x4_t v = *(const u32x4_t*)(at + 32 * k + 8 * q4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[k][j] = v[j];
+      }
+    } else {
+      uint32_t e[4][8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[k][j] = at[(32 * k + 8 * q4 + j) * p.q.s[2]];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[k][j] = e[k][2 * j] | (e[k][2 * j + 1] << 16);
+      }
+    }
+    float qv[4][8];
+    float mx = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = ok ? w[k][j] : 0u;
+        qv[k][2 * j] = word_elem(x, 0, p.q.dtype);
+        qv[k][2 * j + 1] = word_elem(x, 16, p.q.dtype);
+        mx = fmaxf(mx, fmaxf(fabsf(qv[k][2 * j]), fabsf(qv[k][2 * j + 1])));
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    int e = mx > 0.0f ? (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127 - 14 : 0;
+    e = max(-100, min(100, e));
+    cs[qt] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_sm;
+    const float qinv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qop[qt][k][j] = pack_f16(qv[k][j] * qinv, qv[k][j + 4] * qinv);
+    }
+  }
+
+  float m_run[QT], l_run[QT];
+  f32x4_t acc[QT][8];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = -INFINITY;
+    l_run[qt] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[qt][k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  int voff = -1000;        // scales up to 2^(voff + P_TOP) are in range (uniform)
+  float vlim = -1.0f;      // that limit: a larger one moves voff
+
+  // Keep-mask: the wave turns the next SEG tiles' rows of the mask into one word of 32 keys per member
+  // of its row block, lanes 0..31 for one member and 32..63 for the next.
+  const int last_row = min(u.row0 + 16 * QT, u.rows) - 1;
+  const int members = last_row / p.nrep - first_member + 1;
+  auto make_words = [&](const int i0) {
+    for (int i = i0; i < min(i0 + SEG, nw); ++i) {
+      const int64_t key = u.key0 + tile_key(i) + (lane & 31);
+      uint32_t any = 0;
+      for (int a = 0; a < members; a += 2) {
+        const int n = a + (lane >> 5);
+        bool keep = false;
+        if (n < members && key < p.mask_len) {
+          keep = ((const int64_t*)p.mask)[(u.b0 + first_member + n) * p.mask_sb + key * p.mask_sk] != 0;
+        }
+        const uint64_t bits = __ballot(keep);
+        any |= (uint32_t)bits | (uint32_t)(bits >> 32);
+        if (lane < 2) words->w[i - i0][a + lane] = lane == 0 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+      }
+      if (lane == 0) words->w[i - i0][32] = any;
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  const int krow = 4 * (c16 & 3) + (c16 >> 2);  // key of QK A-row c16 in its half
+  // byte c16 & 3 of two dwords -> bytes 0 and 2
+  const uint32_t vsel = 0x0c040c00u + (c16 & 3) * 0x00010001u;
+
+  auto process = [&](const int i, SharedTile& B) {
+    const int tb = tile_key(i);
+    if constexpr (MASK == MASK_KEEP) {
+      if (i % SEG == 0) make_words(i);
+    }
+    if (i + 2 < nw) wait_loads<2 * LPT>();
+    else if (i + 1 < nw) wait_loads<LPT>();
+    else wait_loads<0>();
+    if (u.pack && tb <= u.S - 1 && u.S - 1 < tb + TILE) {
+      // the new token: quantised, written to cache row S - 1 and over that key's row of the tile. Lane
+      // j holds dims 2j and 2j + 1, a group is GH adjacent lanes.
+      constexpr int GH = SD / (2 * G);
+      const int key = u.S - 1 - tb;
+      const int hk = key >> 4;
+      const int r = key & 15;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const View& x = t == 0 ? p.knew : p.vnew;
+        const int64_t at = u.crow * x.s[0] + u.kvh * x.s[1];
+        const float x0 = load_float(x.data, x.dtype, at + 2 * lane * x.s[2]);
+        const float x1 = load_float(x.data, x.dtype, at + (2 * lane + 1) * x.s[2]);
+        const float scale = token_scale(group_max<GH>(fmaxf(fabsf(x0), fabsf(x1))));
+        const uint8_t byte = (uint8_t)(token_level(x0, scale) | token_level(x1, scale) << 4);
+        uint8_t* row = t == 0 ? (uint8_t*)&B.k[hk][4 * r + ((lane >> 4) ^ ((r >> 2) & 3))] + (lane & 15)
+                              : (uint8_t*)&B.v[hk][0] + r * 64 + lane;
+        *row = byte;
+        const_cast<uint8_t*>(t == 0 ? kb : vb)[(int64_t)(u.S - 1) * 64 + lane] = byte;
+        if ((lane & (GH - 1)) == 0) {
+          (t == 0 ? B.ks : B.vs)[key * G + lane / GH] = scale;
+          const_cast<float*>(t == 0 ? ksb : vsb)[(int64_t)(u.S - 1) * G + lane / GH] = scale;
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+
+    // ---- scores, raw units: key slot e = 4t + r of lane group q4 is key tb + 16 t + 4 r + q4
+    float s[QT][8];
+    {
+      float ks[8][G];
+      read_scales<G>(B.ks, q4, ks);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t* kd = (const uint32_t*)&B.k[t][0];
+#pragma unroll
+        for (int m = 0; m < G; ++m) {
+          u32x4_t ka[CPG];
+#pragma unroll
+          for (int cc = 0; cc < CPG; ++cc) {
+            ka[cc] = decode_octet_f16(kd[4 * (4 * krow + ((m * CPG + cc) ^ (c16 & 3))) + q4]);
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            f32x4_t a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int cc = 0; cc < CPG; ++cc) a = mfma_f16(ka[cc], qop[qt][m * CPG + cc], a);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int e = 4 * t + r;
+              s[qt][e] = m == 0 ? a[r] * ks[e][m] : fmaf(a[r], ks[e][m], s[qt][e]);
+            }
+          }
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+    }
+    // V operands of 32-dim chunk c: A row i of the two products is byte i of the chunk's 16 (its low
+    // and its high nibble), so that a product's 16 dims belong to one group. Lane (q4, c16) takes its
+    // byte of key rows q4 + 4e, key slots (2j, 2j+1) paired.
+    u32x4_t va[4][2];
+    {
+      const uint32_t* vrow = (const uint32_t*)&B.v[0][0] + 16 * q4 + (c16 >> 2);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a0 = vrow[64 * (2 * j) + 4 * k], a1 = vrow[64 * (2 * j + 1) + 4 * k];
+          const uint32_t y = __builtin_amdgcn_perm(a1, a0, vsel);
+          va[k][0][j] = nib_pair_f16(y);
+          va[k][1][j] = nib_pair_f16(y >> 4);
+        }
+      }
+    }
+    float vs[8][G];
+    read_scales<G>(B.vs, q4, vs);
+
+    // ---- masks
+    if constexpr (MASK == MASK_KEEP) {
+      const uint32_t* w = words->w[i % SEG];
+      const uint32_t any = w[32];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const uint32_t mine = w[member[qt]];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[qt][e] = (mine >> (q4 + 4 * e) & 1) != 0 ? s[qt][e] : -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int m = 0; m < G; ++m) vs[e][m] = (any >> (q4 + 4 * e) & 1) != 0 ? vs[e][m] : 0.0f;
+      }
+    }
+    if constexpr (MASK == MASK_BIAS) {
+      // additive, in exp2 units: the scores are turned into those first
+      uint32_t any = 0;  // keys that some query row of the wave attends to
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const float* row = (const float*)p.mask + (u.b0 + first_member + member[qt]) * p.mask_sb;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int64_t key = u.key0 + tb + q4 + 4 * e;
+          const float bias = key < p.mask_len ? row[key * p.mask_sk] : -INFINITY;
+          const bool on = bias != -INFINITY;
+          s[qt][e] = on ? fmaf(s[qt][e], cs[qt], bias) : -INFINITY;
+          any |= ((__ballot(on) >> (16 * q4)) & 0xffffu) != 0 ? 1u << e : 0u;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int m = 0; m < G; ++m) vs[e][m] = (any >> e & 1) != 0 ? vs[e][m] : 0.0f;
+      }
+    }
+    if (tb + TILE > u.t1) {  // keys past the split's range (their scales read as 0)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[qt][e] = tb + q4 + 4 * e < u.t1 ? s[qt][e] : -INFINITY;
+      }
+    }
+
+    // ---- running references: the value scales' exponent of the wave, each row's maximum
+    float vmax = vs[0][0];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+      for (int m = 0; m < G; ++m) vmax = fmaxf(vmax, vs[e][m]);
+    }
+    if (__any(vmax > vlim)) {
+      vmax = fmaxf(vmax, __shfl_xor(vmax, 16, 64));
+      vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
+      const int e = __builtin_amdgcn_readfirstlane(exponent_above(vmax));
+      const int next = max(voff, e - P_TOP);
+      if (voff > -1000 && next > voff) {
+        const float alpha = __builtin_amdgcn_exp2f((float)(voff - next));
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[qt][k] *= alpha;
+          l_run[qt] *= alpha;
+        }
+      }
+      voff = next;
+      vlim = e >= MAX_E ? INFINITY : __uint_as_float((uint32_t)(127 + voff + P_TOP) << 23);
+    }
+    const float fvoff = (float)voff;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float lm = s[qt][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) lm = fmaxf(lm, s[qt][e]);
+      if constexpr (MASK != MASK_BIAS) lm *= cs[qt];
+      if (__any(lm > m_run[qt] + LAZY)) {
+        float mt = fmaxf(lm, __shfl_xor(lm, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        const float m_new = fmaxf(m_run[qt], mt);
+        // accumulators are still zero while m_run is -inf
+        const float alpha = m_run[qt] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[qt] - m_new);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[qt][k] *= alpha;
+        l_run[qt] *= alpha;
+        m_run[qt] = m_new;
+      }
+      // -inf only while every score so far is: 0 then, for 2^(-inf)
+      const float m_use = m_run[qt] == -INFINITY ? 0.0f : m_run[qt];
+      float psum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (MASK == MASK_BIAS) {
+          s[qt][e] = __builtin_amdgcn_exp2f((s[qt][e] - m_use) - fvoff);
+        } else {
+          s[qt][e] = __builtin_amdgcn_exp2f(fmaf(s[qt][e], cs[qt], -(m_use + fvoff)));
+        }
+        psum += s[qt][e];
+      }
+      l_run[qt] += psum;
+    }
+
+    // ---- P' per group and the P V products
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int m = 0; m < G; ++m) {
+      u32x4_t hi[QT], lo[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f16x2_t h = {(_Float16)(s[qt][2 * j] * vs[2 * j][m]),
+                             (_Float16)(s[qt][2 * j + 1] * vs[2 * j + 1][m])};
+          hi[qt][j] = __builtin_bit_cast(uint32_t, h);
+          if constexpr (EXACT) {
+            lo[qt][j] = pack_f16(fmaf(s[qt][2 * j], vs[2 * j][m], -(float)h[0]),
+                                 fmaf(s[qt][2 * j + 1], vs[2 * j + 1][m], -(float)h[1]));
+          }
+        }
+      }
+#pragma unroll
+      for (int k = m * CPG; k < (m + 1) * CPG; ++k) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) acc[qt][2 * k + t] = mfma_f16(va[k][t], hi[qt], acc[qt][2 * k + t]);
+          if constexpr (EXACT) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) acc[qt][2 * k + t] = mfma_f16(va[k][t], lo[qt], acc[qt][2 * k + t]);
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  // 3-deep ring: the loads of the next two tiles are in flight while one is processed
+  for (int i = 0; i < nw; i += 3) {
+    if (i + 2 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 2), u.S, tile2, lane);
+    process(i, tile0);
+    if (i + 1 >= nw) break;
+    if (i + 3 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 3), u.S, tile0, lane);
+    process(i + 1, tile1);
+    if (i + 2 >= nw) break;
+    if (i + 4 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 4), u.S, tile1, lane);
+    process(i + 2, tile2);
+  }
+
+  // ---- the waves' states to LDS (over the tiles, which every wave has read), joined there
+  __syncthreads();
+  const float vscale = voff > -1000 ? __builtin_amdgcn_exp2f((float)voff) : 0.0f;
+  WavePartial<QT>& mine = part[wave];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    float l = l_run[qt];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const int row = 16 * qt + c16;
+    if (q4 == 0) {
+      mine.m[row] = m_run[qt];
+      mine.l[row] = l * vscale;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // dims 32k + 8 q4 + 2r + t
+      float* o = &mine.o[row][32 * k + 8 * q4];
+      const f32x4_t a = acc[qt][2 * k] * vscale, b = acc[qt][2 * k + 1] * vscale;
+      *(f32x4_t*)o = f32x4_t{a[0], b[0], a[1], b[1]};
+      *(f32x4_t*)(o + 4) = f32x4_t{a[2], b[2], a[3], b[3]};
+    }
+  }
+  __syncthreads();
+  const int tid = threadIdx.x;
+  const int ns = p.nsp + p.nso;
+#pragma unroll
+  for (int pass = 0; pass < 2 * QT; ++pass) {
+    const int row = 8 * pass + (tid >> 5);
+    const int d = 4 * (tid & 31);
+    if (u.row0 + row >= u.rows) continue;
+    float M = -INFINITY, L = 0.0f;
+    float mw[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      mw[w] = part[w].m[row];
+      M = fmaxf(M, mw[w]);
+    }
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float wt = partial_weight(mw[w], M);
+      L += wt * part[w].l[row];
+      o += wt * *(const f32x4_t*)&part[w].o[row][d];
+    }
+    const int n = (u.row0 + row) / p.nrep;
+    const int qh = u.kvh * p.nrep + u.row0 + row - n * p.nrep;
+    const int64_t b = u.b0 + n;
+    if (ns == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        store_float(p.out.data, p.out.dtype, b * p.out.s[0] + qh * p.out.s[1] + (d + j) * p.out.s[2],
+                    o[j] / L);
+      }
+    } else {
+      const int64_t slot = (b * p.Hq + qh) * ns + u.split;
+      *(f32x4_t*)&p.ws_acc[slot * SD + d] = o;
+      if (d == 0) {
+        p.ws_m[slot] = M;
+        p.ws_l[slot] = L;
+      }
+    }
+  }
+}
+
+// Blocks: the prefix units first (KV head fastest, so that the row blocks that share keys lie on the
+// same XCD where there are 8 KV heads; then row block, split, prompt), then the own units.
+template <int QT, int G, int MASK, bool EXACT>
+__global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p) {
+  __shared__ SharedLds<QT> lds;
+  __shared__ MaskWords words[MASK == MASK_KEEP ? WAVES : 1];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  MaskWords* mine = &words[MASK == MASK_KEEP ? wave : 0];
+  uint32_t i = blockIdx.x;
+  Unit u;
+  if (i < p.prefix_blocks) {
+    u.kvh = i % p.Hkv;
+    i /= p.Hkv;
+    const int rb = i % p.rb_prefix;
+    i /= p.rb_prefix;
+    u.split = i % p.nsp;
+    const int prompt = i / p.nsp;
+    u.c = &p.prefix;
+    u.crow = prompt;
+    u.S = (int)p.prefix_len;
+    u.t0 = u.split * (int)p.chunk_p;
+    u.t1 = min(u.S, u.t0 + (int)p.chunk_p);
+    u.key0 = 0;
+    u.row0 = rb * 16 * QT;
+    u.rows = p.N * p.nrep;
+    u.b0 = (int64_t)prompt * p.N;
+    u.pack = false;
+    run_unit<QT, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, lds.part);
+  } else {
+    i -= p.prefix_blocks;
+    u.kvh = i % p.Hkv;
+    i /= p.Hkv;
+    const int rb = i % p.rb_own;
+    i /= p.rb_own;
+    const int split = i % p.nso;
+    const int b = i / p.nso;
+    u.split = p.nsp + split;
+    u.c = &p.own;
+    u.crow = b;
+    u.S = (int)p.own_len;
+    u.t0 = split * (int)p.chunk_o;
+    u.t1 = min(u.S, u.t0 + (int)p.chunk_o);
+    u.key0 = p.prefix_len;
+    u.row0 = rb * 16;
+    u.rows = p.nrep;
+    u.b0 = b;
+    u.pack = p.pack && u.t1 == u.S;
+    run_unit<1, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, (WavePartial<1>*)lds.part);
+  }
+}
+
+template <int QT, int G, int MASK>
+void launch_exact(const SharedParams& p, dim3 grid, hipStream_t st) {
+  if (p.out.dtype == LQ_BF16) {
+    hipLaunchKernelGGL((shared_mfma_kernel<QT, G, MASK, false>), grid, dim3(THREADS), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((shared_mfma_kernel<QT, G, MASK, true>), grid, dim3(THREADS), 0, st, p);
+  }
+}
+
+template <int QT, int G>
+void launch_mask(const SharedParams& p, dim3 grid, hipStream_t st) {
+  if (p.mask == nullptr) launch_exact<QT, G, MASK_NONE>(p, grid, st);
+  else if (p.mask_keep) launch_exact<QT, G, MASK_KEEP>(p, grid, st);
+  else launch_exact<QT, G, MASK_BIAS>(p, grid, st);
+}
+
+template <int G>
+void launch_tiles(const SharedParams& p, dim3 grid, hipStream_t st) {
+  if (p.col_tiles == 1) launch_mask<1, G>(p, grid, st);
+  else launch_mask<2, G>(p, grid, st);
+}
+
+bool cache_ok(const CacheView& c, int64_t len, int64_t G) {
+  // contiguous key rows: 64 packed bytes per key, D/g scale words per key; 4-byte aligned; 32-bit
+  // extents of one (row, KV head) block
+  if (c.kps[3] != 1 || c.vps[3] != 1 || c.kps[2] != 64 || c.vps[2] != 64) return false;
+  if (c.kss[3] != 1 || c.vss[3] != 1 || c.kss[2] != G || c.vss[2] != G) return false;
+  for (int64_t s : {c.kps[0], c.kps[1], c.vps[0], c.vps[1]}) {
+    if (s % 4 != 0) return false;
+  }
+  for (const void* d : {(const void*)c.kp, (const void*)c.vp, (const void*)c.ks, (const void*)c.vs}) {
+    if (((uintptr_t)d & 3) != 0) return false;
+  }
+  return len * 64 < (int64_t)1 << 31;
+}
+
+}  // namespace
+
+bool shared_fast_shape_ok(int64_t head_dim, int group_size) {
+  return head_dim == SD && (group_size == 32 || group_size == 64 || group_size == 128);
+}
+
+bool shared_fast_ok(const SharedParams& p) {
+  if (diag(LQ_DIAG_ATTN_FORCE_GENERIC)) return false;
+  if (!shared_fast_shape_ok(p.D, p.g)) return false;
+  if (p.q.dtype != LQ_BF16 && p.q.dtype != LQ_F16) return false;
+  const int64_t G = SD / p.g;
+  if (!cache_ok(p.prefix, p.prefix_len, G) || !cache_ok(p.own, p.own_len, G)) return false;
+  return ((uintptr_t)p.mask & (p.mask_keep ? 7 : 3)) == 0;
+}
+
+// Column tiles of 16 query rows per wave in the prefix units.
+static int col_tiles_of(int64_t rows) { return rows <= 16 ? 1 : 2; }
+
+SharedPlan plan_shared_fast(int64_t P, int64_t N, int64_t Hkv, int64_t nrep, int64_t prefix_len,
+                            int64_t own_len) {
+  const int64_t resident = 2 * (int64_t)device_cus();  // workgroups: 2 per CU
+  const int64_t rows = N * nrep;
+  const int64_t block = 16 * col_tiles_of(rows);
+  const int64_t units = std::max<int64_t>(1, P * Hkv * ((rows + block - 1) / block));
+  const int64_t own_units = std::max<int64_t>(1, P * N * Hkv * ((nrep + 15) / 16));
+  constexpr int64_t STEP = WAVES * TILE;
+  return SharedPlan{split_of(prefix_len, resident / units, STEP),
+                    split_of(own_len, resident / own_units, STEP)};
+}
+
+int launch_shared_fast(SharedParams p, hipStream_t st) {
+  const int64_t rows = (int64_t)p.N * p.nrep;
+  p.col_tiles = col_tiles_of(rows);
+  p.rb_prefix = (int)((rows + 16 * p.col_tiles - 1) / (16 * p.col_tiles));
+  p.rb_own = (p.nrep + 15) / 16;
+  const int64_t pb = (int64_t)p.P * p.Hkv * p.rb_prefix * p.nsp;
+  const int64_t ob = (int64_t)p.B * p.Hkv * p.rb_own * p.nso;
+  if (pb + ob >= (int64_t)1 << 31) {
+    return fail(LQ_ERR_UNSUPPORTED, "%lld workgroups exceed the launch limits", (long long)(pb + ob));
+  }
+  p.prefix_blocks = (uint32_t)pb;
+  const View& q = p.q;
+  p.q_rows = q.s[2] == 1 && ((uintptr_t)q.data & 15) == 0 && q.s[0] % 8 == 0 && q.s[1] % 8 == 0;
+  const dim3 grid((unsigned)(pb + ob));
+  switch (SD / p.g) {
+    case 4: launch_tiles<4>(p, grid, st); break;
+    case 2: launch_tiles<2>(p, grid, st); break;
+    default: launch_tiles<1>(p, grid, st); break;
+  }
+  return check_launch("lq_int4_shared_decode_attention (mfma)");
+}
+
+}  // namespace lq

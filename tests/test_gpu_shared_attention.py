@@ -7,6 +7,11 @@ the sums' weights and values against A = sum_j w_j |v_j| / sum_j w_j:
     it); both the sum of the weights and the weighted values have it: 2 ln 2 delta;
   * the matrix-core kernel rounds weight, value scale and their product to fp16 for bf16 outputs:
     3 * 2^-11; for other outputs it keeps 2^-20 of them;
+  * fp16 has steps of 2^-24 below 2^-14: a weighted scale P' = w vs 2^(7-e), 2^e at most twice the
+    largest value scale, is off by half a step at most, which with levels of at most 8 is
+    8 * 2^-25 * 2^(e-7) <= 2^-28 times the largest value scale per key, whatever the weight (where one
+    key has all the weight and level 0, the others' weights can be far below that). A weight below
+    2^-126 of the largest is 0 in fp32: 8 * 2^-126 of the largest scale per key;
   * fp32 sums over the keys of a split and the merge: 2^-24 per addition in a row, fewer than 2^8 of
     them in the matrix-core kernel's lanes per rescale step, linear in the keys else: keys * 2^-23.
 """
@@ -43,13 +48,23 @@ def cache_of(gpu, rows, hkv, length, cap, d, g, seed, scale=1.0, fill=0):
     return c
 
 
+def pack_token(x, packed, scale, row, g):
+    """The token's levels and scales: absmax * fl(1/7), levels by IEEE quotients, half to even."""
+    xg = x.float().reshape(*x.shape[:-1], -1, g)
+    sc = (xg.abs().amax(-1, keepdim=True) * torch.tensor(1 / 7, device=x.device)).clamp_min(1e-8)
+    n = (xg / sc).round().clamp(-8, 7).to(torch.int32).reshape(x.shape) & 15
+    packed[:, :, row:row + 1] = (n[..., 0::2] | n[..., 1::2] << 4).to(torch.uint8)
+    scale[:, :, row:row + 1] = sc[..., 0]
+
+
 def reference(q, cache, seq_len, nrep, g, bias=None):
-    """(out, A, delta) in 64 bits: out [B, Hq, D], the weighted |v|, and the scores' error unit."""
+    """(out, A, delta, vs) in 64 bits: out [B, Hq, D], the weighted |v|, the scores' error unit, and the
+    largest value scale (a group's largest level is 7)."""
     pre, lp = cache.prefix, cache.prefix.length
     B, hq, d = q.shape[0], q.shape[1], q.shape[-1]
     N = B // pre.k_packed.shape[0]
     q = q.reshape(B, hq, d).double()
-    outs, mags, deltas = [], [], []
+    outs, mags, deltas, top = [], [], [], 0.0
     for b in range(B):
         rows = [(pre, b // N, lp), (cache, b, seq_len - lp)]
         k, v = (torch.cat([oik.dequantize(getattr(c, n + "_packed")[i:i + 1, :, :m].cpu(),
@@ -63,12 +78,13 @@ def reference(q, cache, seq_len, nrep, g, bias=None):
             v = torch.where(gone[None, :, None], 0.0, v)
             s = torch.where(gone, -math.inf, s + bias[b])
             mag = torch.where(gone, 0.0, mag)
+        top = max(top, v.abs().max().item() / 7)
         w = torch.exp2(s - s.amax(-1, keepdim=True))
         w = w / w.sum(-1, keepdim=True)
         outs.append((w[:, None] @ v)[:, 0])
         mags.append((w[:, None] @ v.abs())[:, 0])
         deltas.append(mag.amax(-1, keepdim=True))
-    return torch.stack(outs), torch.stack(mags), torch.stack(deltas)
+    return torch.stack(outs), torch.stack(mags), torch.stack(deltas), top
 
 
 def fast_expected(dtype, d, g):
@@ -76,14 +92,15 @@ def fast_expected(dtype, d, g):
 
 
 def assert_near(out, ref, dtype, d, keys, fast, what=""):
-    want, mag, delta = ref
+    want, mag, delta, top = ref
     out = out.double()
     empty = torch.isnan(want)
     assert torch.equal(torch.isnan(out), empty), what
     rel = 2 * math.log(2) * (d + 16) * 2.0 ** -24 * delta + keys * 2.0 ** -23
     if fast:
         rel = rel + (3 * 2.0 ** -11 if dtype == BF16 else 2.0 ** -20)
-    bound = torch.finfo(dtype).eps / 2 * want.abs() + rel * mag + 1e-30
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + rel * mag
+    bound = bound + keys * top * (2.0 ** -28 if fast else 2.0 ** -123) + 1e-300
     if dtype == FP16:
         bound = bound + 2.0 ** -25  # half a step of its subnormal values
     worst = ((out - want).abs() / bound)[~empty]
@@ -112,8 +129,9 @@ def run(gpu, P, N, hkv, nrep, lp, lo, d, g, dtype, seed=0, mask=None, token=True
     with require_env("LQ_ATTN_REQUIRE_FAST", fast):
         out = ia.shared_prefix_decode_attention(q, own, S, nrep, g, mask, k, v)
     if k is not None:
-        _abi.int4_pack_kv_pair(k, v, *before, torch.tensor([lo - 1], device=gpu), g)
-    # the caches: the token's row as the pack kernel writes it, everything else as it was
+        pack_token(k, before[0], before[2], lo - 1, g)
+        pack_token(v, before[1], before[3], lo - 1, g)
+    # the caches: the token's row, everything else as it was
     for t, w in zip((own.k_packed, own.v_packed, own.k_scale, own.v_scale), before):
         assert torch.equal(t.view(torch.uint8), w.view(torch.uint8))
     for t, w in zip((pre.k_packed, pre.v_packed, pre.k_scale, pre.v_scale), pre_before):
@@ -252,6 +270,29 @@ def test_layouts(gpu):
                 q, None, None, (pre.k_packed, pre.v_packed, pre.k_scale, pre.v_scale),
                 (own.k_packed, own.v_packed, own.k_scale, own.v_scale), None, o, lp, lp + lo, nrep, g)
             assert_near(o, ref, dt, 128, lp + lo, True)
+
+
+def test_token_scale(gpu):
+    """The token's scales: within one unit in the last place of the pack kernel's quotients, and those
+    of int4_quant_dequant on the GPU, in both kernels."""
+    B, hkv, g = 64, 8, 32
+    own = cache_of(gpu, B, hkv, 5, 8, 128, g, 2)
+    own.prefix = cache_of(gpu, 8, hkv, 40, 40, 128, g, 1)
+    k, v = torch.randn(2, B, hkv, 1, 128, device=gpu).to(BF16)
+    q = torch.randn(B, hkv * 4, 1, 128, device=gpu).to(BF16)
+    packed = ia._allocate_layer_cache(B, hkv, 8, 128, 4, gpu)
+    _abi.int4_pack_kv_pair(k, v, packed.k_packed, packed.v_packed, packed.k_scale, packed.v_scale,
+                           torch.tensor([4], device=gpu), g)
+    for generic in (False, True):
+        own.k_scale[:, :, 4], own.v_scale[:, :, 4] = 0, 0
+        with require_env("LQ_ATTN_FORCE_GENERIC", generic):
+            ia.shared_prefix_decode_attention(q, own, 45, 4, g, None, k, v)
+        for x, s, w, n in ((k, own.k_scale, packed.k_scale, own.k_packed),
+                           (v, own.v_scale, packed.v_scale, own.v_packed)):
+            got, want = s[:, :, 4], w[:, :, 4]
+            assert (got.view(torch.int32) - want.view(torch.int32)).abs().max() <= 1
+            values = oik.dequantize(n[:, :, 4:5].cpu(), s[:, :, 4:5].cpu(), g)
+            assert torch.equal(values.to(BF16), ia.int4_quant_dequant(x, g).cpu())
 
 
 def test_matches_the_plain_decode_attention(gpu):
