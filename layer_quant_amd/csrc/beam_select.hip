@@ -4,18 +4,19 @@
 // beam's logits. Within a beam the order of the totals is the order of the logits, so that one pass over
 // the logits gives both.
 //
-// select_part_kernel: a workgroup of 4 waves takes a part of one beam's row in runs of 1024 logits per
-// wave (16 per lane). Each lane keeps a running maximum and the sum of e^(x - maximum); each wave keeps a
-// list of the logits above a threshold that only rises: the num-th largest of the lanes' maxima where
-// at least that many lanes pass it (num logits are then at least as large), and the num-th largest of the
-// list where the list is full. The num-th largest of the values in a wave's registers is found bit by
-// bit with ballots (kth_word), with no exchange between lanes. The part leaves (max, sum) and its num
-// largest logits, ties by the lower token.
+// select_part_kernel: a workgroup of 4 waves takes a part of one beam's row, up to 64 logits per lane, all
+// loaded at once and kept in registers as they are. A pass over them makes the lanes' maxima and sums;
+// the num-th largest of the 256 maxima is a threshold that num logits reach, and few others (about 34
+// for 32, of 16384 random ones). A second pass over the registers collects those in lists, which
+// are cut down to their num largest, ties by the lower token. The num-th largest of the values in a
+// wave's registers is found bit by bit with ballots (kth_word), with no exchange between lanes. Lists that
+// overflow (many equal logits, sorted ones) are cut on the way, which raises the threshold. The part
+// leaves (max, sum), its num largest logits and a bound that they all reach.
 //
-// select_final_kernel: one workgroup per prompt makes lse[n] and the totals of the parts' candidates in
-// 64 bits (their order then goes wrong only where totals are closer than the sums' rounding, about
-// 1e-7), reduces them 256 per wave to num per wave until one wave holds them, sorts those and writes
-// them out, by rank or by place.
+// select_final_kernel: one workgroup per prompt makes lse[n] and the totals in 64 bits (their order then
+// goes wrong only where totals are closer than the sums' rounding, about 1e-7). num candidates reach
+// the largest of the parts' bounds; those that do (a few hundred) are reduced, wave by wave, to
+// the num best, which one wave sorts and writes out, by rank or by place.
 #include <math.h>
 
 #include <algorithm>
@@ -32,9 +33,12 @@ constexpr int THREADS = 64 * WAVES;
 constexpr int PER = 16;             // logits per lane and run
 constexpr int RUN = 64 * PER;       // logits per wave and run
 constexpr int LIST = 256;           // entries of a wave's candidate list (4 per lane)
-constexpr int FINAL_WAVES = 16;     // waves of a prompt's workgroup
-constexpr int FINAL_MAX = 256 * FINAL_WAVES;  // candidates of a prompt
-static_assert(MAX_BEAMS * MAX_NUM <= FINAL_MAX, "one part per beam always fits");
+constexpr int FINAL_LIST = 1024;    // entries of a prompt's candidate list
+
+struct PartResult {
+  float m, s;      // maximum and sum of e^(x - m)
+  uint32_t bound;  // order of a logit that num of them reach; 0: there are fewer
+};
 
 struct SelectParams {
   View logits;          // strides of (prompt, beam, token)
@@ -49,10 +53,10 @@ struct SelectParams {
   int64_t pad;
   int P, N, num, slots;
   int64_t V;
-  int parts, runs;      // parts of a row, runs of a part
-  float* ws_m;          // [rows][parts]
-  float* ws_s;
-  uint64_t* ws_key;     // [rows][parts][num]: order of the logit, then of the token; 0: none
+  int parts, cap;       // parts of a row, places for a part's candidates
+  PartResult* ws_part;  // [rows][parts]
+  uint64_t* ws_key;     // [rows][parts][cap]: order of the logit, then of the token; 0: none
+  uint32_t inv_cap, inv_parts;  // ceil(2^32 / cap) and .. / parts (0 for 1), for quotients by them
 };
 
 constexpr float LOG2E_F = 1.44269504f;
@@ -206,143 +210,150 @@ __device__ __forceinline__ void cut_list(uint64_t* list, int& n, int k, uint64_t
   }
 }
 
+// The 16 logits of a lane in a run, as they are in memory.
 template <int DT>
-struct Vec {
-  static constexpr int N = DT == LQ_F32 ? 4 : 8;  // logits of 16 bytes
-  static constexpr int LOADS = PER / N;
-  uint4 raw[LOADS];
-};
+struct Raw {
+  static constexpr int SIZE = DT == LQ_F32 ? 4 : 2;
+  static constexpr int N = 16 / SIZE;  // logits of 16 bytes
+  static constexpr int WORDS = PER * SIZE / 4;
+  uint32_t w[WORDS];
 
-template <int DT>
-__device__ __forceinline__ void unpack(const Vec<DT>& v, float (&x)[PER]) {
-#pragma unroll
-  for (int j = 0; j < Vec<DT>::LOADS; ++j) {
-    const uint32_t w[4] = {v.raw[j].x, v.raw[j].y, v.raw[j].z, v.raw[j].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == LQ_F32) {
-        x[4 * j + i] = __uint_as_float(w[i]);
-      } else {
-        x[8 * j + 2 * i] = word_elem(w[i], 0, DT);
-        x[8 * j + 2 * i + 1] = word_elem(w[i], 16, DT);
-      }
-    }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (DT == LQ_F32) return __uint_as_float(w[i]);
+    else return word_elem(w[i / 2], 16 * (i % 2), DT);
   }
-}
+};
 
 // 16 bytes at any address: the order of a row's sums must not depend on where the row starts, so that
 // beams with equal logits get equal totals (a row of an odd vocabulary starts at any multiple of 2 bytes).
 struct __attribute__((packed, aligned(2))) Unaligned16 {
-  uint4 v;
+  uint32_t v[4];
 };
 
 // DENSE: the logits of a row are contiguous and loaded 16 bytes per lane, but for the row's last run.
-// Otherwise, and there, one element at a time.
-template <int DT, bool DENSE>
+// Otherwise, and there, one element at a time. Wave w takes runs w, w + 4, .. of the part's 4 R.
+template <int DT, bool DENSE, int R>
 __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
   __shared__ uint64_t lists[WAVES][LIST];
+  __shared__ uint32_t maxima[THREADS];
+  __shared__ uint32_t threshold;
   __shared__ int counts[WAVES];
   __shared__ float wave_m[WAVES], wave_s[WAVES];
-  constexpr int VN = Vec<DT>::N;
+  constexpr int VN = Raw<DT>::N;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int64_t row = blockIdx.y;
   const int64_t prompt = row / p.N, beam = row - prompt * p.N;
   if (p.finished != nullptr && p.finished[prompt * p.fs[0] + beam * p.fs[1]] != 0) return;
   const int64_t base = prompt * p.logits.s[0] + beam * p.logits.s[1];
-  const char* first = (const char*)p.logits.data + base * (DT == LQ_F32 ? 4 : 2);
-  const int r0 = blockIdx.x * p.runs;
-  const int nruns = (int)min((int64_t)p.runs, (p.V + RUN - 1) / RUN - r0);
+  const char* first = (const char*)p.logits.data + base * Raw<DT>::SIZE;
+  const uint32_t V = (uint32_t)p.V;
   const int k = p.num;
   uint64_t* list = lists[wave];
 
-  // token of the lane's logit i of the run from token `start` on
+  // first token of run r of the wave, and token of the lane's logit i in it
+  auto start_of = [&](int r) -> uint32_t { return (blockIdx.x * (WAVES * R) + r * WAVES + wave) * RUN; };
   auto token = [&](uint32_t start, int i) -> uint32_t {
     return DENSE ? start + ((i / VN) * 64 + lane) * VN + i % VN : start + i * 64 + lane;
   };
-  auto load = [&](int r, Vec<DT>& v) {
-    const int64_t start = (int64_t)(r0 + r) * RUN;
-    if constexpr (DENSE) {
-      if (r >= nruns || start + RUN > p.V) return;
-      const Unaligned16* at = (const Unaligned16*)(first + start * (DT == LQ_F32 ? 4 : 2)) + lane;
-#pragma unroll
-      for (int j = 0; j < Vec<DT>::LOADS; ++j) v.raw[j] = at[64 * j].v;
-    }
-  };
 
-  float ml = -INFINITY, sl = 0.0f;  // the lane's maximum and sum
-  int n = 0;                        // entries of the list
-  uint64_t bar = 0;                 // only larger keys are taken, whose logits reach barf
-  float barf = -INFINITY;
-  Vec<DT> next;
-  load(wave, next);
-  for (int r = wave; r < nruns; r += WAVES) {
-    const uint32_t start = (uint32_t)(r0 + r) * RUN;
-    float x[PER];
-    uint32_t valid = 0xffffu;
-    if (DENSE && (int64_t)start + RUN <= p.V) {
-      unpack<DT>(next, x);
-      load(r + WAVES, next);
+  Raw<DT> x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t start = start_of(r);
+    if (DENSE && start + RUN <= V) {
+      const Unaligned16* at = (const Unaligned16*)(first + (int64_t)start * Raw<DT>::SIZE) + lane;
+#pragma unroll
+      for (int j = 0; j < PER / VN; ++j) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[r].w[4 * j + u] = at[64 * j].v[u];
+      }
     } else {
-      valid = 0;
+      // tokens past the row as -inf
+      constexpr uint32_t NONE = DT == LQ_F32 ? 0xff800000u : DT == LQ_BF16 ? 0xff80u : 0xfc00u;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t t = token(start, i);
-        x[i] = -INFINITY;
-        if (t < (uint32_t)p.V) {
-          x[i] = load_float(p.logits.data, DT, base + (int64_t)t * p.logits.s[2]);
-          valid |= 1u << i;
-        }
-      }
-    }
-    float mx = x[0];
+      for (int u = 0; u < Raw<DT>::WORDS; ++u) x[r].w[u] = 0;
+      if (start < V) {
 #pragma unroll
-    for (int i = 1; i < PER; ++i) mx = fmaxf(mx, x[i]);
-    if (mx > ml) {
-      sl *= __builtin_amdgcn_exp2f((ml - mx) * LOG2E_F);
-      ml = mx;
-    }
-    const float m0 = ml == -INFINITY ? 0.0f : ml;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sl += __builtin_amdgcn_exp2f((x[i] - m0) * LOG2E_F);
-
-    const uint64_t lanes = __ballot(mx >= barf);
-    if (lanes == 0) continue;
-    if (count(lanes) >= k) {
-      // k lanes' largest logits at least reach it: the k-th largest of those is a threshold
-      uint32_t v[1] = {valid != 0 ? order_bits(mx) : 0};
-      const int have = count(__ballot(v[0] != 0));
-      if (have >= k) {
-        bool exact = false;
-        uint32_t w = 0;
-        if (have == k) {
-          w = wave_fold(v[0] != 0 ? v[0] : ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
-        } else {
-          w = kth_word<1>(v, k, exact);
-        }
-        uint64_t low = (uint64_t)w << 32;
-        if (!exact && count_from<1>(v, w) > k + 8) {
-          // many lanes tie (banned or equal logits): of those the ones with the lowest tokens count
-          uint32_t t = 0;
-#pragma unroll
-          for (int i = PER - 1; i >= 0; --i) {
-            if (x[i] == mx && (valid >> i & 1) != 0) t = 0xffffffffu - token(start, i);
+        for (int i = 0; i < PER; ++i) {
+          const uint32_t t = token(start, i);
+          const int64_t at = base + (int64_t)t * p.logits.s[2];
+          uint32_t bits = NONE;
+          if constexpr (DT == LQ_F32) {
+            if (t < V) bits = ((const uint32_t*)p.logits.data)[at];
+            x[r].w[i] = bits;
+          } else {
+            if (t < V) bits = ((const uint16_t*)p.logits.data)[at];
+            x[r].w[i / 2] |= bits << (16 * (i % 2));
           }
-          const int need = k - count(__ballot(v[0] > w));
-          v[0] = v[0] == w ? t : 0;
-          low |= kth_word<1>(v, need, exact);
         }
-        if (low != 0 && low - 1 > bar) {
-          bar = low - 1;
-          barf = from_order_bits(w);
-        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < Raw<DT>::WORDS; ++u) x[r].w[u] = DT == LQ_F32 ? NONE : NONE | NONE << 16;
       }
     }
+  }
+
+  float mx = -INFINITY, run_max[R];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (__ballot(x[i] >= barf) == 0) continue;
-      const uint64_t key = make_key(x[i], token(start, i));
-      bool ok = x[i] >= barf && (valid >> i & 1) != 0 && key > bar;
+  for (int r = 0; r < R; ++r) {
+    run_max[r] = x[r][0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) run_max[r] = fmaxf(run_max[r], x[r][i]);
+    mx = fmaxf(mx, run_max[r]);
+  }
+  maxima[threadIdx.x] = token(start_of(0), 0) < V ? order_bits(mx) : 0;  // 0: a lane without a token
+  const float m0 = mx == -INFINITY ? 0.0f : mx;
+  float sl = 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sl += __builtin_amdgcn_exp2f((x[r][i] - m0) * LOG2E_F);
+  }
+  const float wm = group_max<64>(mx);
+  const float ws = group_sum<64>(sl * (mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx - wm) * LOG2E_F)));
+  if (lane == 0) {
+    wave_m[wave] = wm;
+    wave_s[wave] = ws;
+  }
+  __syncthreads();
+
+  // the threshold: only keys above bar are taken, whose logits reach barf
+  if (wave == 0) {
+    uint32_t v[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v[w] = maxima[64 * w + lane];
+    bool exact;
+    const uint32_t w = count_from<WAVES>(v, 1) > k ? kth_word<WAVES>(v, k, exact) : 0;
+    if (lane == 0) threshold = w;
+  }
+  __syncthreads();
+  const uint32_t bound = __builtin_amdgcn_readfirstlane(threshold);
+  uint64_t bar = 0;
+  float barf = -INFINITY;
+  if (bound != 0) {
+    bar = ((uint64_t)bound << 32) - 1;
+    barf = from_order_bits(bound);
+  }
+  int n = 0;  // entries of the wave's list
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (__ballot(run_max[r] >= barf) == 0) continue;
+    // the lane's logits that reach the threshold, taken one per lane at a time
+    uint32_t hits = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) hits |= x[r][i] >= barf ? 1u << i : 0u;
+    while (__ballot(hits != 0) != 0) {
+      const bool more = hits != 0;
+      const int i = more ? __builtin_ctz(hits) : 0;
+      hits &= hits - 1;  // (0 stays 0)
+      uint32_t w = x[r].w[0];
+#pragma unroll
+      for (int u = 1; u < Raw<DT>::WORDS; ++u) w = i * Raw<DT>::SIZE / 4 == u ? x[r].w[u] : w;
+      const float xi = DT == LQ_F32 ? __uint_as_float(w) : word_elem(w, 16 * (i & 1), DT);
+      const uint32_t t = token(start_of(r), i);
+      const uint64_t key = make_key(xi, t);
+      bool ok = more && xi >= barf && t < V && key > bar;
       uint64_t b = __ballot(ok);
       if (n + count(b) > LIST) {
         cut_list(list, n, k, bar, barf);
@@ -352,19 +363,13 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
       if (ok) list[n + below(b)] = key;
       n += count(b);
     }
-    __builtin_amdgcn_wave_barrier();
   }
-  if (n > k) cut_list(list, n, k, bar, barf);
-
-  const float wm = group_max<64>(ml);
-  const float ws = group_sum<64>(sl * (ml == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml - wm) * LOG2E_F)));
-  if (lane == 0) {
-    counts[wave] = n;
-    wave_m[wave] = wm;
-    wave_s[wave] = ws;
-  }
+  __builtin_amdgcn_wave_barrier();
+  if (n > 64) cut_list(list, n, k, bar, barf);
+  if (lane == 0) counts[wave] = n;
   __syncthreads();
   if (wave != 0) return;
+
   const int64_t slot = row * p.parts + blockIdx.x;
   float M = wave_m[0], S = 0.0f;
 #pragma unroll
@@ -373,25 +378,35 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
   for (int w = 0; w < WAVES; ++w) {
     S += wave_s[w] * (wave_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((wave_m[w] - M) * LOG2E_F));
   }
+  // the part's candidates: the lists as they are where they fit (num of them reach the bound, the final
+  // workgroup looks at the others' totals anyway), else the num largest
   uint64_t key[WAVES];
   bool take[WAVES];
+  int have = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) key[w] = lane < counts[w] ? lists[w][lane] : 0;
-  __builtin_amdgcn_wave_barrier();
-  take_keys<WAVES>(key, k, take);
+  for (int w = 0; w < WAVES; ++w) {
+    have += counts[w];
+    key[w] = lane < counts[w] ? lists[w][lane] : 0;
+    take[w] = key[w] != 0;
+  }
+  if (have > p.cap) take_keys<WAVES>(key, k, take);
   int total = 0;
+  uint32_t low = ~0u;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
     const uint64_t b = __ballot(take[w]);
-    if (take[w]) list[total + below(b)] = key[w];
+    if (take[w]) {
+      p.ws_key[slot * p.cap + total + below(b)] = key[w];
+      low = min(low, (uint32_t)(key[w] >> 32));
+    }
     total += count(b);
   }
-  __builtin_amdgcn_wave_barrier();
+  for (int i = total + lane; i < p.cap; i += 64) p.ws_key[slot * p.cap + i] = 0;
+  if (have > p.cap) low = wave_fold(low, [](uint32_t a, uint32_t b) { return min(a, b); });
+  else low = bound;
   if (lane == 0) {
-    p.ws_m[slot] = M;
-    p.ws_s[slot] = S;
+    p.ws_part[slot] = PartResult{M, S, total >= k ? low : 0};
   }
-  if (lane < k) p.ws_key[slot * k + lane] = lane < total ? list[lane] : 0;
 }
 
 // A candidate of a prompt: its total and flat index n * V + token. Larger totals first, then the lower
@@ -429,33 +444,62 @@ __device__ __forceinline__ void take_candidates(const Candidate (&c)[4], const b
   narrow<4>(v, take, need);
 }
 
-__global__ __launch_bounds__(64 * FINAL_WAVES) void select_final_kernel(SelectParams p) {
+// FW waves per prompt. Everything that does not depend on the sums is loaded first.
+template <int FW>
+__global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
   __shared__ double base[MAX_BEAMS];   // score - lse; -inf: no candidate above -inf
   __shared__ bool alone[MAX_BEAMS];    // a finished beam
-  __shared__ double c_total[2][FINAL_WAVES * MAX_NUM];
-  __shared__ uint32_t c_index[2][FINAL_WAVES * MAX_NUM];
-  __shared__ int c_count[2][FINAL_WAVES];
+  __shared__ double c_total[FINAL_LIST], d_total[4 * MAX_NUM];
+  __shared__ uint32_t c_index[FINAL_LIST], d_index[4 * MAX_NUM];
+  __shared__ double bounds[FW];
+  __shared__ int c_count, d_count;
   const int64_t prompt = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int k = p.num;
-  for (int n = wave; n < p.N; n += FINAL_WAVES) {
-    const int64_t row = prompt * p.N + n;
+  const uint32_t V = (uint32_t)p.V;
+  const uint32_t slots = (uint32_t)p.N * p.parts;  // of the prompt
+  const uint32_t all = slots * p.cap;
+  const PartResult* parts = p.ws_part + prompt * slots;
+  const uint64_t* keys = p.ws_key + prompt * slots * p.cap;
+  if (threadIdx.x == 0) c_count = d_count = 0;
+  // BATCH candidates per thread at a time, the first ones before the sums are made
+  constexpr int BATCH = 8;
+  uint64_t batch[BATCH];
+  auto load_batch = [&](uint32_t from) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const uint32_t at = from + i * 64 * FW + threadIdx.x;
+      batch[i] = at < all ? keys[at] : 0;
+    }
+  };
+  load_batch(0);
+  PartResult first_part = {};
+  if (threadIdx.x < slots) first_part = parts[threadIdx.x];
+
+  for (int n = wave; n < p.N; n += FW) {
     const bool fin = p.finished != nullptr && p.finished[prompt * p.fs[0] + n * p.fs[1]] != 0;
     const float score = p.scores[prompt * p.ss[0] + n * p.ss[1]];
     double b = score;
     if (!fin) {
+      // each lane's parts with a running maximum, then the lanes
       float m = -INFINITY;
-      for (int c = lane; c < p.parts; c += 64) m = fmaxf(m, p.ws_m[row * p.parts + c]);
-      m = group_max<64>(m);
       double s = 0.0;
       for (int c = lane; c < p.parts; c += 64) {
-        const float mc = p.ws_m[row * p.parts + c], sc = p.ws_s[row * p.parts + c];
-        s += (double)(sc * (mc == -INFINITY ? 0.0f : exp2f((mc - m) * LOG2E_F)));
+        const PartResult r = parts[n * p.parts + c];
+        const float m2 = fmaxf(m, r.m);
+        if (m2 != -INFINITY) {
+          s = s * exp2f((m - m2) * LOG2E_F) + (double)(r.s * exp2f((r.m - m2) * LOG2E_F));
+        } else {
+          s += r.s;  // 0, or a NaN
+        }
+        m = m2;
       }
+      const float M = group_max<64>(m);
+      s = M != -INFINITY && m == -INFINITY ? s : s * (M == -INFINITY ? 1.0f : exp2f((m - M) * LOG2E_F));
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-      b = (double)score - ((double)m + log(s));
+      b = (double)score - ((double)M + log(s));
     }
     if (lane == 0) {
       alone[n] = fin;
@@ -464,76 +508,156 @@ __global__ __launch_bounds__(64 * FINAL_WAVES) void select_final_kernel(SelectPa
   }
   __syncthreads();
 
-  // first level: candidates from the parts' lists, 256 per wave
-  const int per_row = p.parts * k;
-  const int all = p.N * per_row;  // <= FINAL_MAX
-  const uint32_t V = (uint32_t)p.V;
+  auto beam_of = [&](uint32_t slot) -> uint32_t {
+    return p.inv_parts != 0 ? __umulhi(slot, p.inv_parts) : slot;
+  };
+  // the largest of the parts' bounds: at least k totals reach it
+  double bound = -INFINITY;
+  for (uint32_t i = threadIdx.x; i < slots; i += 64 * FW) {
+    const uint32_t n = beam_of(i);
+    const uint32_t w = i == threadIdx.x ? first_part.bound : parts[i].bound;
+    if (!alone[n] && base[n] != -INFINITY && w != 0) bound = fmax(bound, base[n] + (double)from_order_bits(w));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) bound = fmax(bound, __shfl_xor(bound, o, 64));
+  if (lane == 0) bounds[wave] = bound;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < FW; ++w) bound = fmax(bound, bounds[w]);
+
+  // the candidate at place `at`, with its key; whether there is one that reaches the bound
+  auto candidate = [&](uint32_t at, uint64_t key, Candidate& c) -> bool {
+    if (at >= all) return false;
+    const uint32_t slot = __umulhi(at, p.inv_cap);
+    const uint32_t i = at - slot * p.cap;
+    const uint32_t n = beam_of(slot);
+    const double b = base[n];
+    c = Candidate{-INFINITY, 0};
+    if (alone[n] || b == -INFINITY) {
+      // a finished beam's own score at the pad token, then the lowest tokens at -inf
+      if (slot != n * p.parts || i >= (uint32_t)k || i >= V) return false;
+      uint32_t token = i;
+      if (alone[n]) {
+        token = i == 0 ? (uint32_t)p.pad : (i <= (uint32_t)p.pad ? i - 1 : i);
+        if (i == 0) c.total = b;
+      }
+      c.index = n * V + token;
+    } else {
+      if (key == 0) return false;
+      c.total = b + (double)from_order_bits((uint32_t)(key >> 32));
+      c.index = n * V + (0xffffffffu - (uint32_t)key);
+    }
+    return c.total >= bound;
+  };
+  auto append = [&](bool yes, const Candidate& v, double* totals, uint32_t* indexes, int& at, int room) {
+    const uint64_t b = __ballot(yes);
+    if (b == 0) return;
+    int first = 0;
+    if (lane == 0) first = atomicAdd(&at, count(b));
+    first = __builtin_amdgcn_readfirstlane(first) + below(b);
+    if (yes && first < room) {
+      totals[first] = v.total;
+      indexes[first] = v.index;
+    }
+  };
+
+  // the candidates that reach the bound, in one list
   Candidate c[4];
   bool on[4], take[4];
+  for (uint32_t from = 0; from < all; from += BATCH * 64 * FW) {
+    if (from > 0) load_batch(from);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int at = 256 * wave + 64 * e + lane;
-    c[e] = Candidate{-INFINITY, 0};
-    on[e] = false;
-    if (at < all) {
-      const int n = at / per_row;
-      const int j = at - n * per_row;
-      if (alone[n] || base[n] == -INFINITY) {
-        // a finished beam's own score at the pad token, then the lowest tokens at -inf
-        on[e] = j < k && (uint32_t)j < V;
-        uint32_t token = j;
-        if (alone[n]) {
-          token = j == 0 ? (uint32_t)p.pad : ((uint32_t)j <= (uint32_t)p.pad ? j - 1 : j);
-          if (j == 0) c[e].total = base[n];
-        }
-        c[e].index = n * V + token;
-      } else {
-        const uint64_t key = p.ws_key[(prompt * p.N + n) * per_row + j];
-        on[e] = key != 0;
-        c[e].total = base[n] + (double)from_order_bits((uint32_t)(key >> 32));
-        c[e].index = n * V + (0xffffffffu - (uint32_t)key);
-      }
+    for (int i = 0; i < BATCH; ++i) {
+      const uint32_t at = from + i * 64 * FW + threadIdx.x;
+      if (at - lane >= all) break;
+      const bool yes = candidate(at, batch[i], c[0]);
+      append(yes, c[0], c_total, c_index, c_count, FINAL_LIST);
     }
   }
-  int level = 0;
-  int waves = (all + 255) / 256;  // waves with candidates
-  while (true) {
-    if (wave < waves) {
+  __syncthreads();
+  if (c_count > FINAL_LIST) {
+    // too many (most of them equal): each wave's k best of its own, 192 new ones at a time beside the
+    // best so far (c[0]), and the waves' in the list
+    __syncthreads();
+    if (threadIdx.x == 0) c_count = 0;
+    double* own_total = &c_total[wave * MAX_NUM];
+    uint32_t* own_index = &c_index[wave * MAX_NUM];
+    c[0] = Candidate{-INFINITY, 0};
+    on[0] = false;
+    for (uint32_t slice = wave * 192; slice < all; slice += FW * 192) {
+      bool any = false;
+#pragma unroll
+      for (int e = 1; e < 4; ++e) {
+        const uint32_t at = slice + 64 * (e - 1) + lane;
+        on[e] = candidate(at, at < all ? keys[at] : 0, c[e]);
+        any = any || on[e];
+      }
+      if (__ballot(any) == 0) continue;
       take_candidates(c, on, k, take);
       int total = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t b = __ballot(take[e]);
         if (take[e]) {
-          c_total[level & 1][wave * k + total + below(b)] = c[e].total;
-          c_index[level & 1][wave * k + total + below(b)] = c[e].index;
+          own_total[total + below(b)] = c[e].total;
+          own_index[total + below(b)] = c[e].index;
         }
         total += count(b);
       }
-      if (lane == 0) c_count[level & 1][wave] = total;
+      __builtin_amdgcn_wave_barrier();
+      on[0] = lane < total;
+      if (on[0]) c[0] = Candidate{own_total[lane], own_index[lane]};
+      __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    if (waves == 1) break;
-    // next level: the waves' k places, 256 per wave
-    const int places = waves * k;
-    waves = (places + 255) / 256;
+    append(on[0], c[0], c_total, c_index, c_count, FINAL_LIST);
+    __syncthreads();
+  }
+  // the list, 256 entries per wave, to one of k entries per wave, and those to k
+  const int entries = c_count;
+  if (256 * wave < entries) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int at = 256 * wave + 64 * e + lane;
-      on[e] = at < places && at % k < c_count[level & 1][at / k];
-      c[e] = on[e] ? Candidate{c_total[level & 1][at], c_index[level & 1][at]} : Candidate{-INFINITY, 0};
+      const int i = 256 * wave + 64 * e + lane;
+      on[e] = i < entries;
+      c[e] = on[e] ? Candidate{c_total[i], c_index[i]} : Candidate{-INFINITY, 0};
     }
-    ++level;
+    take_candidates(c, on, k, take);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) append(take[e], c[e], d_total, d_index, d_count, 4 * MAX_NUM);
+  }
+  if (entries > 256) {
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 64 * e + lane;
+      on[e] = i < d_count;
+      c[e] = on[e] ? Candidate{d_total[i], d_index[i]} : Candidate{-INFINITY, 0};
+    }
+    take_candidates(c, on, k, take);
+    __builtin_amdgcn_wave_barrier();
+    int total = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint64_t b = __ballot(take[e]);
+      if (take[e]) {
+        d_total[total + below(b)] = c[e].total;
+        d_index[total + below(b)] = c[e].index;
+      }
+      total += count(b);
+    }
   }
   if (wave != 0) return;
+  __builtin_amdgcn_wave_barrier();
 
   // the k chosen ones (there are k: num <= N * V), one per lane, by rank
-  const double total = lane < k ? c_total[level & 1][lane] : -INFINITY;
-  const uint32_t index = lane < k ? c_index[level & 1][lane] : 0xffffffffu;
+  const double total = lane < k ? d_total[lane] : -INFINITY;
+  const uint32_t index = lane < k ? d_index[lane] : 0xffffffffu;
   int rank = 0;
   for (int j = 0; j < k; ++j) {
-    const double t = c_total[level & 1][j];
-    const uint32_t i = c_index[level & 1][j];
+    const double t = d_total[j];
+    const uint32_t i = d_index[j];
     rank += t > total || (t == total && i < index) ? 1 : 0;
   }
   const int beam = (int)(index / V);
@@ -567,28 +691,31 @@ __global__ __launch_bounds__(64 * FINAL_WAVES) void select_final_kernel(SelectPa
   }
 }
 
-// Parts of a row: of whole rounds of 4 runs, about 2048 workgroups in all, as far as the prompt's
-// candidates still fit the final workgroup.
-struct SelectPlan {
-  int parts, runs;
-};
+// Runs per wave of a part: 4 (64 logits per lane), or fewer where that leaves under two workgroups per CU.
+int plan_runs(int64_t rows, int64_t V) {
+  const int64_t runs = rows * ((V + RUN - 1) / RUN);
+  for (int r = 4; r > 1; r /= 2) {
+    if (runs / (WAVES * r) >= 2 * (int64_t)device_cus()) return r;
+  }
+  return 1;
+}
 
-SelectPlan plan_select(int64_t P, int64_t N, int64_t V, int num) {
-  const int64_t runs = (V + RUN - 1) / RUN;
-  const int64_t most = std::max<int64_t>(1, FINAL_MAX / (N * num));
-  const int64_t want = std::min(most, std::max<int64_t>(1, (2048 + P * N - 1) / (P * N)));
-  int64_t per = (runs + want - 1) / want;
-  per = (per + WAVES - 1) / WAVES * WAVES;
-  return SelectPlan{(int)((runs + per - 1) / per), (int)per};
+// Places for a part's candidates: room for the few beside the num largest that usually reach its bound.
+int cap_of(int num) { return num + num / 2 + 8; }
+
+int parts_of(int64_t V, int runs) { return (int)((V + RUN * WAVES * runs - 1) / (RUN * WAVES * runs)); }
+
+template <int DT, bool DENSE>
+void launch_runs(const SelectParams& p, int runs, dim3 grid, hipStream_t st) {
+  if (runs == 4) hipLaunchKernelGGL((select_part_kernel<DT, DENSE, 4>), grid, dim3(THREADS), 0, st, p);
+  else if (runs == 2) hipLaunchKernelGGL((select_part_kernel<DT, DENSE, 2>), grid, dim3(THREADS), 0, st, p);
+  else hipLaunchKernelGGL((select_part_kernel<DT, DENSE, 1>), grid, dim3(THREADS), 0, st, p);
 }
 
 template <int DT>
-void launch_part(const SelectParams& p, dim3 grid, hipStream_t st) {
-  if (p.logits.s[2] == 1) {
-    hipLaunchKernelGGL((select_part_kernel<DT, true>), grid, dim3(THREADS), 0, st, p);
-  } else {
-    hipLaunchKernelGGL((select_part_kernel<DT, false>), grid, dim3(THREADS), 0, st, p);
-  }
+void launch_part(const SelectParams& p, int runs, dim3 grid, hipStream_t st) {
+  if (p.logits.s[2] == 1) launch_runs<DT, true>(p, runs, grid, st);
+  else launch_runs<DT, false>(p, runs, grid, st);
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -600,8 +727,9 @@ using namespace lq;
 
 extern "C" size_t lq_beam_select_workspace(int64_t prompts, int64_t beams, int64_t vocab, int num) {
   if (prompts <= 0 || beams <= 0 || vocab <= 0 || num <= 0) return 0;
-  const size_t slots = (size_t)(prompts * beams) * (size_t)plan_select(prompts, beams, vocab, num).parts;
-  return 2 * align256(slots * 4) + slots * (size_t)num * 8;
+  const int64_t rows = prompts * beams;
+  const size_t slots = (size_t)rows * (size_t)parts_of(vocab, plan_runs(rows, vocab));
+  return align256(slots * sizeof(PartResult)) + slots * (size_t)cap_of(num) * 8;
 }
 
 extern "C" int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores,
@@ -682,20 +810,26 @@ extern "C" int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores,
   p.num = (int)num;
   p.slots = keep_slots;
   p.V = V;
-  const SelectPlan plan = plan_select(P, N, V, (int)num);
-  p.parts = plan.parts;
-  p.runs = plan.runs;
+  const int runs = plan_runs(P * N, V);
+  p.parts = parts_of(V, runs);
   const size_t slots = (size_t)(P * N) * (size_t)p.parts;
   char* ws = (char*)workspace;
-  p.ws_m = (float*)ws;
-  p.ws_s = (float*)(ws + align256(slots * 4));
-  p.ws_key = (uint64_t*)(ws + 2 * align256(slots * 4));
+  p.cap = cap_of((int)num);
+  p.inv_cap = (uint32_t)((((uint64_t)1 << 32) + p.cap - 1) / p.cap);
+  p.inv_parts = p.parts == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + p.parts - 1) / p.parts);
+  p.ws_part = (PartResult*)ws;
+  p.ws_key = (uint64_t*)(ws + align256(slots * sizeof(PartResult)));
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)p.parts, (unsigned)(P * N));
-  if (p.logits.dtype == LQ_BF16) launch_part<LQ_BF16>(p, grid, st);
-  else if (p.logits.dtype == LQ_F16) launch_part<LQ_F16>(p, grid, st);
-  else launch_part<LQ_F32>(p, grid, st);
+  if (p.logits.dtype == LQ_BF16) launch_part<LQ_BF16>(p, runs, grid, st);
+  else if (p.logits.dtype == LQ_F16) launch_part<LQ_F16>(p, runs, grid, st);
+  else launch_part<LQ_F32>(p, runs, grid, st);
   if ((rc = check_launch("lq_beam_select")) != LQ_OK) return rc;
-  hipLaunchKernelGGL(select_final_kernel, dim3((unsigned)P), dim3(64 * FINAL_WAVES), 0, st, p);
+  // four waves for up to three rounds of candidates, sixteen above
+  if (N * p.parts * p.cap <= 3 * 256) {
+    hipLaunchKernelGGL(select_final_kernel<4>, dim3((unsigned)P), dim3(256), 0, st, p);
+  } else {
+    hipLaunchKernelGGL(select_final_kernel<16>, dim3((unsigned)P), dim3(1024), 0, st, p);
+  }
   return check_launch("lq_beam_select (final)");
 }
