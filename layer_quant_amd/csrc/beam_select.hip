@@ -36,8 +36,9 @@ constexpr int LIST = 256;           // entries of a wave's candidate list (4 per
 constexpr int FINAL_LIST = 1024;    // entries of a prompt's candidate list
 
 struct PartResult {
-  float m, s;      // maximum and sum of e^(x - m)
-  uint32_t bound;  // order of a logit that num of them reach; 0: there are fewer
+  float m, s;      // log2e times the maximum, and the sum of 2^(x log2e - m)
+  uint32_t bound;  // order of a logit that num of the part's reach; 0: there are fewer
+  uint32_t share;  // the same for ceil(num / parts) of them, the part's share of num
 };
 
 struct SelectParams {
@@ -54,12 +55,15 @@ struct SelectParams {
   int P, N, num, slots;
   int64_t V;
   int parts, cap;       // parts of a row, places for a part's candidates
+  int share;            // ceil(num / parts)
   PartResult* ws_part;  // [rows][parts]
   uint64_t* ws_key;     // [rows][parts][cap]: order of the logit, then of the token; 0: none
   uint32_t inv_cap, inv_parts;  // ceil(2^32 / cap) and .. / parts (0 for 1), for quotients by them
 };
 
 constexpr float LOG2E_F = 1.44269504f;
+constexpr uint32_t ORDER_NONE = 0x007fffffu;  // order_bits(-inf): words below it are no numbers
+constexpr float LOWEST = -3.0e38f;  // stands for the maximum where there is no logit above -inf
 
 // An unsigned integer in the order of the floats (-0 counts as 0).
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -236,7 +240,7 @@ template <int DT, bool DENSE, int R>
 __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
   __shared__ uint64_t lists[WAVES][LIST];
   __shared__ uint32_t maxima[THREADS];
-  __shared__ uint32_t threshold;
+  __shared__ uint32_t threshold[2];  // order of a logit that num (the share of num) of the part's reach
   __shared__ int counts[WAVES];
   __shared__ float wave_m[WAVES], wave_s[WAVES];
   constexpr int VN = Raw<DT>::N;
@@ -294,24 +298,29 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
     }
   }
 
-  float mx = -INFINITY, run_max[R];
+  // the lane's maximum and sum, S = sum 2^(x log2e - c) with c = log2e times the maximum so far. The
+  // product is exact inside the multiply-add, so that the terms near the maximum are off by the
+  // exponential alone; log2e's own rounding drops out when the logarithm is divided by it again, but for
+  // 1e-8 times the entropy.
+  float mx = -INFINITY, run_max[R], c = LOWEST, sl = 0.0f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     run_max[r] = x[r][0];
 #pragma unroll
     for (int i = 1; i < PER; ++i) run_max[r] = fmaxf(run_max[r], x[r][i]);
     mx = fmaxf(mx, run_max[r]);
+    const float c2 = fmaxf(c, run_max[r] * LOG2E_F);
+    if (r > 0) sl *= __builtin_amdgcn_exp2f(c - c2);
+    c = c2;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sl += __builtin_amdgcn_exp2f(fmaf(x[r][i], LOG2E_F, -c));
+    // the logits stay as they were loaded: unpacked for the second pass too, they took twice the registers
+#pragma unroll
+    for (int u = 0; u < Raw<DT>::WORDS; ++u) asm volatile("" : "+v"(x[r].w[u]));
   }
   maxima[threadIdx.x] = token(start_of(0), 0) < V ? order_bits(mx) : 0;  // 0: a lane without a token
-  const float m0 = mx == -INFINITY ? 0.0f : mx;
-  float sl = 0.0f;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sl += __builtin_amdgcn_exp2f((x[r][i] - m0) * LOG2E_F);
-  }
-  const float wm = group_max<64>(mx);
-  const float ws = group_sum<64>(sl * (mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx - wm) * LOG2E_F)));
+  const float wm = group_max<64>(c);
+  const float ws = group_sum<64>(sl * __builtin_amdgcn_exp2f(c - wm));
   if (lane == 0) {
     wave_m[wave] = wm;
     wave_s[wave] = ws;
@@ -319,16 +328,26 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
   __syncthreads();
 
   // the threshold: only keys above bar are taken, whose logits reach barf
-  if (wave == 0) {
+  if (wave < 2) {
     uint32_t v[WAVES];
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) v[w] = maxima[64 * w + lane];
+    const int need = wave == 0 ? k : p.share;
+    const int have = count_from<WAVES>(v, 1);
     bool exact;
-    const uint32_t w = count_from<WAVES>(v, 1) > k ? kth_word<WAVES>(v, k, exact) : 0;
-    if (lane == 0) threshold = w;
+    uint32_t w = 0;
+    if (have > need) {
+      w = kth_word<WAVES>(v, need, exact);
+    } else if (have == need) {
+      uint32_t low = ~0u;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) low = v[i] != 0 ? min(low, v[i]) : low;
+      w = wave_fold(low, [](uint32_t a, uint32_t b) { return min(a, b); });
+    }
+    if (lane == 0) threshold[wave] = w;
   }
   __syncthreads();
-  const uint32_t bound = __builtin_amdgcn_readfirstlane(threshold);
+  const uint32_t bound = __builtin_amdgcn_readfirstlane(threshold[0]);
   uint64_t bar = 0;
   float barf = -INFINITY;
   if (bound != 0) {
@@ -336,32 +355,55 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
     barf = from_order_bits(bound);
   }
   int n = 0;  // entries of the wave's list
+  if (bound != 0) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (__ballot(run_max[r] >= barf) == 0) continue;
-    // the lane's logits that reach the threshold, taken one per lane at a time
-    uint32_t hits = 0;
+    for (int r = 0; r < R; ++r) {
+      if (__ballot(run_max[r] >= barf) == 0) continue;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) hits |= x[r][i] >= barf ? 1u << i : 0u;
-    while (__ballot(hits != 0) != 0) {
-      const bool more = hits != 0;
-      const int i = more ? __builtin_ctz(hits) : 0;
-      hits &= hits - 1;  // (0 stays 0)
-      uint32_t w = x[r].w[0];
-#pragma unroll
-      for (int u = 1; u < Raw<DT>::WORDS; ++u) w = i * Raw<DT>::SIZE / 4 == u ? x[r].w[u] : w;
-      const float xi = DT == LQ_F32 ? __uint_as_float(w) : word_elem(w, 16 * (i & 1), DT);
-      const uint32_t t = token(start_of(r), i);
-      const uint64_t key = make_key(xi, t);
-      bool ok = more && xi >= barf && t < V && key > bar;
-      uint64_t b = __ballot(ok);
-      if (n + count(b) > LIST) {
-        cut_list(list, n, k, bar, barf);
-        ok = ok && key > bar;
-        b = __ballot(ok);
+      for (int i = 0; i < PER; ++i) {
+        const uint64_t b = __ballot(x[r][i] >= barf);
+        if (b == 0) continue;
+        const int at = n + below(b);
+        if (x[r][i] >= barf && at < LIST) list[at] = make_key(x[r][i], token(start_of(r), i));
+        n += count(b);
       }
-      if (ok) list[n + below(b)] = key;
-      n += count(b);
+    }
+  }
+  // no threshold, more logits at it than the list holds, or the row's end among them (its places past
+  // the last token are -inf): once more, the list cut where it is full
+  if (bound == 0 || n > LIST || barf == -INFINITY) {
+    n = 0;
+    for (int r = 0; r < R; ++r) {
+      Raw<DT> y = x[0];
+#pragma unroll
+      for (int q = 1; q < R; ++q) {
+#pragma unroll
+        for (int u = 0; u < Raw<DT>::WORDS; ++u) y.w[u] = q == r ? x[q].w[u] : y.w[u];
+      }
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) hits |= y[i] >= barf ? 1u << i : 0u;
+      // one per lane at a time
+      while (__ballot(hits != 0) != 0) {
+        const bool more = hits != 0;
+        const int i = more ? __builtin_ctz(hits) : 0;
+        hits &= hits - 1;  // (0 stays 0)
+        uint32_t w = y.w[0];
+#pragma unroll
+        for (int u = 1; u < Raw<DT>::WORDS; ++u) w = i * Raw<DT>::SIZE / 4 == u ? y.w[u] : w;
+        const float xi = DT == LQ_F32 ? __uint_as_float(w) : word_elem(w, 16 * (i & 1), DT);
+        const uint32_t t = token(start_of(r), i);
+        const uint64_t key = make_key(xi, t);
+        bool ok = more && xi >= barf && t < V && key > bar;
+        uint64_t b = __ballot(ok);
+        if (n + count(b) > LIST) {
+          cut_list(list, n, k, bar, barf);
+          ok = ok && key > bar;
+          b = __ballot(ok);
+        }
+        if (ok) list[n + below(b)] = key;
+        n += count(b);
+      }
     }
   }
   __builtin_amdgcn_wave_barrier();
@@ -376,7 +418,7 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
   for (int w = 1; w < WAVES; ++w) M = fmaxf(M, wave_m[w]);
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
-    S += wave_s[w] * (wave_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((wave_m[w] - M) * LOG2E_F));
+    S += wave_s[w] * __builtin_amdgcn_exp2f(wave_m[w] - M);
   }
   // the part's candidates: the lists as they are where they fit (num of them reach the bound, the final
   // workgroup looks at the others' totals anyway), else the num largest
@@ -405,7 +447,7 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
   if (have > p.cap) low = wave_fold(low, [](uint32_t a, uint32_t b) { return min(a, b); });
   else low = bound;
   if (lane == 0) {
-    p.ws_part[slot] = PartResult{M, S, total >= k ? low : 0};
+    p.ws_part[slot] = PartResult{M, S, total >= k ? low : 0, threshold[1]};
   }
 }
 
@@ -451,8 +493,12 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
   __shared__ bool alone[MAX_BEAMS];    // a finished beam
   __shared__ double c_total[FINAL_LIST], d_total[4 * MAX_NUM];
   __shared__ uint32_t c_index[FINAL_LIST], d_index[4 * MAX_NUM];
-  __shared__ double bounds[FW];
-  __shared__ int c_count, d_count;
+  __shared__ uint32_t bound_bits;
+  __shared__ uint32_t shares[MAX_BEAMS], least[MAX_BEAMS];
+  __shared__ int c_count, d_count, has_apart;
+  __shared__ int ranks[256], first_of[MAX_BEAMS];
+  __shared__ double r_total[MAX_NUM];
+  __shared__ uint32_t r_index[MAX_NUM];
   const int64_t prompt = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -462,7 +508,12 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
   const uint32_t all = slots * p.cap;
   const PartResult* parts = p.ws_part + prompt * slots;
   const uint64_t* keys = p.ws_key + prompt * slots * p.cap;
-  if (threadIdx.x == 0) c_count = d_count = 0;
+  if (threadIdx.x == 0) {
+    c_count = d_count = has_apart = 0;
+    bound_bits = 0;
+  }
+  if (threadIdx.x < 256) ranks[threadIdx.x] = 0;
+  if (threadIdx.x < MAX_BEAMS) first_of[threadIdx.x] = MAX_NUM;
   // BATCH candidates per thread at a time, the first ones before the sums are made
   constexpr int BATCH = 8;
   uint64_t batch[BATCH];
@@ -483,23 +534,20 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
     double b = score;
     if (!fin) {
       // each lane's parts with a running maximum, then the lanes
-      float m = -INFINITY;
-      double s = 0.0;
-      for (int c = lane; c < p.parts; c += 64) {
-        const PartResult r = parts[n * p.parts + c];
+      float m = LOWEST, s = 0.0f;
+      uint32_t share = ~0u;
+      for (int i = lane; i < p.parts; i += 64) {
+        const PartResult r = parts[n * p.parts + i];
+        share = min(share, r.share);
         const float m2 = fmaxf(m, r.m);
-        if (m2 != -INFINITY) {
-          s = s * exp2f((m - m2) * LOG2E_F) + (double)(r.s * exp2f((r.m - m2) * LOG2E_F));
-        } else {
-          s += r.s;  // 0, or a NaN
-        }
+        s = s * exp2f(m - m2) + r.s * exp2f(r.m - m2);
         m = m2;
       }
       const float M = group_max<64>(m);
-      s = M != -INFINITY && m == -INFINITY ? s : s * (M == -INFINITY ? 1.0f : exp2f((m - M) * LOG2E_F));
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-      b = (double)score - ((double)M + log(s));
+      s = group_sum<64>(s * exp2f(m - M));
+      share = wave_fold(share, [](uint32_t a, uint32_t b) { return min(a, b); });
+      if (lane == 0) shares[n] = share;
+      b = (double)score - ((double)M + log2((double)s)) / (double)LOG2E_F;
     }
     if (lane == 0) {
       alone[n] = fin;
@@ -511,43 +559,65 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
   auto beam_of = [&](uint32_t slot) -> uint32_t {
     return p.inv_parts != 0 ? __umulhi(slot, p.inv_parts) : slot;
   };
-  // the largest of the parts' bounds: at least k totals reach it
-  double bound = -INFINITY;
+  // At least k totals reach the largest of the parts' bounds, and the largest over the beams of the
+  // smallest of its parts' share bounds (as the order of an fp32 number, a step below the rounded total).
+  uint32_t most = 0;
   for (uint32_t i = threadIdx.x; i < slots; i += 64 * FW) {
     const uint32_t n = beam_of(i);
-    const uint32_t w = i == threadIdx.x ? first_part.bound : parts[i].bound;
-    if (!alone[n] && base[n] != -INFINITY && w != 0) bound = fmax(bound, base[n] + (double)from_order_bits(w));
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) bound = fmax(bound, __shfl_xor(bound, o, 64));
-  if (lane == 0) bounds[wave] = bound;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < FW; ++w) bound = fmax(bound, bounds[w]);
-
-  // the candidate at place `at`, with its key; whether there is one that reaches the bound
-  auto candidate = [&](uint32_t at, uint64_t key, Candidate& c) -> bool {
-    if (at >= all) return false;
-    const uint32_t slot = __umulhi(at, p.inv_cap);
-    const uint32_t i = at - slot * p.cap;
-    const uint32_t n = beam_of(slot);
-    const double b = base[n];
-    c = Candidate{-INFINITY, 0};
-    if (alone[n] || b == -INFINITY) {
-      // a finished beam's own score at the pad token, then the lowest tokens at -inf
-      if (slot != n * p.parts || i >= (uint32_t)k || i >= V) return false;
-      uint32_t token = i;
-      if (alone[n]) {
-        token = i == 0 ? (uint32_t)p.pad : (i <= (uint32_t)p.pad ? i - 1 : i);
-        if (i == 0) c.total = b;
-      }
-      c.index = n * V + token;
-    } else {
-      if (key == 0) return false;
-      c.total = b + (double)from_order_bits((uint32_t)(key >> 32));
-      c.index = n * V + (0xffffffffu - (uint32_t)key);
+    uint32_t w = i == threadIdx.x ? first_part.bound : parts[i].bound;
+    if (i == n * p.parts) w = max(w, shares[n]);
+    if (!alone[n] && base[n] != -INFINITY && w != 0) {
+      const uint32_t o = order_bits((float)(base[n] + (double)from_order_bits(w)));
+      most = max(most, o > ORDER_NONE ? o - 1 : o);
     }
+  }
+  most = wave_fold(most, [](uint32_t a, uint32_t b) { return max(a, b); });
+  if (lane == 0) atomicMax(&bound_bits, most);
+  __syncthreads();
+  const double bound = bound_bits == 0 ? -INFINITY : (double)from_order_bits(bound_bits);
+  // the order of a logit below those of beam n that reach it (the difference rounded to fp32, two steps
+  // down)
+  for (int n = threadIdx.x; n < p.N; n += 64 * FW) {
+    const bool apart = alone[n] || base[n] == -INFINITY;
+    const uint32_t w = order_bits((float)(bound - base[n]));
+    least[n] = apart ? ~0u : bound == -INFINITY || w <= 2 ? 1u : w - 2;
+    if (apart) has_apart = 1;
+  }
+  __syncthreads();
+
+  auto place = [&](uint32_t at, uint32_t& n, uint32_t& i) -> bool {  // place i of beam n's first part
+    const uint32_t slot = __umulhi(at, p.inv_cap);
+    n = beam_of(slot);
+    i = at - slot * p.cap;
+    return slot == n * p.parts;
+  };
+  // the candidate with its key; whether it reaches the bound
+  auto candidate = [&](uint32_t n, uint64_t key, Candidate& c) -> bool {
+    c.total = base[n] + (double)from_order_bits((uint32_t)(key >> 32));
+    c.index = n * V + (0xffffffffu - (uint32_t)key);
     return c.total >= bound;
+  };
+  // the i-th candidate of a beam without logits: a finished beam's own score at the pad token, then the
+  // lowest tokens at -inf
+  auto apart_candidate = [&](uint32_t n, uint32_t i, Candidate& c) -> bool {
+    if (i >= (uint32_t)k || i >= V) return false;
+    uint32_t token = i;
+    c.total = -INFINITY;
+    if (alone[n]) {
+      token = i == 0 ? (uint32_t)p.pad : (i <= (uint32_t)p.pad ? i - 1 : i);
+      if (i == 0) c.total = base[n];
+    }
+    c.index = n * V + token;
+    return c.total >= bound;
+  };
+  auto any_candidate = [&](uint32_t at, Candidate& c) -> bool {
+    uint32_t n, i;
+    c = Candidate{-INFINITY, 0};
+    if (at >= all) return false;
+    const bool lead = place(at, n, i);
+    if (least[n] == ~0u) return lead && apart_candidate(n, i, c);
+    const uint64_t key = keys[at];
+    return (uint32_t)(key >> 32) >= least[n] && candidate(n, key, c);
   };
   auto append = [&](bool yes, const Candidate& v, double* totals, uint32_t* indexes, int& at, int room) {
     const uint64_t b = __ballot(yes);
@@ -570,7 +640,16 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
     for (int i = 0; i < BATCH; ++i) {
       const uint32_t at = from + i * 64 * FW + threadIdx.x;
       if (at - lane >= all) break;
-      const bool yes = candidate(at, batch[i], c[0]);
+      const uint32_t n = beam_of(__umulhi(min(at, all - 1), p.inv_cap));
+      const bool maybe = (uint32_t)(batch[i] >> 32) >= least[n];  // (0 past the end and where there is none)
+      if (__ballot(maybe) == 0) continue;
+      append(maybe && candidate(n, batch[i], c[0]), c[0], c_total, c_index, c_count, FINAL_LIST);
+    }
+  }
+  if (has_apart) {
+    for (uint32_t at = threadIdx.x; at - lane < (uint32_t)(p.N * k); at += 64 * FW) {
+      const uint32_t n = at / (uint32_t)k;
+      const bool yes = at < (uint32_t)(p.N * k) && least[n] == ~0u && apart_candidate(n, at - n * k, c[0]);
       append(yes, c[0], c_total, c_index, c_count, FINAL_LIST);
     }
   }
@@ -589,7 +668,7 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
 #pragma unroll
       for (int e = 1; e < 4; ++e) {
         const uint32_t at = slice + 64 * (e - 1) + lane;
-        on[e] = candidate(at, at < all ? keys[at] : 0, c[e]);
+        on[e] = any_candidate(at, c[e]);
         any = any || on[e];
       }
       if (__ballot(any) == 0) continue;
@@ -613,79 +692,70 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
     append(on[0], c[0], c_total, c_index, c_count, FINAL_LIST);
     __syncthreads();
   }
-  // the list, 256 entries per wave, to one of k entries per wave, and those to k
-  const int entries = c_count;
-  if (256 * wave < entries) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = 256 * wave + 64 * e + lane;
-      on[e] = i < entries;
-      c[e] = on[e] ? Candidate{c_total[i], c_index[i]} : Candidate{-INFINITY, 0};
-    }
-    take_candidates(c, on, k, take);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) append(take[e], c[e], d_total, d_index, d_count, 4 * MAX_NUM);
-  }
+  // more than 256 entries are reduced, 256 per wave, to a list of k entries per wave
+  int entries = c_count;
+  const double* totals = c_total;
+  const uint32_t* indexes = c_index;
   if (entries > 256) {
-    __syncthreads();
-    if (wave != 0) return;
+    if (256 * wave < entries) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = 64 * e + lane;
-      on[e] = i < d_count;
-      c[e] = on[e] ? Candidate{d_total[i], d_index[i]} : Candidate{-INFINITY, 0};
-    }
-    take_candidates(c, on, k, take);
-    __builtin_amdgcn_wave_barrier();
-    int total = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint64_t b = __ballot(take[e]);
-      if (take[e]) {
-        d_total[total + below(b)] = c[e].total;
-        d_index[total + below(b)] = c[e].index;
+      for (int e = 0; e < 4; ++e) {
+        const int i = 256 * wave + 64 * e + lane;
+        on[e] = i < entries;
+        c[e] = on[e] ? Candidate{c_total[i], c_index[i]} : Candidate{-INFINITY, 0};
       }
-      total += count(b);
+      take_candidates(c, on, k, take);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) append(take[e], c[e], d_total, d_index, d_count, 4 * MAX_NUM);
+    }
+    __syncthreads();
+    entries = d_count;
+    totals = d_total;
+    indexes = d_index;
+  }
+  // their ranks: thread t counts for entry t % 256 the better ones of a stretch
+  {
+    const int i = threadIdx.x & 255;
+    const int stretch = (entries + FW / 4 - 1) / (FW / 4);
+    const int j0 = (threadIdx.x >> 8) * stretch, j1 = min(entries, j0 + stretch);
+    const double total = i < entries ? totals[i] : -INFINITY;
+    const uint32_t index = i < entries ? indexes[i] : 0xffffffffu;
+    int better = 0;
+    if ((i & ~63) < entries) {  // (uniform per wave)
+#pragma unroll 4
+      for (int j = j0; j < j1; ++j) {
+        const double t = totals[j];
+        better += t > total || (t == total && indexes[j] < index) ? 1 : 0;
+      }
+      if (i < entries) atomicAdd(&ranks[i], better);
     }
   }
-  if (wave != 0) return;
-  __builtin_amdgcn_wave_barrier();
-
-  // the k chosen ones (there are k: num <= N * V), one per lane, by rank
-  const double total = lane < k ? d_total[lane] : -INFINITY;
-  const uint32_t index = lane < k ? d_index[lane] : 0xffffffffu;
-  int rank = 0;
-  for (int j = 0; j < k; ++j) {
-    const double t = d_total[j];
-    const uint32_t i = d_index[j];
-    rank += t > total || (t == total && i < index) ? 1 : 0;
+  __syncthreads();
+  if (threadIdx.x < entries && ranks[threadIdx.x] < k) {
+    const int r = ranks[threadIdx.x];
+    r_total[r] = totals[threadIdx.x];
+    r_index[r] = indexes[threadIdx.x];
   }
+  __syncthreads();
+  if (wave != 0) return;
+
+  // the k chosen ones in order, one per lane (num <= N * V: there are k)
+  const bool chosen = lane < k;
+  const uint32_t index = chosen ? r_index[lane] : 0;
   const int beam = (int)(index / V);
-  int at = rank;
+  int at = lane;
   if (p.slots) {
     // a beam's best continuation keeps the beam's place, the others take the free places in order
-    uint64_t used = 0;
-    bool best = lane < k;
-    for (int j = 0; j < k; ++j) {
-      const int b = __builtin_amdgcn_readlane(beam, j);
-      const int r = __builtin_amdgcn_readlane(rank, j);
-      used |= (uint64_t)1 << b;
-      best = best && !(b == beam && r < rank);
-    }
-    int before = 0;  // other continuations of a better rank that have no place of their own
-    const uint64_t bests = __ballot(best);
-    for (int j = 0; j < k; ++j) {
-      const int r = __builtin_amdgcn_readlane(rank, j);
-      before += (bests >> j & 1) == 0 && r < rank ? 1 : 0;
-    }
-    uint64_t free = ~used;
-    if (!best) {
-      for (int j = 0; j < before; ++j) free &= free - 1;
-    }
-    at = best ? beam : __builtin_ctzll(free);
+    if (chosen) atomicMin(&first_of[beam], lane);
+    __builtin_amdgcn_wave_barrier();
+    const bool best = chosen && first_of[beam] == lane;
+    uint64_t free = __ballot(lane < p.N && first_of[lane] == MAX_NUM);
+    const int before = below(__ballot(chosen && !best));
+    for (int j = 0; j < before; ++j) free &= free - 1;
+    at = best ? beam : __builtin_ctzll(free | (uint64_t)1 << 63);
   }
-  if (lane < k) {
-    p.out_score[prompt * p.os[0][0] + at * p.os[0][1]] = (float)total;
+  if (chosen) {
+    p.out_score[prompt * p.os[0][0] + at * p.os[0][1]] = (float)r_total[lane];
     p.out_beam[prompt * p.os[1][0] + at * p.os[1][1]] = beam;
     p.out_token[prompt * p.os[2][0] + at * p.os[2][1]] = index - (uint32_t)beam * V;
   }
@@ -815,6 +885,7 @@ extern "C" int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores,
   const size_t slots = (size_t)(P * N) * (size_t)p.parts;
   char* ws = (char*)workspace;
   p.cap = cap_of((int)num);
+  p.share = (int)((num + p.parts - 1) / p.parts);
   p.inv_cap = (uint32_t)((((uint64_t)1 << 32) + p.cap - 1) / p.cap);
   p.inv_parts = p.parts == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + p.parts - 1) / p.parts);
   p.ws_part = (PartResult*)ws;
