@@ -2,8 +2,8 @@
 // of row p*N + beams[p][n].
 //
 // One launch moves any number of tensors (the INT4 caches' live rows, MX or float states, convolution
-// states of all layers). A thread owns one unit (up to 16 bytes) of a row's contents, at the same place
-// in all N rows of a prompt: it loads that unit of every row's source first and stores afterwards, so
+// states of all layers). A thread owns a few units (up to 16 bytes) of a row's contents, at the same places
+// in all N rows of a prompt: it loads those of every row's source first and stores afterwards, so
 // that a row may be the source of some rows and the destination of another, in any permutation, with
 // no second buffer and no order between threads. Rows that keep their beam are neither read nor
 // written.
@@ -46,52 +46,80 @@ struct ReorderParams {
 };
 static_assert(sizeof(ReorderParams) <= 4096, "a launch's arguments");
 
-template <class T, int NMAX>
-__device__ __forceinline__ void move_unit(char* at, int64_t sb, const int (&src)[NMAX]) {
-  T v[NMAX];
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// Units per thread: as many as keep the loaded units of all NMAX rows within 64 to 128 registers.
+constexpr int units_per_thread(int nmax) { return nmax <= 8 ? 4 : nmax <= 16 ? 2 : 1; }
+
+// Unit `first` + i THREADS of the row for i < U, of all rows: the sources' first, then the stores. (The
+// values are vector types: an array of uint4 structs stays in scratch memory here.)
+template <class T, int NMAX, int U>
+__device__ __forceinline__ void move_units(const RowShape& sh, char* base, uint32_t first,
+                                           const int (&src)[NMAX]) {
+  char* at[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t u = min(first + i * THREADS, sh.total - 1);
+    if (sh.units == sh.total) {
+      at[i] = base + (uint64_t)u * sizeof(T);
+    } else {
+      const uint32_t run = u / sh.units;
+      const uint32_t i1 = run / sh.n2;
+      const uint32_t i0 = i1 / sh.n1;
+      at[i] = base + i0 * sh.s0 + (i1 - i0 * sh.n1) * sh.s1 + (run - i1 * sh.n2) * sh.s2 +
+              (uint64_t)(u - run * sh.units) * sizeof(T);
+    }
+  }
+  T v[NMAX][U];
 #pragma unroll
   for (int n = 0; n < NMAX; ++n) {
-    if (src[n] != n) v[n] = *(const T*)(at + src[n] * sb);
+    if (src[n] != n) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[n][i] = *(const T*)(at[i] + src[n] * sh.sb);
+    }
   }
 #pragma unroll
   for (int n = 0; n < NMAX; ++n) {
-    if (src[n] != n) *(T*)(at + n * sb) = v[n];
+    if (src[n] != n) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (first + i * THREADS < sh.total) *(T*)(at[i] + n * sh.sb) = v[n][i];
+      }
+    }
   }
 }
 
 template <int NMAX>
 __global__ __launch_bounds__(THREADS) void reorder_kernel(ReorderParams p) {
+  constexpr int U = units_per_thread(NMAX);
   int si = 0;
   while (si + 1 < p.nshapes && blockIdx.x >= p.shapes[si + 1].first_block) ++si;
   const RowShape& sh = p.shapes[si];
   const uint32_t rel = blockIdx.x - sh.first_block;
   const uint32_t tp = rel / sh.blocks;
-  const uint32_t u = (rel - tp * sh.blocks) * THREADS + threadIdx.x;
+  const uint32_t first = (rel - tp * sh.blocks) * (THREADS * U) + threadIdx.x;
   const uint32_t tensor = tp / p.P;
   const int64_t prompt = tp - tensor * p.P;
 
+  int64_t beam[NMAX];
+#pragma unroll
+  for (int n = 0; n < NMAX; ++n) {
+    beam[n] = p.beams[prompt * p.beams_sp + min(n, p.N - 1) * p.beams_sn];
+  }
   int src[NMAX];
 #pragma unroll
   for (int n = 0; n < NMAX; ++n) {
-    src[n] = n;
-    if (n < p.N) {
-      const int64_t b = p.beams[prompt * p.beams_sp + n * p.beams_sn];
-      if (b >= 0 && b < p.N) src[n] = (int)b;
-    }
+    src[n] = n < p.N && beam[n] >= 0 && beam[n] < p.N ? (int)beam[n] : n;
   }
-  if (u >= sh.total) return;
-  const uint32_t run = u / sh.units;
-  const uint32_t i1 = run / sh.n2;
-  const uint32_t i0 = i1 / sh.n1;
-  char* at = p.base[sh.first_tensor + tensor] + prompt * p.N * sh.sb + i0 * sh.s0 +
-             (i1 - i0 * sh.n1) * sh.s1 + (run - i1 * sh.n2) * sh.s2 +
-             ((int64_t)(u - run * sh.units) << sh.unit_log2);
+  if (first >= sh.total) return;
+  char* base = p.base[sh.first_tensor + tensor] + prompt * p.N * sh.sb;
   switch (sh.unit_log2) {
-    case 4: move_unit<uint4, NMAX>(at, sh.sb, src); break;
-    case 3: move_unit<uint2, NMAX>(at, sh.sb, src); break;
-    case 2: move_unit<uint32_t, NMAX>(at, sh.sb, src); break;
-    case 1: move_unit<uint16_t, NMAX>(at, sh.sb, src); break;
-    default: move_unit<uint8_t, NMAX>(at, sh.sb, src); break;
+    case 4: move_units<u32x4_t, NMAX, U>(sh, base, first, src); break;
+    case 3: move_units<u32x2_t, NMAX, U>(sh, base, first, src); break;
+    case 2: move_units<uint32_t, NMAX, U>(sh, base, first, src); break;
+    case 1: move_units<uint16_t, NMAX, U>(sh, base, first, src); break;
+    default: move_units<uint8_t, NMAX, U>(sh, base, first, src); break;
   }
 }
 
@@ -102,7 +130,7 @@ struct Item {
 };
 
 // The row geometry of t over its first `rows` entries of dim 2 (-1: all); total 0 when it is empty.
-int row_shape(const lq_tensor& t, int64_t rows, Item& item) {
+int row_shape(const lq_tensor& t, int64_t rows, int64_t per_block, Item& item) {
   const int64_t es = dtype_size(t.dtype);
   int64_t n[3] = {1, 1, 1}, s[3] = {0, 0, 0};  // dims 1 .. 3, in bytes
   for (int d = 1; d < t.ndim; ++d) {
@@ -146,17 +174,17 @@ int row_shape(const lq_tensor& t, int64_t rows, Item& item) {
   r.s2 = os[0];
   r.units = (uint32_t)units;
   r.total = (uint32_t)total;
-  r.blocks = (uint32_t)((total + THREADS - 1) / THREADS);
+  r.blocks = (uint32_t)((total + per_block - 1) / per_block);
   item.shape = r;
   return LQ_OK;
 }
 
-int launch(const ReorderParams& p, int64_t blocks, hipStream_t st) {
+int launch(const ReorderParams& p, int nmax, int64_t blocks, hipStream_t st) {
   const dim3 grid((unsigned)blocks), block(THREADS);
-  if (p.N <= 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, block, 0, st, p);
-  else if (p.N <= 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, block, 0, st, p);
-  else if (p.N <= 16) hipLaunchKernelGGL(reorder_kernel<16>, grid, block, 0, st, p);
-  else if (p.N <= 32) hipLaunchKernelGGL(reorder_kernel<32>, grid, block, 0, st, p);
+  if (nmax == 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, block, 0, st, p);
+  else if (nmax == 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, block, 0, st, p);
+  else if (nmax == 16) hipLaunchKernelGGL(reorder_kernel<16>, grid, block, 0, st, p);
+  else if (nmax == 32) hipLaunchKernelGGL(reorder_kernel<32>, grid, block, 0, st, p);
   else hipLaunchKernelGGL(reorder_kernel<64>, grid, block, 0, st, p);
   return check_launch("lq_reorder_beams");
 }
@@ -182,6 +210,8 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
     return fail(LQ_ERR_UNSUPPORTED, "%d tensors in one call unsupported (<= %d)", count,
                 LQ_REORDER_MAX_TENSORS);
   }
+  const int nmax = N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64;
+  const int64_t per_block = (int64_t)THREADS * units_per_thread(nmax);
   Item items[LQ_REORDER_MAX_TENSORS];
   int used = 0;
   for (int i = 0; i < count; ++i) {
@@ -209,7 +239,7 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
       }
     }
     Item it{};
-    if ((rc = row_shape(t, live, it)) != LQ_OK) return rc;
+    if ((rc = row_shape(t, live, per_block, it)) != LQ_OK) return rc;
     if (it.shape.total == 0) continue;
     items[used++] = it;
   }
@@ -253,7 +283,7 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
     if (blocks == 0) {
       return fail(LQ_ERR_UNSUPPORTED, "%lld prompts exceed the launch limits", (long long)P);
     }
-    if ((rc = launch(p, blocks, st)) != LQ_OK) return rc;
+    if ((rc = launch(p, nmax, blocks, st)) != LQ_OK) return rc;
   }
   return LQ_OK;
 }
