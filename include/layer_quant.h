@@ -328,7 +328,7 @@ int lq_int4_shared_decode_attention(
  * are not read. Continuations of a beam whose score or log-sum-exp is not finite (a NaN or +inf
  * logit, no logit above -inf) count as -inf, and so do the other tokens of a finished beam. (Logits
  * beyond 2^127 in magnitude count as infinite.)
- *   logits    [P, N, V]  f32/f16/bf16, any strides
+ *   logits    [P, N, V] or [P * N, V]  f32/f16/bf16, any strides
  *   scores    [P, N]     f32
  *   finished  NULL or [P, N] u8 (0: not finished)
  *   out_scores [P, num] f32 (the totals), out_beams [P, num] i64 (n), out_tokens [P, num] i64 (t)

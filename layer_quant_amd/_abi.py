@@ -463,14 +463,17 @@ class _Scratch:
         self._lock = threading.Lock()
 
     def get(self, index: int, stream: int, nbytes: int) -> torch.Tensor:
-        device = torch.device("cuda", index)
         if torch.cuda.is_current_stream_capturing():
-            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+            return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
         key = (index, stream)
+        buf = self._bufs.get(key)
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
         with self._lock:
             buf = self._bufs.get(key)
             if buf is None or buf.numel() < nbytes:
-                buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+                buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8,
+                                  device=torch.device("cuda", index))
                 self._bufs[key] = buf
             return buf
 
@@ -714,7 +717,7 @@ def int4_shared_decode_attention(q: torch.Tensor, k_new: torch.Tensor | None,
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None,
                 out_scores: torch.Tensor, out_beams: torch.Tensor, out_tokens: torch.Tensor,
                 pad_token: int, keep_slots: bool) -> None:
-    """The best continuations of logits [P, N, V] and scores [P, N] (finished: uint8 [P, N] or None)
+    """The best continuations of logits [P, N, V] or [P*N, V] and scores [P, N] (finished: uint8 [P, N] or None)
     into the outputs [P, num]."""
     host = _host or host_binding()
     if host:
@@ -724,7 +727,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
             return check(rc, "lq_beam_select")
     dev = _require_gpu(logits, scores, finished, out_scores, out_beams, out_tokens)
     stream = _stream(dev)
-    need = int(lib().lq_beam_select_workspace(*logits.shape, out_scores.shape[1]))
+    need = int(lib().lq_beam_select_workspace(*scores.shape, logits.shape[-1], out_scores.shape[1]))
     ws = _scratch.get(dev.index, stream, need) if need else None
     rc = lib().lq_beam_select(desc(logits), desc(scores), desc(finished), desc(out_scores),
                               desc(out_beams), desc(out_tokens), int(pad_token),

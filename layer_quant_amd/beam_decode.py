@@ -44,7 +44,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: int | None = No
     if logits.dim() == 2:
         if logits.shape[0] != prompts * beams:
             raise ValueError(f"Expected logits of {prompts} x {beams} rows, got {logits.shape[0]}")
-        logits = logits.unflatten(0, (prompts, beams))
     elif logits.dim() != 3 or logits.shape[:2] != scores.shape:
         raise ValueError(f"Expected logits [{prompts}, {beams}, vocab], got {tuple(logits.shape)}")
     if finished is not None:

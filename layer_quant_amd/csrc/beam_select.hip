@@ -808,7 +808,8 @@ extern "C" int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores,
                               int64_t pad_token, int keep_slots, void* workspace,
                               size_t workspace_bytes, void* stream) {
   int rc;
-  if ((rc = check_tensor(logits, "logits", 3, true)) != LQ_OK) return rc;
+  const int ldim = logits != nullptr && logits->ndim == 2 ? 2 : 3;
+  if ((rc = check_tensor(logits, "logits", ldim, true)) != LQ_OK) return rc;
   if ((rc = check_tensor(scores, "scores", 2, false, LQ_F32)) != LQ_OK) return rc;
   if (finished != nullptr && (rc = check_tensor(finished, "finished", 2, false, LQ_U8)) != LQ_OK) {
     return rc;
@@ -816,8 +817,12 @@ extern "C" int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores,
   if ((rc = check_tensor(out_scores, "out_scores", 2, false, LQ_F32)) != LQ_OK) return rc;
   if ((rc = check_tensor(out_beams, "out_beams", 2, false, LQ_I64)) != LQ_OK) return rc;
   if ((rc = check_tensor(out_tokens, "out_tokens", 2, false, LQ_I64)) != LQ_OK) return rc;
-  const int64_t P = logits->shape[0], N = logits->shape[1], V = logits->shape[2];
+  const int64_t P = scores->shape[0], N = scores->shape[1], V = logits->shape[ldim - 1];
   const int64_t num = out_scores->shape[1];
+  if (ldim == 2 ? logits->shape[0] != P * N : logits->shape[0] != P || logits->shape[1] != N) {
+    return fail(LQ_ERR_INVALID_ARG, "logits must be [%lld, %lld, V] or [%lld, V]", (long long)P,
+                (long long)N, (long long)(P * N));
+  }
   const lq_tensor* rows[2] = {scores, finished};
   for (const lq_tensor* t : rows) {
     if (t != nullptr && (t->shape[0] != P || t->shape[1] != N)) {
@@ -864,6 +869,11 @@ extern "C" int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores,
 
   SelectParams p{};
   p.logits = make_view(logits);
+  if (ldim == 2) {
+    p.logits.s[2] = logits->stride[1];
+    p.logits.s[1] = logits->stride[0];
+    p.logits.s[0] = logits->stride[0] * N;
+  }
   p.scores = (const float*)scores->data;
   for (int i = 0; i < 2; ++i) {
     p.ss[i] = scores->stride[i];

@@ -369,10 +369,10 @@ PyObject* py_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int slots = PyObject_IsTrue(a[7]);
   if (slots < 0) return nullptr;
   const lq_tensor* const* p = t.ptr;
-  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim != 3 || p[3] == nullptr || p[3]->ndim != 2 ||
-               p[3]->shape[1] > INT32_MAX);
-  const size_t need = entries.select_workspace(p[0]->shape[0], p[0]->shape[1], p[0]->shape[2],
-                                               (int)p[3]->shape[1]);
+  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim < 1 || p[1] == nullptr || p[1]->ndim != 2 ||
+               p[3] == nullptr || p[3]->ndim != 2 || p[3]->shape[1] > INT32_MAX);
+  const size_t need = entries.select_workspace(p[1]->shape[0], p[1]->shape[1],
+                                               p[0]->shape[p[0]->ndim - 1], (int)p[3]->shape[1]);
   return launch_with(t.device, a[8], need, [&](void* ws, size_t bytes, void* s) {
     return entries.select(p[0], p[1], p[2], p[3], p[4], p[5], pad, slots, ws, bytes, s);
   });
