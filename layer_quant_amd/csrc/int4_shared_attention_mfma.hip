@@ -136,6 +136,42 @@ __device__ __forceinline__ int exponent_above(float v) {
   return min(max(e, -60), MAX_E);
 }
 
+// A query row's 32 values of this lane (two per word) as fp16 operands q * 2^-e, 2^e being `scale`, e such
+// that the row's largest value lies in [2^14, 2^15); zeros where the row is none.
+template <int DT>
+__device__ __forceinline__ void scale_query(const uint32_t (&w)[4][4], bool ok, u32x4_t (&op)[4],
+                                            float& scale) {
+  float qv[4][8];
+  float mx = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = ok ? w[k][j] : 0u;
+      qv[k][2 * j] = word_elem(x, 0, DT);
+      qv[k][2 * j + 1] = word_elem(x, 16, DT);
+      mx = fmaxf(mx, fmaxf(fabsf(qv[k][2 * j]), fabsf(qv[k][2 * j + 1])));
+    }
+  }
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  int e = mx > 0.0f ? (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127 - 14 : 0;
+  e = max(-100, min(100, e));
+  scale = __uint_as_float((uint32_t)(127 + e) << 23);
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) op[k][j] = pack_f16(qv[k][j] * inv, qv[k][j + 4] * inv);
+  }
+}
+
+// The products a0 b0 and a1 b1 as an fp16 pair, each rounded once (v_fma_mixlo/mixhi_f16; as two multiplies
+// and a conversion the pair takes three instructions).
+__device__ __forceinline__ f16x2_t mul_f16(float a0, float b0, float a1, float b1) {
+  return f16x2_t{(_Float16)__builtin_fmaf(a0, b0, 0.0f), (_Float16)__builtin_fmaf(a1, b1, 0.0f)};
+}
+
 template <int QT, int G, int MASK, bool EXACT>
 __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, SharedTile* ring,
                                          MaskWords* words, WavePartial<QT>* part) {
@@ -197,29 +233,9 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
         for (int j = 0; j < 4; ++j) w[k][j] = e[k][2 * j] | (e[k][2 * j + 1] << 16);
       }
     }
-    float qv[4][8];
-    float mx = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t x = ok ? w[k][j] : 0u;
-        qv[k][2 * j] = word_elem(x, 0, p.q.dtype);
-        qv[k][2 * j + 1] = word_elem(x, 16, p.q.dtype);
-        mx = fmaxf(mx, fmaxf(fabsf(qv[k][2 * j]), fabsf(qv[k][2 * j + 1])));
-      }
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    int e = mx > 0.0f ? (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127 - 14 : 0;
-    e = max(-100, min(100, e));
-    cs[qt] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_sm;
-    const float qinv = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) qop[qt][k][j] = pack_f16(qv[k][j] * qinv, qv[k][j + 4] * qinv);
-    }
+    if (p.q.dtype == LQ_BF16) scale_query<LQ_BF16>(w, ok, qop[qt], cs[qt]);
+    else scale_query<LQ_F16>(w, ok, qop[qt], cs[qt]);
+    cs[qt] *= p.scale_sm;
   }
 
   float m_run[QT], l_run[QT];
@@ -393,15 +409,20 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     }
 
     // ---- running references: the value scales' exponent of the wave, each row's maximum
-    float vmax = vs[0][0];
+    float vmax;
+    if constexpr (MASK == MASK_NONE) {  // each lane its part of the tile's 32 G scales
+      vmax = B.vs[lane & (32 * G - 1)];
+      if constexpr (G == 4) vmax = fmaxf(vmax, B.vs[64 + lane]);
+    } else {
+      vmax = vs[0][0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 8; ++e) {
 #pragma unroll
-      for (int m = 0; m < G; ++m) vmax = fmaxf(vmax, vs[e][m]);
+        for (int m = 0; m < G; ++m) vmax = fmaxf(vmax, vs[e][m]);
+      }
     }
     if (__any(vmax > vlim)) {
-      vmax = fmaxf(vmax, __shfl_xor(vmax, 16, 64));
-      vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
+      vmax = group_max<64>(vmax);
       const int e = __builtin_amdgcn_readfirstlane(exponent_above(vmax));
       const int next = max(voff, e - P_TOP);
       if (voff > -1000 && next > voff) {
@@ -458,8 +479,7 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
       for (int qt = 0; qt < QT; ++qt) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const f16x2_t h = {(_Float16)(s[qt][2 * j] * vs[2 * j][m]),
-                             (_Float16)(s[qt][2 * j + 1] * vs[2 * j + 1][m])};
+          const f16x2_t h = mul_f16(s[qt][2 * j], vs[2 * j][m], s[qt][2 * j + 1], vs[2 * j + 1][m]);
           hi[qt][j] = __builtin_bit_cast(uint32_t, h);
           if constexpr (EXACT) {
             lo[qt][j] = pack_f16(fmaf(s[qt][2 * j], vs[2 * j][m], -(float)h[0]),
