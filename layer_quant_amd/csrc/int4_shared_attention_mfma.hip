@@ -190,11 +190,10 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   auto tile_key = [&](const int i) { return u.t0 + (wave + WAVES * i) * TILE; };
   // K slot l of a half holds row l >> 2, unit (l & 3) ^ ((l >> 4) & 3)
   const int kvo = (lane >> 2) * 64 + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
-  SharedTile& tile0 = ring[0 * WAVES + wave];
-  SharedTile& tile1 = ring[1 * WAVES + wave];
-  SharedTile& tile2 = ring[2 * WAVES + wave];
-  if (nw > 0) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(0), u.S, tile0, lane);
-  if (nw > 1) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(1), u.S, tile1, lane);
+  auto tile_at = [&](const int slot) -> SharedTile& { return ring[slot * WAVES + wave]; };
+  for (int i = 0; i < 2; ++i) {
+    if (i < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i), u.S, tile_at(i), lane);
+  }
 
   // Query operands: lane (q4, c16) of column tile qt holds query row row0 + 16 qt + c16, dims
   // 32c + 8 q4 + (0,4,1,5,2,6,3,7) for chunk c, as fp16 q * 2^-e; cs turns its raw scores into exp2
@@ -255,20 +254,41 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   const int last_row = min(u.row0 + 16 * QT, u.rows) - 1;
   const int members = last_row / p.nrep - first_member + 1;
   auto make_words = [&](const int i0) {
-    for (int i = i0; i < min(i0 + SEG, nw); ++i) {
-      const int64_t key = u.key0 + tile_key(i) + (lane & 31);
-      uint32_t any = 0;
-      for (int a = 0; a < members; a += 2) {
-        const int n = a + (lane >> 5);
-        bool keep = false;
-        if (n < members && key < p.mask_len) {
-          keep = ((const int64_t*)p.mask)[(u.b0 + first_member + n) * p.mask_sb + key * p.mask_sk] != 0;
+    constexpr int BATCH = 8;  // loads in flight
+    const int pairs = (members + 1) / 2;
+    const int tiles = min(SEG, nw - i0);
+    int i = 0, a = 0;  // tile and pair of the batch's first load
+    for (int left = tiles * pairs; left > 0; left -= BATCH) {
+      int ti[BATCH], ta[BATCH];
+      bool keep[BATCH];
+#pragma unroll
+      for (int f = 0; f < BATCH; ++f) {
+        ti[f] = i;
+        ta[f] = a;
+        const int n = 2 * a + (lane >> 5);
+        const int64_t key = u.key0 + tile_key(i0 + i) + (lane & 31);
+        keep[f] = false;
+        if (f < left && n < members && key < p.mask_len) {
+          keep[f] = ((const int64_t*)p.mask)[(u.b0 + first_member + n) * p.mask_sb + key * p.mask_sk] != 0;
         }
-        const uint64_t bits = __ballot(keep);
-        any |= (uint32_t)bits | (uint32_t)(bits >> 32);
-        if (lane < 2) words->w[i - i0][a + lane] = lane == 0 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+        if (++a == pairs) {
+          a = 0;
+          ++i;
+        }
       }
-      if (lane == 0) words->w[i - i0][32] = any;
+#pragma unroll
+      for (int f = 0; f < BATCH; ++f) {
+        const uint64_t bits = __ballot(keep[f]);
+        if (f < left && lane < 2) {
+          words->w[ti[f]][2 * ta[f] + lane] = lane == 0 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane < tiles) {
+      uint32_t any = 0;
+      for (int n = 0; n < members; ++n) any |= words->w[lane][n];
+      words->w[lane][32] = any;
     }
     __builtin_amdgcn_wave_barrier();
   };
@@ -504,21 +524,20 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     __builtin_amdgcn_wave_barrier();
   };
 
-  // 3-deep ring: the loads of the next two tiles are in flight while one is processed
-  for (int i = 0; i < nw; i += 3) {
-    if (i + 2 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 2), u.S, tile2, lane);
-    process(i, tile0);
-    if (i + 1 >= nw) break;
-    if (i + 3 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 3), u.S, tile0, lane);
-    process(i + 1, tile1);
-    if (i + 2 >= nw) break;
-    if (i + 4 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 4), u.S, tile1, lane);
-    process(i + 2, tile2);
+  // 3-deep ring: the loads of the next two tiles are in flight while one is processed. (One body for all
+  // ring positions: unrolled by three, the kernel's two units fill the instruction cache.)
+  int slot = 0;
+  for (int i = 0; i < nw; ++i) {
+    const int fill = slot == 0 ? 2 : slot - 1;
+    if (i + 2 < nw) issue_tile<G>(kb, vb, ksb, vsb, kvo, tile_key(i + 2), u.S, tile_at(fill), lane);
+    process(i, tile_at(slot));
+    slot = slot == 2 ? 0 : slot + 1;
   }
 
+  const float vscale = voff > -1000 ? __builtin_amdgcn_exp2f((float)voff) : 0.0f;
+  const int ns = p.nsp + p.nso;
   // ---- the waves' states to LDS (over the tiles, which every wave has read), joined there
   __syncthreads();
-  const float vscale = voff > -1000 ? __builtin_amdgcn_exp2f((float)voff) : 0.0f;
   WavePartial<QT>& mine = part[wave];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -540,7 +559,6 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   }
   __syncthreads();
   const int tid = threadIdx.x;
-  const int ns = p.nsp + p.nso;
 #pragma unroll
   for (int pass = 0; pass < 2 * QT; ++pass) {
     const int row = 8 * pass + (tid >> 5);
@@ -580,8 +598,8 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   }
 }
 
-// Blocks: the prefix units first (KV head fastest, so that the row blocks that share keys lie on the
-// same XCD where there are 8 KV heads; then row block, split, prompt), then the own units.
+// Workgroups: the prefix units first, the longer ones (KV head fastest, so that the row blocks that share
+// keys lie on the same XCD where there are 8 KV heads; then row block, split, prompt), then the own units.
 template <int QT, int G, int MASK, bool EXACT>
 __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p) {
   __shared__ SharedLds<QT> lds;
@@ -608,27 +626,27 @@ __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p)
     u.b0 = (int64_t)prompt * p.N;
     u.pack = false;
     run_unit<QT, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, lds.part);
-  } else {
-    i -= p.prefix_blocks;
-    u.kvh = i % p.Hkv;
-    i /= p.Hkv;
-    const int rb = i % p.rb_own;
-    i /= p.rb_own;
-    const int split = i % p.nso;
-    const int b = i / p.nso;
-    u.split = p.nsp + split;
-    u.c = &p.own;
-    u.crow = b;
-    u.S = (int)p.own_len;
-    u.t0 = split * (int)p.chunk_o;
-    u.t1 = min(u.S, u.t0 + (int)p.chunk_o);
-    u.key0 = p.prefix_len;
-    u.row0 = rb * 16;
-    u.rows = p.nrep;
-    u.b0 = b;
-    u.pack = p.pack && u.t1 == u.S;
-    run_unit<1, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, (WavePartial<1>*)lds.part);
+    return;
   }
+  i -= p.prefix_blocks;
+  u.kvh = i % p.Hkv;
+  i /= p.Hkv;
+  const int rb = i % p.rb_own;
+  i /= p.rb_own;
+  const int split = i % p.nso;
+  const int b = i / p.nso;
+  u.split = p.nsp + split;
+  u.c = &p.own;
+  u.crow = b;
+  u.S = (int)p.own_len;
+  u.t0 = split * (int)p.chunk_o;
+  u.t1 = min(u.S, u.t0 + (int)p.chunk_o);
+  u.key0 = p.prefix_len;
+  u.row0 = rb * 16;
+  u.rows = p.nrep;
+  u.b0 = b;
+  u.pack = p.pack && u.t1 == u.S;
+  run_unit<1, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, (WavePartial<1>*)lds.part);
 }
 
 template <int QT, int G, int MASK>
