@@ -40,6 +40,8 @@ struct SharedParams {
   int col_tiles;            // 16-row column tiles of a prefix unit's wave
   int rb_prefix, rb_own;    // row blocks of a prefix and of an own unit
   uint32_t prefix_blocks;   // workgroups of the prefix units
+  uint32_t own_units;       // own units, times splits
+  int own_waves;            // waves per own unit
 };
 
 // Splits of the two key ranges.

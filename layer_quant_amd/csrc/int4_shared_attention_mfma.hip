@@ -77,6 +77,7 @@ struct Unit {
   int row0, rows;    // first query row of the block, query rows of the unit
   int64_t b0;        // row of member 0 in q
   int split;         // partial slot
+  int waves;         // waves of the workgroup that share the unit (1, 2 or 4)
   bool pack;         // the token goes into cache row S - 1
 };
 
@@ -186,8 +187,9 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   const float* ksb = c.ks + u.crow * c.kss[0] + u.kvh * c.kss[1];
   const float* vsb = c.vs + u.crow * c.vss[0] + u.kvh * c.vss[1];
   const int ntile = (u.t1 - u.t0 + TILE - 1) / TILE;
-  const int nw = ntile > wave ? (ntile - wave + WAVES - 1) / WAVES : 0;
-  auto tile_key = [&](const int i) { return u.t0 + (wave + WAVES * i) * TILE; };
+  const int member_wave = wave & (u.waves - 1);
+  const int nw = ntile > member_wave ? (ntile - member_wave + u.waves - 1) / u.waves : 0;
+  auto tile_key = [&](const int i) { return u.t0 + (member_wave + u.waves * i) * TILE; };
   // K slot l of a half holds row l >> 2, unit (l & 3) ^ ((l >> 4) & 3)
   const int kvo = (lane >> 2) * 64 + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
   auto tile_at = [&](const int slot) -> SharedTile& { return ring[slot * WAVES + wave]; };
@@ -558,23 +560,16 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     }
   }
   __syncthreads();
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int pass = 0; pass < 2 * QT; ++pass) {
-    const int row = 8 * pass + (tid >> 5);
-    const int d = 4 * (tid & 31);
-    if (u.row0 + row >= u.rows) continue;
+  const int w0 = wave & ~(u.waves - 1);  // the unit's first wave
+  for (int i = threadIdx.x - 64 * w0; i < 16 * QT * (SD / 4); i += 64 * u.waves) {
+    const int row = i / (SD / 4);
+    const int d = 4 * (i % (SD / 4));
+    if (u.row0 + row >= u.rows) break;
     float M = -INFINITY, L = 0.0f;
-    float mw[WAVES];
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      mw[w] = part[w].m[row];
-      M = fmaxf(M, mw[w]);
-    }
+    for (int w = w0; w < w0 + u.waves; ++w) M = fmaxf(M, part[w].m[row]);
     f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float wt = partial_weight(mw[w], M);
+    for (int w = w0; w < w0 + u.waves; ++w) {
+      const float wt = partial_weight(part[w].m[row], M);
       L += wt * part[w].l[row];
       o += wt * *(const f32x4_t*)&part[w].o[row][d];
     }
@@ -625,10 +620,15 @@ __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p)
     u.rows = p.N * p.nrep;
     u.b0 = (int64_t)prompt * p.N;
     u.pack = false;
+    u.waves = WAVES;
     run_unit<QT, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, lds.part);
     return;
   }
-  i -= p.prefix_blocks;
+  // (a wave without a unit takes the last one's place with no query rows)
+  u.waves = p.own_waves;
+  i = (i - p.prefix_blocks) * (WAVES / p.own_waves) + (uint32_t)wave / p.own_waves;
+  const bool none = i >= p.own_units;
+  if (none) i = p.own_units - 1;
   u.kvh = i % p.Hkv;
   i /= p.Hkv;
   const int rb = i % p.rb_own;
@@ -646,6 +646,11 @@ __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p)
   u.rows = p.nrep;
   u.b0 = b;
   u.pack = p.pack && u.t1 == u.S;
+  if (none) {
+    u.t1 = u.t0;  // no keys
+    u.row0 = u.rows;
+    u.pack = false;
+  }
   run_unit<1, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, (WavePartial<1>*)lds.part);
 }
 
@@ -711,8 +716,13 @@ SharedPlan plan_shared_fast(int64_t P, int64_t N, int64_t Hkv, int64_t nrep, int
   const int64_t units = std::max<int64_t>(1, P * Hkv * ((rows + block - 1) / block));
   const int64_t own_units = std::max<int64_t>(1, P * N * Hkv * ((nrep + 15) / 16));
   constexpr int64_t STEP = WAVES * TILE;
-  return SharedPlan{split_of(prefix_len, resident / units, STEP),
-                    split_of(own_len, resident / own_units, STEP)};
+  SharedPlan plan{split_of(prefix_len, resident / units, STEP),
+                  split_of(own_len, resident / own_units, 2 * STEP)};
+  // a wave of one tile spends its time in set-up and merging: two where that leaves a workgroup per CU
+  if (plan.prefix.chunk == STEP && units * ((prefix_len + 2 * STEP - 1) / (2 * STEP)) >= device_cus()) {
+    plan.prefix = split_of(prefix_len, resident / units, 2 * STEP);
+  }
+  return plan;
 }
 
 int launch_shared_fast(SharedParams p, hipStream_t st) {
@@ -721,8 +731,12 @@ int launch_shared_fast(SharedParams p, hipStream_t st) {
   p.rb_prefix = (int)((rows + 16 * p.col_tiles - 1) / (16 * p.col_tiles));
   p.rb_own = (p.nrep + 15) / 16;
   const int64_t pb = (int64_t)p.P * p.Hkv * p.rb_prefix * p.nsp;
-  const int64_t ob = (int64_t)p.B * p.Hkv * p.rb_own * p.nso;
-  if (pb + ob >= (int64_t)1 << 31) {
+  const int64_t units = (int64_t)p.B * p.Hkv * p.rb_own * p.nso;
+  const int64_t tiles = (std::min(p.chunk_o, p.own_len) + TILE - 1) / TILE;
+  p.own_waves = tiles <= 2 ? 1 : tiles <= 4 ? 2 : 4;
+  const int64_t ob = (units * p.own_waves + WAVES - 1) / WAVES;
+  p.own_units = (uint32_t)units;
+  if (pb + units >= (int64_t)1 << 31) {
     return fail(LQ_ERR_UNSUPPORTED, "%lld workgroups exceed the launch limits", (long long)(pb + ob));
   }
   p.prefix_blocks = (uint32_t)pb;
