@@ -705,12 +705,15 @@ bool shared_fast_ok(const SharedParams& p) {
   return ((uintptr_t)p.mask & (p.mask_keep ? 7 : 3)) == 0;
 }
 
+// Workgroups that run at once: two per CU (LDS and registers).
+static int64_t resident_workgroups() { return 2 * (int64_t)device_cus(); }
+
 // Column tiles of 16 query rows per wave in the prefix units.
 static int col_tiles_of(int64_t rows) { return rows <= 16 ? 1 : 2; }
 
 SharedPlan plan_shared_fast(int64_t P, int64_t N, int64_t Hkv, int64_t nrep, int64_t prefix_len,
                             int64_t own_len) {
-  const int64_t resident = 2 * (int64_t)device_cus();  // workgroups: 2 per CU
+  const int64_t resident = resident_workgroups();
   const int64_t rows = N * nrep;
   const int64_t block = 16 * col_tiles_of(rows);
   const int64_t units = std::max<int64_t>(1, P * Hkv * ((rows + block - 1) / block));
@@ -732,8 +735,13 @@ int launch_shared_fast(SharedParams p, hipStream_t st) {
   p.rb_own = (p.nrep + 15) / 16;
   const int64_t pb = (int64_t)p.P * p.Hkv * p.rb_prefix * p.nsp;
   const int64_t units = (int64_t)p.B * p.Hkv * p.rb_own * p.nso;
+  // Waves per own unit: a whole workgroup where every one has its place at once, the shortest chain of
+  // steps (1 prompt x 16, ctx 2000, 100 own rows: 15.3 us, 16.6 with two waves, 19.8 with one); where they
+  // wait for places behind the prefix, fewer and fuller ones (8 x 8, ctx 16384: 64 own rows 60.8 us with
+  // four waves, 58.4 with one; 100 rows 63.1, 58.4 with two, 62.2 with one; 200 rows 64.4, 61.9 with two,
+  // 64.4 with one).
   const int64_t tiles = (std::min(p.chunk_o, p.own_len) + TILE - 1) / TILE;
-  p.own_waves = tiles <= 2 ? 1 : tiles <= 4 ? 2 : 4;
+  p.own_waves = pb + units <= resident_workgroups() ? 4 : tiles <= 2 ? 1 : tiles <= 8 ? 2 : 4;
   const int64_t ob = (units * p.own_waves + WAVES - 1) / WAVES;
   p.own_units = (uint32_t)units;
   if (pb + units >= (int64_t)1 << 31) {
