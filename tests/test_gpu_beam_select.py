@@ -57,7 +57,7 @@ def check(logits, scores, num=None, **kw):
     s, w = got[0].cpu().double().numpy(), want[0]
     live = np.isfinite(w)
     assert np.array_equal(live, np.isfinite(s)) and np.array_equal(s[~live], w[~live])
-    assert np.all(np.abs(s - w)[live] <= 2.0 ** -24 * np.abs(w[live]) + 2.0 ** -19)
+    assert np.all(np.abs(s[live] - w[live]) <= 2.0 ** -24 * np.abs(w[live]) + 2.0 ** -19)
     return got
 
 
@@ -109,6 +109,21 @@ def test_ties_and_borders(gpu, V):
     scores[:, 0] = 0
     logits, _ = random(gpu, P, N, V, torch.float32, 3)
     check(logits, scores)
+
+
+@pytest.mark.parametrize("N,num", [(8, 32), (16, 32), (64, 64)])
+@pytest.mark.parametrize("V", [700, 9001, 40000])
+def test_many_equal_totals(gpu, N, num, V):
+    """More candidates at the border than the final list holds, and lists that overflow."""
+    gen = torch.Generator(device=gpu).manual_seed(V + N)
+    scores = torch.zeros(2, N, device=gpu)
+    row = torch.randint(0, 2, (1, V), device=gpu, generator=gen).float()
+    for logits in (torch.zeros(2 * N, V, device=gpu), row.expand(2 * N, V),
+                   torch.where(row > 0, 0.0, -torch.inf).expand(2 * N, V).to(torch.bfloat16),
+                   torch.full((2 * N, V), -torch.inf, device=gpu)):
+        check(logits, scores, num)
+        check(logits, scores, slots=True)
+        check(logits, scores, num, finished=torch.arange(2 * N, device=gpu).reshape(2, N) % 3 == 0, pad=V - 1)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -163,6 +163,18 @@ def test_shapes(gpu, P, N, hkv, nrep, lp, lo, g, dtype):
     run(gpu, P, N, hkv, nrep, lp, lo, 128, g, dtype, seed=lp + lo)
 
 
+@pytest.mark.parametrize("lo", [1, 40, 64, 65, 100, 129, 250, 300])
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_own_rows(gpu, lo, masked):
+    """Own units behind a prefix that fills the GPU: one, two or four waves each, odd numbers of them."""
+    P, N, hkv, nrep, lp, g = 5, 13, 8, 4, 2500, 32
+    mask = None
+    if masked:
+        gen = torch.Generator(device=gpu).manual_seed(lo)
+        mask = (torch.rand(P * N, lp + lo, device=gpu, generator=gen) < 0.8).long()
+    run(gpu, P, N, hkv, nrep, lp, lo, 128, g, BF16, lo, mask)
+
+
 @pytest.mark.parametrize("d,g,dtype", [(64, 32, BF16), (128, 32, FP32), (128, 16, BF16), (96, 96, FP16),
                                        (512, 64, BF16), (80, 2, FP32)])
 def test_general_kernel(gpu, d, g, dtype):
