@@ -529,15 +529,18 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
   if (threadIdx.x < slots) first_part = parts[threadIdx.x];
 
   for (int n = wave; n < p.N; n += FW) {
-    const bool fin = p.finished != nullptr && p.finished[prompt * p.fs[0] + n * p.fs[1]] != 0;
+    // the lane's first part is loaded beside the flag and the score
+    PartResult r = {LOWEST, 0.0f, 0, ~0u};
+    if (lane < p.parts) r = parts[n * p.parts + lane];
     const float score = p.scores[prompt * p.ss[0] + n * p.ss[1]];
+    const bool fin = p.finished != nullptr && p.finished[prompt * p.fs[0] + n * p.fs[1]] != 0;
     double b = score;
     if (!fin) {
       // each lane's parts with a running maximum, then the lanes
-      float m = LOWEST, s = 0.0f;
-      uint32_t share = ~0u;
-      for (int i = lane; i < p.parts; i += 64) {
-        const PartResult r = parts[n * p.parts + i];
+      float m = r.m, s = r.s;
+      uint32_t share = r.share;
+      for (int i = lane + 64; i < p.parts; i += 64) {
+        r = parts[n * p.parts + i];
         share = min(share, r.share);
         const float m2 = fmaxf(m, r.m);
         s = s * exp2f(m - m2) + r.s * exp2f(r.m - m2);

@@ -200,26 +200,25 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   // Query operands: lane (q4, c16) of column tile qt holds query row row0 + 16 qt + c16, dims
   // 32c + 8 q4 + (0,4,1,5,2,6,3,7) for chunk c, as fp16 q * 2^-e; cs turns its raw scores into exp2
   // units. Rows past the unit's count hold 0.
+  // The rows' bits are loaded here and converted behind the mask's loads.
   u32x4_t qop[QT][4];
   float cs[QT];
   int member[QT];  // the row's member, relative to the row block's first
+  uint32_t qbits[QT][4][4];
   const int first_member = u.row0 / p.nrep;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    const int row = u.row0 + 16 * qt + c16;
-    const bool ok = row < u.rows;
-    const int r = ok ? row : u.rows - 1;
+    const int r = min(u.row0 + 16 * qt + c16, u.rows - 1);
     const int n = r / p.nrep;
     member[qt] = n - first_member;
     const int64_t base = (u.b0 + n) * p.q.s[0] + (int64_t)(u.kvh * p.nrep + r - n * p.nrep) * p.q.s[1];
-    uint32_t w[4][4];
     const uint16_t* at = (const uint16_t*)p.q.data + base;
     if (p.q_rows) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const u32x4_t v = *(const u32x4_t*)(at + 32 * k + 8 * q4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[k][j] = v[j];
+        for (int j = 0; j < 4; ++j) qbits[qt][k][j] = v[j];
       }
     } else {
       uint32_t e[4][8];
@@ -231,12 +230,9 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[k][j] = e[k][2 * j] | (e[k][2 * j + 1] << 16);
+        for (int j = 0; j < 4; ++j) qbits[qt][k][j] = e[k][2 * j] | (e[k][2 * j + 1] << 16);
       }
     }
-    if (p.q.dtype == LQ_BF16) scale_query<LQ_BF16>(w, ok, qop[qt], cs[qt]);
-    else scale_query<LQ_F16>(w, ok, qop[qt], cs[qt]);
-    cs[qt] *= p.scale_sm;
   }
 
   float m_run[QT], l_run[QT];
@@ -295,6 +291,17 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     __builtin_amdgcn_wave_barrier();
   };
 
+  if constexpr (MASK == MASK_KEEP) {
+    if (nw > 0) make_words(0);
+  }
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const bool ok = u.row0 + 16 * qt + c16 < u.rows;
+    if (p.q.dtype == LQ_BF16) scale_query<LQ_BF16>(qbits[qt], ok, qop[qt], cs[qt]);
+    else scale_query<LQ_F16>(qbits[qt], ok, qop[qt], cs[qt]);
+    cs[qt] *= p.scale_sm;
+  }
+
   const int krow = 4 * (c16 & 3) + (c16 >> 2);  // key of QK A-row c16 in its half
   // byte c16 & 3 of two dwords -> bytes 0 and 2
   const uint32_t vsel = 0x0c040c00u + (c16 & 3) * 0x00010001u;
@@ -302,7 +309,7 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
   auto process = [&](const int i, SharedTile& B) {
     const int tb = tile_key(i);
     if constexpr (MASK == MASK_KEEP) {
-      if (i % SEG == 0) make_words(i);
+      if (i > 0 && i % SEG == 0) make_words(i);
     }
     if (i + 2 < nw) wait_loads<2 * LPT>();
     else if (i + 1 < nw) wait_loads<LPT>();
