@@ -17,6 +17,14 @@
 // goes wrong only where totals are closer than the sums' rounding, about 1e-7). num candidates reach
 // the largest of the parts' bounds; those that do (a few hundred) are reduced, wave by wave, to
 // the num best, which one wave sorts and writes out, by rank or by place.
+//
+// What it measured (MI355X, kernel trace, parts + final): 256 rows of 131072 bf16 logits (67 MB), 32 of
+// each of 16 prompts, 19.2 + 10.4 us; 64 rows, 8 of each of 8 prompts, 9.8 + 6.6; 15 rows of 50257 fp32
+// 6.6 + 6.6; 4 rows of 32000 6.2 + 5.7. The largest is bound by the VALU (about 13 instructions per logit,
+// of which the exponential takes two issue slots), the others by the latency of two launches and of
+// their loads. Tried: one block reduction per selected token (1301 us for the largest); lists per run with a
+// rising threshold (57 us); the list code inside the 64 unrolled comparisons (part kernel 46.8 us: the
+// instruction cache; 23.0 with it outside).
 #include <math.h>
 
 #include <algorithm>
