@@ -453,29 +453,26 @@ class _Workspace:
 _workspace = _Workspace()
 
 
-class _Scratch:
-    """Scratch of the calls that need no particular contents: per (device, stream), grown on demand.
-    A call that is being captured gets a buffer of the graph's own memory instead, so that graphs
-    captured on one stream do not share it and an eager call that grows the buffer leaves theirs."""
+class _Scratch(threading.local):
+    """Scratch of the calls that need no particular contents: per thread, device and stream, grown on
+    demand. A call writes it in one launch and reads it in the next, between which another thread may
+    launch on the same stream: each thread has its own. A call that is being captured gets a buffer of
+    the graph's own memory, so that graphs captured on one stream do not share it and an eager call
+    that grows the buffer leaves theirs."""
 
     def __init__(self):
         self._bufs: dict[tuple[int, int], torch.Tensor] = {}
-        self._lock = threading.Lock()
 
     def get(self, index: int, stream: int, nbytes: int) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
         key = (index, stream)
         buf = self._bufs.get(key)
-        if buf is not None and buf.numel() >= nbytes:
-            return buf
-        with self._lock:
-            buf = self._bufs.get(key)
-            if buf is None or buf.numel() < nbytes:
-                buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8,
-                                  device=torch.device("cuda", index))
-                self._bufs[key] = buf
-            return buf
+        if buf is None or buf.numel() < nbytes:
+            buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8,
+                              device=torch.device("cuda", index))
+            self._bufs[key] = buf
+        return buf
 
 
 _scratch = _Scratch()
@@ -717,8 +714,8 @@ def int4_shared_decode_attention(q: torch.Tensor, k_new: torch.Tensor | None,
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None,
                 out_scores: torch.Tensor, out_beams: torch.Tensor, out_tokens: torch.Tensor,
                 pad_token: int, keep_slots: bool) -> None:
-    """The best continuations of logits [P, N, V] or [P*N, V] and scores [P, N] (finished: uint8 [P, N] or None)
-    into the outputs [P, num]."""
+    """The best continuations of logits [P, N, V] or [P*N, V] and scores [P, N] (finished: uint8
+    [P, N] or None) into the outputs [P, num]."""
     host = _host or host_binding()
     if host:
         rc = host.beam_select(logits, scores, finished, out_scores, out_beams, out_tokens, pad_token,

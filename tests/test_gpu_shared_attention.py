@@ -16,6 +16,7 @@ the sums' weights and values against A = sum_j w_j |v_j| / sum_j w_j:
     them in the matrix-core kernel's lanes per rescale step, linear in the keys else: keys * 2^-23.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -351,6 +352,36 @@ def test_stream_and_capture(gpu):
             g_.replay()
             ref = reference(q, own, S, nrep, g)
             assert_near(out, ref, BF16, 128, S, True, f"replay {i}")
+
+
+def test_threads_on_one_stream(gpu):
+    """Two threads whose calls (a launch that leaves partials, a merge that reads them) interleave on one
+    stream."""
+    hkv, nrep, g = 8, 4, 32
+    calls = []
+    for P, N, lp, seed in ((1, 4, 2000, 1), (2, 3, 1500, 2)):
+        own = cache_of(gpu, P * N, hkv, 20, 32, 128, g, seed)
+        own.prefix = cache_of(gpu, P, hkv, lp, lp, 128, g, seed + 10)
+        q = torch.randn(P * N, hkv * nrep, 1, 128, device=gpu).to(BF16)
+        calls.append((q, own, lp + 20, nrep, g))
+    alone = [ia.shared_prefix_decode_attention(*c) for c in calls]
+    outs = [[], []]
+    start = threading.Barrier(2)
+
+    def work(i):
+        start.wait()
+        for _ in range(200):
+            outs[i].append(ia.shared_prefix_decode_attention(*calls[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(outs[i]) == 200
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
 
 
 def test_long_prefix_offsets(gpu):
