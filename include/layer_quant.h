@@ -354,7 +354,7 @@ int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores, const lq_te
  *   rows   NULL, or for each tensor how many entries of dim 2 are moved (the live rows of a cache
  *          [B, Hkv, cap, .]; what lies behind them stays), -1 for the whole tensor
  *   beams  [P, N] i64
- * The tensors must not overlap (one listed twice is refused). One launch for up to 256 tensors of up
+ * The tensors must not overlap (one listed twice, or over the beams, is refused). One launch for up to 256 tensors of up
  * to 16 row shapes. No counterpart in the reference.
  */
 #define LQ_REORDER_MAX_BEAMS 64

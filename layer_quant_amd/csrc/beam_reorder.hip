@@ -18,6 +18,7 @@ constexpr int MAX_BEAMS = LQ_REORDER_MAX_BEAMS;
 constexpr int THREADS = 256;
 constexpr int MAX_SHAPES = 16;    // different row geometries in a launch
 constexpr int MAX_TENSORS = 256;  // tensors in a launch
+constexpr int64_t MAX_BLOCKS = ((int64_t)1 << 32) / THREADS - 1;  // a launch holds less than 2^32 threads
 
 // Contents of a row: a n0 x n1 x n2 array of runs (byte strides s0, s1, s2) of `units` units.
 struct RowShape {
@@ -129,6 +130,7 @@ __global__ __launch_bounds__(THREADS) void reorder_kernel(ReorderParams p) {
 struct Item {
   RowShape shape;
   char* base;
+  int64_t span;  // bytes from base on
 };
 
 // The row geometry of t over its first `rows` entries of dim 2 (-1: all); total 0 when it is empty.
@@ -179,6 +181,13 @@ int row_shape(const lq_tensor& t, int64_t rows, int64_t per_block, Item& item) {
   r.blocks = (uint32_t)((total + per_block - 1) / per_block);
   item.shape = r;
   return LQ_OK;
+}
+
+// The bytes that t spans, from its first element's on.
+int64_t span_bytes(const lq_tensor& t) {
+  int64_t last = 0;
+  for (int d = 0; d < t.ndim; ++d) last += (t.shape[d] - 1) * t.stride[d];
+  return (last + 1) * dtype_size(t.dtype);
 }
 
 int launch(const ReorderParams& p, int nmax, int64_t blocks, hipStream_t st) {
@@ -243,6 +252,7 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
     Item it{};
     if ((rc = row_shape(t, live, per_block, it)) != LQ_OK) return rc;
     if (it.shape.total == 0) continue;
+    it.span = span_bytes(t);
     items[used++] = it;
   }
   if (used == 0 || P == 0 || N <= 1) return LQ_OK;
@@ -250,6 +260,14 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
   for (int i = 1; i < used; ++i) {
     if (items[i].base == items[i - 1].base) {
       return fail(LQ_ERR_INVALID_ARG, "a tensor is listed twice");
+    }
+  }
+  // a workgroup may read its beams after another has moved rows
+  const char* beams_at = (const char*)beams->data;
+  const int64_t beams_span = span_bytes(*beams);
+  for (int i = 0; i < used; ++i) {
+    if (beams_at < items[i].base + items[i].span && items[i].base < beams_at + beams_span) {
+      return fail(LQ_ERR_INVALID_ARG, "a tensor overlaps the beams");
     }
   }
 
@@ -273,7 +291,7 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
       const int64_t each = (int64_t)sh.blocks * P;
       for (int j = i; j < used && taken < MAX_TENSORS; ++j) {
         if (done[j] || !(items[j].shape == sh)) continue;
-        if (blocks + each >= (int64_t)1 << 31) break;
+        if (blocks + each > MAX_BLOCKS) break;
         p.base[taken++] = items[j].base;
         blocks += each;
         done[j] = true;

@@ -338,7 +338,7 @@ extern "C" int lq_int4_shared_decode_attention(
     }
   }
   if (B == 0 || Hq == 0) return LQ_OK;
-  if (B * Hq >= (int64_t)1 << 31) {
+  if (B * Hq * 64 >= (int64_t)1 << 32) {  // threads of the generic kernel's launch
     return fail(LQ_ERR_UNSUPPORTED, "%lld rows x %lld heads exceed the launch limits", (long long)B,
                 (long long)Hq);
   }

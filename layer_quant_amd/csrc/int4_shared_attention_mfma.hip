@@ -766,7 +766,7 @@ int launch_shared_fast(SharedParams p, hipStream_t st) {
   p.own_waves = pb + units <= resident_workgroups() ? 4 : tiles <= 2 ? 1 : tiles <= 8 ? 2 : 4;
   const int64_t ob = (units * p.own_waves + WAVES - 1) / WAVES;
   p.own_units = (uint32_t)units;
-  if (pb + units >= (int64_t)1 << 31) {
+  if ((pb + ob) * THREADS >= (int64_t)1 << 32) {  // threads of a launch
     return fail(LQ_ERR_UNSUPPORTED, "%lld workgroups exceed the launch limits", (long long)(pb + ob));
   }
   p.prefix_blocks = (uint32_t)pb;

@@ -83,6 +83,15 @@ def test_reorder_refuses():
     assert reorder([fake((8,), U8, data=0x10000 + 64 * i) for i in range(513)], b) == -2
 
 
+def test_reorder_refuses_its_beams():
+    """Entries that a workgroup reads while another moves them: the tensor itself and any overlap."""
+    b = fake((2, 4), I64, data=0x20000)
+    for data in (0x20000, 0x20000 - 8 * 15, 0x20000 + 63):
+        assert reorder([fake((8, 16), U8, data=data)], b) == -1
+        assert "overlaps the beams" in _abi.last_error()
+    assert reorder([fake((8,), I64, data=0x20000)], fake((2, 4), I64, (1, 2), data=0x20000)) == -1
+
+
 def shared(B=6, P=2, hq=8, hkv=2, d=128, g=32, cap=100, ocap=20, lp=50, S=60, nrep=4, mask=None,
            token=True, ws=0x10000, wsb=1 << 40, **over):
     new = fake((B, hkv, 1, d), BF16) if token else None
