@@ -27,8 +27,9 @@
 // the rate that lq_int4_decode_attention reaches on that volume (one member per prompt 35 us; its 6.5 TB/s
 // come with the eightfold volume), behind the set-up (4 us: query rows, first tiles), the partials of 2048
 // (row, head)s in 8 splits (9 MB) and the own units, which start as the prefix's workgroups end (6 us). 64
-// members of one prompt (group 128, fp16, ctx 8192: 256 query rows per KV head, 37.4 us) are bound by the
-// VALU: every row block of 32 decodes the same tiles again. A few members at a short prompt (1 x 4, ctx 777:
+// members of one prompt (group 128, fp16, ctx 8192: 256 query rows per KV head, 34.8 us) take 400 VALU
+// instructions and 48 MFMAs per tile and 32 rows, as every row block decodes the same tiles again: half of
+// the time is their issue, the rest the set-up, the join and waits that two waves per SIMD leave open. A few members at a short prompt (1 x 4, ctx 777:
 // 7.6 us) are one tile per wave: latency of the loads, set-up and join.
 //
 // Why 32 rows and not more per wave: the accumulators (64 registers), the query operands (32) and a tile's
@@ -741,11 +742,17 @@ SharedPlan plan_shared_fast(int64_t P, int64_t N, int64_t Hkv, int64_t nrep, int
   const int64_t units = std::max<int64_t>(1, P * Hkv * ((rows + block - 1) / block));
   const int64_t own_units = std::max<int64_t>(1, P * N * Hkv * ((nrep + 15) / 16));
   constexpr int64_t STEP = WAVES * TILE;
-  SharedPlan plan{split_of(prefix_len, resident / units, STEP),
+  // One prefix workgroup per CU leaves the other place to the own units and halves the set-ups and partials;
+  // two hide each other's waits. The first pays up to about 12 tiles per wave (9 with 16 query rows) and one
+  // more for each of the first 6 own tiles. Measured with one and with two, group 32: 60 own rows, 1 prompt
+  // x 16, 4 tiles 22.3 us for 26.3, 8 x 8, 10 tiles 30.1 for 33.7, 14 tiles 36.5 for 37.4, 18 tiles 43.0 for
+  // 41.2; 200 own rows, 8 x 8, 18 tiles 43.4 for 44.2, 24 tiles 52.9 for 50.2; 4 x 4 (16 query rows), 60
+  // own rows, 10 tiles 22.9 for 25.5, 14 tiles 27.9 for 28.4, 16 tiles 30.4 for 29.8.
+  const int64_t own_tiles = std::min<int64_t>(6, (own_len + TILE - 1) / TILE);
+  SharedPlan plan{split_of(prefix_len, device_cus() / units, STEP),
                   split_of(own_len, resident / own_units, 2 * STEP)};
-  // a wave of one tile spends its time in set-up and merging: two where that leaves a workgroup per CU
-  if (plan.prefix.chunk == STEP && units * ((prefix_len + 2 * STEP - 1) / (2 * STEP)) >= device_cus()) {
-    plan.prefix = split_of(prefix_len, resident / units, 2 * STEP);
+  if (plan.prefix.chunk > ((block == 16 ? 9 : 12) + own_tiles) * STEP) {
+    plan.prefix = split_of(prefix_len, resident / units, STEP);
   }
   return plan;
 }
