@@ -176,6 +176,22 @@ def test_many_own_rows(gpu, lo, masked):
     run(gpu, P, N, hkv, nrep, lp, lo, 128, g, BF16, lo, mask)
 
 
+@pytest.mark.parametrize("mask", ["none", "keep", "bias"])
+@pytest.mark.parametrize("nrep,lp", [(1, 4300), (17, 2300), (17, 2047)])
+def test_long_units(gpu, nrep, lp, mask):
+    """More prefix units than places: every wave takes 16 to 34 tiles, masks among them in stretches."""
+    P, N, hkv, lo, g = 8, 1, 64, 40, 64
+    gen = torch.Generator(device=gpu).manual_seed(lp)
+    keep = (torch.rand(P * N, lp + lo, device=gpu, generator=gen) < 0.7).long()
+    keep[1, 100:2000] = 0
+    keep[2, :lp] = 0
+    m = {"none": None, "keep": keep}.get(mask)
+    if mask == "bias":
+        m = torch.where(keep != 0, torch.randn(keep.shape, device=gpu, generator=gen), -torch.inf)
+        m = m[:, None, None, :]
+    run(gpu, P, N, hkv, nrep, lp, lo, 128, g, BF16, lp, m)
+
+
 @pytest.mark.parametrize("d,g,dtype", [(64, 32, BF16), (128, 32, FP32), (128, 16, BF16), (96, 96, FP16),
                                        (512, 64, BF16), (80, 2, FP32)])
 def test_general_kernel(gpu, d, g, dtype):
