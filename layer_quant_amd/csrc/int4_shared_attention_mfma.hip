@@ -8,18 +8,18 @@
 // At the end the 4 partial softmax states are joined through LDS, and the split's (m, l, acc) goes to
 // the workspace (or, where it is the only split, out).
 //
-// Products use v_mfma_f32_16x16x32_f16, D[16x16] += A[16x32] * B[32x16] (lane l holds A row l%16 and B
-// column l%16, each with K slots 8*(l/16) .. +7, and D rows 4*(l/16) .. +3 of column l%16):
+// Products use v_mfma_f32_16x16x32_f16 and _bf16, D[16x16] += A[16x32] * B[32x16] (lane l holds A row l%16
+// and B column l%16, each with K slots 8*(l/16) .. +7, and D rows 4*(l/16) .. +3 of column l%16):
 //   S^T[key][query] per group m: A = K rows as exact fp16 integers, B = Q^T scaled by a power of two
 //     per query row so that its largest value lies in [2^14, 2^15) (16-bit queries are then exact in
 //     fp16, products exact, sums fp32); the groups' partial sums are scaled by the fp32 key scales and
 //     added in fp32.
-//   O^T[dim][query]: A = V^T as exact fp16 integers, B = P'_m[key][query] = 2^(s - M) * vscale[key][m],
-//     formed in fp32 and rounded to fp16 (bf16 outputs; relative 2^-11, less than the output's own
-//     rounding of 2^-8) or split into fp16 hi + lo (other outputs; about 22 bits).
-// M is the lazily moved running maximum of the row's scores plus an offset of the wave that follows the
-// largest value scale seen, so that P' stays below 2^15 and is exact to 2^-24 of 2^7 at the largest
-// score and scale: fp16 has no exponent range to spare for both.
+//   O^T[dim][query]: A = V^T as exact bf16 values n / 16, B = P'_m[key][query] = 2^(s - M) * vscale[key][m],
+//     M the lazily moved running maximum of the row's scores. P' is formed in fp32 and split into bf16
+//     terms, each the rounding of what the terms before it leave: two for bf16 outputs (off by 2^-16
+//     relative at most, 2^-8 of the output's own rounding), three for others (all 24 bits). A term has
+//     the exponent range of fp32, so that a key's share keeps its precision whatever the other keys'
+//     scales and weights are.
 //
 // What bounds it (MI355X, kernel trace, group 32 unless said): 8 prompts x 8 members at ctx 16384 take 55.7
 // us, 174 MB of which 168 are the prompts' rows. With the products left out the kernel takes as long, with
@@ -45,6 +45,9 @@
 namespace lq {
 namespace {
 
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
 constexpr int SD = 128;     // head_dim
 constexpr int TILE = 32;    // keys per wave step
 constexpr int WAVES = 4;
@@ -52,7 +55,6 @@ constexpr int THREADS = 64 * WAVES;
 constexpr int SEG = 16;     // tiles of a wave whose keep-mask words are made together
 constexpr int OROW = SD + 4;  // floats per row of a wave's partial output (rows 4 banks apart)
 constexpr float LAZY = 8.0f;  // running-max slack of the lazy rescale
-constexpr int P_TOP = 7;      // P' of the largest score and value scale is about 2^P_TOP
 
 enum { MASK_NONE = 0, MASK_BIAS = 1, MASK_KEEP = 2 };
 
@@ -144,15 +146,6 @@ __device__ __forceinline__ void read_scales(const float* s, int q4, float (&out)
   }
 }
 
-// Power of two at or above v as its exponent, kept between -60 and MAX_E: weights 2^(s - M) of 2^(8 - e)
-// at most still add up below 2^127, and those of 2^-e are normal 2^-20 times over.
-constexpr int MAX_E = 100;
-__device__ __forceinline__ int exponent_above(float v) {
-  const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
-  const int e = (int)(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0 ? 1 : 0);
-  return min(max(e, -60), MAX_E);
-}
-
 // A query row's 32 values of this lane (two per word) as fp16 operands q * 2^-e, 2^e being `scale`, e such
 // that the row's largest value lies in [2^14, 2^15); zeros where the row is none.
 template <int DT>
@@ -183,13 +176,35 @@ __device__ __forceinline__ void scale_query(const uint32_t (&w)[4][4], bool ok, 
   }
 }
 
-// The products a0 b0 and a1 b1 as an fp16 pair, each rounded once (v_fma_mixlo/mixhi_f16; as two multiplies
-// and a conversion the pair takes three instructions).
-__device__ __forceinline__ f16x2_t mul_f16(float a0, float b0, float a1, float b1) {
-  return f16x2_t{(_Float16)__builtin_fmaf(a0, b0, 0.0f), (_Float16)__builtin_fmaf(a1, b1, 0.0f)};
+// Two value nibbles (bits 3:0 and 19:16 of x) as a bf16 pair n / 16 (exact).
+__device__ __forceinline__ uint32_t nib_pair_16th(uint32_t x) {
+  const float a = __builtin_amdgcn_cvt_off_f32_i4((int)x);
+  const float b = __builtin_amdgcn_cvt_off_f32_i4((int)(x >> 16));
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
-template <int QT, int G, int MASK, bool EXACT>
+__device__ __forceinline__ f32x4_t mfma_bf16(u32x4_t a, u32x4_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// a and b as TERMS bf16 pairs t[0] + t[1] + ..: each rounds what is left (to nearest), which the next
+// subtraction gives exactly. The subtraction a - t.lo * 1 - t.hi * 0 is one v_dot2_f32_bf16, with the
+// multipliers (-1, 0) in a register: as an inline constant, -1.0 stands for another pair in this instruction.
+template <int TERMS>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t minus_lo, uint32_t (&t)[TERMS]) {
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    const bf16x2_t r = __builtin_convertvector(f32x2_t{a, b}, bf16x2_t);
+    t[i] = __builtin_bit_cast(uint32_t, r);
+    if (i + 1 < TERMS) {
+      a = __builtin_amdgcn_fdot2_f32_bf16(r, __builtin_bit_cast(bf16x2_t, minus_lo), a, false);
+      b = __builtin_amdgcn_fdot2_f32_bf16(r, __builtin_bit_cast(bf16x2_t, 0xbf800000u), b, false);
+    }
+  }
+}
+
+template <int QT, int G, int MASK, int TERMS>
 __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, SharedTile* ring,
                                          MaskWords* words, WavePartial<QT>* part) {
   constexpr int CPG = 4 / G;  // 32-dim chunks per group
@@ -260,8 +275,8 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[qt][k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  int voff = -1000;        // scales up to 2^(voff + P_TOP) are in range (uniform)
-  float vlim = -1.0f;      // that limit: a larger one moves voff
+  uint32_t minus_lo = 0x0000bf80u;  // bf16 (-1, 0)
+  asm("" : "+s"(minus_lo));
 
   // Keep-mask: the wave turns the next SEG tiles' rows of the mask into one word of 32 keys per member
   // of its row block, lanes 0..31 for one member and 32..63 for the next.
@@ -400,8 +415,10 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
         for (int j = 0; j < 4; ++j) {
           const uint32_t a0 = vrow[64 * (2 * j) + 4 * k], a1 = vrow[64 * (2 * j + 1) + 4 * k];
           const uint32_t y = __builtin_amdgcn_perm(a1, a0, vsel);
-          va[k][0][j] = nib_pair_f16(y);
-          va[k][1][j] = nib_pair_f16(y >> 4);
+          uint32_t high = y >> 4;
+          asm("" : "+v"(high));  // (one shift for both of its nibbles: their word is an operand select)
+          va[k][0][j] = nib_pair_16th(y);
+          va[k][1][j] = nib_pair_16th(high);
         }
       }
     }
@@ -453,36 +470,7 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
       }
     }
 
-    // ---- running references: the value scales' exponent of the wave, each row's maximum
-    float vmax;
-    if constexpr (MASK == MASK_NONE) {  // each lane its part of the tile's 32 G scales
-      vmax = B.vs[lane & (32 * G - 1)];
-      if constexpr (G == 4) vmax = fmaxf(vmax, B.vs[64 + lane]);
-    } else {
-      vmax = vs[0][0];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-#pragma unroll
-        for (int m = 0; m < G; ++m) vmax = fmaxf(vmax, vs[e][m]);
-      }
-    }
-    if (__any(vmax > vlim)) {
-      vmax = group_max<64>(vmax);
-      const int e = __builtin_amdgcn_readfirstlane(exponent_above(vmax));
-      const int next = max(voff, e - P_TOP);
-      if (voff > -1000 && next > voff) {
-        const float alpha = __builtin_amdgcn_exp2f((float)(voff - next));
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) acc[qt][k] *= alpha;
-          l_run[qt] *= alpha;
-        }
-      }
-      voff = next;
-      vlim = e >= MAX_E ? INFINITY : __uint_as_float((uint32_t)(127 + voff + P_TOP) << 23);
-    }
-    const float fvoff = (float)voff;
+    // ---- weights, below a running maximum of each row's scores
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       float lm = s[qt][0];
@@ -506,9 +494,9 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (MASK == MASK_BIAS) {
-          s[qt][e] = __builtin_amdgcn_exp2f((s[qt][e] - m_use) - fvoff);
+          s[qt][e] = __builtin_amdgcn_exp2f(s[qt][e] - m_use);
         } else {
-          s[qt][e] = __builtin_amdgcn_exp2f(fmaf(s[qt][e], cs[qt], -(m_use + fvoff)));
+          s[qt][e] = __builtin_amdgcn_exp2f(fmaf(s[qt][e], cs[qt], -m_use));
         }
         psum += s[qt][e];
       }
@@ -519,28 +507,27 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int m = 0; m < G; ++m) {
-      u32x4_t hi[QT], lo[QT];
+      u32x4_t pt[TERMS][QT];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const f16x2_t h = mul_f16(s[qt][2 * j], vs[2 * j][m], s[qt][2 * j + 1], vs[2 * j + 1][m]);
-          hi[qt][j] = __builtin_bit_cast(uint32_t, h);
-          if constexpr (EXACT) {
-            lo[qt][j] = pack_f16(fmaf(s[qt][2 * j], vs[2 * j][m], -(float)h[0]),
-                                 fmaf(s[qt][2 * j + 1], vs[2 * j + 1][m], -(float)h[1]));
-          }
+          uint32_t t[TERMS];
+          split_pair<TERMS>(s[qt][2 * j] * vs[2 * j][m], s[qt][2 * j + 1] * vs[2 * j + 1][m], minus_lo, t);
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) pt[i][qt][j] = t[i];
         }
       }
 #pragma unroll
       for (int k = m * CPG; k < (m + 1) * CPG; ++k) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < TERMS; ++i) {
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) acc[qt][2 * k + t] = mfma_f16(va[k][t], hi[qt], acc[qt][2 * k + t]);
-          if constexpr (EXACT) {
+          for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) acc[qt][2 * k + t] = mfma_f16(va[k][t], lo[qt], acc[qt][2 * k + t]);
+            for (int qt = 0; qt < QT; ++qt) {
+              acc[qt][2 * k + t] = mfma_bf16(va[k][t], pt[i][qt], acc[qt][2 * k + t]);
+            }
           }
         }
       }
@@ -559,7 +546,6 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     slot = slot == 2 ? 0 : slot + 1;
   }
 
-  const float vscale = voff > -1000 ? __builtin_amdgcn_exp2f((float)voff) : 0.0f;
   const int ns = p.nsp + p.nso;
   // ---- the waves' states to LDS (over the tiles, which every wave has read), joined there
   __syncthreads();
@@ -572,12 +558,12 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
     const int row = 16 * qt + c16;
     if (q4 == 0) {
       mine.m[row] = m_run[qt];
-      mine.l[row] = l * vscale;
+      mine.l[row] = l;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {  // dims 32k + 8 q4 + 2r + t
       float* o = &mine.o[row][32 * k + 8 * q4];
-      const f32x4_t a = acc[qt][2 * k] * vscale, b = acc[qt][2 * k + 1] * vscale;
+      const f32x4_t a = acc[qt][2 * k] * 16.0f, b = acc[qt][2 * k + 1] * 16.0f;
       *(f32x4_t*)o = f32x4_t{a[0], b[0], a[1], b[1]};
       *(f32x4_t*)(o + 4) = f32x4_t{a[2], b[2], a[3], b[3]};
     }
@@ -618,7 +604,7 @@ __device__ __forceinline__ void run_unit(const SharedParams& p, const Unit& u, S
 
 // Workgroups: the prefix units first, the longer ones (KV head fastest, so that the row blocks that share
 // keys lie on the same XCD where there are 8 KV heads; then row block, split, prompt), then the own units.
-template <int QT, int G, int MASK, bool EXACT>
+template <int QT, int G, int MASK, int TERMS>
 __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p) {
   __shared__ SharedLds<QT> lds;
   __shared__ MaskWords words[MASK == MASK_KEEP ? WAVES : 1];
@@ -644,7 +630,7 @@ __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p)
     u.b0 = (int64_t)prompt * p.N;
     u.pack = false;
     u.waves = WAVES;
-    run_unit<QT, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, lds.part);
+    run_unit<QT, G, MASK, TERMS>(p, u, &lds.tiles[0][0], mine, lds.part);
     return;
   }
   // (a wave without a unit takes the last one's place with no query rows)
@@ -674,23 +660,23 @@ __global__ __launch_bounds__(THREADS, 2) void shared_mfma_kernel(SharedParams p)
     u.row0 = u.rows;
     u.pack = false;
   }
-  run_unit<1, G, MASK, EXACT>(p, u, &lds.tiles[0][0], mine, (WavePartial<1>*)lds.part);
+  run_unit<1, G, MASK, TERMS>(p, u, &lds.tiles[0][0], mine, (WavePartial<1>*)lds.part);
 }
 
 template <int QT, int G, int MASK>
-void launch_exact(const SharedParams& p, dim3 grid, hipStream_t st) {
+void launch_terms(const SharedParams& p, dim3 grid, hipStream_t st) {
   if (p.out.dtype == LQ_BF16) {
-    hipLaunchKernelGGL((shared_mfma_kernel<QT, G, MASK, false>), grid, dim3(THREADS), 0, st, p);
+    hipLaunchKernelGGL((shared_mfma_kernel<QT, G, MASK, 2>), grid, dim3(THREADS), 0, st, p);
   } else {
-    hipLaunchKernelGGL((shared_mfma_kernel<QT, G, MASK, true>), grid, dim3(THREADS), 0, st, p);
+    hipLaunchKernelGGL((shared_mfma_kernel<QT, G, MASK, 3>), grid, dim3(THREADS), 0, st, p);
   }
 }
 
 template <int QT, int G>
 void launch_mask(const SharedParams& p, dim3 grid, hipStream_t st) {
-  if (p.mask == nullptr) launch_exact<QT, G, MASK_NONE>(p, grid, st);
-  else if (p.mask_keep) launch_exact<QT, G, MASK_KEEP>(p, grid, st);
-  else launch_exact<QT, G, MASK_BIAS>(p, grid, st);
+  if (p.mask == nullptr) launch_terms<QT, G, MASK_NONE>(p, grid, st);
+  else if (p.mask_keep) launch_terms<QT, G, MASK_KEEP>(p, grid, st);
+  else launch_terms<QT, G, MASK_BIAS>(p, grid, st);
 }
 
 template <int G>
