@@ -112,21 +112,28 @@ def share_prompt(model, cache_params, num_beams: int) -> None:
                                        layer.k_scale.shape[-1], layer.k_packed.device)
         own.prefix = layer
         caches[layer_idx] = own
-    registry = _mx_registry(model)
-    renewed = {}
+    module = __import__(model.__class__.__module__, fromlist=["selective_state_update"])
+    registries = [_mx_registry(model)]
+    held_by_module = getattr(module, "_mamba_decode_state_kernel_caches", None)
+    if held_by_module is not None and held_by_module is not registries[0]:
+        registries.append(held_by_module)
     for held, i in _float_states(cache_params):
         old = held[i]
         held[i] = old.repeat_interleave(num_beams, dim=0)
-        mx = registry.get(id(old))
-        if mx is not None:
-            renewed[id(held[i])] = replace(
-                mx, q_state=mx.q_state.repeat_interleave(num_beams, dim=0),
-                shared_exp=mx.shared_exp.repeat_interleave(num_beams, dim=0),
-                micro_exp=mx.micro_exp.repeat_interleave(num_beams, dim=0))
-    if registry:
-        model._mamba_decode_state_kernel_caches = renewed
-        module = __import__(model.__class__.__module__, fromlist=["selective_state_update"])
-        module._mamba_decode_state_kernel_caches = dict(renewed)
+        # this state's entries alone: other hybrid caches stay registered (an entry under the new
+        # tensor's id can only be that of a state that is gone)
+        renewed = {}
+        for entries in registries:
+            mx = entries.pop(id(old), None)
+            entries.pop(id(held[i]), None)
+            if mx is None:
+                continue
+            if id(mx) not in renewed:
+                renewed[id(mx)] = replace(
+                    mx, q_state=mx.q_state.repeat_interleave(num_beams, dim=0),
+                    shared_exp=mx.shared_exp.repeat_interleave(num_beams, dim=0),
+                    micro_exp=mx.micro_exp.repeat_interleave(num_beams, dim=0))
+            entries[id(held[i])] = renewed[id(mx)]
 
 
 def reorder_states(model, cache_params, beams: torch.Tensor) -> None:
