@@ -159,11 +159,14 @@ def beam_search(model, logits: torch.Tensor, cache_params, num_beams: int, max_n
     scores [P, N] fp32), the beams of a prompt in descending order of their summed log-probabilities.
 
     logits [P, V] are the prompts' last ones and cache_params their hybrid cache, `start` the
-    position of the first new token, attention_mask the prompts' 2-D keep-mask, if any. A beam that
-    has chosen eos_token_id goes on with pad_token at its score.
+    position of the first new token (right behind the INT4 caches' rows), attention_mask the prompts'
+    2-D keep-mask, if any. A beam that has chosen eos_token_id goes on with pad_token at its score.
     """
     if max_new_tokens < 1:
         raise ValueError(f"max_new_tokens must be >= 1, got {max_new_tokens}")
+    for layer_idx, layer in ia._cache_dict(cache_params).items():
+        if layer.length != start:
+            raise ValueError(f"start={start} is not behind the {layer.length} rows of layer {layer_idx}")
     prompts = logits.shape[0]
     device = logits.device
     scores, _, tokens = beam_select(logits[:, None], torch.zeros(prompts, 1, device=device),

@@ -325,6 +325,9 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
     if shared_len and (q_len != 1 or required_len <= shared_len):
         raise ValueError(f"a cache behind {shared_len} shared rows takes one later token at a time, "
                          f"got {q_len} up to position {required_len - 1}")
+    if shared_len and required_len - 1 > shared_len + current.length:
+        raise ValueError(f"position {required_len - 1} leaves unwritten rows behind the "
+                         f"{shared_len + current.length} of the cache")
     layer_cache = _ensure_layer_cache(past_key_value, self.layer_idx, bsz,
                                       self.num_key_value_heads, required_len - shared_len,
                                       self.head_dim, group_size, hidden_states.device)

@@ -85,3 +85,30 @@ def test_share_prompt_drops_entries_of_freed_states(model):
         bd.share_prompt(model, b, 2)
     for registry in (model._mamba_decode_state_kernel_caches, fk._mamba_decode_state_kernel_caches):
         assert not any(id(s) in registry for s in b.ssm_states)
+
+
+def int4_layer(batch, length):
+    layer = ia._allocate_layer_cache(batch, 1, 16, 128, 2, torch.device("cpu"))
+    layer.length = length
+    return layer
+
+
+@pytest.mark.parametrize("start", [0, 8, 10, 11])
+def test_beam_search_refuses_a_start_off_its_caches(model, start):
+    """The first new token stands right behind the prompts' rows: rows in between would be attended
+    without having been written."""
+    cache = hybrid(model, 2)
+    ia._cache_dict(cache).update({1: int4_layer(2, 9), 4: int4_layer(2, 9)})
+    before = list(cache.ssm_states)
+    with pytest.raises(ValueError, match="start"):
+        bd.beam_search(model, torch.zeros(2, 64), cache, 4, 3, start=start)
+    assert all(a is b for a, b in zip(cache.ssm_states, before))
+    assert all(layer.prefix is None for layer in ia._cache_dict(cache).values())
+
+
+def test_beam_search_refuses_caches_of_different_lengths(model):
+    cache = hybrid(model, 2)
+    ia._cache_dict(cache).update({1: int4_layer(2, 9), 4: int4_layer(2, 8)})
+    for start in (8, 9):
+        with pytest.raises(ValueError, match="start"):
+            bd.beam_search(model, torch.zeros(2, 64), cache, 4, 3, start=start)
