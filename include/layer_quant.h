@@ -348,14 +348,15 @@ int lq_beam_select(const lq_tensor* logits, const lq_tensor* scores, const lq_te
 
 /*
  * The states of P prompts x N beams follow the selected beams, in place: for each of `count` tensors
- * (an array of descriptors, any dtype, 1 to 4 dims, P * N rows, any strides without a broadcast
- * dimension) row p*N + n takes the contents that row p*N + beams[p][n] had before the call. Rows with
- * beams[p][n] == n stay as they are, and so do rows whose entry is outside [0, N).
+ * (an array of descriptors, any dtype, 1 to 4 dims, P * N rows, any strides of which each, by size,
+ * reaches past the extent of the smaller ones: no two elements share memory) row p*N + n takes the
+ * contents that row p*N + beams[p][n] had before the call. Rows with beams[p][n] == n stay as they are,
+ * and so do rows whose entry is outside [0, N).
  *   rows   NULL, or for each tensor how many entries of dim 2 are moved (the live rows of a cache
  *          [B, Hkv, cap, .]; what lies behind them stays), -1 for the whole tensor
  *   beams  [P, N] i64
- * The tensors must not overlap (one listed twice, or over the beams, is refused). One launch for up to 256 tensors of up
- * to 16 row shapes. No counterpart in the reference.
+ * The tensors must not overlap (one listed twice, over itself or over the beams is refused). One launch
+ * for up to 256 tensors of up to 16 row shapes. No counterpart in the reference.
  */
 #define LQ_REORDER_MAX_BEAMS 64
 #define LQ_REORDER_MAX_TENSORS 512

@@ -68,8 +68,9 @@ def reorder_beams(tensors, beams: torch.Tensor, rows=None) -> None:
     p*N + beams[p, n] had before the call. Entries outside [0, N) leave their row as it is.
 
     beams int64 [P, N] (N <= 64); the tensors of any dtype the ABI knows and any strides, up to 512,
-    none overlapping another or the beams. rows[i]: how many entries of dim 2 of tensor i are moved (the live rows
-    of an INT4 cache), None for all. One launch for a model's states, in any permutation.
+    none overlapping itself, another or the beams. rows[i]: how many entries of dim 2 of tensor i are
+    moved (the live rows of an INT4 cache), None for all. One launch for a model's states, in any
+    permutation.
     """
     if rows is not None and len(rows) != len(tensors):
         raise ValueError(f"{len(rows)} row counts for {len(tensors)} tensors")
