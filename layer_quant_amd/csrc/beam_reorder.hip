@@ -273,6 +273,10 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
     Item it{};
     if ((rc = row_shape(t, live, per_block, it)) != LQ_OK) return rc;
     if (it.shape.total == 0) continue;
+    // before anything is moved: a call that fails leaves every tensor as it was
+    if (N > 1 && (int64_t)it.shape.blocks * P > MAX_BLOCKS) {
+      return fail(LQ_ERR_UNSUPPORTED, "tensor %d: %lld prompts exceed the launch limits", i, (long long)P);
+    }
     it.span = span_bytes(t);
     items[used++] = it;
   }
@@ -320,9 +324,6 @@ extern "C" int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, i
       }
       if (!done[i]) break;
       p.shapes[p.nshapes++] = sh;
-    }
-    if (blocks == 0) {
-      return fail(LQ_ERR_UNSUPPORTED, "%lld prompts exceed the launch limits", (long long)P);
     }
     if ((rc = launch(p, nmax, blocks, st)) != LQ_OK) return rc;
   }

@@ -26,3 +26,15 @@ def test_elements_that_overlap(shape, stride):
 def test_any_order_without_an_overlap(shape, stride):
     """Rows innermost, gaps, extents of one: passed on (one beam per prompt, so nothing is launched)."""
     assert reorder([fake(shape, U8, stride, data=0x900000)], fake((8, 1), I64)) == 0
+
+
+def test_launch_limits_before_the_first_launch():
+    """A tensor that no launch takes is refused before any other is moved, wherever it stands in the list."""
+    P = 1 << 20
+    b = fake((P, 2), I64)
+    small = fake((2 * P, 16), U8, data=0x10000000)
+    wide = fake((2 * P, 140000), U8, data=0x1000000000)  # 18 workgroups of 8 KiB for each of 2^20 prompts
+    for tensors in ([wide], [small, wide], [wide, small]):
+        assert reorder(tensors, b) == -2
+        assert "launch limits" in _abi.last_error()
+    assert reorder([fake((2 * P, 140000), U8, data=0x1000000000)], fake((2 * P, 1), I64)) == 0  # nothing moves
