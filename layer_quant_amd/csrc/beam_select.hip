@@ -484,9 +484,13 @@ __device__ __forceinline__ void take_candidates(const Candidate (&c)[4], const b
   int need = k;
   narrow<4>(v, take, need);
   if (need == 0) return;
-  // (the low words are compared above 0: their lowest bit is set aside and does not decide)
+  // (words are compared above 0: the other 32 bits go in two steps, 31 of them and the last)
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = v[e] != 0 ? (uint32_t)order_bits64(c[e].total) | 1u : 0;
+  for (int e = 0; e < 4; ++e) v[e] = v[e] != 0 ? (uint32_t)order_bits64(c[e].total) >> 1 | 0x80000000u : 0;
+  narrow<4>(v, take, need);
+  if (need == 0) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = v[e] != 0 ? ((uint32_t)order_bits64(c[e].total) & 1u) + 1 : 0;
   narrow<4>(v, take, need);
   if (need == 0) return;
 #pragma unroll
