@@ -612,13 +612,13 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
     c.index = n * V + (0xffffffffu - (uint32_t)key);
     return c.total >= bound;
   };
-  // the i-th candidate of a beam without logits: a finished beam's own score at the pad token, then the
-  // lowest tokens at -inf
+  // the i-th candidate of a beam without logits: a finished beam's own score, where it has one, at the pad
+  // token, then the lowest tokens at -inf
   auto apart_candidate = [&](uint32_t n, uint32_t i, Candidate& c) -> bool {
     if (i >= (uint32_t)k || i >= V) return false;
     uint32_t token = i;
     c.total = -INFINITY;
-    if (alone[n]) {
+    if (alone[n] && base[n] != -INFINITY) {
       token = i == 0 ? (uint32_t)p.pad : (i <= (uint32_t)p.pad ? i - 1 : i);
       if (i == 0) c.total = base[n];
     }
