@@ -323,11 +323,12 @@ int lq_int4_shared_decode_attention(
 /*
  * Beam selection: for each of P prompts the `num` best continuations of its N beams, num the extent
  * of the outputs' second dim. The total of beam n and token t is scores[n] + logits[n][t] - lse[n],
- * lse[n] the log-sum-exp of the beam's logits; totals are compared in 64 bits, equal ones by the
- * lower n * V + t. A finished beam has one continuation, pad_token at its own score, and its logits
- * are not read. Continuations of a beam whose score or log-sum-exp is not finite (a NaN or +inf
- * logit, no logit above -inf) count as -inf, and so do the other tokens of a finished beam. (Logits
- * beyond 2^127 in magnitude count as infinite.)
+ * lse[n] the log-sum-exp of the beam's logits, off by less than 2^-18 (fp32 sums, the same error for
+ * all of a beam's tokens); totals are compared in 64 bits, equal ones by the lower n * V + t. A finished
+ * beam has one continuation, pad_token at its own score, and its logits are not read. Continuations of
+ * a beam whose score or log-sum-exp is not finite (a NaN or +inf logit, no logit above -inf) count as
+ * -inf, and so do the other tokens of a finished beam. (Logits beyond 2^127 in magnitude count as
+ * infinite.)
  *   logits    [P, N, V] or [P * N, V]  f32/f16/bf16, any strides
  *   scores    [P, N]     f32
  *   finished  NULL or [P, N] u8 (0: not finished)

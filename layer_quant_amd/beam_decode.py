@@ -29,10 +29,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: int | None = No
     beams [P, num] int64, tokens [P, num] int64).
 
     logits [P*N, V] or [P, N, V] in fp32, fp16 or bf16, any strides; scores [P, N] fp32, the beams'
-    running scores. The total of beam n and token t is scores[n] + log_softmax(logits[n])[t]; totals
-    are compared in 64 bits, equal ones by the lower n * V + t. `finished` (bool [P, N]): such a beam
-    has one continuation, pad_token at its own score. Continuations of a beam whose score or
-    log-sum-exp is not finite count as -inf.
+    running scores. The total of beam n and token t is scores[n] + log_softmax(logits[n])[t], its
+    log-sum-exp off by less than 2^-18 (fp32 sums); totals are compared in 64 bits, equal ones by the
+    lower n * V + t. `finished` (bool [P, N]): such a beam has one continuation, pad_token at its own
+    score. Continuations of a beam whose score or log-sum-exp is not finite count as -inf.
 
     In descending order, or with keep_slots (num == N) by place: the best continuation selected of a
     beam stands at that beam's place, the others at the free places in order, so that reorder_beams

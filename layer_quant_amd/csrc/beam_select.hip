@@ -13,10 +13,16 @@
 // overflow (many equal logits, sorted ones) are cut on the way, which raises the threshold. The part
 // leaves (max, sum), its num largest logits and a bound that they all reach.
 //
-// select_final_kernel: one workgroup per prompt makes lse[n] and the totals in 64 bits (their order then
-// goes wrong only where totals are closer than the sums' rounding, about 1e-7). num candidates reach
-// the largest of the parts' bounds; those that do (a few hundred) are reduced, wave by wave, to
+// select_final_kernel: one workgroup per prompt makes lse[n] and the totals in 64 bits. num candidates
+// reach the largest of the parts' bounds; those that do (a few hundred) are reduced, wave by wave, to
 // the num best, which one wave sorts and writes out, by rank or by place.
+//
+// The sums of exponentials are fp32 and off by less than 2^-18, which is their logarithms' error: at most
+// 24 additions in a row (lane 8, wave 6, workgroup 3, parts 7), 7 exponentials (the term's own and its
+// rescales, one step of fp32 each) and their 6 products, 2^-24 each, and the roundings of the exponents,
+// 2^-24 of the distance to the maximum, which weighted with the terms is 17 * 2^-24 at 2^24 tokens.
+// A whole beam has its lse's error, so that totals of one beam keep their order; those of two beams can
+// change places where they are closer than that.
 //
 // What it measured (MI355X, kernel trace, parts + final): 256 rows of 131072 bf16 logits (67 MB), 32 of
 // each of 16 prompts, 19.2 + 10.4 us; 64 rows, 8 of each of 8 prompts, 9.8 + 6.6; 15 rows of 50257 fp32
@@ -320,8 +326,10 @@ __global__ __launch_bounds__(THREADS) void select_part_kernel(SelectParams p) {
     const float c2 = fmaxf(c, run_max[r] * LOG2E_F);
     if (r > 0) sl *= __builtin_amdgcn_exp2f(c - c2);
     c = c2;
+    float four[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (short chains of additions)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sl += __builtin_amdgcn_exp2f(fmaf(x[r][i], LOG2E_F, -c));
+    for (int i = 0; i < PER; ++i) four[i % 4] += __builtin_amdgcn_exp2f(fmaf(x[r][i], LOG2E_F, -c));
+    sl += (four[0] + four[1]) + (four[2] + four[3]);
     // the logits stay as they were loaded: unpacked for the second pass too, they took twice the registers
 #pragma unroll
     for (int u = 0; u < Raw<DT>::WORDS; ++u) asm volatile("" : "+v"(x[r].w[u]));
@@ -548,18 +556,21 @@ __global__ __launch_bounds__(64 * FW) void select_final_kernel(SelectParams p) {
     const bool fin = p.finished != nullptr && p.finished[prompt * p.fs[0] + n * p.fs[1]] != 0;
     double b = score;
     if (!fin) {
-      // each lane's parts with a running maximum, then the lanes
-      float m = r.m, s = r.s;
+      // the largest of the parts' maxima, then their sums
+      float m = r.m;
       uint32_t share = r.share;
       for (int i = lane + 64; i < p.parts; i += 64) {
-        r = parts[n * p.parts + i];
-        share = min(share, r.share);
-        const float m2 = fmaxf(m, r.m);
-        s = s * exp2f(m - m2) + r.s * exp2f(r.m - m2);
-        m = m2;
+        const PartResult& q = parts[n * p.parts + i];
+        share = min(share, q.share);
+        m = fmaxf(m, q.m);
       }
       const float M = group_max<64>(m);
-      s = group_sum<64>(s * exp2f(m - M));
+      double of_lane = r.s * exp2f(r.m - M);
+      for (int i = lane + 64; i < p.parts; i += 64) {
+        const PartResult& q = parts[n * p.parts + i];
+        of_lane += q.s * exp2f(q.m - M);
+      }
+      const float s = group_sum<64>((float)of_lane);
       share = wave_fold(share, [](uint32_t a, uint32_t b) { return min(a, b); });
       if (lane == 0) shares[n] = share;
       b = (double)score - ((double)M + log2((double)s)) / (double)LOG2E_F;
