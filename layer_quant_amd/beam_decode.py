@@ -170,8 +170,8 @@ def beam_search(model, logits: torch.Tensor, cache_params, num_beams: int, max_n
             raise ValueError(f"start={start} is not behind the {layer.length} rows of layer {layer_idx}")
     prompts = logits.shape[0]
     device = logits.device
-    scores, _, tokens = beam_select(logits[:, None], torch.zeros(prompts, 1, device=device),
-                                    num_beams)
+    scores = torch.zeros(prompts, 1, device=device, dtype=torch.float32)
+    scores, _, tokens = beam_select(logits[:, None], scores, num_beams)
     finished = None if eos_token_id is None else tokens == eos_token_id
     share_prompt(model, cache_params, num_beams)
     if attention_mask is not None:

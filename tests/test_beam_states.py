@@ -112,3 +112,38 @@ def test_beam_search_refuses_caches_of_different_lengths(model):
     for start in (8, 9):
         with pytest.raises(ValueError, match="start"):
             bd.beam_search(model, torch.zeros(2, 64), cache, 4, 3, start=start)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """beam_search with the selection in torch, no reordering, and a model that makes the same logits."""
+    seen = SimpleNamespace(scores=[], grad=[])
+
+    def select(logits, scores, num=None, *, finished=None, pad_token=0, keep_slots=False):
+        seen.scores.append(scores)
+        P, N = scores.shape
+        total = scores[..., None] + logits.reshape(P, N, -1).float().log_softmax(-1)
+        best = total.reshape(P, -1).topk(N if num is None else num)
+        V = logits.shape[-1]
+        return best.values, best.indices // V, best.indices % V
+
+    def model(tokens, **kw):
+        seen.grad.append(torch.is_grad_enabled())
+        return SimpleNamespace(logits=torch.arange(64.0).expand(tokens.shape[0], 1, 64))
+
+    monkeypatch.setattr(bd, "beam_select", select)
+    monkeypatch.setattr(bd, "reorder_states", lambda *a: None)
+    seen.run = lambda: bd.beam_search(model, torch.randn(2, 64), SimpleNamespace(), 4, 3, start=5)
+    return seen
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_running_scores_are_fp32_whatever_the_default_dtype(on_cpu, dtype):
+    default = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        tokens, scores = on_cpu.run()
+    finally:
+        torch.set_default_dtype(default)
+    assert tokens.shape == (2, 4, 3) and scores.dtype == torch.float32
+    assert all(s.dtype == torch.float32 for s in on_cpu.scores)
