@@ -153,6 +153,7 @@ def reorder_states(model, cache_params, beams: torch.Tensor) -> None:
     reorder_beams(tensors, beams, rows)
 
 
+@torch.no_grad()
 def beam_search(model, logits: torch.Tensor, cache_params, num_beams: int, max_new_tokens: int, *,
                 start: int, eos_token_id: int | None = None, pad_token: int = 0,
                 attention_mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:

@@ -147,3 +147,10 @@ def test_running_scores_are_fp32_whatever_the_default_dtype(on_cpu, dtype):
         torch.set_default_dtype(default)
     assert tokens.shape == (2, 4, 3) and scores.dtype == torch.float32
     assert all(s.dtype == torch.float32 for s in on_cpu.scores)
+
+
+def test_a_search_records_no_gradients(on_cpu):
+    """States are written in place, step after step: with gradients on, a graph over all steps stayed alive."""
+    assert torch.is_grad_enabled()
+    on_cpu.run()
+    assert on_cpu.grad == [False, False] and torch.is_grad_enabled()
