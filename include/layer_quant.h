@@ -293,10 +293,12 @@ size_t lq_int4_shared_decode_attention_workspace(int64_t prompts, int64_t member
  * q_len = 1 GQA attention of rows that share their prompt's cache. Row b = prompt * N + member of q
  * (N = B / P members for each of the P prompts) attends to rows [0, prefix_len) of its prompt's
  * cache and then to rows [0, seq_len - prefix_len) of its own: the attention of
- * lq_int4_decode_attention over the two in sequence, with each prompt's rows read once for all its
- * members. With k_new and v_new [B, Hkv, 1, D] (both or neither NULL) the step's token is first
- * packed into own row seq_len - prefix_len - 1, with scale = max(absmax * fl(1/7), 1e-8) (within one
- * unit in the last place of lq_int4_pack_kv's quotient) and the levels of lq_int4_pack_kv under it.
+ * lq_int4_decode_attention over the two in sequence. With f16 or bf16 queries, D = 128, groups of 32, 64
+ * or 128 and contiguous cache rows each prompt's rows are read once for every 32 query rows of a KV head;
+ * any other form takes a kernel that reads them for each row and head. With k_new and v_new
+ * [B, Hkv, 1, D] (both or neither NULL) the step's token is first packed into own row
+ * seq_len - prefix_len - 1, with scale = max(absmax * fl(1/7), 1e-8) (within one unit in the last place
+ * of lq_int4_pack_kv's quotient) and the levels of lq_int4_pack_kv under it.
  *   q         [B, Hq, 1, D] or [B, Hq, D]   f32/f16/bf16
  *   prefix_*  the prompts' cache, k_packed/v_packed [P, Hkv, cap, D/2] u8 and scales [P, Hkv, cap,
  *             D/g] f32;  k_packed .. v_scale the rows' own cache, the same with B rows and a

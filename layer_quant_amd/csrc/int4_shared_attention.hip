@@ -10,7 +10,8 @@
 //   * shared_mfma_kernel (int4_shared_attention_mfma.hip): head_dim 128, group 32/64/128, 16-bit
 //     queries; packs the new token itself.
 //   * shared_generic_kernel: any even group dividing any head_dim <= 512, any query type; one wave per
-//     (row, query head, split), fp32 VALU throughout, behind shared_pack_kernel.
+//     (row, query head, split), fp32 VALU throughout, behind shared_pack_kernel. It shares nothing of a
+//     prompt's rows: fp32 queries, ctx 4001, group 32, 2 prompts x 8 members 696 us, 16 x 1 843, 2 x 1 128.
 #include <math.h>
 
 #include "int4_quant.h"

@@ -21,16 +21,19 @@
 //     the exponent range of fp32, so that a key's share keeps its precision whatever the other keys'
 //     scales and weights are.
 //
-// What bounds it (MI355X, kernel trace, group 32 unless said): 8 prompts x 8 members at ctx 16384 take 55.7
-// us, 174 MB of which 168 are the prompts' rows. With the products left out the kernel takes as long, with
-// half the workgroups in place 5 us more, with any other order of the tiles the same: it is the reads, at
-// the rate that lq_int4_decode_attention reaches on that volume (one member per prompt 35 us; its 6.5 TB/s
-// come with the eightfold volume), behind the set-up (4 us: query rows, first tiles), the partials of 2048
-// (row, head)s in 8 splits (9 MB) and the own units, which start as the prefix's workgroups end (6 us). 64
-// members of one prompt (group 128, fp16, ctx 8192: 256 query rows per KV head, 34.8 us) take 400 VALU
-// instructions and 48 MFMAs per tile and 32 rows, as every row block decodes the same tiles again: half of
-// the time is their issue, the rest the set-up, the join and waits that two waves per SIMD leave open. A few members at a short prompt (1 x 4, ctx 777:
-// 7.6 us) are one tile per wave: latency of the loads, set-up and join.
+// What bounds it (MI355X, kernel trace, group 32 unless said): 8 prompts x 8 members at ctx 16384 take 62
+// us, 174 MB of which 168 are the prompts' rows. The loads alone take 34 us, with the scores and weights
+// but without the P V products 41: it is issue, 23.0 M VALU instructions (4 cycles each, 37 us of the
+// SIMDs) and 1.6 M MFMAs (16 cycles, 10 us), about 650 and 48 per tile and 32 rows, at two waves per SIMD.
+// Of a tile's VALU instructions 192 split P' in two terms, three per key, row and group. (As one fp16 value
+// in one instruction for two keys the kernel took 56 us, with 11 bits of each product and the range of
+// fp16.) 64 members of one prompt (group 128, fp16, ctx 8192: 256 query rows per KV head) take 37 us, the
+// loads alone 13, without the P V products 24: every row block decodes the same tiles again. 2 x 8 under a
+// keep-mask, ctx 4001: 19.5 us, the loads and masks alone 12.6, without the P V products 17.3. A few
+// members at a short prompt (1 x 4, ctx 777: 8.0 us) are one tile per wave: latency of the loads, set-up
+// and join. An additive mask is slow (8 x 8, ctx 16384: 273 us a call, 95 with the keep-mask, 68 without):
+// its 16 values per lane and tile are loaded inside the tile's work, and with two column tiles at group 32
+// and 64 they do not fit the registers beside it.
 //
 // Why 32 rows and not more per wave: the accumulators (64 registers), the query operands (32) and a tile's
 // decoded values and scales fill the 256 registers of two waves per SIMD. Why a tile per wave and not one
@@ -731,9 +734,9 @@ SharedPlan plan_shared_fast(int64_t P, int64_t N, int64_t Hkv, int64_t nrep, int
   // One prefix workgroup per CU leaves the other place to the own units and halves the set-ups and partials;
   // two hide each other's waits. The first pays up to about 12 tiles per wave (9 with 16 query rows) and one
   // more for each of the first 6 own tiles. Measured with one and with two, group 32: 60 own rows, 1 prompt
-  // x 16, 4 tiles 22.3 us for 26.3, 8 x 8, 10 tiles 30.1 for 33.7, 14 tiles 36.5 for 37.4, 18 tiles 43.0 for
-  // 41.2; 200 own rows, 8 x 8, 18 tiles 43.4 for 44.2, 24 tiles 52.9 for 50.2; 4 x 4 (16 query rows), 60
-  // own rows, 10 tiles 22.9 for 25.5, 14 tiles 27.9 for 28.4, 16 tiles 30.4 for 29.8.
+  // x 16, 4 tiles 21.0 us for 26.9, 8 x 8, 10 tiles 32.1 for 33.8, 14 tiles 39.7 for 39.0, 18 tiles 47.1 for
+  // 43.7; 200 own rows, 8 x 8, 14 tiles 39.8 for 41.5, 18 tiles 47.2 for 46.4, 24 tiles 58.2 for 53.8; 4 x 4
+  // (16 query rows), 60 own rows, 10 tiles 23.3 for 25.4, 14 tiles 28.6 for 28.5, 16 tiles 31.3 for 30.0.
   const int64_t own_tiles = std::min<int64_t>(6, (own_len + TILE - 1) / TILE);
   SharedPlan plan{split_of(prefix_len, device_cus() / units, STEP),
                   split_of(own_len, resident / own_units, 2 * STEP)};
@@ -751,10 +754,9 @@ int launch_shared_fast(SharedParams p, hipStream_t st) {
   const int64_t pb = (int64_t)p.P * p.Hkv * p.rb_prefix * p.nsp;
   const int64_t units = (int64_t)p.B * p.Hkv * p.rb_own * p.nso;
   // Waves per own unit: a whole workgroup where every one has its place at once, the shortest chain of
-  // steps (1 prompt x 16, ctx 2000, 100 own rows: 15.3 us, 16.6 with two waves, 19.8 with one); where they
-  // wait for places behind the prefix, fewer and fuller ones (8 x 8, ctx 16384: 64 own rows 60.8 us with
-  // four waves, 58.4 with one; 100 rows 63.1, 58.4 with two, 62.2 with one; 200 rows 64.4, 61.9 with two,
-  // 64.4 with one).
+  // steps (1 prompt x 16, ctx 2000, 100 own rows: 14.9 us, 15.9 with two waves, 18.8 with one); where they
+  // wait for places behind the prefix, fewer and fuller ones (8 x 8, ctx 16384: 100 rows 64.1 us with four
+  // waves, 63.6 with two, 65.2 with one; 200 rows 68.0, 64.6 and 67.4; 64 rows 66.4, 66.1 and 66.5).
   const int64_t tiles = (std::min(p.chunk_o, p.own_len) + TILE - 1) / TILE;
   p.own_waves = pb + units <= resident_workgroups() ? 4 : tiles <= 2 ? 1 : tiles <= 8 ? 2 : 4;
   const int64_t ob = (units * p.own_waves + WAVES - 1) / WAVES;

@@ -241,7 +241,9 @@ def shared_prefix_decode_attention(query_states: torch.Tensor, cache: Int4KVLaye
                                    value_states: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [P*N, Hq, 1, D] over a cache with a shared prefix -> [P*N, Hq, D] in q's dtype
     (no reference counterpart): row p*N + n attends to prefix rows [0, prefix.length) of prompt p and
-    then to its own rows, seq_len keys in all. Each prompt's rows are read once for its N members.
+    then to its own rows, seq_len keys in all. With 16-bit queries, head_dim 128 and groups of 32, 64 or
+    128 each prompt's rows are read once for 32 query rows of a KV head (8 members of 4 heads); any other
+    form reads them for each query head.
 
     With key_states and value_states [P*N, Hkv, 1, D] the step's token is first packed into own row
     seq_len - prefix.length - 1, and cache.length follows. The mask is that of _decode_attention over
