@@ -367,6 +367,62 @@ int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, int count,
                      const lq_tensor* beams, void* stream);
 
 /*
+ * Causal attention of whole prompts over their own keys (no counterpart in the reference, whose forward
+ * hands prompts to a library attention on repeated K and V, hybrid_quant/int4_8b_attention.py:693-714):
+ *   out[t] = sum over s <= t of t's own prompt of softmax_s(scale * q[t] . k[s]) v[s]
+ * Query head h reads KV head h / (Hq / Hkv). Scores, softmax and sums in fp32.
+ *   packed: q, out [T, Hq, D], k, v [T, Hkv, D], starts int32 or int64 [S + 1] on the device, contiguous:
+ *     prompt s has rows [starts[s], starts[s + 1]), in ascending order (an empty one has none). Rows in
+ *     front of starts[0] and behind starts[S] get zeros. Starts outside [0, T] count as 0 or T; prompts
+ *     that are not in ascending order give unspecified values.
+ *   a batch: starts NULL, q, out [B, L, Hq, D], k, v [B, L, Hkv, D], every batch row a prompt
+ *   q, k, v and out of one dtype (f32, f16 or bf16), any strides; D <= 256
+ * Rows behind a query's own never reach its result, whatever they hold.
+ */
+int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor* v,
+                        const lq_tensor* starts, const lq_tensor* out, float scale, void* stream);
+
+/*
+ * The Mamba2 recurrence over whole prompts (the form of lq_selective_state_update for more than one
+ * token; the reference leaves prompts to its remote module). Per head, over the rows of a prompt:
+ *   dt = dt (+ dt_bias); dt = log(1 + e^dt) if dt_softplus; dt clamped to [dt_min, dt_max]
+ *   S  = exp(A dt) S + dt x B^T     (S [P, N], from initial or zero)
+ *   y  = S C (+ D x);  y *= z * sigmoid(z) when z is given
+ * States in fp32; rounded where they are written.
+ *   packed: x, z, out [T, H, P], dt [T, H], B, C [T, G, N] (H % G == 0) and starts as for
+ *     lq_prompt_attention; a batch: starts NULL, x [B, L, H, P] and so on
+ *   A [H], D NULL or [H], dt_bias NULL or [H]; initial NULL or [S, H, P, N], states NULL or [S, H, P, N]
+ *   (the state behind each prompt; an empty one's is its initial state). They may be one tensor; else no
+ *   output may overlap an input. x, B and C of one dtype, the others of any float dtype; any strides.
+ *   N <= 256. The workspace needs no particular contents; `packed` is 1 where starts are given, `batch`
+ *   then ignored but for 0.
+ */
+size_t lq_prompt_scan_workspace(int64_t batch, int64_t rows, int packed, int64_t heads,
+                                int64_t head_dim, int64_t dstate);
+int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_tensor* A, const lq_tensor* B,
+                   const lq_tensor* C, const lq_tensor* starts, const lq_tensor* D,
+                   const lq_tensor* z, const lq_tensor* dt_bias, const lq_tensor* initial,
+                   const lq_tensor* states, const lq_tensor* out, int dt_softplus, float dt_min,
+                   float dt_max, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log-probabilities of given tokens under logits [R, V] or [B, L, V] (f32, f16 or bf16, any strides),
+ * with the entropy of each row and its likeliest tokens (no counterpart in the reference):
+ *   logprobs[r] = logits[r][tokens[r]] - lse[r], entropy[r] = lse[r] - sum_v p[r][v] logits[r][v]
+ *   tokens [R] or [B, L] i64, any strides; one outside [0, V) gives 0
+ *   logprobs [R] f32, entropy NULL or [R] f32, top_logprobs and top_tokens NULL or [R, top] f32 and i64
+ *   (R = B * L), contiguous; top <= 32: the largest logits in descending order, equal ones by the lower
+ *   token
+ * A row with a NaN or +inf logit, or without one above -inf, gives NaN (and tokens 0, 1, ...); logits
+ * beyond 2^127 in magnitude count as infinite. The workspace needs no particular contents.
+ */
+size_t lq_token_logprobs_workspace(int64_t rows, int64_t vocab, int top);
+int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* tokens, const lq_tensor* logprobs,
+                      const lq_tensor* entropy, const lq_tensor* top_logprobs,
+                      const lq_tensor* top_tokens, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
  * MX state layouts. Every MX entry point takes either layout and tells them apart by the shapes
  * of q_state and micro_exp (N = 16 * shared_exp.shape[3]):
  *   reference layout (hybrid_quant/mamba_state_8b_kernel.py:11-25, 575-598):

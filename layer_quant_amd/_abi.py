@@ -84,6 +84,11 @@ EXPORTED_SYMBOLS = (
     "lq_beam_select_workspace",
     "lq_beam_select",
     "lq_reorder_beams",
+    "lq_prompt_attention",
+    "lq_prompt_scan_workspace",
+    "lq_prompt_scan",
+    "lq_token_logprobs_workspace",
+    "lq_token_logprobs",
 )
 
 
@@ -177,6 +182,17 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.lq_reorder_beams.restype = ctypes.c_int
     lib.lq_reorder_beams.argtypes = [_P, ctypes.POINTER(ctypes.c_int64), ctypes.c_int, _P,
                                      ctypes.c_void_p]
+    lib.lq_prompt_attention.restype = ctypes.c_int
+    lib.lq_prompt_attention.argtypes = [_P] * 5 + [ctypes.c_float, ctypes.c_void_p]
+    lib.lq_prompt_scan_workspace.restype = ctypes.c_size_t
+    lib.lq_prompt_scan_workspace.argtypes = [ctypes.c_int64] * 2 + [ctypes.c_int] + [ctypes.c_int64] * 3
+    lib.lq_prompt_scan.restype = ctypes.c_int
+    lib.lq_prompt_scan.argtypes = [_P] * 12 + [ctypes.c_int, ctypes.c_float, ctypes.c_float,
+                                               ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    lib.lq_token_logprobs_workspace.restype = ctypes.c_size_t
+    lib.lq_token_logprobs_workspace.argtypes = [ctypes.c_int64] * 2 + [ctypes.c_int]
+    lib.lq_token_logprobs.restype = ctypes.c_int
+    lib.lq_token_logprobs.argtypes = [_P] * 6 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
 
 
 def lib() -> ctypes.CDLL:
@@ -205,7 +221,8 @@ _HOST_ENTRIES = (
     "lq_mx_encode", "lq_mx_state_update", "lq_mx_state_update_device_step",
     "lq_selective_state_update", "lq_max_position", "lq_keep_mask_bias",
     "lq_int4_shared_decode_attention_workspace", "lq_int4_shared_decode_attention",
-    "lq_beam_select_workspace", "lq_beam_select", "lq_reorder_beams",
+    "lq_beam_select_workspace", "lq_beam_select", "lq_reorder_beams", "lq_prompt_attention",
+    "lq_prompt_scan_workspace", "lq_prompt_scan", "lq_token_logprobs_workspace", "lq_token_logprobs",
 )
 
 
@@ -748,3 +765,66 @@ def reorder_beams(tensors, rows, beams: torch.Tensor) -> None:
         live = (ctypes.c_int64 * max(len(tensors), 1))(*(-1 if r is None else int(r) for r in rows))
     rc = lib().lq_reorder_beams(table, live, len(tensors), desc(beams), _stream(dev))
     check(rc, "lq_reorder_beams")
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     starts: torch.Tensor | None, out: torch.Tensor, scale: float) -> torch.Tensor:
+    """Causal attention of packed prompts [T, heads, D] with starts [S + 1], or of a batch
+    [B, L, heads, D] -> out."""
+    host = _host or host_binding()
+    if host:
+        rc = host.prompt_attention(q, k, v, starts, out, scale)
+        if rc is not None:
+            check(rc, "lq_prompt_attention")
+            return out
+    dev = _require_gpu(q, k, v, starts, out)
+    rc = lib().lq_prompt_attention(desc(q), desc(k), desc(v), desc(starts), desc(out), float(scale),
+                                   _stream(dev))
+    check(rc, "lq_prompt_attention")
+    return out
+
+
+def prompt_scan(x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out, dt_softplus: bool,
+                dt_min: float, dt_max: float) -> torch.Tensor:
+    """The Mamba2 recurrence over packed prompts or a batch: y -> out, the states behind the prompts
+    -> states (or None)."""
+    host = _host or host_binding()
+    if host:
+        rc = host.prompt_scan(x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out, dt_softplus,
+                              dt_min, dt_max, _scratch.get)
+        if rc is not None:
+            check(rc, "lq_prompt_scan")
+            return out
+    dev = _require_gpu(x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out)
+    stream = _stream(dev)
+    batch, rows = (1, x.shape[0]) if starts is not None else x.shape[:2]
+    need = int(lib().lq_prompt_scan_workspace(batch, rows, int(starts is not None), *x.shape[-2:],
+                                              B.shape[-1]))
+    ws = _scratch.get(dev.index, stream, need) if need else None
+    rc = lib().lq_prompt_scan(*map(desc, (x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out)),
+                              1 if dt_softplus else 0, float(dt_min), float(dt_max),
+                              None if ws is None else ws.data_ptr(), need, stream)
+    check(rc, "lq_prompt_scan")
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprobs: torch.Tensor,
+                   entropy: torch.Tensor | None, top_logprobs: torch.Tensor | None,
+                   top_tokens: torch.Tensor | None) -> None:
+    """Log-probabilities of tokens [R] or [B, L] under logits [R, V] or [B, L, V], entropy and the
+    likeliest tokens, into the contiguous outputs [B * L] and [B * L, top]."""
+    host = _host or host_binding()
+    if host:
+        rc = host.token_logprobs(logits, tokens, logprobs, entropy, top_logprobs, top_tokens,
+                                 _scratch.get)
+        if rc is not None:
+            return check(rc, "lq_token_logprobs")
+    dev = _require_gpu(logits, tokens, logprobs, entropy, top_logprobs, top_tokens)
+    stream = _stream(dev)
+    need = int(lib().lq_token_logprobs_workspace(tokens.numel(), logits.shape[-1],
+                                                 0 if top_tokens is None else top_tokens.shape[1]))
+    ws = _scratch.get(dev.index, stream, need) if need else None
+    rc = lib().lq_token_logprobs(desc(logits), desc(tokens), desc(logprobs), desc(entropy),
+                                 desc(top_logprobs), desc(top_tokens),
+                                 None if ws is None else ws.data_ptr(), need, stream)
+    check(rc, "lq_token_logprobs")

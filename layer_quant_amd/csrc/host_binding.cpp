@@ -35,6 +35,11 @@ struct Entries {
   decltype(&lq_beam_select_workspace) select_workspace;
   decltype(&lq_beam_select) select;
   decltype(&lq_reorder_beams) reorder;
+  decltype(&lq_prompt_attention) prompt_attention;
+  decltype(&lq_prompt_scan_workspace) scan_workspace;
+  decltype(&lq_prompt_scan) scan;
+  decltype(&lq_token_logprobs_workspace) logprobs_workspace;
+  decltype(&lq_token_logprobs) logprobs;
 } entries;
 constexpr int kEntries = sizeof(Entries) / sizeof(void*);
 
@@ -111,6 +116,12 @@ bool to_int(PyObject* o, int& v) {
 bool to_uint64(PyObject* o, uint64_t& v) {
   if (!PyLong_CheckExact(o)) return false;
   v = PyLong_AsUnsignedLongLongMask(o);
+  return true;
+}
+
+bool to_float(PyObject* o, float& v) {
+  if (!PyFloat_CheckExact(o)) return false;
+  v = (float)PyFloat_AS_DOUBLE(o);
   return true;
 }
 
@@ -405,6 +416,55 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// q, k, v, starts, out, scale
+PyObject* py_prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!has_args(n, 6)) return nullptr;
+  Tensors<5> t;
+  float scale;
+  LQ_NOT_PLAIN(!t.add_all(a) || !to_float(a[5], scale));
+  return launch(t.device, [&](void* s) {
+    return entries.prompt_attention(t.ptr[0], t.ptr[1], t.ptr[2], t.ptr[3], t.ptr[4], scale, s);
+  });
+}
+
+// x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out, softplus, the step's limits, scratch getter
+PyObject* py_prompt_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!has_args(n, 16)) return nullptr;
+  Tensors<12> t;
+  float lo, hi;
+  LQ_NOT_PLAIN(!t.add_all(a) || !to_float(a[13], lo) || !to_float(a[14], hi));
+  const int softplus = PyObject_IsTrue(a[12]);
+  if (softplus < 0) return nullptr;
+  const lq_tensor* const* p = t.ptr;
+  const bool packed = p[5] != nullptr;
+  const int nd = packed ? 3 : 4;
+  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim != nd || p[3] == nullptr || p[3]->ndim != nd);
+  const size_t need = entries.scan_workspace(packed ? 1 : p[0]->shape[0], p[0]->shape[nd - 3], packed,
+                                             p[0]->shape[nd - 2], p[0]->shape[nd - 1],
+                                             p[3]->shape[nd - 1]);
+  return launch_with(t.device, a[15], need, [&](void* ws, size_t bytes, void* s) {
+    return entries.scan(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], p[11],
+                        softplus, lo, hi, ws, bytes, s);
+  });
+}
+
+// logits, tokens, logprobs, entropy, top_logprobs, top_tokens, scratch getter
+PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!has_args(n, 7)) return nullptr;
+  Tensors<6> t;
+  LQ_NOT_PLAIN(!t.add_all(a));
+  const lq_tensor* const* p = t.ptr;
+  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim < 2 || p[0]->ndim > 3 ||
+               (p[5] != nullptr && (p[5]->ndim != 2 || p[5]->shape[1] > INT32_MAX)));
+  const int nd = p[0]->ndim;
+  const int64_t rows = (nd == 3 ? p[0]->shape[0] : 1) * p[0]->shape[nd - 2];
+  const size_t need = entries.logprobs_workspace(rows, p[0]->shape[nd - 1],
+                                                 p[5] == nullptr ? 0 : (int)p[5]->shape[1]);
+  return launch_with(t.device, a[6], need, [&](void* ws, size_t bytes, void* s) {
+    return entries.logprobs(p[0], p[1], p[2], p[3], p[4], p[5], ws, bytes, s);
+  });
+}
+
 // bind(current raw stream function, addresses of the entry points in the order of Entries)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!has_args(n, 1 + kEntries)) return nullptr;
@@ -454,6 +514,9 @@ PyMethodDef methods[] = {LQ_METHOD("bind", py_bind),
                          LQ_METHOD("int4_shared_decode_attention", py_shared),
                          LQ_METHOD("beam_select", py_select),
                          LQ_METHOD("reorder_beams", py_reorder),
+                         LQ_METHOD("prompt_attention", py_prompt_attention),
+                         LQ_METHOD("prompt_scan", py_prompt_scan),
+                         LQ_METHOD("token_logprobs", py_token_logprobs),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lq_host", nullptr, -1, methods,

@@ -51,6 +51,19 @@ bool diag(uint32_t bit);
 int check_tensor(const lq_tensor* t, const char* name, int ndim, bool float_dtype,
                  int exact_dtype = -1);
 
+// check_tensor, but a tensor without elements may come without memory (torch gives it none).
+inline int check_tensor_or_empty(const lq_tensor* t, const char* name, int ndim, bool float_dtype,
+                                 int exact_dtype = -1) {
+  if (t == nullptr || t->data != nullptr || t->ndim < 1 || t->ndim > 4) {
+    return check_tensor(t, name, ndim, float_dtype, exact_dtype);
+  }
+  lq_tensor with_data = *t;
+  for (int i = 0; i < t->ndim; ++i) {
+    if (t->shape[i] == 0) with_data.data = &with_data;
+  }
+  return check_tensor(&with_data, name, ndim, float_dtype, exact_dtype);
+}
+
 // Largest element offset reachable through a descriptor (for bounds reasoning on the host).
 int64_t max_offset(const lq_tensor* t);
 
