@@ -124,7 +124,9 @@ enum {
    * against 10.4 + 4.4 us of kernel time) and at batch 8, ctx 2072, 0.7 us faster at batch 8,
    * ctx 16384 */
   LQ_DIAG_ATTN_FOLD_MERGE = 1u << 8,
-  LQ_DIAG_ALL = (1u << 9) - 1
+  LQ_DIAG_PROMPT_FORCE_GENERIC = 1u << 9,
+  LQ_DIAG_PROMPT_REQUIRE_MFMA = 1u << 10,
+  LQ_DIAG_ALL = (1u << 11) - 1
 };
 
 /* The current LQ_DIAG_* bits. */

@@ -46,6 +46,8 @@ DIAG_BITS = {
     "LQ_SSM_FORCE_GENERIC": 1 << 6,
     "LQ_SSM_REQUIRE_ROWS": 1 << 7,
     "LQ_ATTN_FOLD_MERGE": 1 << 8,
+    "LQ_PROMPT_FORCE_GENERIC": 1 << 9,
+    "LQ_PROMPT_REQUIRE_MFMA": 1 << 10,
 }
 
 DTYPE_CODES = {

@@ -14,6 +14,15 @@ struct PromptAttention {
   Spans spans;
   int Hkv, nrep, D;
   float scale;  // log2(e) times the caller's
+  uint32_t q_and, q_xor;  // on pairs of 16-bit query values: the scale's sign, and zeros for scale 0
 };
+
+constexpr int PROMPT_ATTENTION_WAVES = 4;  // of a workgroup, 32 rows each
+
+// The 16-bit kernel (prompt_attention_mfma.hip): whether the tensors are in its form, and its launch,
+// whose scale is positive.
+bool prompt_attention_mfma_fits(const lq_tensor* q, const lq_tensor* k, const lq_tensor* v,
+                                const lq_tensor* out);
+int launch_prompt_attention_mfma(const PromptAttention& p, int dtype, int64_t parts, hipStream_t st);
 
 }  // namespace lq

@@ -21,7 +21,7 @@ namespace {
 
 constexpr int KT = 32;    // keys per tile
 constexpr int ROWS = 32;  // rows per wave
-constexpr int NW = 4;     // waves per workgroup
+constexpr int NW = PROMPT_ATTENTION_WAVES;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -253,8 +253,18 @@ extern "C" int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const
     return fail(LQ_ERR_UNSUPPORTED, "%lld parts of %lld KV heads exceed the launch limits",
                 (long long)parts, (long long)Hkv);
   }
-  const dim3 grid((unsigned)(parts * Hkv)), block(64 * NW);
   const hipStream_t st = (hipStream_t)stream;
+  const bool mfma = !diag(LQ_DIAG_PROMPT_FORCE_GENERIC) && prompt_attention_mfma_fits(q, k, v, out);
+  if (!mfma && diag(LQ_DIAG_PROMPT_REQUIRE_MFMA)) {
+    return fail(LQ_ERR_INVALID_ARG, "the layout takes the general kernel");
+  }
+  if (mfma) {
+    p.q_and = scale == 0.f ? 0 : ~0u;
+    p.q_xor = scale < 0.f ? 0x80008000u : 0;
+    p.scale = scale == 0.f ? 1.f : fabsf(p.scale);
+    return launch_prompt_attention_mfma(p, q->dtype, parts, st);
+  }
+  const dim3 grid((unsigned)(parts * Hkv)), block(64 * NW);
   if (D <= 64) hipLaunchKernelGGL(prompt_attention_f32<64>, grid, block, 0, st, p);
   else if (D <= 128) hipLaunchKernelGGL(prompt_attention_f32<128>, grid, block, 0, st, p);
   else hipLaunchKernelGGL(prompt_attention_f32<256>, grid, block, 0, st, p);

@@ -95,6 +95,31 @@ def test_attention_strides(gpu, dtype):
         within(got, want, bound, f"{form} {dtype}")
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_attention_kernels_by_layout(gpu, dtype, diag):
+    """16-bit rows of 64 or 128 dims, 16-byte aligned, take the matrix kernel, and agree with the general
+    one; anything else takes the general one."""
+    from layer_quant_amd import _abi
+
+    for d in (64, 128):
+        q, k, v = attention_inputs(gpu, 333, 8, 2, d, dtype, seed=11)
+        starts = starts_of([300, 33], gpu)
+        want, weight, score = ref.attention(q, k, v, starts.tolist())
+        bound = ref.attention_bound(want, weight, score, dtype, d)
+        diag.set("LQ_PROMPT_REQUIRE_MFMA")
+        within(prompts.prompt_attention(q, k, v, starts), want, bound, f"matrix {d}")
+        wide = torch.zeros(333, 2, d + 8, device=gpu, dtype=dtype)
+        prompts.prompt_attention(q, wide[..., :d], wide[..., 8:], starts)
+        for bad in (wide[..., 1:d + 1], wide[:1].expand(333, 2, d + 8)[..., :d], k[:, :, ::2].repeat(1, 1, 2)
+                    .transpose(0, 2).contiguous().transpose(0, 2)):
+            with pytest.raises(_abi.LQError, match="general kernel"):
+                prompts.prompt_attention(q, bad, v, starts)
+        diag.clear("LQ_PROMPT_REQUIRE_MFMA")
+        diag.set("LQ_PROMPT_FORCE_GENERIC")
+        within(prompts.prompt_attention(q, k, v, starts), want, bound, f"general {d}")
+        diag.clear("LQ_PROMPT_FORCE_GENERIC")
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_nothing_from_behind(gpu, dtype, bad):
