@@ -22,7 +22,7 @@
 // Masked keys of a row have p = 0, which a value of inf or NaN would turn into NaN. Results that are not
 // finite are rare, so it is they that are looked for: a workgroup with one runs its rows again, and then
 // hands such values to the rows that see them and takes them out of the tile.
-#include "lds_loads.h"
+#include "matrix16.h"
 #include "prompt_attention.h"
 
 namespace lq {
@@ -31,37 +31,6 @@ namespace {
 constexpr int KT = 64;    // keys per tile
 constexpr int ROWS = 32;  // rows per wave
 constexpr float LAZY = 8.f;
-
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-
-template <bool BF>
-__device__ __forceinline__ f32x16_t mfma(u32x4_t a, u32x4_t b, f32x16_t c) {
-  if constexpr (BF) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
-                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-  }
-}
-
-// Two floats rounded to nearest even, a in the low half.
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF) {
-    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-    const bf16x2_t v = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, v);
-  } else {
-    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-    const f16x2_t v = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, v);
-  }
-}
 
 // Chunks by which a tile row's chunks are exchanged. D = 128 (256-byte rows): 16 rows' equal chunks, and
 // 4 rows' runs of 4 chunks, lie in different banks. D = 64: two rows share 256 bytes.
@@ -72,20 +41,6 @@ __device__ __forceinline__ int swizzle_k(int r) {
 template <int D>
 __device__ __forceinline__ int swizzle_v(int r) {
   return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
-}
-
-typedef __attribute__((address_space(3))) char* lds_t;
-
-// As load_to_lds, for rows that other workgroups read as well.
-__device__ __forceinline__ void load_rows_to_lds(i32x4_t desc, lds_t lds, int voff) {
-  const uint32_t addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      :
-      : "s"(addr), "v"(voff), "s"(desc)
-      : "memory", "m0");
 }
 
 template <bool BF, int D, int NW>
@@ -113,17 +68,17 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
   if (sp.gap) {
     if (r < nrows) {
 #pragma unroll
-      for (int i = 0; i < CH / 2; ++i) *(u32x4_t*)(out + 8 * (2 * i + hi)) = u32x4_t{0, 0, 0, 0};
+      for (int i = 0; i < CH / 2; ++i) *(words4_t*)(out + 8 * (2 * i + hi)) = words4_t{0, 0, 0, 0};
     }
     return;
   }
 
-  u32x4_t q[D / 16];  // dims 16 i + 8 hi .. + 7
+  words4_t q[D / 16];  // dims 16 i + 8 hi .. + 7
   {
     const uint16_t* from = (const uint16_t*)p.q.data + lead * p.q.s[0] + row * p.q.s[1] + head * p.q.s[2];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
-      q[i] = *(const u32x4_t*)(from + 16 * i + 8 * hi);
+      q[i] = *(const words4_t*)(from + 16 * i + 8 * hi);
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[i][e] = (q[i][e] & p.q_and) ^ p.q_xor;
     }
@@ -202,8 +157,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
       for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const u32x4_t k = *(__attribute__((address_space(3))) u32x4_t*)(kt + (kaddr ^ (32 * i)) + b * 32 * ROW_BYTES);
-          s[b] = mfma<BF>(k, q[i], s[b]);
+          s[b] = mfma<BF>(lds_read16(kt + (kaddr ^ (32 * i)) + b * 32 * ROW_BYTES), q[i], s[b]);
         }
       }
       if (kb + KT - 1 > wave_first) {
@@ -229,7 +183,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
         for (int b = 0; b < D / 32; ++b) o[b] *= keep;
       }
       const float base = m == -INFINITY ? 0.f : m * p.scale;
-      u32x4_t pk[4];
+      words4_t pk[4];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -245,11 +199,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
           lds_t from = vt + (vaddr ^ (64 * b)) + 16 * j * ROW_BYTES;
-          const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)from);
-          const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4_t*)(from + 8 * ROW_BYTES));
-          const uint2 a0 = __builtin_bit_cast(uint2, lo), a1 = __builtin_bit_cast(uint2, up);
-          o[b] = mfma<BF>(u32x4_t{a0.x, a0.y, a1.x, a1.y}, pk[j], o[b]);
+          o[b] = mfma<BF>(lds_read_columns(from, from + 8 * ROW_BYTES), pk[j], o[b]);
         }
       }
     }
@@ -275,7 +225,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
       for (int i = 0; i < 4; ++i) w[i] = pack2<BF>(o[b][8 * a + 2 * i] * inv, o[b][8 * a + 2 * i + 1] * inv);
       const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
       const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-      *(u32x4_t*)(out + 32 * b + 16 * a + 8 * hi) = u32x4_t{x[0], y[0], x[1], y[1]};
+      *(words4_t*)(out + 32 * b + 16 * a + 8 * hi) = words4_t{x[0], y[0], x[1], y[1]};
     }
   }
 }

@@ -24,6 +24,13 @@ struct PromptScan {
   float* slot_log;    // [slots][H]: log2 of the decay over it
 };
 
+// The matrix kernel (prompt_scan_mfma.hip): whether the call is in its form, and the launch of `parts`
+// segments.
+bool prompt_scan_mfma_fits(const lq_tensor* x, const lq_tensor* B, const lq_tensor* C,
+                           const lq_tensor* z, const lq_tensor* initial, const lq_tensor* states,
+                           const lq_tensor* out);
+void launch_prompt_scan_mfma(const PromptScan& p, bool followed, int64_t parts, hipStream_t st);
+
 // Segments of a prompt (an empty one has one, which hands its state on), and those that others follow.
 __device__ __forceinline__ int segments_of(const PromptScan& p, int len, bool gap) {
   return max((len + p.segment - 1) / p.segment, gap ? 0 : 1);

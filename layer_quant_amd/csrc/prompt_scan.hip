@@ -362,15 +362,22 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   p.slot_state = (float*)workspace;
   p.slot_log = (float*)((char*)workspace + align256((size_t)(slots * H * P * N) * 4));
   const hipStream_t st = (hipStream_t)stream;
+  const bool mfma = !diag(LQ_DIAG_PROMPT_FORCE_GENERIC) &&
+                    prompt_scan_mfma_fits(x, B, C, z, initial, states, out);
+  if (!mfma && diag(LQ_DIAG_PROMPT_REQUIRE_MFMA)) {
+    return fail(LQ_ERR_INVALID_ARG, "the call takes the general kernel");
+  }
   const unsigned blocks = (unsigned)((H * P * N + 255) / 256);
   if (slots > 0) {
-    launch_rows<true>(p, dim3((unsigned)(slots * H), (unsigned)pblocks), st);
+    if (mfma) launch_prompt_scan_mfma(p, true, slots, st);
+    else launch_rows<true>(p, dim3((unsigned)(slots * H), (unsigned)pblocks), st);
     if ((rc = check_launch("lq_prompt_scan (segments)")) != LQ_OK) return rc;
     hipLaunchKernelGGL(scan_carry_kernel, dim3(blocks, (unsigned)slots), dim3(256), 0, st, p);
     if ((rc = check_launch("lq_prompt_scan (carry)")) != LQ_OK) return rc;
   }
   if (parts > 0) {
-    launch_rows<false>(p, dim3((unsigned)(parts * H), (unsigned)pblocks), st);
+    if (mfma) launch_prompt_scan_mfma(p, false, parts, st);
+    else launch_rows<false>(p, dim3((unsigned)(parts * H), (unsigned)pblocks), st);
     if ((rc = check_launch("lq_prompt_scan")) != LQ_OK) return rc;
   }
   return LQ_OK;

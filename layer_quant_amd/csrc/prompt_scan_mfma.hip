@@ -1,0 +1,486 @@
+// prompt_scan.hip's operator for bf16 x, B and C with head_dim 64 and a state of 128, on
+// v_mfma_f32_32x32x16_bf16: prompts in chunks of 64 rows. With c the running sum of A dt log2(e) within a
+// chunk, S the state in front of it and t, s rows of it,
+//   Y[t] = 2^c_t S C_t + sum_{s <= t} M[t][s] x_s,  M[t][s] = 2^(c_t - c_s) dt_s (C_t . B_s), + D where s = t
+//   S'   = 2^c_63 S + sum_s w_s x_s B_s^T,          w_s = 2^(c_63 - c_s) dt_s
+// c is summed in 64 bits and taken apart into a whole number n and a rest: 2^(c_t - c_s) is the product of
+// 2^(n_t - n_s), exact, and of two factors between 0.7 and 1.42 that a row has once. So no decay overflows
+// however fast a state fades, close rows behind a large c keep their digits, and no element of M takes an
+// exponential. (A step's decay is held within 2^-256 and 2^256.)
+//
+// A workgroup of four waves has two heads of one group; wave (head, half) keeps rows p = 32 half .. + 31 of
+// its head's state, transposed, in 64 accumulators. Of B^T x that is the layout in which S is, rounded to
+// bf16, the A operand of S C^T without leaving its registers, once the columns that the transposing reads
+// hand to the lanes are taken in the order sigma: lane bits (8 a + 4 h + b) <-> index (8 h + 4 a + b). The
+// same order makes eight consecutive values of every result meet in one lane.
+// Per chunk:
+//   phase 1  S C^T (16 products) with C's operands shared by the mixing scores B C^T, of which three waves
+//            make one 32 x 32 block each (the fourth lies above the diagonal) for both heads and leave M in
+//            LDS as bf16; the fourth wave makes the next chunk's steps and decays
+//   phase 2  Y += M x (6 products), stores, S' (32 products)
+// B lies in two LDS buffers; C and x are read in phase 1 alone, so that one buffer each is refilled in
+// phase 2: 79 KB per workgroup, two of them per CU.
+//
+// Roundings: M and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result); w x, which a
+// state keeps, as the sum of two bf16 values (2^-16). Everything else is fp32.
+//
+// Rows behind a row in its chunk have M = 0 there, which an x of inf or NaN would turn into NaN: such values
+// are looked for when x is read, added to the rows that see them and left out of M x.
+#include "matrix16.h"
+#include "prompt_scan.h"
+
+namespace lq {
+namespace {
+
+constexpr int Q = 64;      // rows of a chunk
+constexpr int HEADS = 2;   // of a workgroup
+constexpr int P = 64, N = 128;
+
+struct alignas(1024) ChunkLds {
+  char b[2][Q * N * 2];         // rows of 256 bytes; chunk k of row r at k ^ swizzle_b(r)
+  char c[Q * N * 2];            // the same with k ^ (r mod 16)
+  char x[HEADS][Q * P * 2];     // rows of 128 bytes, k ^ 4 ((r / 2) mod 2)
+  char m[HEADS][3][32 * 32 * 2];  // blocks (s, t) = (0, 0), (0, 1), (1, 1): row t, 64 bytes
+  int whole[HEADS][Q];          // n_s
+  float rest[HEADS][Q];         // 2^(c_s - n_s)
+  float step[HEADS][Q];         // dt_s 2^(n_s - c_s)
+  float weight[2][HEADS][Q];    // w_s
+};
+
+// Both four consecutive rows' runs of 4 chunks and 16 rows' equal chunks lie in different banks.
+__device__ __forceinline__ int swizzle_b(int r) { return 4 * (r & 3) | ((r >> 2) & 3); }
+
+// index of lane (or result row) m
+__device__ __forceinline__ int sigma(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
+
+// Inclusive sums over the wave's lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double prefix_sum(double v) {
+  v += moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);  // row_bcast 15, 31
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+
+// Eight consecutive state values.
+__device__ __forceinline__ void load8(const char* at, int dtype, float (&v)[8]) {
+  if (dtype == LQ_F32) {
+    const float4 a = ((const float4*)at)[0], b = ((const float4*)at)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    return;
+  }
+  const words4_t w = *(const words4_t*)at;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = word_elem(w[i >> 1], (i & 1) * 16, dtype);
+}
+__device__ __forceinline__ void store8(char* at, int dtype, const float (&v)[8]) {
+  if (dtype == LQ_F32) {
+    ((float4*)at)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    ((float4*)at)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    return;
+  }
+  words4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = dtype == LQ_BF16 ? pack2<true>(v[2 * i], v[2 * i + 1]) : pack2<false>(v[2 * i], v[2 * i + 1]);
+  }
+  *(words4_t*)at = w;
+}
+
+__device__ __forceinline__ int size_of(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
+
+// FOLLOWED: as in scan_rows_kernel.
+template <bool FOLLOWED>
+__global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
+  __shared__ ChunkLds lds;
+  // the workgroups of a group's heads on one XCD (blocks go round the eight), as they read the same B and C
+  const int pairs = p.H / HEADS, idx = blockIdx.x % pairs, t0 = blockIdx.x / pairs;
+  const int pair = pairs % 8 == 0 ? (idx & 7) * (pairs / 8) + (idx >> 3) : idx;
+  Span sp;
+  if (!find_span(p.spans, t0,
+                 [&](int len, bool gap) {
+                   return FOLLOWED ? followed_segments_of(p, len, gap) : segments_of(p, len, gap);
+                 },
+                 sp)) {
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), hw = wave >> 1, half = wave & 1;
+  const int h0 = pair * HEADS, h = h0 + hw, g = h0 / p.ratio;
+  const int64_t lead = p.spans.starts == nullptr ? sp.index : 0;
+  const int from = sp.part * p.segment, to = min(sp.len, from + p.segment);
+  uint16_t* out = (uint16_t*)p.out.data + lead * p.out.s[0] + (int64_t)(sp.begin + from) * p.out.s[1];
+  if (sp.gap) {
+    for (int i = tid; i < (to - from) * HEADS * (P / 8); i += 256) {
+      const int r = i / (HEADS * P / 8), k = i % (HEADS * P / 8);
+      *(words4_t*)(out + r * p.out.s[1] + (h0 + k / (P / 8)) * p.out.s[2] + k % (P / 8) * 8) = words4_t{0, 0, 0, 0};
+    }
+    return;
+  }
+  const int nseg = segments_of(p, sp.len, false);
+  const int slot = FOLLOWED ? t0 : sp.before + sp.part;
+  if (!FOLLOWED && nseg > 1 && sp.part == 0) return;  // finished by the first launch
+  if (slot > p.slots) return;                         // starts out of order ask for more than there are
+  const bool alone = FOLLOWED && sp.part > 0;         // from no state, and no y
+
+  // the state: [32-block][i], n = 32 block + 16 (i / 8) + 8 hi + i mod 8 of row pw
+  const int pw = 32 * half + sigma(col);
+  f32x16_t st[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) st[b] = f32x16_t{};
+  const int64_t slot_at = (((int64_t)slot * p.H + h) * P + pw) * N + 8 * hi;
+  if (!alone && (sp.part > 0 || p.initial.data != nullptr)) {
+    const bool carried = sp.part > 0;
+    const int dtype = carried ? (int)LQ_F32 : p.initial.dtype;
+    const char* at = carried ? (const char*)(p.slot_state + slot_at - (int64_t)p.H * P * N)
+                             : (const char*)p.initial.data +
+                                   (sp.index * p.initial.s[0] + h * p.initial.s[1] + pw * p.initial.s[2] + 8 * hi) *
+                                       size_of(dtype);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float v[8];
+        load8(at + (32 * b + 16 * u) * size_of(dtype), dtype, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) st[b][8 * u + i] = v[i];
+      }
+    }
+  }
+
+  // loads of a chunk: each wave 16 rows of B and of C, and 32 of one head's x
+  const int bs = (int)p.B.s[1] * 2, cs = (int)p.C.s[1] * 2, xs = (int)p.x.s[1] * 2;
+  const int64_t row0 = sp.begin + from;
+  const char* bbase = (const char*)p.B.data + (lead * p.B.s[0] + row0 * p.B.s[1] + g * p.B.s[2]) * 2;
+  const char* cbase = (const char*)p.C.data + (lead * p.C.s[0] + row0 * p.C.s[1] + g * p.C.s[2]) * 2;
+  const char* xbase = (const char*)p.x.data + (lead * p.x.s[0] + row0 * p.x.s[1] + h * p.x.s[2]) * 2;
+  const int rows = to - from, chunks = (rows + Q - 1) / Q;
+  auto load_chunk = [&](int k) {
+    const int have = min(Q, rows - k * Q);
+    const i32x4_t bd = make_desc(bbase + (int64_t)k * Q * bs, (have - 1) * bs + N * 2);
+    const i32x4_t xd = make_desc(xbase + (int64_t)k * Q * xs, (have - 1) * xs + P * 2);
+    lds_t b_to = (lds_t)&lds.b[k & 1][wave * 4096], c_to = (lds_t)&lds.c[wave * 4096];
+    lds_t x_to = (lds_t)&lds.x[hw][half * 4096];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = wave * 16 + j * 4 + (lane >> 4);
+      load_rows_to_lds(bd, b_to + j * 1024, r * bs + 16 * ((lane & 15) ^ swizzle_b(r)));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = half * 32 + j * 8 + (lane >> 3);
+      load_rows_to_lds(xd, x_to + j * 1024, r * xs + 16 * ((lane & 7) ^ (4 * ((r >> 1) & 1))));
+    }
+    if (!alone) {
+      const i32x4_t cd = make_desc(cbase + (int64_t)k * Q * cs, (have - 1) * cs + N * 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = wave * 16 + j * 4 + (lane >> 4);
+        load_rows_to_lds(cd, c_to + j * 1024, r * cs + 16 * ((lane & 15) ^ (r & 15)));
+      }
+    }
+  };
+
+  // the fourth wave: steps of a chunk, lane = row (rows past the end have dt = 0 and change nothing)
+  float raw[HEADS] = {0.f, 0.f}, bias[HEADS];
+  double A[HEADS];
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    A[j] = (double)load_float(p.A.data, p.A.dtype, (h0 + j) * p.A.s[0]) * 1.4426950408889634;
+    bias[j] = p.bias.data == nullptr ? 0.f : load_float(p.bias.data, p.bias.dtype, (h0 + j) * p.bias.s[0]);
+  }
+  const int64_t dt_at = lead * p.dt.s[0] + row0 * p.dt.s[1] + h0 * p.dt.s[2];
+  auto load_steps = [&](int k) {
+    const int r = k * Q + lane;
+    if (r >= rows) return;
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j) {
+      raw[j] = load_float(p.dt.data, p.dt.dtype, dt_at + (int64_t)r * p.dt.s[1] + j * p.dt.s[2]);
+    }
+  };
+  struct Steps {
+    int whole[HEADS];
+    float rest[HEADS], step[HEADS], weight[HEADS];
+  } next;
+  auto make_steps = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j) {
+      const bool in = k * Q + lane < rows;
+      const float dt = in ? scan_step(p, raw[j], bias[j]) : 0.f;
+      // (a NaN step has a decay here, and its NaN in what it multiplies)
+      const double c = prefix_sum(in ? fmin(fmax(A[j] * dt, -256.0), 256.0) : 0.0);
+      const uint64_t u = __builtin_bit_cast(uint64_t, c);
+      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, 63);
+      const uint32_t up = __builtin_amdgcn_readlane((uint32_t)(u >> 32), 63);
+      const double all = __builtin_bit_cast(double, ((uint64_t)up << 32) | lo), whole = __builtin_rint(c);
+      const float rest = (float)(c - whole);
+      next.whole[j] = (int)whole;
+      next.rest[j] = __builtin_amdgcn_exp2f(rest);
+      next.step[j] = dt * __builtin_amdgcn_exp2f(-rest);
+      next.weight[j] = in ? dt * __builtin_amdgcn_exp2f((float)(all - c)) : 0.f;
+    }
+  };
+  auto put_steps = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j) {
+      lds.whole[j][lane] = next.whole[j];
+      lds.rest[j][lane] = next.rest[j];
+      lds.step[j][lane] = next.step[j];
+      lds.weight[k & 1][j][lane] = next.weight[j];
+    }
+  };
+
+  const float D = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, h0 * p.D.s[0]);
+  const float D1 = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, (h0 + 1) * p.D.s[0]);
+  // operand addresses within the tiles; a product step exchanges chunks (^)
+  const int sb = wave == 2, tb = wave != 0;  // the mixing block of waves 0 to 2
+  const int brow = 32 * sb + sigma(col);
+  const int b_row_at = brow * 256 + 16 * (hi ^ swizzle_b(brow));
+  const int c_row_at = col * 256 + 16 * (hi ^ (col & 15));
+  const int j16 = lane & 15, g1 = (lane >> 4) & 1;
+  const int col_chunk = 2 * g1 + (j16 & 1), col_half = 8 * ((j16 >> 1) & 1), tr = 8 * hi + (j16 >> 2);
+  const int b_col_at0 = tr * 256 + 16 * (col_chunk ^ swizzle_b(tr)) + col_half;
+  const int b_col_at1 = (tr + 4) * 256 + 16 * (col_chunk ^ swizzle_b(tr + 4)) + col_half;
+  const int x_col_at = tr * 128 + 16 * ((4 * half + col_chunk) ^ (4 * (j16 >> 3))) + col_half;
+  const int m_at = col * 64 + 16 * (hi ^ ((col >> 2) & 3));
+  float log_decay = 0.f;
+
+  if (chunks > 0) {
+    if (wave == 3) {
+      load_steps(0);
+      make_steps(0);
+      put_steps(0);
+      load_steps(1);
+    }
+    load_chunk(0);
+  }
+  for (int k = 0; k < chunks; ++k) {
+    const int buf = k & 1;
+    wait_loads<0>();
+    __syncthreads();
+    lds_t xt = (lds_t)&lds.x[hw][0], bt = (lds_t)&lds.b[buf][0], ct = (lds_t)&lds.c[0];
+    words4_t xa[4];  // x of rows s = 16 i + 8 hi .. + 7 in column pw
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lds_t at = xt + x_col_at + i * 16 * 128;
+      xa[i] = lds_read_columns(at, at + 4 * 128);
+    }
+    f32x16_t y[2] = {};
+    words4_t xc[4];  // the same without what is not finite
+    if (!alone) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xc[i] = xa[i];
+      f32x16_t mix = {};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        words4_t s16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s16[e] = pack2<true>(st[i >> 1][8 * (i & 1) + 2 * e], st[i >> 1][8 * (i & 1) + 2 * e + 1]);
+        }
+        const words4_t c0 = lds_read16(ct + (c_row_at ^ (32 * i)));
+        const words4_t c1 = lds_read16(ct + (c_row_at ^ (32 * i)) + 32 * 256);
+        y[0] = mfma<true>(s16, c0, y[0]);
+        y[1] = mfma<true>(s16, c1, y[1]);
+        if (wave < 3) mix = mfma<true>(lds_read16(bt + (b_row_at ^ (32 * i))), tb ? c1 : c0, mix);
+      }
+      if (wave < 3) {
+        // mix[8 u + e]: row s = 32 sb + 16 u + 8 hi + e, column t = 32 tb + col
+#pragma unroll
+        for (int j = 0; j < HEADS; ++j) {
+          const int at_t = lds.whole[j][32 * tb + col];
+          const float rest = lds.rest[j][32 * tb + col];
+          words4_t w[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float v[8];
+            const int s0 = 32 * sb + 16 * u + 8 * hi;
+            const int4 n0 = *(const int4*)&lds.whole[j][s0], n1 = *(const int4*)&lds.whole[j][s0 + 4];
+            const float4 d0 = *(const float4*)&lds.step[j][s0], d1 = *(const float4*)&lds.step[j][s0 + 4];
+            const int n[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+            const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              v[e] = __builtin_amdgcn_ldexpf(mix[8 * u + e] * (d[e] * rest), at_t - n[e]);
+            }
+            if (sb == tb) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int s = 16 * u + 8 * hi + e;
+                v[e] = s < col ? v[e] : s == col ? v[e] + (j ? D1 : D) : 0.f;
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[u][e] = pack2<true>(v[2 * e], v[2 * e + 1]);
+          }
+          lds_t at = (lds_t)&lds.m[j][sb + tb][0];
+          *(__attribute__((address_space(3))) words4_t*)(at + m_at) = w[0];
+          *(__attribute__((address_space(3))) words4_t*)(at + (m_at ^ 32)) = w[1];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        y[b] *= __builtin_amdgcn_ldexpf(lds.rest[hw][32 * b + col], lds.whole[hw][32 * b + col]);
+      }
+      // the largest exponent of the lane's x
+      typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+      u16x2_t most = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, xa[i >> 2][i & 3] & 0x7fff7fffu));
+      }
+      if (__any(most[0] >= 0x7f80 || most[1] >= 0x7f80)) {
+        for (int s = 0; s < Q; ++s) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int q = 32 * half + 16 * (i >> 3) + 8 * hi + (i & 7);
+            const float v = bf16_bits_to_float(*(const uint16_t*)&lds.x[hw][s * 128 + 16 * ((q >> 3) ^ (4 * ((s >> 1) & 1))) + 2 * (q & 7)]);
+            if (v - v == 0.f) continue;
+            if (s <= col) y[0][i] += v;
+            if (s <= 32 + col) y[1][i] += v;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          uint32_t w = xc[i >> 2][i & 3];
+          if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+          if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+          xc[i >> 2][i & 3] = w;
+        }
+      }
+    }
+    const int whole = lds.whole[hw][Q - 1];  // the chunk's decay
+    const float rest = lds.rest[hw][Q - 1];
+    if (wave == 3 && k + 1 < chunks) {
+      make_steps(k + 1);
+      load_steps(k + 2);
+    }
+    __syncthreads();
+    if (k + 1 < chunks) {
+      load_chunk(k + 1);
+      if (wave == 3) put_steps(k + 1);
+    }
+    if (!alone) {
+      lds_t mt = (lds_t)&lds.m[hw][0][0];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        y[0] = mfma<true>(xc[i], lds_read16(mt + (m_at ^ (32 * i))), y[0]);
+        y[1] = mfma<true>(xc[i], lds_read16(mt + 2048 + (m_at ^ (32 * i))), y[1]);
+        y[1] = mfma<true>(xc[i + 2], lds_read16(mt + 4096 + (m_at ^ (32 * i))), y[1]);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int r = k * Q + 32 * b + col;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int q = 32 * half + 16 * u + 8 * hi;
+          if (p.z.data != nullptr) {
+            const words4_t z = *(const words4_t*)((const uint16_t*)p.z.data + lead * p.z.s[0] +
+                                                  (row0 + r) * p.z.s[1] + h * p.z.s[2] + q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[b][8 * u + e] *= scan_silu(word_elem(z[e >> 1], (e & 1) * 16, LQ_BF16));
+          }
+          words4_t w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pack2<true>(y[b][8 * u + 2 * e], y[b][8 * u + 2 * e + 1]);
+          *(words4_t*)(out + r * p.out.s[1] + h * p.out.s[2] + q) = w;
+        }
+      }
+    }
+    const float keep = __builtin_amdgcn_ldexpf(rest, whole);
+    log_decay += (float)whole + __builtin_amdgcn_logf(rest);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) st[b] *= keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 w0 = *(const float4*)&lds.weight[buf][hw][16 * i + 8 * hi];
+      const float4 w1 = *(const float4*)&lds.weight[buf][hw][16 * i + 8 * hi + 4];
+      const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+      words4_t top, rest;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = w[2 * e] * __uint_as_float(xa[i][e] << 16);
+        const float b = w[2 * e + 1] * __uint_as_float(xa[i][e] & 0xffff0000u);
+        const uint32_t ab = pack2<true>(a, b);
+        top[e] = ab;
+        rest[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const words4_t bc = lds_read_columns(bt + (b_col_at0 ^ (64 * b)) + i * 16 * 256,
+                                             bt + (b_col_at1 ^ (64 * b)) + i * 16 * 256);
+        st[b] = mfma<true>(bc, top, st[b]);
+        st[b] = mfma<true>(bc, rest, st[b]);
+      }
+    }
+  }
+
+  const bool last = !FOLLOWED && sp.part == nseg - 1 && p.states.data != nullptr;
+  if (!FOLLOWED && !last) return;
+  const int dtype = FOLLOWED ? (int)LQ_F32 : p.states.dtype;
+  char* at = FOLLOWED ? (char*)(p.slot_state + slot_at)
+                      : (char*)p.states.data +
+                            (sp.index * p.states.s[0] + h * p.states.s[1] + pw * p.states.s[2] + 8 * hi) *
+                                size_of(dtype);
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = st[b][8 * u + i];
+      store8(at + (32 * b + 16 * u) * size_of(dtype), dtype, v);
+    }
+  }
+  if (FOLLOWED && half == 0 && lane == 0) p.slot_log[(int64_t)slot * p.H + h] = log_decay;
+}
+
+// Values in a row, every row 16-byte aligned.
+bool rows_fit(const lq_tensor* t) {
+  if (t == nullptr) return true;
+  const int nd = t->ndim;
+  if (t->stride[nd - 1] != 1 || ((uintptr_t)t->data & 15) != 0) return false;
+  for (int i = 0; i < nd - 1; ++i) {
+    if (t->shape[i] > 1 && t->stride[i] * dtype_size(t->dtype) % 16 != 0) return false;
+  }
+  return true;
+}
+
+}  // namespace
+
+bool prompt_scan_mfma_fits(const lq_tensor* x, const lq_tensor* B, const lq_tensor* C,
+                           const lq_tensor* z, const lq_tensor* initial, const lq_tensor* states,
+                           const lq_tensor* out) {
+  const int nd = x->ndim;
+  const int64_t H = x->shape[nd - 2], G = B->shape[nd - 2];
+  if (x->dtype != LQ_BF16 || out->dtype != LQ_BF16 || (z != nullptr && z->dtype != LQ_BF16)) return false;
+  if (x->shape[nd - 1] != P || B->shape[nd - 1] != N || H / G % HEADS != 0) return false;
+  const lq_tensor* ts[7] = {x, B, C, z, initial, states, out};
+  for (const lq_tensor* t : ts) {
+    if (!rows_fit(t)) return false;
+  }
+  const lq_tensor* loaded[3] = {x, B, C};
+  for (const lq_tensor* t : loaded) {
+    const int64_t s = t->stride[nd - 3];
+    if (t->shape[nd - 3] > 1 && (s < t->shape[nd - 1] || s > (1 << 22))) return false;
+  }
+  return true;
+}
+
+void launch_prompt_scan_mfma(const PromptScan& p, bool followed, int64_t parts, hipStream_t st) {
+  const dim3 grid((unsigned)(parts * (p.H / HEADS))), block(256);
+  if (followed) hipLaunchKernelGGL(scan_chunks_kernel<true>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(scan_chunks_kernel<false>, grid, block, 0, st, p);
+}
+
+}  // namespace lq
