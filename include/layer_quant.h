@@ -396,10 +396,10 @@ int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor*
  *   A [H], D NULL or [H], dt_bias NULL or [H]; initial NULL or [S, H, P, N], states NULL or [S, H, P, N]
  *   (the state behind each prompt; an empty one's is its initial state). They may be one tensor; else no
  *   output may overlap an input. x, B and C of one dtype, the others of any float dtype; any strides.
- *   N <= 256. The workspace needs no particular contents; `packed` is 1 where starts are given, `batch`
- *   then ignored but for 0.
+ *   N <= 256. The workspace needs no particular contents; dtype is x's, `prompts` S and `rows` T (packed
+ *   1) or L (packed 0).
  */
-size_t lq_prompt_scan_workspace(int64_t batch, int64_t rows, int packed, int64_t heads,
+size_t lq_prompt_scan_workspace(int dtype, int64_t prompts, int64_t rows, int packed, int64_t heads,
                                 int64_t head_dim, int64_t dstate);
 int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_tensor* A, const lq_tensor* B,
                    const lq_tensor* C, const lq_tensor* starts, const lq_tensor* D,

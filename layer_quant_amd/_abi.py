@@ -187,7 +187,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.lq_prompt_attention.restype = ctypes.c_int
     lib.lq_prompt_attention.argtypes = [_P] * 5 + [ctypes.c_float, ctypes.c_void_p]
     lib.lq_prompt_scan_workspace.restype = ctypes.c_size_t
-    lib.lq_prompt_scan_workspace.argtypes = [ctypes.c_int64] * 2 + [ctypes.c_int] + [ctypes.c_int64] * 3
+    lib.lq_prompt_scan_workspace.argtypes = ([ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_int]
+                                             + [ctypes.c_int64] * 3)
     lib.lq_prompt_scan.restype = ctypes.c_int
     lib.lq_prompt_scan.argtypes = [_P] * 12 + [ctypes.c_int, ctypes.c_float, ctypes.c_float,
                                                ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
@@ -799,9 +800,9 @@ def prompt_scan(x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out, dt_
             return out
     dev = _require_gpu(x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out)
     stream = _stream(dev)
-    batch, rows = (1, x.shape[0]) if starts is not None else x.shape[:2]
-    need = int(lib().lq_prompt_scan_workspace(batch, rows, int(starts is not None), *x.shape[-2:],
-                                              B.shape[-1]))
+    prompts, rows = (starts.numel() - 1, x.shape[0]) if starts is not None else x.shape[:2]
+    need = int(lib().lq_prompt_scan_workspace(DTYPE_CODES.get(x.dtype, 0), prompts, rows,
+                                              int(starts is not None), *x.shape[-2:], B.shape[-1]))
     ws = _scratch.get(dev.index, stream, need) if need else None
     rc = lib().lq_prompt_scan(*map(desc, (x, dt, A, B, C, starts, D, z, dt_bias, initial, states, out)),
                               1 if dt_softplus else 0, float(dt_min), float(dt_max),

@@ -438,10 +438,11 @@ PyObject* py_prompt_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const lq_tensor* const* p = t.ptr;
   const bool packed = p[5] != nullptr;
   const int nd = packed ? 3 : 4;
-  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim != nd || p[3] == nullptr || p[3]->ndim != nd);
-  const size_t need = entries.scan_workspace(packed ? 1 : p[0]->shape[0], p[0]->shape[nd - 3], packed,
-                                             p[0]->shape[nd - 2], p[0]->shape[nd - 1],
-                                             p[3]->shape[nd - 1]);
+  LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim != nd || p[3] == nullptr || p[3]->ndim != nd ||
+               (packed && p[5]->ndim != 1));
+  const size_t need = entries.scan_workspace(p[0]->dtype, packed ? p[5]->shape[0] - 1 : p[0]->shape[0],
+                                             p[0]->shape[nd - 3], packed, p[0]->shape[nd - 2],
+                                             p[0]->shape[nd - 1], p[3]->shape[nd - 1]);
   return launch_with(t.device, a[15], need, [&](void* ws, size_t bytes, void* s) {
     return entries.scan(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], p[11],
                         softplus, lo, hi, ws, bytes, s);

@@ -68,4 +68,16 @@ __device__ __forceinline__ void load_rows_to_lds(i32x4_t desc, lds_t lds, int vo
       : "memory", "m0");
 }
 
+// The same with 4 bytes per lane.
+__device__ __forceinline__ void load_words_to_lds(i32x4_t desc, lds_t lds, int voff) {
+  const uint32_t addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds"
+      :
+      : "s"(addr), "v"(voff), "s"(desc)
+      : "memory", "m0");
+}
+
 }  // namespace lq

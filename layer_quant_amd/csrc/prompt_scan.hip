@@ -6,10 +6,11 @@
 //   y_t = S_t C_t + D x_t,  y_t *= silu(z_t)
 //
 // A prompt's rows fall into segments. Where a prompt has more than one, so that a few long prompts fill
-// the GPU too, a first launch finds the state that each segment but the last adds by itself (the first
-// segment starts from the given state and is finished there), a second one carries the states from
-// segment to segment, and the last launch runs the others from the state in front of them. A prompt of
-// one segment takes the last launch alone. The segment's length follows from the sizes (plan_segment).
+// the GPU too, a first launch finds what each segment but the last adds to the state by itself, a second
+// one carries the states from segment to segment, and the last launch runs every segment from the state in
+// front of it. (The first segment's is a copy, as the given states may be the tensor that the last segment
+// writes.) A prompt of one segment takes the last launch alone. The segment's length follows from the sizes
+// (plan_segment).
 //
 // scan_rows_kernel walks the rows one by one with the state in registers, fp32 throughout: the kernel of
 // fp32 and fp16 inputs and of every geometry that the matrix kernel does not take. A thread holds 4 p x
@@ -50,17 +51,13 @@ __device__ __forceinline__ float sums_of_four(const float (&v)[4], int lane) {
   return r;
 }
 
-// FOLLOWED: the segments that others of their prompt follow (blockIdx: slot), else those that are left.
-template <int NPL, bool FOLLOWED>
+template <int NPL, bool ADDS>
 __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
   __shared__ RowTile<NPL> tile;
-  const int h = blockIdx.x % p.H, t0 = blockIdx.x / p.H;
-  Span sp;
-  const bool mine = find_span(
-      p.spans, t0,
-      [&](int len, bool gap) { return FOLLOWED ? followed_segments_of(p, len, gap) : segments_of(p, len, gap); },
-      sp);
-  if (!mine) return;
+  const int h = blockIdx.x % p.H;
+  const Segment seg = find_segment<ADDS>(p, blockIdx.x / p.H);
+  if (!seg.valid) return;
+  const Span& sp = seg.span;
   const int tid = threadIdx.x, lane = tid & 63, nl = lane & 15;
   const int pb = blockIdx.y * PB, width = min(PB, p.P - pb);
   const int p0 = (tid >> 6) * 16 + (lane >> 4) * 4;  // of the thread's 4 p
@@ -75,24 +72,17 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
     }
     return;
   }
-  const int nseg = segments_of(p, sp.len, false);
-  const int slot = FOLLOWED ? t0 : sp.before + sp.part;
-  if (!FOLLOWED && nseg > 1 && sp.part == 0) return;  // finished by the first launch
-  if (slot > p.slots) return;                         // starts out of order ask for more than there are
-  const bool alone = FOLLOWED && sp.part > 0;         // from no state, and no y
-
   float st[4][NPL];
-  const int64_t slot_at = (((int64_t)slot * p.H + h) * p.P + pb + p0) * p.N;
-  const int64_t prev_at = slot_at - (int64_t)p.H * p.P * p.N;
+  const int64_t slot_at = (((int64_t)seg.slot * p.H + h) * p.P + pb + p0) * p.N;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
       const int n = 64 * (j >> 2) + 4 * nl + (j & 3);
       float v = 0.f;
-      if (!alone && p0 + i < width && n < p.N) {
-        if (sp.part > 0) {
-          v = p.slot_state[prev_at + (int64_t)i * p.N + n];
+      if (!ADDS && p0 + i < width && n < p.N) {
+        if (seg.several) {
+          v = p.slot_state[slot_at + (int64_t)i * p.N + n];
         } else if (p.initial.data != nullptr) {
           v = load_float(p.initial.data, p.initial.dtype,
                          sp.index * p.initial.s[0] + h * p.initial.s[1] +
@@ -155,12 +145,12 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
           }
         }
       }
-      if (!alone) {
+      if (!ADDS) {
         const float sum = sums_of_four(y, lane);
         if ((lane & 3) == 0) tile.y[r][p0 + ((lane >> 2) & 3)] = sum;
       }
     }
-    if (!alone) {
+    if (!ADDS) {
       __syncthreads();
       for (int i = tid; i < rows * PB; i += blockDim.x) {
         const int r = i / PB, c = i % PB;
@@ -173,17 +163,18 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
       }
     }
   }
-  if (FOLLOWED) {
+  if (ADDS) {
+    const int64_t next_at = slot_at + (int64_t)p.H * p.P * p.N;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int j = 0; j < NPL; ++j) {
         const int n = 64 * (j >> 2) + 4 * nl + (j & 3);
-        if (p0 + i < width && n < p.N) p.slot_state[slot_at + (int64_t)i * p.N + n] = st[i][j];
+        if (p0 + i < width && n < p.N) p.slot_state[next_at + (int64_t)i * p.N + n] = st[i][j];
       }
     }
-    if (tid == 0 && blockIdx.y == 0) p.slot_log[(int64_t)slot * p.H + h] = log_decay;
-  } else if (sp.part == nseg - 1 && p.states.data != nullptr) {
+    if (tid == 0 && blockIdx.y == 0) p.slot_log[(int64_t)(seg.slot + 1) * p.H + h] = log_decay;
+  } else if (to == sp.len && p.states.data != nullptr) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -200,25 +191,68 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
   }
 }
 
-// The states behind the segments of a prompt from what each adds by itself, in place. blockIdx.y: slot;
-// the first slot of a prompt carries all of its own.
+constexpr int AHEAD = 8;
+
+// The states in front of a prompt's segments from what the segments in front of them add, in place.
+// blockIdx.y: slot; a prompt's first one carries all of its own. Four consecutive values per thread.
 __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
   Span sp;
-  if (!find_span(p.spans, blockIdx.y,
-                 [&](int len, bool gap) { return followed_segments_of(p, len, gap); }, sp)) {
+  const auto slots = [&](int len, bool gap) { return slots_of_span(p, len, gap); };
+  if (!find_span(p.spans, blockIdx.y, slots, sp) || sp.part != 0) return;
+  const int many = min(slots_of_span(p, sp.len, false), p.slots - (int)blockIdx.y);
+  const int64_t size = (int64_t)p.H * p.P * p.N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= size) return;
+  float* state = p.slot_state + (int64_t)blockIdx.y * size + i;
+  const int have = (int)min((int64_t)4, size - i);
+  float held[4];
+  int head[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t at = i + min(e, have - 1);
+    const int n = (int)(at % p.N), pp = (int)(at / p.N % p.P);
+    head[e] = (int)(at / ((int64_t)p.P * p.N));
+    held[e] = 0.f;
+    if (p.initial.data != nullptr) {
+      held[e] = load_float(p.initial.data, p.initial.dtype,
+                           sp.index * p.initial.s[0] + head[e] * p.initial.s[1] + pp * p.initial.s[2] +
+                               n * p.initial.s[3]);
+    }
+  }
+  if (size % 4 == 0 && p.P * p.N % 4 == 0) {
+    const float* lg = p.slot_log + (int64_t)blockIdx.y * p.H + head[0];
+    float4 h4 = make_float4(held[0], held[1], held[2], held[3]);
+    *(float4*)state = h4;
+    // eight loads go out before the first is needed
+    for (int j = 1; j < many; j += AHEAD) {
+      float4 add[AHEAD];
+      float keep[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const int k = min(j + e, many - 1);
+        add[e] = *(const float4*)(state + k * size);
+        keep[e] = lg[(int64_t)k * p.H];
+      }
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        if (j + e >= many) break;
+        const float a = __builtin_amdgcn_exp2f(keep[e]);
+        h4.x = fmaf(h4.x, a, add[e].x);
+        h4.y = fmaf(h4.y, a, add[e].y);
+        h4.z = fmaf(h4.z, a, add[e].z);
+        h4.w = fmaf(h4.w, a, add[e].w);
+        *(float4*)(state + (j + e) * size) = h4;
+      }
+    }
     return;
   }
-  if (sp.part != 0) return;
-  const int many = min(followed_segments_of(p, sp.len, false), p.slots - (int)blockIdx.y);
-  const int64_t size = (int64_t)p.H * p.P * p.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= size) return;
-  const int h = (int)(i / ((int64_t)p.P * p.N));
-  float* state = p.slot_state + (int64_t)blockIdx.y * size + i;
-  const float* lg = p.slot_log + (int64_t)blockIdx.y * p.H + h;
-  float held = state[0];
-  for (int j = 1; j < many; ++j) {
-    held = fmaf(held, __builtin_amdgcn_exp2f(lg[(int64_t)j * p.H]), state[j * size]);
-    state[j * size] = held;
+  for (int e = 0; e < have; ++e) {
+    float v = held[e];
+    state[e] = v;
+    for (int j = 1; j < many; ++j) {
+      v = fmaf(v, __builtin_amdgcn_exp2f(p.slot_log[((int64_t)blockIdx.y + j) * p.H + head[e]]),
+               state[j * size + e]);
+      state[j * size + e] = v;
+    }
   }
 }
 
@@ -232,19 +266,22 @@ int64_t plan_segment(int64_t rows, int64_t heads) {
   return seg < MIN_SEGMENT ? MIN_SEGMENT : seg;
 }
 
-// Segments that others follow, at most.
-int64_t slots_of(int64_t batch, int64_t rows, int64_t segment, bool packed) {
-  return packed ? rows / segment : rows == 0 ? 0 : batch * ((rows + segment - 1) / segment - 1);
+// Slots, at most: a prompt has a segment more than its rows fill, or, as one of several segments has more
+// rows than one of them, less than two for each segment's rows.
+int64_t slots_of(int64_t prompts, int64_t rows, int64_t segment, bool packed) {
+  const int64_t n = (rows + segment - 1) / segment;
+  if (n < 2) return 0;
+  return packed ? min(rows / segment + prompts, 2 * rows / segment) : prompts * n;
 }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-template <bool FOLLOWED>
+template <bool ADDS>
 void launch_rows(const PromptScan& p, dim3 grid, hipStream_t st) {
   const dim3 block(64 * min(4, (p.P + 15) / 16));
-  if (p.N <= 64) hipLaunchKernelGGL((scan_rows_kernel<4, FOLLOWED>), grid, block, 0, st, p);
-  else if (p.N <= 128) hipLaunchKernelGGL((scan_rows_kernel<8, FOLLOWED>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((scan_rows_kernel<16, FOLLOWED>), grid, block, 0, st, p);
+  if (p.N <= 64) hipLaunchKernelGGL((scan_rows_kernel<4, ADDS>), grid, block, 0, st, p);
+  else if (p.N <= 128) hipLaunchKernelGGL((scan_rows_kernel<8, ADDS>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((scan_rows_kernel<16, ADDS>), grid, block, 0, st, p);
 }
 
 }  // namespace
@@ -252,12 +289,14 @@ void launch_rows(const PromptScan& p, dim3 grid, hipStream_t st) {
 
 using namespace lq;
 
-extern "C" size_t lq_prompt_scan_workspace(int64_t batch, int64_t rows, int packed, int64_t heads,
-                                           int64_t head_dim, int64_t dstate) {
-  if (batch <= 0 || rows <= 0 || heads <= 0 || head_dim <= 0 || dstate <= 0) return 0;
-  const int64_t total = packed ? rows : batch * rows;
-  const int64_t slots = slots_of(batch, rows, plan_segment(total, heads), packed != 0);
-  return align256((size_t)(slots * heads * head_dim * dstate) * 4) + align256((size_t)(slots * heads) * 4);
+extern "C" size_t lq_prompt_scan_workspace(int dtype, int64_t prompts, int64_t rows, int packed,
+                                           int64_t heads, int64_t head_dim, int64_t dstate) {
+  if (prompts <= 0 || rows <= 0 || heads <= 0 || head_dim <= 0 || dstate <= 0) return 0;
+  const int64_t total = packed ? rows : prompts * rows;
+  const int64_t slots = slots_of(prompts, rows, plan_segment(total, heads), packed != 0);
+  const bool mfma = prompt_scan_mfma_geometry(dtype, heads, head_dim, dstate);
+  return align256((size_t)(slots * heads * head_dim * dstate) * 4) + align256((size_t)(slots * heads) * 4) +
+         (mfma ? prompt_scan_mfma_workspace(total, heads) : 0);
 }
 
 extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_tensor* A,
@@ -322,15 +361,17 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
                 (long long)total, (long long)S);
   }
   p.segment = (int)plan_segment(total, H);
-  const int64_t slots = slots_of(batch, rows, p.segment, nd == 3);
+  const int64_t slots = slots_of(S, rows, p.segment, nd == 3);
   const int64_t parts =
       nd == 4 ? batch * (rows == 0 ? 1 : (rows + p.segment - 1) / p.segment) : rows / p.segment + S + 2;
   const int64_t pblocks = (P + PB - 1) / PB;
-  if (parts * H * pblocks >= ((int64_t)1 << 32) / 256 || slots > 65535) {
+  const int64_t chunks = nd == 4 ? batch * ((rows + 63) / 64) : rows / 64 + S;
+  if (parts * H * pblocks >= ((int64_t)1 << 32) / 256 || slots > 65535 ||
+      chunks * ((H + 31) / 32) >= ((int64_t)1 << 32) / 256) {
     return fail(LQ_ERR_UNSUPPORTED, "%lld parts of %lld heads exceed the launch limits",
                 (long long)parts, (long long)H);
   }
-  const size_t need = lq_prompt_scan_workspace(batch, rows, nd == 3, H, P, N);
+  const size_t need = lq_prompt_scan_workspace(x->dtype, S, rows, nd == 3, H, P, N);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     return fail(LQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
@@ -361,6 +402,8 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   p.dt_max = dt_max;
   p.slot_state = (float*)workspace;
   p.slot_log = (float*)((char*)workspace + align256((size_t)(slots * H * P * N) * 4));
+  p.steps = (float*)((char*)p.slot_log + align256((size_t)(slots * H) * 4));
+  p.rows = total;
   const hipStream_t st = (hipStream_t)stream;
   const bool mfma = !diag(LQ_DIAG_PROMPT_FORCE_GENERIC) &&
                     prompt_scan_mfma_fits(x, B, C, z, initial, states, out);
@@ -368,11 +411,15 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
     return fail(LQ_ERR_INVALID_ARG, "the call takes the general kernel");
   }
   const unsigned blocks = (unsigned)((H * P * N + 255) / 256);
+  if (mfma && total > 0) {
+    launch_prompt_scan_steps(p, chunks, st);
+    if ((rc = check_launch("lq_prompt_scan (steps)")) != LQ_OK) return rc;
+  }
   if (slots > 0) {
     if (mfma) launch_prompt_scan_mfma(p, true, slots, st);
     else launch_rows<true>(p, dim3((unsigned)(slots * H), (unsigned)pblocks), st);
     if ((rc = check_launch("lq_prompt_scan (segments)")) != LQ_OK) return rc;
-    hipLaunchKernelGGL(scan_carry_kernel, dim3(blocks, (unsigned)slots), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(scan_carry_kernel, dim3((blocks + 3) / 4, (unsigned)slots), dim3(256), 0, st, p);
     if ((rc = check_launch("lq_prompt_scan (carry)")) != LQ_OK) return rc;
   }
   if (parts > 0) {

@@ -1,12 +1,14 @@
 // prompt_scan.hip's operator for bf16 x, B and C with head_dim 64 and a state of 128, on
 // v_mfma_f32_32x32x16_bf16: prompts in chunks of 64 rows. With c the running sum of A dt log2(e) within a
 // chunk, S the state in front of it and t, s rows of it,
-//   Y[t] = 2^c_t S C_t + sum_{s <= t} M[t][s] x_s,  M[t][s] = 2^(c_t - c_s) dt_s (C_t . B_s), + D where s = t
+//   Y[t] = 2^c_t S C_t + sum_{s <= t} M[t][s] x_s + D x_t,  M[t][s] = 2^(c_t - c_s) dt_s (C_t . B_s)
 //   S'   = 2^c_63 S + sum_s w_s x_s B_s^T,          w_s = 2^(c_63 - c_s) dt_s
 // c is summed in 64 bits and taken apart into a whole number n and a rest: 2^(c_t - c_s) is the product of
 // 2^(n_t - n_s), exact, and of two factors between 0.7 and 1.42 that a row has once. So no decay overflows
 // however fast a state fades, close rows behind a large c keep their digits, and no element of M takes an
-// exponential. (A step's decay is held within 2^-256 and 2^256.)
+// exponential. (A step's decay is held within 2^-256 and 2^256.) scan_steps_kernel makes these numbers of
+// every row and head beforehand: in this kernel one wave made them while the others waited, 260 us of 539
+// for a prompt of 16384 rows.
 //
 // A workgroup of four waves has two heads of one group; wave (head, half) keeps rows p = 32 half .. + 31 of
 // its head's state, transposed, in 64 accumulators. Of B^T x that is the layout in which S is, rounded to
@@ -16,16 +18,18 @@
 // Per chunk:
 //   phase 1  S C^T (16 products) with C's operands shared by the mixing scores B C^T, of which three waves
 //            make one 32 x 32 block each (the fourth lies above the diagonal) for both heads and leave M in
-//            LDS as bf16; the fourth wave makes the next chunk's steps and decays
-//   phase 2  Y += M x (6 products), stores, S' (32 products)
-// B lies in two LDS buffers; C and x are read in phase 1 alone, so that one buffer each is refilled in
-// phase 2: 79 KB per workgroup, two of them per CU.
+//            LDS as bf16
+//   phase 2  Y += M x + D x (6 and 4 products), stores, S' (16 or 32 products)
+// B lies in two LDS buffers; C, x and the decays are read in phase 1 alone, so that one buffer each is
+// refilled in phase 2: 79 KB per workgroup, two of them per CU.
 //
-// Roundings: M and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result); w x, which a
-// state keeps, as the sum of two bf16 values (2^-16). Everything else is fp32.
+// Roundings: M, D and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result); w x, which a
+// state keeps, to the sum of two bf16 values (2^-16) where the states leave in fp32 and to one (2^-8, less
+// than they lose then) where they leave in 16 bits. Everything else is fp32.
 //
-// Rows behind a row in its chunk have M = 0 there, which an x of inf or NaN would turn into NaN: such values
-// are looked for when x is read, added to the rows that see them and left out of M x.
+// Rows behind a row in its chunk have M = 0 there, which an x of inf or NaN would turn into NaN. Such a value
+// stays in the state, so that it is enough to look at the state behind a segment: one that is not finite has
+// the segment run again, and then they are added to the rows that see them and left out of M x.
 #include "matrix16.h"
 #include "prompt_scan.h"
 
@@ -35,23 +39,6 @@ namespace {
 constexpr int Q = 64;      // rows of a chunk
 constexpr int HEADS = 2;   // of a workgroup
 constexpr int P = 64, N = 128;
-
-struct alignas(1024) ChunkLds {
-  char b[2][Q * N * 2];         // rows of 256 bytes; chunk k of row r at k ^ swizzle_b(r)
-  char c[Q * N * 2];            // the same with k ^ (r mod 16)
-  char x[HEADS][Q * P * 2];     // rows of 128 bytes, k ^ 4 ((r / 2) mod 2)
-  char m[HEADS][3][32 * 32 * 2];  // blocks (s, t) = (0, 0), (0, 1), (1, 1): row t, 64 bytes
-  int whole[HEADS][Q];          // n_s
-  float rest[HEADS][Q];         // 2^(c_s - n_s)
-  float step[HEADS][Q];         // dt_s 2^(n_s - c_s)
-  float weight[2][HEADS][Q];    // w_s
-};
-
-// Both four consecutive rows' runs of 4 chunks and 16 rows' equal chunks lie in different banks.
-__device__ __forceinline__ int swizzle_b(int r) { return 4 * (r & 3) | ((r >> 2) & 3); }
-
-// index of lane (or result row) m
-__device__ __forceinline__ int sigma(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
 
 // Inclusive sums over the wave's lanes.
 template <int CTRL, int ROWS>
@@ -70,6 +57,70 @@ __device__ __forceinline__ double prefix_sum(double v) {
   v += moved<0x143, 0xc>(v);
   return v;
 }
+
+struct alignas(1024) ChunkLds {
+  char b[2][Q * N * 2];         // rows of 256 bytes; chunk k of row r at k ^ swizzle_b(r)
+  char c[Q * N * 2];            // the same with k ^ (r mod 16)
+  char x[HEADS][Q * P * 2];     // rows of 128 bytes, k ^ 4 ((r / 2) mod 2)
+  char m[HEADS][3][32 * 32 * 2];  // blocks (s, t) = (0, 0), (0, 1), (1, 1): row t, 64 bytes
+  float weight[2][HEADS][Q];    // w_s
+  int whole[HEADS][Q];          // n_s
+  float rest[HEADS][Q];         // 2^(c_s - n_s)
+  float step[HEADS][Q];         // dt_s 2^(n_s - c_s)
+};
+
+// scan_steps_kernel's arrays, in p.steps: [array][head][row]
+enum { WEIGHT, WHOLE, REST, STEP };
+
+constexpr int STEP_HEADS = 16;  // of a workgroup of scan_steps_kernel
+
+// A chunk's decays and steps, lane = row.
+__global__ __launch_bounds__(256) void scan_steps_kernel(PromptScan p) {
+  __shared__ float tile[Q][STEP_HEADS + 1];
+  const int blocks = (p.H + STEP_HEADS - 1) / STEP_HEADS, hb = blockIdx.x % blocks * STEP_HEADS;
+  Span sp;
+  if (!find_span(p.spans, blockIdx.x / blocks, [&](int len, bool gap) { return gap ? 0 : (len + Q - 1) / Q; },
+                 sp)) {
+    return;
+  }
+  const int64_t lead = p.spans.starts == nullptr ? sp.index : 0, row0 = sp.begin + sp.part * Q;
+  const int have = min(Q, sp.len - sp.part * Q), heads = min(STEP_HEADS, p.H - hb);
+  for (int i = threadIdx.x; i < have * STEP_HEADS; i += 256) {
+    const int r = i / STEP_HEADS, j = i % STEP_HEADS;
+    if (j >= heads) continue;
+    tile[r][j] = load_float(p.dt.data, p.dt.dtype,
+                            lead * p.dt.s[0] + (row0 + r) * p.dt.s[1] + (hb + j) * p.dt.s[2]);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  for (int j = threadIdx.x >> 6; j < heads; j += 4) {
+    const int h = hb + j;
+    const double A = (double)load_float(p.A.data, p.A.dtype, h * p.A.s[0]) * 1.4426950408889634;
+    const float bias = p.bias.data == nullptr ? 0.f : load_float(p.bias.data, p.bias.dtype, h * p.bias.s[0]);
+    const bool in = lane < have;
+    const float dt = in ? scan_step(p, tile[lane][j], bias) : 0.f;
+    // (a NaN step has a decay here, and its NaN in what it multiplies)
+    const double c = prefix_sum(in ? fmin(fmax(A * dt, -256.0), 256.0) : 0.0);
+    const uint64_t u = __builtin_bit_cast(uint64_t, c);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, 63);
+    const uint32_t up = __builtin_amdgcn_readlane((uint32_t)(u >> 32), 63);
+    const double all = __builtin_bit_cast(double, ((uint64_t)up << 32) | lo), whole = __builtin_rint(c);
+    const float rest = (float)(c - whole);
+    if (!in) continue;
+    float* to = p.steps + h * p.rows + lead * p.spans.rows + row0 + lane;
+    const int64_t array = p.H * p.rows;
+    to[WEIGHT * array] = dt * __builtin_amdgcn_exp2f((float)(all - c));
+    to[WHOLE * array] = __int_as_float((int)whole);
+    to[REST * array] = __builtin_amdgcn_exp2f(rest);
+    to[STEP * array] = dt * __builtin_amdgcn_exp2f(-rest);
+  }
+}
+
+// Both four consecutive rows' runs of 4 chunks and 16 rows' equal chunks lie in different banks.
+__device__ __forceinline__ int swizzle_b(int r) { return 4 * (r & 3) | ((r >> 2) & 3); }
+
+// index of lane (or result row) m
+__device__ __forceinline__ int sigma(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
 
 // Eight consecutive state values.
 __device__ __forceinline__ void load8(const char* at, int dtype, float (&v)[8]) {
@@ -98,21 +149,16 @@ __device__ __forceinline__ void store8(char* at, int dtype, const float (&v)[8])
 
 __device__ __forceinline__ int size_of(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
 
-// FOLLOWED: as in scan_rows_kernel.
-template <bool FOLLOWED>
+// ADDS: find_segment's. LO: w x as the sum of two bf16 values.
+template <bool ADDS, bool LO>
 __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
   __shared__ ChunkLds lds;
   // the workgroups of a group's heads on one XCD (blocks go round the eight), as they read the same B and C
-  const int pairs = p.H / HEADS, idx = blockIdx.x % pairs, t0 = blockIdx.x / pairs;
+  const int pairs = p.H / HEADS, idx = blockIdx.x % pairs;
   const int pair = pairs % 8 == 0 ? (idx & 7) * (pairs / 8) + (idx >> 3) : idx;
-  Span sp;
-  if (!find_span(p.spans, t0,
-                 [&](int len, bool gap) {
-                   return FOLLOWED ? followed_segments_of(p, len, gap) : segments_of(p, len, gap);
-                 },
-                 sp)) {
-    return;
-  }
+  const Segment seg = find_segment<ADDS>(p, blockIdx.x / pairs);
+  if (!seg.valid) return;
+  const Span& sp = seg.span;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), hw = wave >> 1, half = wave & 1;
   const int h0 = pair * HEADS, h = h0 + hw, g = h0 / p.ratio;
@@ -126,25 +172,19 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
     }
     return;
   }
-  const int nseg = segments_of(p, sp.len, false);
-  const int slot = FOLLOWED ? t0 : sp.before + sp.part;
-  if (!FOLLOWED && nseg > 1 && sp.part == 0) return;  // finished by the first launch
-  if (slot > p.slots) return;                         // starts out of order ask for more than there are
-  const bool alone = FOLLOWED && sp.part > 0;         // from no state, and no y
-
   // the state: [32-block][i], n = 32 block + 16 (i / 8) + 8 hi + i mod 8 of row pw
   const int pw = 32 * half + sigma(col);
   f32x16_t st[4];
+  const int64_t slot_at = (((int64_t)seg.slot * p.H + h) * P + pw) * N + 8 * hi;
+  auto load_state = [&] {
 #pragma unroll
-  for (int b = 0; b < 4; ++b) st[b] = f32x16_t{};
-  const int64_t slot_at = (((int64_t)slot * p.H + h) * P + pw) * N + 8 * hi;
-  if (!alone && (sp.part > 0 || p.initial.data != nullptr)) {
-    const bool carried = sp.part > 0;
-    const int dtype = carried ? (int)LQ_F32 : p.initial.dtype;
-    const char* at = carried ? (const char*)(p.slot_state + slot_at - (int64_t)p.H * P * N)
-                             : (const char*)p.initial.data +
-                                   (sp.index * p.initial.s[0] + h * p.initial.s[1] + pw * p.initial.s[2] + 8 * hi) *
-                                       size_of(dtype);
+    for (int b = 0; b < 4; ++b) st[b] = f32x16_t{};
+    if (ADDS || (!seg.several && p.initial.data == nullptr)) return;
+    const int dtype = seg.several ? (int)LQ_F32 : p.initial.dtype;
+    const char* at = seg.several ? (const char*)(p.slot_state + slot_at)
+                                 : (const char*)p.initial.data +
+                                       (sp.index * p.initial.s[0] + h * p.initial.s[1] + pw * p.initial.s[2] + 8 * hi) *
+                                           size_of(dtype);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
 #pragma unroll
@@ -155,7 +195,7 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
         for (int i = 0; i < 8; ++i) st[b][8 * u + i] = v[i];
       }
     }
-  }
+  };
 
   // loads of a chunk: each wave 16 rows of B and of C, and 32 of one head's x
   const int bs = (int)p.B.s[1] * 2, cs = (int)p.C.s[1] * 2, xs = (int)p.x.s[1] * 2;
@@ -180,7 +220,15 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
       const int r = half * 32 + j * 8 + (lane >> 3);
       load_rows_to_lds(xd, x_to + j * 1024, r * xs + 16 * ((lane & 7) ^ (4 * ((r >> 1) & 1))));
     }
-    if (!alone) {
+    const char* steps = (const char*)(p.steps + h * p.rows + lead * p.spans.rows + row0 + k * Q);
+    const int64_t array = (int64_t)p.H * p.rows * 4;
+    float* const to[4] = {&lds.weight[k & 1][hw][0], (float*)&lds.whole[hw][0], &lds.rest[hw][0], &lds.step[hw][0]};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int a = 2 * half + j;
+      load_words_to_lds(make_desc(steps + a * array, have * 4), (lds_t)to[a], 4 * lane);
+    }
+    if (!ADDS) {
       const i32x4_t cd = make_desc(cbase + (int64_t)k * Q * cs, (have - 1) * cs + N * 2);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -190,57 +238,8 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
     }
   };
 
-  // the fourth wave: steps of a chunk, lane = row (rows past the end have dt = 0 and change nothing)
-  float raw[HEADS] = {0.f, 0.f}, bias[HEADS];
-  double A[HEADS];
-#pragma unroll
-  for (int j = 0; j < HEADS; ++j) {
-    A[j] = (double)load_float(p.A.data, p.A.dtype, (h0 + j) * p.A.s[0]) * 1.4426950408889634;
-    bias[j] = p.bias.data == nullptr ? 0.f : load_float(p.bias.data, p.bias.dtype, (h0 + j) * p.bias.s[0]);
-  }
-  const int64_t dt_at = lead * p.dt.s[0] + row0 * p.dt.s[1] + h0 * p.dt.s[2];
-  auto load_steps = [&](int k) {
-    const int r = k * Q + lane;
-    if (r >= rows) return;
-#pragma unroll
-    for (int j = 0; j < HEADS; ++j) {
-      raw[j] = load_float(p.dt.data, p.dt.dtype, dt_at + (int64_t)r * p.dt.s[1] + j * p.dt.s[2]);
-    }
-  };
-  struct Steps {
-    int whole[HEADS];
-    float rest[HEADS], step[HEADS], weight[HEADS];
-  } next;
-  auto make_steps = [&](int k) {
-#pragma unroll
-    for (int j = 0; j < HEADS; ++j) {
-      const bool in = k * Q + lane < rows;
-      const float dt = in ? scan_step(p, raw[j], bias[j]) : 0.f;
-      // (a NaN step has a decay here, and its NaN in what it multiplies)
-      const double c = prefix_sum(in ? fmin(fmax(A[j] * dt, -256.0), 256.0) : 0.0);
-      const uint64_t u = __builtin_bit_cast(uint64_t, c);
-      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, 63);
-      const uint32_t up = __builtin_amdgcn_readlane((uint32_t)(u >> 32), 63);
-      const double all = __builtin_bit_cast(double, ((uint64_t)up << 32) | lo), whole = __builtin_rint(c);
-      const float rest = (float)(c - whole);
-      next.whole[j] = (int)whole;
-      next.rest[j] = __builtin_amdgcn_exp2f(rest);
-      next.step[j] = dt * __builtin_amdgcn_exp2f(-rest);
-      next.weight[j] = in ? dt * __builtin_amdgcn_exp2f((float)(all - c)) : 0.f;
-    }
-  };
-  auto put_steps = [&](int k) {
-#pragma unroll
-    for (int j = 0; j < HEADS; ++j) {
-      lds.whole[j][lane] = next.whole[j];
-      lds.rest[j][lane] = next.rest[j];
-      lds.step[j][lane] = next.step[j];
-      lds.weight[k & 1][j][lane] = next.weight[j];
-    }
-  };
-
-  const float D = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, h0 * p.D.s[0]);
-  const float D1 = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, (h0 + 1) * p.D.s[0]);
+  const float D = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, h * p.D.s[0]);
+  const uint32_t D16 = pack2<true>(D, 0.f);
   // operand addresses within the tiles; a product step exchanges chunks (^)
   const int sb = wave == 2, tb = wave != 0;  // the mixing block of waves 0 to 2
   const int brow = 32 * sb + sigma(col);
@@ -252,17 +251,11 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
   const int b_col_at1 = (tr + 4) * 256 + 16 * (col_chunk ^ swizzle_b(tr + 4)) + col_half;
   const int x_col_at = tr * 128 + 16 * ((4 * half + col_chunk) ^ (4 * (j16 >> 3))) + col_half;
   const int m_at = col * 64 + 16 * (hi ^ ((col >> 2) & 3));
-  float log_decay = 0.f;
-
-  if (chunks > 0) {
-    if (wave == 3) {
-      load_steps(0);
-      make_steps(0);
-      put_steps(0);
-      load_steps(1);
-    }
-    load_chunk(0);
-  }
+  float log_decay;
+  for (int careful = 0; careful < 2; ++careful) {
+  load_state();
+  log_decay = 0.f;
+  if (chunks > 0) load_chunk(0);
   for (int k = 0; k < chunks; ++k) {
     const int buf = k & 1;
     wait_loads<0>();
@@ -275,10 +268,7 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
       xa[i] = lds_read_columns(at, at + 4 * 128);
     }
     f32x16_t y[2] = {};
-    words4_t xc[4];  // the same without what is not finite
-    if (!alone) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xc[i] = xa[i];
+    if (!ADDS) {
       f32x16_t mix = {};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -294,7 +284,10 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
         if (wave < 3) mix = mfma<true>(lds_read16(bt + (b_row_at ^ (32 * i))), tb ? c1 : c0, mix);
       }
       if (wave < 3) {
-        // mix[8 u + e]: row s = 32 sb + 16 u + 8 hi + e, column t = 32 tb + col
+        // mix[8 u + e]: row s = 32 sb + 16 u + 8 hi + e, column t = 32 tb + col. (t is hidden from the
+        // compiler, which would keep the comparisons' masks through the loop, more than there are registers.)
+        int t = col;
+        asm volatile("" : "+v"(t));
 #pragma unroll
         for (int j = 0; j < HEADS; ++j) {
           const int at_t = lds.whole[j][32 * tb + col];
@@ -314,10 +307,7 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
             }
             if (sb == tb) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int s = 16 * u + 8 * hi + e;
-                v[e] = s < col ? v[e] : s == col ? v[e] + (j ? D1 : D) : 0.f;
-              }
+              for (int e = 0; e < 8; ++e) v[e] = 16 * u + 8 * hi + e <= t ? v[e] : 0.f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[u][e] = pack2<true>(v[2 * e], v[2 * e + 1]);
@@ -331,14 +321,7 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
       for (int b = 0; b < 2; ++b) {
         y[b] *= __builtin_amdgcn_ldexpf(lds.rest[hw][32 * b + col], lds.whole[hw][32 * b + col]);
       }
-      // the largest exponent of the lane's x
-      typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-      u16x2_t most = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, xa[i >> 2][i & 3] & 0x7fff7fffu));
-      }
-      if (__any(most[0] >= 0x7f80 || most[1] >= 0x7f80)) {
+      if (careful) {
         for (int s = 0; s < Q; ++s) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -349,30 +332,37 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
             if (s <= 32 + col) y[1][i] += v;
           }
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          uint32_t w = xc[i >> 2][i & 3];
-          if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-          if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
-          xc[i >> 2][i & 3] = w;
-        }
       }
     }
-    const int whole = lds.whole[hw][Q - 1];  // the chunk's decay
-    const float rest = lds.rest[hw][Q - 1];
-    if (wave == 3 && k + 1 < chunks) {
-      make_steps(k + 1);
-      load_steps(k + 2);
-    }
+    const int last_row = min(Q, rows - k * Q) - 1;
+    const int whole = lds.whole[hw][last_row];  // the chunk's decay
+    const float rest = lds.rest[hw][last_row];
     __syncthreads();
-    if (k + 1 < chunks) {
-      load_chunk(k + 1);
-      if (wave == 3) put_steps(k + 1);
-    }
-    if (!alone) {
+    if (k + 1 < chunks) load_chunk(k + 1);
+    if (!ADDS) {
       lds_t mt = (lds_t)&lds.m[hw][0][0];
+      words4_t xc[4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint32_t w = xa[i >> 2][i & 3];
+        if (careful) {
+          if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+          if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+        }
+        xc[i >> 2][i & 3] = w;
+      }
+      int t = col;
+      asm volatile("" : "+v"(t));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        words4_t diagonal;  // D where s = t
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int s = 16 * i + 8 * hi + 2 * e;
+          diagonal[e] = t == s ? D16 : t == s + 1 ? D16 << 16 : 0;
+        }
+        y[0] = mfma<true>(xc[i], diagonal, y[0]);
+        y[1] = mfma<true>(xc[i + 2], diagonal, y[1]);
         y[0] = mfma<true>(xc[i], lds_read16(mt + (m_at ^ (32 * i))), y[0]);
         y[1] = mfma<true>(xc[i], lds_read16(mt + 2048 + (m_at ^ (32 * i))), y[1]);
         y[1] = mfma<true>(xc[i + 2], lds_read16(mt + 4096 + (m_at ^ (32 * i))), y[1]);
@@ -406,32 +396,39 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
       const float4 w0 = *(const float4*)&lds.weight[buf][hw][16 * i + 8 * hi];
       const float4 w1 = *(const float4*)&lds.weight[buf][hw][16 * i + 8 * hi + 4];
       const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      words4_t top, rest;
+      words4_t top, lower;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float a = w[2 * e] * __uint_as_float(xa[i][e] << 16);
         const float b = w[2 * e + 1] * __uint_as_float(xa[i][e] & 0xffff0000u);
         const uint32_t ab = pack2<true>(a, b);
         top[e] = ab;
-        rest[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
+        if (LO) lower[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const words4_t bc = lds_read_columns(bt + (b_col_at0 ^ (64 * b)) + i * 16 * 256,
                                              bt + (b_col_at1 ^ (64 * b)) + i * 16 * 256);
         st[b] = mfma<true>(bc, top, st[b]);
-        st[b] = mfma<true>(bc, rest, st[b]);
+        if (LO) st[b] = mfma<true>(bc, lower, st[b]);
       }
     }
   }
 
-  const bool last = !FOLLOWED && sp.part == nseg - 1 && p.states.data != nullptr;
-  if (!FOLLOWED && !last) return;
-  const int dtype = FOLLOWED ? (int)LQ_F32 : p.states.dtype;
-  char* at = FOLLOWED ? (char*)(p.slot_state + slot_at)
-                      : (char*)p.states.data +
-                            (sp.index * p.states.s[0] + h * p.states.s[1] + pw * p.states.s[2] + 8 * hi) *
-                                size_of(dtype);
+  if (ADDS) break;
+  // a value that is not finite, wherever it came from, is still in the state
+  float odd = 0.f;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) odd = fmaf(st[i >> 4][i & 15], 0.f, odd);
+  if (careful || !__syncthreads_or(odd != 0.f)) break;
+  }
+
+  if (!ADDS && (to != sp.len || p.states.data == nullptr)) return;
+  const int dtype = ADDS ? (int)LQ_F32 : p.states.dtype;
+  char* at = ADDS ? (char*)(p.slot_state + slot_at + (int64_t)p.H * P * N)
+                  : (char*)p.states.data +
+                        (sp.index * p.states.s[0] + h * p.states.s[1] + pw * p.states.s[2] + 8 * hi) *
+                            size_of(dtype);
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
 #pragma unroll
@@ -442,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
       store8(at + (32 * b + 16 * u) * size_of(dtype), dtype, v);
     }
   }
-  if (FOLLOWED && half == 0 && lane == 0) p.slot_log[(int64_t)slot * p.H + h] = log_decay;
+  if (ADDS && half == 0 && lane == 0) p.slot_log[(int64_t)(seg.slot + 1) * p.H + h] = log_decay;
 }
 
 // Values in a row, every row 16-byte aligned.
@@ -458,13 +455,17 @@ bool rows_fit(const lq_tensor* t) {
 
 }  // namespace
 
+bool prompt_scan_mfma_geometry(int dtype, int64_t heads, int64_t head_dim, int64_t dstate) {
+  return dtype == LQ_BF16 && heads % HEADS == 0 && head_dim == P && dstate == N;
+}
+
 bool prompt_scan_mfma_fits(const lq_tensor* x, const lq_tensor* B, const lq_tensor* C,
                            const lq_tensor* z, const lq_tensor* initial, const lq_tensor* states,
                            const lq_tensor* out) {
   const int nd = x->ndim;
   const int64_t H = x->shape[nd - 2], G = B->shape[nd - 2];
-  if (x->dtype != LQ_BF16 || out->dtype != LQ_BF16 || (z != nullptr && z->dtype != LQ_BF16)) return false;
-  if (x->shape[nd - 1] != P || B->shape[nd - 1] != N || H / G % HEADS != 0) return false;
+  if (!prompt_scan_mfma_geometry(x->dtype, H, x->shape[nd - 1], B->shape[nd - 1])) return false;
+  if (H / G % HEADS != 0 || out->dtype != LQ_BF16 || (z != nullptr && z->dtype != LQ_BF16)) return false;
   const lq_tensor* ts[7] = {x, B, C, z, initial, states, out};
   for (const lq_tensor* t : ts) {
     if (!rows_fit(t)) return false;
@@ -477,10 +478,20 @@ bool prompt_scan_mfma_fits(const lq_tensor* x, const lq_tensor* B, const lq_tens
   return true;
 }
 
-void launch_prompt_scan_mfma(const PromptScan& p, bool followed, int64_t parts, hipStream_t st) {
+size_t prompt_scan_mfma_workspace(int64_t rows, int64_t heads) { return (size_t)(rows * heads) * 16; }
+
+void launch_prompt_scan_steps(const PromptScan& p, int64_t chunks, hipStream_t st) {
+  const int64_t blocks = (p.H + STEP_HEADS - 1) / STEP_HEADS;
+  hipLaunchKernelGGL(scan_steps_kernel, dim3((unsigned)(chunks * blocks)), dim3(256), 0, st, p);
+}
+
+void launch_prompt_scan_mfma(const PromptScan& p, bool adds, int64_t parts, hipStream_t st) {
   const dim3 grid((unsigned)(parts * (p.H / HEADS))), block(256);
-  if (followed) hipLaunchKernelGGL(scan_chunks_kernel<true>, grid, block, 0, st, p);
-  else hipLaunchKernelGGL(scan_chunks_kernel<false>, grid, block, 0, st, p);
+  const bool lo = p.states.data != nullptr && p.states.dtype == LQ_F32;
+  if (adds && lo) hipLaunchKernelGGL((scan_chunks_kernel<true, true>), grid, block, 0, st, p);
+  else if (adds) hipLaunchKernelGGL((scan_chunks_kernel<true, false>), grid, block, 0, st, p);
+  else if (lo) hipLaunchKernelGGL((scan_chunks_kernel<false, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((scan_chunks_kernel<false, false>), grid, block, 0, st, p);
 }
 
 }  // namespace lq

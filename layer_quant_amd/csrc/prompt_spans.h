@@ -22,7 +22,7 @@ struct Span {
   int begin;  // first row (0 in a batch)
   int len;
   int part;    // the part of this span
-  int before;  // parts behind the first one that the spans in front of this one have together
+  int before;  // slots of the spans in front of this one
   bool gap;    // rows of no prompt
 };
 
@@ -44,9 +44,9 @@ __device__ __forceinline__ int wave_prefix_sum(int v, int lane) {
 }
 
 // The span and part behind t parts; false where there are not so many. parts(len, gap) gives a span's
-// number. Every lane of a wave calls it with the same t.
-template <class F>
-__device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, Span& out) {
+// number, slots(len, gap) another one that is summed. Every lane of a wave calls it with the same t.
+template <class F, class G>
+__device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, G&& slots, Span& out) {
   if (s.starts == nullptr) {
     const int n = parts(s.rows, false);
     if (n == 0 || t >= n * s.S) return false;
@@ -54,7 +54,7 @@ __device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, Span
     out.part = t - out.index * n;
     out.begin = 0;
     out.len = s.rows;
-    out.before = out.index * (n - 1);
+    out.before = out.index * slots(s.rows, false);
     out.gap = false;
     return true;
   }
@@ -70,7 +70,7 @@ __device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, Span
     const bool gap = i == 0 || i >= s.S + 1;
     const int n = parts(len, gap);
     const int upto = wave_prefix_sum(n, lane);
-    const int later = wave_prefix_sum(gap || n == 0 ? 0 : n - 1, lane);
+    const int own_slots = slots(len, gap), later = wave_prefix_sum(own_slots, lane);
     const uint64_t have = __ballot(t < run + upto);
     if (have != 0) {
       const int l = __builtin_ctzll(have);
@@ -80,13 +80,18 @@ __device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, Span
       const int own = __builtin_amdgcn_readlane(n, l);
       out.part = t - (run + __builtin_amdgcn_readlane(upto, l) - own);
       out.gap = out.index < 0 || out.index >= s.S;
-      out.before = behind + __builtin_amdgcn_readlane(later, l) - (out.gap ? 0 : own - 1);
+      out.before = behind + __builtin_amdgcn_readlane(later, l) - __builtin_amdgcn_readlane(own_slots, l);
       return true;
     }
     run += __builtin_amdgcn_readlane(upto, 63);
     behind += __builtin_amdgcn_readlane(later, 63);
   }
   return false;
+}
+
+template <class F>
+__device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, Span& out) {
+  return find_span(s, t, parts, [](int, bool) { return 0; }, out);
 }
 
 // host: validates `starts` (NULL, or int32/int64 [S + 1]) against packed rows

@@ -35,7 +35,8 @@ def attention_bound(ref, weight, score, dtype, head_dim):
     weight, and the weights' sum, by that much."""
     half = torch.finfo(dtype).eps / 2
     moved = ((head_dim + 2) * 2.0 ** -23 * score + (score + 1) * 2.0 ** -21)[..., None]
-    return half * ref.abs() + (half + 2 * moved + 2.0 ** -18) * weight + torch.finfo(dtype).tiny
+    least = torch.finfo(dtype).tiny * half  # half a step below the smallest normal number
+    return half * ref.abs() + (half + 2 * moved + 2.0 ** -18) * weight + least
 
 
 def softplus(x):

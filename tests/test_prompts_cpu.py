@@ -69,7 +69,7 @@ def scan(ws=0x10000, nbytes=None, softplus=1, lo=0.0, hi=float("inf"), **change)
              states=((2, 8, 64, 128), F32), out=((600, 8, 64), BF))
     a.update(change)
     t = {k: None if v is None else fake(*v) for k, v in a.items()}
-    need = _abi.lib().lq_prompt_scan_workspace(1, a["x"][0][0], 1, 8, 64, 128)
+    need = _abi.lib().lq_prompt_scan_workspace(3, 2, a["x"][0][0], 1, 8, 64, 128)
     return _abi.lib().lq_prompt_scan(*(t[k] for k in a), softplus, lo, hi, ws,
                                      need if nbytes is None else nbytes, None)
 
@@ -108,11 +108,13 @@ def test_scan_of_nothing():
                 out=((0, 8, 64), BF), starts=((1,), I32), states=((0, 8, 64, 128), F32))
     assert scan(**none) == 0
     lib = _abi.lib()
-    assert lib.lq_prompt_scan_workspace(1, 0, 1, 8, 64, 128) == 0
-    assert lib.lq_prompt_scan_workspace(0, 5, 0, 8, 64, 128) == 0
+    f32, bf = _abi.DTYPE_CODES[F32], _abi.DTYPE_CODES[BF]
+    assert lib.lq_prompt_scan_workspace(bf, 1, 0, 1, 8, 64, 128) == 0
+    assert lib.lq_prompt_scan_workspace(bf, 0, 5, 0, 8, 64, 128) == 0
     # prompts of one segment carry nothing
-    assert lib.lq_prompt_scan_workspace(4, 200, 0, 8, 64, 128) == 0
-    assert lib.lq_prompt_scan_workspace(1, 16384, 1, 128, 64, 128) > 0
+    assert lib.lq_prompt_scan_workspace(f32, 4, 200, 0, 8, 64, 128) == 0
+    assert lib.lq_prompt_scan_workspace(f32, 1, 16384, 1, 128, 64, 128) > 0
+    assert lib.lq_prompt_scan_workspace(bf, 4, 200, 0, 8, 64, 128) == 4 * 200 * 8 * 16
 
 
 def scores(logits=((4, 100), BF), tokens=((4,), I64), lp=((4,), F32), entropy=((4,), F32),
