@@ -56,8 +56,29 @@ __device__ __forceinline__ words4_t lds_read_columns(lds_t first, lds_t second) 
   return words4_t{a.x, a.y, b.x, b.y};
 }
 
+// A barrier that publishes the waves' LDS reads and writes and leaves their loads from memory in flight
+// (__syncthreads waits for those too).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" : : : "memory");
+}
+
+// A descriptor of wave-uniform values in scalar registers, also where the compiler has run out of them.
+__device__ __forceinline__ i32x4_t scalar_desc(i32x4_t d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_readfirstlane(d[i]);
+  return d;
+}
+
+// `bytes` of memory for the buffer builtins: what lies past them reads as zero and is not written.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, BUF_DWORD3);
+}
+
 // As load_to_lds, for memory that other workgroups read as well.
 __device__ __forceinline__ void load_rows_to_lds(i32x4_t desc, lds_t lds, int voff) {
+  desc = scalar_desc(desc);
   const uint32_t addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
@@ -70,6 +91,7 @@ __device__ __forceinline__ void load_rows_to_lds(i32x4_t desc, lds_t lds, int vo
 
 // The same with 4 bytes per lane.
 __device__ __forceinline__ void load_words_to_lds(i32x4_t desc, lds_t lds, int voff) {
+  desc = scalar_desc(desc);
   const uint32_t addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   asm volatile(
       "s_mov_b32 m0, %0\n\t"

@@ -93,6 +93,6 @@ __device__ __forceinline__ float scan_step(const PromptScan& p, float dt, float 
   return dt < p.dt_min ? p.dt_min : dt > p.dt_max ? p.dt_max : dt;
 }
 
-__device__ __forceinline__ float scan_silu(float z) { return z / (1.f + __expf(-z)); }
+__device__ __forceinline__ float scan_silu(float z) { return z * __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 }  // namespace lq

@@ -20,8 +20,8 @@
 //            make one 32 x 32 block each (the fourth lies above the diagonal) for both heads and leave M in
 //            LDS as bf16
 //   phase 2  Y += M x + D x (6 and 4 products), stores, S' (16 or 32 products)
-// B lies in two LDS buffers; C, x and the decays are read in phase 1 alone, so that one buffer each is
-// refilled in phase 2: 79 KB per workgroup, two of them per CU.
+// B lies in two LDS buffers; x goes to registers at once, and C and the decays are read in phase 1 alone, so
+// that one buffer each does, refilled from then on: 79 KB per workgroup, two of them per CU.
 //
 // Roundings: M, D and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result); w x, which a
 // state keeps, to the sum of two bf16 values (2^-16) where the states leave in fp32 and to one (2^-8, less
@@ -149,37 +149,24 @@ __device__ __forceinline__ void store8(char* at, int dtype, const float (&v)[8])
 
 __device__ __forceinline__ int size_of(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
 
-// ADDS: find_segment's. LO: w x as the sum of two bf16 values.
-template <bool ADDS, bool LO>
-__global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
-  __shared__ ChunkLds lds;
-  // the workgroups of a group's heads on one XCD (blocks go round the eight), as they read the same B and C
-  const int pairs = p.H / HEADS, idx = blockIdx.x % pairs;
-  const int pair = pairs % 8 == 0 ? (idx & 7) * (pairs / 8) + (idx >> 3) : idx;
-  const Segment seg = find_segment<ADDS>(p, blockIdx.x / pairs);
-  if (!seg.valid) return;
+// A segment of two heads; whether it has to run again, with CAREFUL. ADDS: find_segment's. LO: w x as the
+// sum of two bf16 values.
+template <bool ADDS, bool LO, bool CAREFUL>
+__device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& seg, int pair, int tid,
+                                            ChunkLds& lds) {
   const Span& sp = seg.span;
-  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
+  const int lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), hw = wave >> 1, half = wave & 1;
   const int h0 = pair * HEADS, h = h0 + hw, g = h0 / p.ratio;
   const int64_t lead = p.spans.starts == nullptr ? sp.index : 0;
   const int from = sp.part * p.segment, to = min(sp.len, from + p.segment);
-  uint16_t* out = (uint16_t*)p.out.data + lead * p.out.s[0] + (int64_t)(sp.begin + from) * p.out.s[1];
-  if (sp.gap) {
-    for (int i = tid; i < (to - from) * HEADS * (P / 8); i += 256) {
-      const int r = i / (HEADS * P / 8), k = i % (HEADS * P / 8);
-      *(words4_t*)(out + r * p.out.s[1] + (h0 + k / (P / 8)) * p.out.s[2] + k % (P / 8) * 8) = words4_t{0, 0, 0, 0};
-    }
-    return;
-  }
   // the state: [32-block][i], n = 32 block + 16 (i / 8) + 8 hi + i mod 8 of row pw
   const int pw = 32 * half + sigma(col);
   f32x16_t st[4];
   const int64_t slot_at = (((int64_t)seg.slot * p.H + h) * P + pw) * N + 8 * hi;
-  auto load_state = [&] {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) st[b] = f32x16_t{};
-    if (ADDS || (!seg.several && p.initial.data == nullptr)) return;
+  for (int b = 0; b < 4; ++b) st[b] = f32x16_t{};
+  if (!ADDS && (seg.several || p.initial.data != nullptr)) {
     const int dtype = seg.several ? (int)LQ_F32 : p.initial.dtype;
     const char* at = seg.several ? (const char*)(p.slot_state + slot_at)
                                  : (const char*)p.initial.data +
@@ -195,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
         for (int i = 0; i < 8; ++i) st[b][8 * u + i] = v[i];
       }
     }
-  };
+  }
 
   // loads of a chunk: each wave 16 rows of B and of C, and 32 of one head's x
   const int bs = (int)p.B.s[1] * 2, cs = (int)p.C.s[1] * 2, xs = (int)p.x.s[1] * 2;
@@ -203,23 +190,30 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
   const char* bbase = (const char*)p.B.data + (lead * p.B.s[0] + row0 * p.B.s[1] + g * p.B.s[2]) * 2;
   const char* cbase = (const char*)p.C.data + (lead * p.C.s[0] + row0 * p.C.s[1] + g * p.C.s[2]) * 2;
   const char* xbase = (const char*)p.x.data + (lead * p.x.s[0] + row0 * p.x.s[1] + h * p.x.s[2]) * 2;
+  const char* obase = (const char*)p.out.data + (lead * p.out.s[0] + row0 * p.out.s[1] + h * p.out.s[2]) * 2;
+  const int os = (int)p.out.s[1] * 2, o_at = col * os + 64 * half + 16 * hi;
   const int rows = to - from, chunks = (rows + Q - 1) / Q;
-  auto load_chunk = [&](int k) {
-    const int have = min(Q, rows - k * Q);
-    const i32x4_t bd = make_desc(bbase + (int64_t)k * Q * bs, (have - 1) * bs + N * 2);
-    const i32x4_t xd = make_desc(xbase + (int64_t)k * Q * xs, (have - 1) * xs + P * 2);
-    lds_t b_to = (lds_t)&lds.b[k & 1][wave * 4096], c_to = (lds_t)&lds.c[wave * 4096];
-    lds_t x_to = (lds_t)&lds.x[hw][half * 4096];
+  auto load_b = [&](int k) {
+    const i32x4_t bd = make_desc(bbase + (int64_t)k * Q * bs, (min(Q, rows - k * Q) - 1) * bs + N * 2);
+    lds_t to = (lds_t)&lds.b[k & 1][wave * 4096];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = wave * 16 + j * 4 + (lane >> 4);
-      load_rows_to_lds(bd, b_to + j * 1024, r * bs + 16 * ((lane & 15) ^ swizzle_b(r)));
+      load_rows_to_lds(bd, to + j * 1024, r * bs + 16 * ((lane & 15) ^ swizzle_b(r)));
     }
+  };
+  auto load_x = [&](int k) {
+    const i32x4_t xd = make_desc(xbase + (int64_t)k * Q * xs, (min(Q, rows - k * Q) - 1) * xs + P * 2);
+    lds_t to = (lds_t)&lds.x[hw][half * 4096];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = half * 32 + j * 8 + (lane >> 3);
-      load_rows_to_lds(xd, x_to + j * 1024, r * xs + 16 * ((lane & 7) ^ (4 * ((r >> 1) & 1))));
+      load_rows_to_lds(xd, to + j * 1024, r * xs + 16 * ((lane & 7) ^ (4 * ((r >> 1) & 1))));
     }
+  };
+  auto load_rest = [&](int k) {
+    const int have = min(Q, rows - k * Q);
+    lds_t c_to = (lds_t)&lds.c[wave * 4096];
     const char* steps = (const char*)(p.steps + h * p.rows + lead * p.spans.rows + row0 + k * Q);
     const int64_t array = (int64_t)p.H * p.rows * 4;
     float* const to[4] = {&lds.weight[k & 1][hw][0], (float*)&lds.whole[hw][0], &lds.rest[hw][0], &lds.step[hw][0]};
@@ -241,47 +235,92 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
   const float D = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, h * p.D.s[0]);
   const uint32_t D16 = pack2<true>(D, 0.f);
   // operand addresses within the tiles; a product step exchanges chunks (^)
-  const int sb = wave == 2, tb = wave != 0;  // the mixing block of waves 0 to 2
+  const int sb = wave >= 2, tb = wave != 0;  // the mixing block of waves 0 to 2
   const int brow = 32 * sb + sigma(col);
-  const int b_row_at = brow * 256 + 16 * (hi ^ swizzle_b(brow));
-  const int c_row_at = col * 256 + 16 * (hi ^ (col & 15));
+  int b_row_at = brow * 256 + 16 * (hi ^ swizzle_b(brow));
+  int c_row_at = col * 256 + 16 * (hi ^ (col & 15));
   const int j16 = lane & 15, g1 = (lane >> 4) & 1;
   const int col_chunk = 2 * g1 + (j16 & 1), col_half = 8 * ((j16 >> 1) & 1), tr = 8 * hi + (j16 >> 2);
-  const int b_col_at0 = tr * 256 + 16 * (col_chunk ^ swizzle_b(tr)) + col_half;
-  const int b_col_at1 = (tr + 4) * 256 + 16 * (col_chunk ^ swizzle_b(tr + 4)) + col_half;
+  int b_col_at0 = tr * 256 + 16 * (col_chunk ^ swizzle_b(tr)) + col_half;
+  int b_col_at1 = (tr + 4) * 256 + 16 * (col_chunk ^ swizzle_b(tr + 4)) + col_half;
   const int x_col_at = tr * 128 + 16 * ((4 * half + col_chunk) ^ (4 * (j16 >> 3))) + col_half;
-  const int m_at = col * 64 + 16 * (hi ^ ((col >> 2) & 3));
-  float log_decay;
-  for (int careful = 0; careful < 2; ++careful) {
-  load_state();
-  log_decay = 0.f;
-  if (chunks > 0) load_chunk(0);
+  int m_at = col * 64 + 16 * (hi ^ ((col >> 2) & 3));
+  float log_decay = 0.f;
+  if (chunks > 0) {
+    load_b(0);
+    load_x(0);
+    load_rest(0);
+  }
   for (int k = 0; k < chunks; ++k) {
     const int buf = k & 1;
-    wait_loads<0>();
-    __syncthreads();
+    // the chunk's loads; the four stores of the last one's y, a whole chunk's, were issued behind them
+    if (ADDS || k == 0) wait_loads<0>();
+    else wait_loads<4>();
+    lds_barrier();
+    // hidden from the compiler, which would keep every exchanged form of them in a register of its own
+    asm volatile("" : "+v"(b_row_at), "+v"(c_row_at), "+v"(b_col_at0), "+v"(b_col_at1), "+v"(m_at));
     lds_t xt = (lds_t)&lds.x[hw][0], bt = (lds_t)&lds.b[buf][0], ct = (lds_t)&lds.c[0];
+    float added = 0.f;
     words4_t xa[4];  // x of rows s = 16 i + 8 hi .. + 7 in column pw
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       lds_t at = xt + x_col_at + i * 16 * 128;
       xa[i] = lds_read_columns(at, at + 4 * 128);
     }
-    f32x16_t y[2] = {};
+    f32x16_t y[2] = {}, seen[2] = {};
+    if (CAREFUL) {
+      for (int s = 0; s < Q; ++s) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int q = 32 * half + 16 * (i >> 3) + 8 * hi + (i & 7);
+          const float v = bf16_bits_to_float(
+              *(const uint16_t*)&lds.x[hw][s * 128 + 16 * ((q >> 3) ^ (4 * ((s >> 1) & 1))) + 2 * (q & 7)]);
+          if (v - v == 0.f) continue;
+          if (s <= col) seen[0][i] += v;
+          if (s <= 32 + col) seen[1][i] += v;
+        }
+      }
+      float gone = 0.f;  // of row pw: to its state as well
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint32_t w = xa[i >> 2][i & 3];
+        const float a = __uint_as_float(w << 16), b = __uint_as_float(w & 0xffff0000u);
+        if (a - a != 0.f) gone += a, w &= 0xffff0000u;
+        if (b - b != 0.f) gone += b, w &= 0xffffu;
+        xa[i >> 2][i & 3] = w;
+      }
+      added = gone + __shfl_xor(gone, 32, 64);
+    }
+    lds_barrier();  // x is in registers: its buffer is free
+    if (k + 1 < chunks) {
+      load_x(k + 1);
+      load_b(k + 1);
+    }
     if (!ADDS) {
       f32x16_t mix = {};
+      // the next step's operands are read before this one's products (the scheduler, short of registers,
+      // would read each right before its product and wait for it)
+      words4_t c0 = lds_read16(ct + c_row_at), c1 = lds_read16(ct + c_row_at + 32 * 256);
+      words4_t b0 = lds_read16(bt + b_row_at);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        words4_t next_c0, next_c1, next_b0;
+        if (i < 7) {
+          next_c0 = lds_read16(ct + (c_row_at ^ (32 * (i + 1))));
+          next_c1 = lds_read16(ct + (c_row_at ^ (32 * (i + 1))) + 32 * 256);
+          next_b0 = lds_read16(bt + (b_row_at ^ (32 * (i + 1))));
+        }
         words4_t s16;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s16[e] = pack2<true>(st[i >> 1][8 * (i & 1) + 2 * e], st[i >> 1][8 * (i & 1) + 2 * e + 1]);
         }
-        const words4_t c0 = lds_read16(ct + (c_row_at ^ (32 * i)));
-        const words4_t c1 = lds_read16(ct + (c_row_at ^ (32 * i)) + 32 * 256);
+        __builtin_amdgcn_sched_barrier(0);
+        mix = mfma<true>(b0, tb ? c1 : c0, mix);  // (the fourth wave's is not used)
         y[0] = mfma<true>(s16, c0, y[0]);
         y[1] = mfma<true>(s16, c1, y[1]);
-        if (wave < 3) mix = mfma<true>(lds_read16(bt + (b_row_at ^ (32 * i))), tb ? c1 : c0, mix);
+        __builtin_amdgcn_sched_barrier(0);
+        c0 = next_c0, c1 = next_c1, b0 = next_b0;
       }
       if (wave < 3) {
         // mix[8 u + e]: row s = 32 sb + 16 u + 8 hi + e, column t = 32 tb + col. (t is hidden from the
@@ -320,37 +359,16 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         y[b] *= __builtin_amdgcn_ldexpf(lds.rest[hw][32 * b + col], lds.whole[hw][32 * b + col]);
-      }
-      if (careful) {
-        for (int s = 0; s < Q; ++s) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int q = 32 * half + 16 * (i >> 3) + 8 * hi + (i & 7);
-            const float v = bf16_bits_to_float(*(const uint16_t*)&lds.x[hw][s * 128 + 16 * ((q >> 3) ^ (4 * ((s >> 1) & 1))) + 2 * (q & 7)]);
-            if (v - v == 0.f) continue;
-            if (s <= col) y[0][i] += v;
-            if (s <= 32 + col) y[1][i] += v;
-          }
-        }
+        if (CAREFUL) y[b] += seen[b];
       }
     }
     const int last_row = min(Q, rows - k * Q) - 1;
     const int whole = lds.whole[hw][last_row];  // the chunk's decay
     const float rest = lds.rest[hw][last_row];
-    __syncthreads();
-    if (k + 1 < chunks) load_chunk(k + 1);
+    lds_barrier();
+    if (k + 1 < chunks) load_rest(k + 1);
     if (!ADDS) {
       lds_t mt = (lds_t)&lds.m[hw][0][0];
-      words4_t xc[4];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        uint32_t w = xa[i >> 2][i & 3];
-        if (careful) {
-          if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-          if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
-        }
-        xc[i >> 2][i & 3] = w;
-      }
       int t = col;
       asm volatile("" : "+v"(t));
 #pragma unroll
@@ -361,40 +379,62 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
           const int s = 16 * i + 8 * hi + 2 * e;
           diagonal[e] = t == s ? D16 : t == s + 1 ? D16 << 16 : 0;
         }
-        y[0] = mfma<true>(xc[i], diagonal, y[0]);
-        y[1] = mfma<true>(xc[i + 2], diagonal, y[1]);
-        y[0] = mfma<true>(xc[i], lds_read16(mt + (m_at ^ (32 * i))), y[0]);
-        y[1] = mfma<true>(xc[i], lds_read16(mt + 2048 + (m_at ^ (32 * i))), y[1]);
-        y[1] = mfma<true>(xc[i + 2], lds_read16(mt + 4096 + (m_at ^ (32 * i))), y[1]);
+        y[0] = mfma<true>(xa[i], diagonal, y[0]);
+        y[1] = mfma<true>(xa[i + 2], diagonal, y[1]);
+        y[0] = mfma<true>(xa[i], lds_read16(mt + (m_at ^ (32 * i))), y[0]);
+        y[1] = mfma<true>(xa[i], lds_read16(mt + 2048 + (m_at ^ (32 * i))), y[1]);
+        y[1] = mfma<true>(xa[i + 2], lds_read16(mt + 4096 + (m_at ^ (32 * i))), y[1]);
       }
+      // (rows past the end are past the descriptor, and not stored)
+      const auto od = buffer_of(obase + (int64_t)k * Q * os, (min(Q, rows - k * Q) - 1) * os + P * 2);
+      if (p.z.data != nullptr) {
+        const char* zbase = (const char*)p.z.data + (lead * p.z.s[0] + (row0 + k * Q) * p.z.s[1] + h * p.z.s[2]) * 2;
+        const int zs = (int)p.z.s[1] * 2;
+        const auto zd = buffer_of(zbase, (min(Q, rows - k * Q) - 1) * zs + P * 2);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int r = k * Q + 32 * b + col;
-        if (r >= rows) continue;
+        for (int b = 0; b < 2; ++b) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int q = 32 * half + 16 * u + 8 * hi;
-          if (p.z.data != nullptr) {
-            const words4_t z = *(const words4_t*)((const uint16_t*)p.z.data + lead * p.z.s[0] +
-                                                  (row0 + r) * p.z.s[1] + h * p.z.s[2] + q);
+          for (int u = 0; u < 2; ++u) {
+            const words4_t z = __builtin_bit_cast(words4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                zd, (32 * b + col) * zs + 64 * half + 16 * hi, 32 * u, 0));
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[b][8 * u + e] *= scan_silu(word_elem(z[e >> 1], (e & 1) * 16, LQ_BF16));
           }
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
           words4_t w;
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = pack2<true>(y[b][8 * u + 2 * e], y[b][8 * u + 2 * e + 1]);
-          *(words4_t*)(out + r * p.out.s[1] + h * p.out.s[2] + q) = w;
+          __builtin_amdgcn_raw_buffer_store_b128(w, od, o_at + 32 * b * os, 32 * u, 0);
         }
       }
     }
     const float keep = __builtin_amdgcn_ldexpf(rest, whole);
     log_decay += (float)whole + __builtin_amdgcn_logf(rest);
+    words4_t bc[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) st[b] *= keep;
+    for (int b = 0; b < 4; ++b) bc[b] = lds_read_columns(bt + (b_col_at0 ^ (64 * b)), bt + (b_col_at1 ^ (64 * b)));
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      st[b] *= keep;
+      if (CAREFUL) st[b] += added;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4 w0 = *(const float4*)&lds.weight[buf][hw][16 * i + 8 * hi];
       const float4 w1 = *(const float4*)&lds.weight[buf][hw][16 * i + 8 * hi + 4];
+      words4_t next[4];
+      if (i < 3) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          next[b] = lds_read_columns(bt + (b_col_at0 ^ (64 * b)) + (i + 1) * 16 * 256,
+                                     bt + (b_col_at1 ^ (64 * b)) + (i + 1) * 16 * 256);
+        }
+      }
       const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
       words4_t top, lower;
 #pragma unroll
@@ -405,25 +445,28 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
         top[e] = ab;
         if (LO) lower[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const words4_t bc = lds_read_columns(bt + (b_col_at0 ^ (64 * b)) + i * 16 * 256,
-                                             bt + (b_col_at1 ^ (64 * b)) + i * 16 * 256);
-        st[b] = mfma<true>(bc, top, st[b]);
-        if (LO) st[b] = mfma<true>(bc, lower, st[b]);
+      for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], top, st[b]);
+      if (LO) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], lower, st[b]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) bc[b] = next[b];
     }
   }
 
-  if (ADDS) break;
-  // a value that is not finite, wherever it came from, is still in the state
-  float odd = 0.f;
+  if (!ADDS && !CAREFUL) {
+    // a value that is not finite, wherever it came from, is still in the state
+    float odd = 0.f;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) odd = fmaf(st[i >> 4][i & 15], 0.f, odd);
-  if (careful || !__syncthreads_or(odd != 0.f)) break;
+    for (int i = 0; i < 64; ++i) odd = fmaf(st[i >> 4][i & 15], 0.f, odd);
+    if (__syncthreads_or(odd != 0.f)) return true;
   }
 
-  if (!ADDS && (to != sp.len || p.states.data == nullptr)) return;
+  if (!ADDS && (to != sp.len || p.states.data == nullptr)) return false;
   const int dtype = ADDS ? (int)LQ_F32 : p.states.dtype;
   char* at = ADDS ? (char*)(p.slot_state + slot_at + (int64_t)p.H * P * N)
                   : (char*)p.states.data +
@@ -440,6 +483,36 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
     }
   }
   if (ADDS && half == 0 && lane == 0) p.slot_log[(int64_t)(seg.slot + 1) * p.H + h] = log_decay;
+  return false;
+}
+
+template <bool ADDS, bool LO>
+__global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
+  __shared__ ChunkLds lds;
+  // the workgroups of a group's heads on one XCD (blocks go round the eight), as they read the same B and C
+  const int pairs = p.H / HEADS, idx = blockIdx.x % pairs;
+  const int pair = pairs % 8 == 0 ? (idx & 7) * (pairs / 8) + (idx >> 3) : idx;
+  const Segment seg = find_segment<ADDS>(p, blockIdx.x / pairs);
+  if (!seg.valid) return;
+  const Span& sp = seg.span;
+  if (sp.gap) {
+    const int from = sp.part * p.segment, rows = min(sp.len - from, p.segment);
+    uint16_t* out = (uint16_t*)p.out.data + (int64_t)(sp.begin + from) * p.out.s[1];
+    for (int i = threadIdx.x; i < rows * HEADS * (P / 8); i += 256) {
+      const int r = i / (HEADS * P / 8), k = i % (HEADS * P / 8);
+      *(words4_t*)(out + r * p.out.s[1] + (pair * HEADS + k / (P / 8)) * p.out.s[2] + k % (P / 8) * 8) =
+          words4_t{0, 0, 0, 0};
+    }
+    return;
+  }
+  if (!run_segment<ADDS, LO, false>(p, seg, pair, threadIdx.x, lds)) return;
+  // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
+  // for the second one, through the loop.
+  Segment again = seg;
+  int tid = threadIdx.x, same = pair;
+  asm volatile("" : "+s"(again.span.index), "+s"(again.span.begin), "+s"(again.span.part), "+s"(again.slot));
+  asm volatile("" : "+v"(tid), "+s"(same));
+  run_segment<ADDS, LO, true>(p, again, same, tid, lds);
 }
 
 // Values in a row, every row 16-byte aligned.
@@ -470,8 +543,9 @@ bool prompt_scan_mfma_fits(const lq_tensor* x, const lq_tensor* B, const lq_tens
   for (const lq_tensor* t : ts) {
     if (!rows_fit(t)) return false;
   }
-  const lq_tensor* loaded[3] = {x, B, C};
-  for (const lq_tensor* t : loaded) {
+  const lq_tensor* by_chunk[5] = {x, B, C, z, out};
+  for (const lq_tensor* t : by_chunk) {
+    if (t == nullptr) continue;
     const int64_t s = t->stride[nd - 3];
     if (t->shape[nd - 3] > 1 && (s < t->shape[nd - 1] || s > (1 << 22))) return false;
   }
