@@ -3,10 +3,19 @@
 //
 //   lse = log sum_v exp(l_v),  logprob = l_token - lse,  entropy = lse - sum_v p_v l_v
 //
-// One pass over the logits. A workgroup takes a part of a row into registers, 32 logits per thread, and
-// leaves m = max l log2(e), s = sum 2^z and t = sum 2^z z with z = l log2(e) - m, and its `top` largest
-// logits; the row's workgroup then joins the parts. fp32 sums. Every z is made from the rounded m by one
-// fused multiply-add, the given token's too, so that m's rounding falls out of logprob and entropy.
+// One pass over the logits. A thread takes 32 logits at a time, in 16-byte loads (rows that begin off that
+// alignment: from the aligned address in front of them), and keeps m = max l log2(e), s = sum 2^z and
+// t = sum 2^z z, z = l log2(e) - m, of its own: nothing is exchanged before the row's end. Every z is made
+// from the rounded m by one fused multiply-add, the given token's too, so that m's rounding falls out of
+// logprob and entropy. fp32 sums: a thread adds 8 terms in a row four times over, then the threads in a
+// tree.
+// The likeliest tokens: the k-th largest of a wave's 64 lane maxima is a threshold that k logits reach; those
+// that reach it are few (about 1.4 k of 2048 random ones) and go to the wave's list, which is cut down to
+// its k largest when it is full, and that raises the threshold. The list is kept and cut by ballots.
+//
+// Which form: with 512 rows or more, or 32768 logits or less, a workgroup per row writes the results (256
+// threads, or 1024 where one sweep of theirs covers the row); else each 8192 logits are a workgroup's, and
+// a wave per row joins the parts, a second launch. Measured: MEASURED
 //
 // Order: the larger logit first, of equal ones (and of 0 and -0) the lower token. -inf logits have no
 // part in the sums. A row with a NaN or an infinity, or with -inf alone, has no distribution: NaN.
@@ -17,11 +26,15 @@
 namespace lq {
 namespace {
 
-constexpr int THREADS = 256;
-constexpr int VPT = 32;               // logits per thread
-constexpr int PART = THREADS * VPT;   // logits of a part
+constexpr int VPT = 32;                   // logits of a thread and sweep
+constexpr int NARROW = 256, WIDE = 1024;  // threads of a workgroup
 constexpr int MAX_TOP = 32;
+constexpr int LIST = 256;  // entries of a wave's list, 4 per lane
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+struct Sums {
+  float m, s, t;
+};
 
 struct LogprobParams {
   View logits;  // strides of (batch row, row, token)
@@ -29,20 +42,103 @@ struct LogprobParams {
   float *logprobs, *entropy, *top_logprobs;
   int64_t* top_tokens;
   int rows, parts, top, len;  // len: rows of a batch row
+  int part;                   // logits of a part
   int64_t V;
-  float* stats;    // [rows][parts][4]: m, s, t
-  uint64_t* keys;  // [rows][parts][top]
+  Sums* sums;      // [rows][parts]
+  uint64_t* keys;  // [rows][parts][top]; 0: none
 };
 
-// Larger for the logit that comes first: its bits in order, then the lower token. 0: none.
-__device__ __forceinline__ uint64_t key_of(float l, uint32_t token) {
+// Larger for the logit that comes first: its bits in order, then the lower token. Never 0.
+__device__ __forceinline__ uint32_t order_of(float l) {
   const uint32_t u = __float_as_uint(l + 0.f);
-  const uint32_t up = (u >> 31) ? ~u : u | 0x80000000u;
-  return ((uint64_t)up << 32) | (0xffffffffu - token);
+  return (u >> 31) ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float logit_of(uint64_t key) {
-  const uint32_t up = (uint32_t)(key >> 32);
-  return __uint_as_float((up >> 31) ? up & 0x7fffffffu : ~up);
+__device__ __forceinline__ float logit_of(uint32_t order) {
+  return __uint_as_float((order >> 31) ? order & 0x7fffffffu : ~order);
+}
+
+__device__ __forceinline__ int count(uint64_t ballot) { return __builtin_popcountll(ballot); }
+__device__ __forceinline__ int below(uint64_t ballot) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0));
+}
+
+// The largest word w that `need` or more of the wave's 64 E words reach (0 where there are fewer).
+template <int E>
+__device__ __forceinline__ uint32_t kth_word(const uint32_t (&v)[E], int need) {
+  uint32_t w = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) c += count(__ballot(v[e] >= (w | bit)));
+    if (c >= need) w |= bit;
+    if (c == need) break;  // these and no others: w stands for the need-th
+  }
+  return w;
+}
+
+// The wave's 64 E keys (0: none) reduced to the `top` largest: whether each is one of them.
+template <int E>
+__device__ __forceinline__ uint32_t select_top(const uint32_t (&hi)[E], const uint32_t (&lo)[E], int top) {
+  const uint32_t w = kth_word(hi, top);
+  uint32_t in = 0;
+  int reach = 0, more = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    reach += count(__ballot(hi[e] >= w && hi[e] != 0));
+    more += count(__ballot(hi[e] > w));
+    in |= (uint32_t)(hi[e] >= w && hi[e] != 0) << e;
+  }
+  if (reach <= top) return in;
+  // too many of equal logits: of those, the ones with the lowest tokens
+  uint32_t tie[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) tie[e] = hi[e] == w ? lo[e] : 0;
+  const uint32_t last = kth_word(tie, top - more);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (hi[e] == w && lo[e] < last) in &= ~(1u << e);
+  }
+  return in;
+}
+
+// Orders a wave's reads of its list behind the other lanes' writes.
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); }
+
+// Cuts a wave's list of n keys to its `top` largest; returns how many there are.
+__device__ __forceinline__ int cut_list(uint2* list, int n, int top, int lane) {
+  wave_fence();
+  if (n <= top) return n;
+  uint32_t hi[LIST / 64], lo[LIST / 64];
+#pragma unroll
+  for (int e = 0; e < LIST / 64; ++e) {
+    const uint2 k = 64 * e + lane < n ? list[64 * e + lane] : make_uint2(0, 0);
+    hi[e] = k.y;
+    lo[e] = k.x;
+  }
+  const uint32_t in = select_top(hi, lo, top);
+  int at = 0;
+#pragma unroll
+  for (int e = 0; e < LIST / 64; ++e) {
+    const uint64_t some = __ballot((in >> e) & 1);
+    if ((in >> e) & 1) list[at + below(some)] = make_uint2(lo[e], hi[e]);
+    at += count(some);
+  }
+  wave_fence();
+  return at;
+}
+
+// Sums over another maximum: z' = z + m - to.
+__device__ __forceinline__ Sums moved(Sums v, float to) {
+  const float d = fmaxf(v.m - (to == -INFINITY ? 0.f : to), -200.f);
+  const float w = __builtin_amdgcn_exp2f(d);
+  return {to, w * v.s, w * fmaf(d, v.s, v.t)};
+}
+__device__ __forceinline__ Sums wave_sums(Sums v) {
+  v = moved(v, group_max<64>(v.m));
+  v.s = group_sum<64>(v.s);
+  v.t = group_sum<64>(v.t);
+  return v;
 }
 
 __device__ __forceinline__ int64_t row_at(const LogprobParams& p, int row) {
@@ -50,108 +146,10 @@ __device__ __forceinline__ int64_t row_at(const LogprobParams& p, int row) {
   return b * p.logits.s[0] + (row - b * p.len) * p.logits.s[1];
 }
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t lo = __shfl_xor((uint32_t)v, o, 64), hi = __shfl_xor((uint32_t)(v >> 32), o, 64);
-    const uint64_t w = ((uint64_t)hi << 32) | lo;
-    v = w > v ? w : v;
-  }
-  return v;
-}
-
-template <int DTYPE>
-__global__ __launch_bounds__(THREADS) void logprob_part_kernel(LogprobParams p) {
-  __shared__ float red[3][THREADS / 64];
-  __shared__ uint64_t best[THREADS / 64];
-  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t base = row_at(p, row);
-  const int64_t first = (int64_t)part * PART + tid;
-  float l[VPT];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int64_t v = first + (int64_t)i * THREADS;
-    l[i] = v < p.V ? load_float(p.logits.data, DTYPE, base + v * p.logits.s[2]) : -INFINITY;
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) m = fmaxf(m, l[i]);
-  m = group_max<64>(m);
-  if (lane == 0) red[0][wave] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) m = fmaxf(m, red[0][w]);
-  // a part of -inf alone has s = 0
-  m *= LOG2E;
-  const float mz = m == -INFINITY ? 0.f : m;
-  float s = 0.f, t = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const float z = fmaf(l[i], LOG2E, -mz);
-    const float e = __builtin_amdgcn_exp2f(z);  // NaN stays; 0 for -inf
-    s += e;
-    t = fmaf(e, fmaxf(z, -200.f), t);
-  }
-  s = group_sum<64>(s);
-  t = group_sum<64>(t);
-  __syncthreads();
-  if (lane == 0) {
-    red[1][wave] = s;
-    red[2][wave] = t;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    float* to = p.stats + ((int64_t)row * p.parts + part) * 4;
-    s = t = 0.f;
-    for (int w = 0; w < THREADS / 64; ++w) {
-      s += red[1][w];
-      t += red[2][w];
-    }
-    to[0] = m;
-    to[1] = s;
-    to[2] = t;
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
-    uint64_t b = 0;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int64_t v = first + (int64_t)i * THREADS;
-      if (v >= p.V) continue;
-      const uint64_t key = key_of(l[i], (uint32_t)v);
-      if (key < last && key > b) b = key;
-    }
-    b = wave_max(b);
-    __syncthreads();
-    if (lane == 0) best[wave] = b;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) b = best[w] > b ? best[w] : b;
-    last = b;
-    if (tid == 0) p.keys[((int64_t)row * p.parts + part) * p.top + k] = b;
-  }
-}
-
-// One wave per row.
-__global__ __launch_bounds__(64) void logprob_final_kernel(LogprobParams p) {
-  const int row = blockIdx.x, lane = threadIdx.x;
-  const float* st = p.stats + (int64_t)row * p.parts * 4;
-  float m = -INFINITY;
-  for (int i = lane; i < p.parts; i += 64) m = fmaxf(m, st[4 * i]);
-  m = group_max<64>(m);
-  const float mz = m == -INFINITY ? 0.f : m;
-  float s = 0.f, t = 0.f;
-  for (int i = lane; i < p.parts; i += 64) {
-    const float d = fmaxf(st[4 * i] - mz, -200.f);
-    const float w = __builtin_amdgcn_exp2f(d);
-    s = fmaf(w, st[4 * i + 1], s);
-    t = fmaf(w, fmaf(d, st[4 * i + 1], st[4 * i + 2]), t);
-  }
-  s = group_sum<64>(s);
-  t = group_sum<64>(t);
-  const float log2s = __log2f(s);
-  const bool known = s > 0.f && s < INFINITY && m < INFINITY;
+// A row's results from its sums and, in one wave's registers, its `top` largest keys (lane k: any one).
+__device__ __forceinline__ void put_row(const LogprobParams& p, int row, Sums v, uint64_t key, int lane) {
+  const float base = v.m == -INFINITY ? 0.f : v.m, log2s = __builtin_amdgcn_logf(v.s);
+  const bool known = v.s > 0.f && v.s < INFINITY && v.m < INFINITY;
   const float nan = __builtin_nanf("");
   if (lane == 0) {
     const int b = row / p.len;
@@ -159,26 +157,222 @@ __global__ __launch_bounds__(64) void logprob_final_kernel(LogprobParams p) {
     float lp = 0.f;
     if (token >= 0 && token < p.V) {
       const float l = load_float(p.logits.data, p.logits.dtype, row_at(p, row) + token * p.logits.s[2]);
-      lp = known ? (fmaf(l, LOG2E, -mz) - log2s) * LN2 : nan;
+      lp = known ? (fmaf(l, LOG2E, -base) - log2s) * LN2 : nan;
     }
     p.logprobs[row] = lp;
-    if (p.entropy != nullptr) p.entropy[row] = known ? LN2 * (log2s - t / s) : nan;
+    if (p.entropy != nullptr) p.entropy[row] = known ? LN2 * (log2s - v.t / v.s) : nan;
   }
-  const uint64_t* keys = p.keys + (int64_t)row * p.parts * p.top;
-  uint64_t last = ~0ull;
+  int rank = 0;
   for (int k = 0; k < p.top; ++k) {
-    uint64_t b = 0;
-    for (int i = lane; i < p.parts * p.top; i += 64) {
-      const uint64_t key = keys[i];
-      if (key < last && key > b) b = key;
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)key, k);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(key >> 32), k);
+    rank += (((uint64_t)hi << 32) | lo) > key;
+  }
+  if (lane < p.top) {
+    // (a row that is not known can hold keys that are not numbers, and its order is not one)
+    const int64_t at = (int64_t)row * p.top + (known ? rank : lane);
+    p.top_logprobs[at] = known ? (fmaf(logit_of((uint32_t)(key >> 32)), LOG2E, -base) - log2s) * LN2 : nan;
+    p.top_tokens[at] = known ? (int64_t)(0xffffffffu - (uint32_t)key) : lane;
+  }
+}
+
+// The 32 logits of a thread's sweep from logit `from` on (a multiple of a load's behind the row's aligned
+// beginning), -inf outside [lo, hi). Element i of load j is logit from + j * THREADS * W + tid * W + i.
+template <int DTYPE, int THREADS, bool ROWS>
+__device__ __forceinline__ void load_logits(const LogprobParams& p, int64_t row, int64_t from, int64_t lo,
+                                            int64_t hi, int tid, float (&x)[VPT]) {
+  constexpr int W = DTYPE == LQ_F32 ? 4 : 8, SIZE = DTYPE == LQ_F32 ? 4 : 2;
+  uint4 raw[VPT / W];
+#pragma unroll
+  for (int j = 0; j < VPT / W; ++j) {
+    const int64_t at = from + (int64_t)j * THREADS * W + tid * W;
+    if (ROWS) {
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (at + W > lo && at < hi) raw[j] = *(const uint4*)((const char*)p.logits.data + (row + at) * SIZE);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        x[j * W + i] = at + i >= lo && at + i < hi
+                           ? load_float(p.logits.data, DTYPE, row + (at + i) * p.logits.s[2])
+                           : -INFINITY;
+      }
     }
-    b = wave_max(b);
-    last = b;
-    if (lane == 0) {
-      const int64_t at = (int64_t)row * p.top + k;
-      p.top_logprobs[at] = known ? (fmaf(logit_of(b), LOG2E, -mz) - log2s) * LN2 : nan;
-      p.top_tokens[at] = known ? (int64_t)(0xffffffffu - (uint32_t)b) : k;
+  }
+  if (!ROWS) return;
+#pragma unroll
+  for (int j = 0; j < VPT / W; ++j) {
+    const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      x[j * W + i] = SIZE == 4 ? __uint_as_float(w[i & 3]) : word_elem(w[i >> 1], (i & 1) * 16, DTYPE);
     }
+    const int64_t at = from + (int64_t)j * THREADS * W + tid * W;
+    if (at < lo || at + W > hi) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if (at + i < lo || at + i >= hi) x[j * W + i] = -INFINITY;
+      }
+    }
+  }
+}
+
+// A row, or a part of it. ROWS: its logits lie one behind another.
+template <int DTYPE, int THREADS, bool ROWS>
+__global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
+  constexpr int WAVES = THREADS / 64, SWEEP = THREADS * VPT;
+  constexpr int W = DTYPE == LQ_F32 ? 4 : 8, SIZE = DTYPE == LQ_F32 ? 4 : 2;
+  __shared__ Sums sums[WAVES];
+  __shared__ uint2 lists[WAVES][LIST];
+  __shared__ int counts[WAVES];
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t base = row_at(p, row);
+  // parts lie between aligned addresses, the first one's at or in front of the row's beginning
+  const int skew = ROWS ? (int)(((uintptr_t)p.logits.data + (uintptr_t)(base * SIZE)) & 15) / SIZE : 0;
+  int64_t from = (int64_t)part * p.part - skew;
+  const int64_t lo = max(from, (int64_t)0), hi = min(p.V, from + p.part);
+  Sums v = {-INFINITY, 0.f, 0.f};
+  float limit = -INFINITY;  // `top` logits of the wave's reach it
+  int listed = 0;
+  uint2* list = lists[wave];
+  for (int sweep = 0; from < hi; ++sweep, from += SWEEP) {
+    float x[VPT];
+    load_logits<DTYPE, THREADS, ROWS>(p, base, from, lo, hi, tid, x);
+    float most[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+    for (int i = 4; i < VPT; ++i) most[i & 3] = fmaxf(most[i & 3], x[i]);
+    const float top_l = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    v = moved(v, fmaxf(v.m, top_l * LOG2E));
+    const float m = v.m == -INFINITY ? 0.f : v.m;
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const float z = fmaf(x[i], LOG2E, -m);
+      const float e = __builtin_amdgcn_exp2f(z);  // NaN stays; 0 for -inf
+      s[i & 3] += e;
+      t[i & 3] = fmaf(e, fmaxf(z, -200.f), t[i & 3]);
+    }
+    v.s += (s[0] + s[1]) + (s[2] + s[3]);
+    v.t += (t[0] + t[1]) + (t[2] + t[3]);
+    if (p.top == 0) continue;
+    if (sweep == 0) {
+      const uint32_t word[1] = {order_of(top_l)};
+      limit = logit_of(kth_word(word, p.top));
+      if (!(limit >= -INFINITY)) limit = -INFINITY;  // NaN among the maxima
+    }
+    uint32_t hits = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) hits |= x[i] >= limit ? 1u << i : 0u;
+    // (the few that reach the limit are read again: registers have no index)
+    while (uint64_t some = __ballot(hits != 0)) {
+      const int i = __builtin_ctz(hits | 0x80000000u);
+      const int64_t at = from + (int64_t)(i / W) * SWEEP / (VPT / W) + tid * W + i % W;
+      const bool in = hits != 0 && at >= lo && at < hi;
+      hits &= hits - 1;
+      some = __ballot(in);
+      if (listed + count(some) > LIST) {
+        listed = cut_list(list, listed, p.top, lane);
+        // the smallest that is left is the new limit: `top` logits reach it
+        uint32_t least[1] = {lane < listed ? ~list[lane].y : 0};
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) least[0] = max(least[0], (uint32_t)__shfl_xor(least[0], o, 64));
+        limit = fmaxf(limit, logit_of(~least[0]));
+      }
+      if (in) {
+        const float l = load_float(p.logits.data, DTYPE, base + at * p.logits.s[2]);
+        list[listed + below(some)] = make_uint2(0xffffffffu - (uint32_t)at, order_of(l));
+      }
+      listed += count(some);
+    }
+  }
+  v = wave_sums(v);
+  if (p.top > 0) listed = cut_list(list, listed, p.top, lane);
+  if (lane == 0) {
+    sums[wave] = v;
+    counts[wave] = listed;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  v = wave_sums(lane < WAVES ? sums[lane] : Sums{-INFINITY, 0.f, 0.f});
+  uint64_t key = 0;
+  if (p.top > 0) {
+    // the waves' lists of up to 32 keys: two in a row of 64 lanes
+    constexpr int E = (WAVES + 1) / 2;
+    uint32_t khi[E], klo[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int w = 2 * e + (lane >> 5);
+      const uint2 k = w < WAVES && (lane & 31) < counts[w] ? lists[w][lane & 31] : make_uint2(0, 0);
+      khi[e] = k.y;
+      klo[e] = k.x;
+    }
+    const uint32_t in = select_top(khi, klo, p.top);
+    // (list 0 has been read)
+    int at = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t some = __ballot((in >> e) & 1);
+      if ((in >> e) & 1) list[at + below(some)] = make_uint2(klo[e], khi[e]);
+      at += count(some);
+    }
+    wave_fence();
+    if (lane < at) key = ((uint64_t)list[lane].y << 32) | list[lane].x;
+  }
+  if (p.parts == 1) return put_row(p, row, v, key, lane);
+  const int64_t slot = (int64_t)row * p.parts + part;
+  if (lane == 0) p.sums[slot] = v;
+  if (lane < p.top) p.keys[slot * p.top + lane] = key;
+}
+
+// The parts of a row, one wave per row.
+__global__ __launch_bounds__(64) void logprob_join_kernel(LogprobParams p) {
+  __shared__ uint2 list[LIST];
+  const int row = blockIdx.x, lane = threadIdx.x;
+  const Sums* sums = p.sums + (int64_t)row * p.parts;
+  Sums v = {-INFINITY, 0.f, 0.f};
+  for (int i = lane; i < p.parts; i += 64) {
+    const float to = fmaxf(v.m, sums[i].m);
+    const Sums a = moved(v, to), b = moved(sums[i], to);
+    v = {to, a.s + b.s, a.t + b.t};
+  }
+  v = wave_sums(v);
+  const uint64_t* keys = p.keys + (int64_t)row * p.parts * p.top;
+  const int n = p.parts * p.top;
+  int listed = 0;
+  for (int i = 0; i < n; i += 64) {
+    if (listed + 64 > LIST) listed = cut_list(list, listed, p.top, lane);
+    const uint64_t k = i + lane < n ? keys[i + lane] : 0;
+    const uint64_t some = __ballot(k != 0);
+    if (k != 0) list[listed + below(some)] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
+    listed += count(some);
+  }
+  listed = cut_list(list, listed, p.top, lane);
+  put_row(p, row, v, lane < listed ? ((uint64_t)list[lane].y << 32) | list[lane].x : 0, lane);
+}
+
+// Threads of a workgroup and logits of a part (the whole row: one launch). skew: logits between an aligned
+// address and a row's beginning, at most.
+struct Plan {
+  int threads;
+  int64_t part, parts;
+};
+constexpr int MAX_SKEW = 7;
+Plan plan_of(int64_t rows, int64_t vocab, int skew) {
+  if (rows >= 512) return {NARROW, vocab + MAX_SKEW, 1};
+  if (vocab <= WIDE * VPT - MAX_SKEW) return {WIDE, vocab + MAX_SKEW, 1};  // one sweep
+  const int64_t part = NARROW * VPT;
+  return {NARROW, part, (vocab + skew + part - 1) / part};
+}
+
+template <int DTYPE>
+void launch_logprobs(const LogprobParams& p, int threads, bool in_a_row, hipStream_t st) {
+  const dim3 grid((unsigned)p.rows * (unsigned)p.parts), block(threads);
+  if (threads == WIDE) {
+    if (in_a_row) hipLaunchKernelGGL((logprob_kernel<DTYPE, WIDE, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((logprob_kernel<DTYPE, WIDE, false>), grid, block, 0, st, p);
+  } else {
+    if (in_a_row) hipLaunchKernelGGL((logprob_kernel<DTYPE, NARROW, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((logprob_kernel<DTYPE, NARROW, false>), grid, block, 0, st, p);
   }
 }
 
@@ -191,8 +385,10 @@ using namespace lq;
 
 extern "C" size_t lq_token_logprobs_workspace(int64_t rows, int64_t vocab, int top) {
   if (rows <= 0 || vocab <= 0 || top < 0) return 0;
-  const size_t parts = (size_t)rows * (size_t)((vocab + PART - 1) / PART);
-  return align256(parts * 16) + parts * (size_t)top * 8;
+  const Plan plan = plan_of(rows, vocab, MAX_SKEW);
+  if (plan.parts == 1) return 0;
+  const size_t parts = (size_t)rows * (size_t)plan.parts;
+  return align256(parts * sizeof(Sums)) + parts * (size_t)top * 8;
 }
 
 extern "C" int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* tokens,
@@ -235,20 +431,26 @@ extern "C" int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* token
     return fail(LQ_ERR_INVALID_ARG, "%lld likeliest of a vocabulary of %lld asked for", (long long)top,
                 (long long)V);
   }
-  const int64_t parts = (V + PART - 1) / PART;
+  const int size = dtype_size(logits->dtype);
+  const bool in_a_row = V == 1 || logits->stride[nd - 1] == 1;
+  bool aligned = ((uintptr_t)logits->data & 15) == 0;
+  for (int i = 0; i < nd - 1; ++i) {
+    aligned = aligned && (logits->shape[i] < 2 || logits->stride[i] * size % 16 == 0);
+  }
+  const Plan plan = plan_of(rows, V, in_a_row && !aligned ? MAX_SKEW : 0);
   if (top > MAX_TOP) {
     return fail(LQ_ERR_UNSUPPORTED, "top %lld unsupported (<= %d)", (long long)top, MAX_TOP);
   }
-  if (V > INT32_MAX || rows > INT32_MAX || rows * parts >= ((int64_t)1 << 32) / THREADS) {
+  if (V > INT32_MAX / 2 || rows > INT32_MAX || rows * plan.parts >= ((int64_t)1 << 32) / plan.threads) {
     return fail(LQ_ERR_UNSUPPORTED, "%lld rows of %lld logits exceed the launch limits",
                 (long long)rows, (long long)V);
   }
   const size_t need = lq_token_logprobs_workspace(rows, V, (int)top);
-  if (workspace == nullptr || workspace_bytes < need) {
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     return fail(LQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
   }
-  if (((uintptr_t)workspace & 255) != 0) {
+  if (need > 0 && ((uintptr_t)workspace & 255) != 0) {
     return fail(LQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   }
   LogprobParams p{};
@@ -267,17 +469,17 @@ extern "C" int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* token
   }
   p.rows = (int)rows;
   p.len = (int)len;
-  p.parts = (int)parts;
+  p.parts = (int)plan.parts;
+  p.part = (int)plan.part;
   p.top = (int)top;
   p.V = V;
-  p.stats = (float*)workspace;
-  p.keys = (uint64_t*)((char*)workspace + align256((size_t)(rows * parts) * 16));
+  p.sums = (Sums*)workspace;
+  p.keys = (uint64_t*)((char*)workspace + align256((size_t)(rows * plan.parts) * sizeof(Sums)));
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(rows * parts)), block(THREADS);
-  if (logits->dtype == LQ_BF16) hipLaunchKernelGGL(logprob_part_kernel<LQ_BF16>, grid, block, 0, st, p);
-  else if (logits->dtype == LQ_F16) hipLaunchKernelGGL(logprob_part_kernel<LQ_F16>, grid, block, 0, st, p);
-  else hipLaunchKernelGGL(logprob_part_kernel<LQ_F32>, grid, block, 0, st, p);
-  if ((rc = check_launch("lq_token_logprobs")) != LQ_OK) return rc;
-  hipLaunchKernelGGL(logprob_final_kernel, dim3((unsigned)rows), dim3(64), 0, st, p);
-  return check_launch("lq_token_logprobs (final)");
+  if (logits->dtype == LQ_BF16) launch_logprobs<LQ_BF16>(p, plan.threads, in_a_row, st);
+  else if (logits->dtype == LQ_F16) launch_logprobs<LQ_F16>(p, plan.threads, in_a_row, st);
+  else launch_logprobs<LQ_F32>(p, plan.threads, in_a_row, st);
+  if ((rc = check_launch("lq_token_logprobs")) != LQ_OK || plan.parts == 1) return rc;
+  hipLaunchKernelGGL(logprob_join_kernel, dim3((unsigned)rows), dim3(64), 0, st, p);
+  return check_launch("lq_token_logprobs (join)");
 }

@@ -142,9 +142,9 @@ def scores(logits=((4, 100), BF), tokens=((4,), I64), lp=((4,), F32), entropy=((
     (-2, dict(tl=((4, 33), F32), tt=((4, 33), I64))),
     (-2, dict(logits=((1 << 24, 100), BF), tokens=((1 << 24,), I64), lp=((1 << 24,), F32),
               entropy=((1 << 24,), F32), tl=None, tt=None)),
-    (-3, dict(ws=None)),
-    (-3, dict(nbytes=8)),
-    (-3, dict(ws=0x10010))])
+    (-3, dict(logits=((4, 40000), BF), ws=None)),
+    (-3, dict(logits=((4, 40000), BF), nbytes=8)),
+    (-3, dict(logits=((4, 40000), BF), ws=0x10010))])
 def test_scores_refusals(rc, change):
     assert scores(**change) == rc, _abi.last_error()
 
