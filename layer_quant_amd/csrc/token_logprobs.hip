@@ -62,17 +62,43 @@ __device__ __forceinline__ int below(uint64_t ballot) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0));
 }
 
-// The largest word w that `need` or more of the wave's 64 E words reach (0 where there are fewer).
+// op over the wave's lanes: rotations within rows of 16, then the four rows.
+template <class F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F op) {
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x122, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x121, 0xf, 0xf, false));
+  return op(op(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+            op(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+// A word that `need` or more of the wave's 64 E words (0: none) reach, and of those that many do the largest
+// or one that exactly `need` reach; 0 where there are fewer. Bit by bit from the highest in which the
+// words differ.
 template <int E>
 __device__ __forceinline__ uint32_t kth_word(const uint32_t (&v)[E], int need) {
-  uint32_t w = 0;
+  uint32_t some = 0, every = ~0u;
+  int words = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    some |= v[e];
+    every &= v[e] == 0 ? ~0u : v[e];
+    words += count(__ballot(v[e] != 0));
+  }
+  if (words < need) return 0;
+  some = wave_fold(some, [](uint32_t x, uint32_t y) { return x | y; });
+  uint32_t w = wave_fold(every, [](uint32_t x, uint32_t y) { return x & y; });
+  uint32_t differ = some & ~w;
 #pragma unroll 1
-  for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+  while (differ != 0) {
+    const uint32_t bit = 0x80000000u >> __builtin_clz(differ);
+    differ ^= bit;
     int c = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) c += count(__ballot(v[e] >= (w | bit)));
     if (c >= need) w |= bit;
-    if (c == need) break;  // these and no others: w stands for the need-th
+    if (c == need) break;
   }
   return w;
 }
@@ -128,6 +154,51 @@ __device__ __forceinline__ int cut_list(uint2* list, int n, int top, int lane) {
   return at;
 }
 
+// The `top` largest of a list of n <= 64 E keys, one per lane and in order: lane k has the k-th (0: none).
+template <int E>
+__device__ __forceinline__ uint64_t sort_list(uint2* list, int n, int top, int lane) {
+  wave_fence();
+  if (n > 64) {
+    uint32_t hi[E], lo[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint2 k = 64 * e + lane < n ? list[64 * e + lane] : make_uint2(0, 0);
+      hi[e] = k.y;
+      lo[e] = k.x;
+    }
+    // the equal ones at the end may stay, as long as a lane is there for each
+    const uint32_t w = kth_word(hi, top);
+    uint32_t in = 0;
+    int reach = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      reach += count(__ballot(hi[e] >= w));
+      in |= (uint32_t)(hi[e] >= w) << e;
+    }
+    if (reach > 64) in = select_top(hi, lo, top);
+    n = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t some = __ballot((in >> e) & 1);
+      if ((in >> e) & 1) list[n + below(some)] = make_uint2(lo[e], hi[e]);
+      n += count(some);
+    }
+    wave_fence();
+  }
+  const uint2 k = lane < n ? list[lane] : make_uint2(0, 0);
+  int rank = 0;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const uint32_t lo = __builtin_amdgcn_readlane(k.x, i), hi = __builtin_amdgcn_readlane(k.y, i);
+    rank += hi > k.y || (hi == k.y && lo > k.x);
+  }
+  wave_fence();
+  if (lane < n && rank < 64) list[rank] = k;
+  wave_fence();
+  const uint2 sorted = lane < min(n, top) ? list[lane] : make_uint2(0, 0);
+  return ((uint64_t)sorted.y << 32) | sorted.x;
+}
+
 // Sums over another maximum: z' = z + m - to.
 __device__ __forceinline__ Sums moved(Sums v, float to) {
   const float d = fmaxf(v.m - (to == -INFINITY ? 0.f : to), -200.f);
@@ -146,7 +217,7 @@ __device__ __forceinline__ int64_t row_at(const LogprobParams& p, int row) {
   return b * p.logits.s[0] + (row - b * p.len) * p.logits.s[1];
 }
 
-// A row's results from its sums and, in one wave's registers, its `top` largest keys (lane k: any one).
+// A row's results from its sums and, in one wave's registers, its `top` largest keys (lane k: the k-th).
 __device__ __forceinline__ void put_row(const LogprobParams& p, int row, Sums v, uint64_t key, int lane) {
   const float base = v.m == -INFINITY ? 0.f : v.m, log2s = __builtin_amdgcn_logf(v.s);
   const bool known = v.s > 0.f && v.s < INFINITY && v.m < INFINITY;
@@ -162,15 +233,9 @@ __device__ __forceinline__ void put_row(const LogprobParams& p, int row, Sums v,
     p.logprobs[row] = lp;
     if (p.entropy != nullptr) p.entropy[row] = known ? LN2 * (log2s - v.t / v.s) : nan;
   }
-  int rank = 0;
-  for (int k = 0; k < p.top; ++k) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)key, k);
-    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(key >> 32), k);
-    rank += (((uint64_t)hi << 32) | lo) > key;
-  }
   if (lane < p.top) {
-    // (a row that is not known can hold keys that are not numbers, and its order is not one)
-    const int64_t at = (int64_t)row * p.top + (known ? rank : lane);
+    // (a row that is not known can hold logits that are not numbers, and its order is not one)
+    const int64_t at = (int64_t)row * p.top + lane;
     p.top_logprobs[at] = known ? (fmaf(logit_of((uint32_t)(key >> 32)), LOG2E, -base) - log2s) * LN2 : nan;
     p.top_tokens[at] = known ? (int64_t)(0xffffffffu - (uint32_t)key) : lane;
   }
@@ -223,7 +288,9 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
   constexpr int W = DTYPE == LQ_F32 ? 4 : 8, SIZE = DTYPE == LQ_F32 ? 4 : 2;
   __shared__ Sums sums[WAVES];
   __shared__ uint2 lists[WAVES][LIST];
+  __shared__ uint2 joined[512];
   __shared__ int counts[WAVES];
+  __shared__ uint32_t reached;  // the order of a logit that `top` logits of a wave reach
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t base = row_at(p, row);
@@ -232,9 +299,13 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
   int64_t from = (int64_t)part * p.part - skew;
   const int64_t lo = max(from, (int64_t)0), hi = min(p.V, from + p.part);
   Sums v = {-INFINITY, 0.f, 0.f};
-  float limit = -INFINITY;  // `top` logits of the wave's reach it
+  float limit = -INFINITY;  // `top` logits of the part reach it
   int listed = 0;
   uint2* list = lists[wave];
+  if (p.top > 0) {
+    if (tid == 0) reached = 0;
+    __syncthreads();
+  }
   for (int sweep = 0; from < hi; ++sweep, from += SWEEP) {
     float x[VPT];
     load_logits<DTYPE, THREADS, ROWS>(p, base, from, lo, hi, tid, x);
@@ -256,10 +327,13 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
     v.t += (t[0] + t[1]) + (t[2] + t[3]);
     if (p.top == 0) continue;
     if (sweep == 0) {
-      const uint32_t word[1] = {order_of(top_l)};
-      limit = logit_of(kth_word(word, p.top));
-      if (!(limit >= -INFINITY)) limit = -INFINITY;  // NaN among the maxima
+      const uint32_t word[1] = {order_of(top_l)}, w = kth_word(word, p.top);
+      if (lane == 0) atomicMax(&reached, w);
+      __syncthreads();
     }
+    const uint32_t w = *(volatile uint32_t*)&reached;
+    // (a NaN maximum is no limit)
+    limit = w > order_of(INFINITY) || w < order_of(-INFINITY) ? -INFINITY : fmaxf(limit, logit_of(w));
     uint32_t hits = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) hits |= x[i] >= limit ? 1u << i : 0u;
@@ -276,6 +350,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
         uint32_t least[1] = {lane < listed ? ~list[lane].y : 0};
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) least[0] = max(least[0], (uint32_t)__shfl_xor(least[0], o, 64));
+        if (lane == 0) atomicMax(&reached, ~least[0]);
         limit = fmaxf(limit, logit_of(~least[0]));
       }
       if (in) {
@@ -286,7 +361,9 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
     }
   }
   v = wave_sums(v);
-  if (p.top > 0) listed = cut_list(list, listed, p.top, lane);
+  // the lists together: 512 keys at most
+  constexpr int E = 8, MOST = 64 * E / WAVES;
+  if (listed > MOST) listed = cut_list(list, listed, p.top, lane);
   if (lane == 0) {
     sums[wave] = v;
     counts[wave] = listed;
@@ -296,27 +373,14 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
   v = wave_sums(lane < WAVES ? sums[lane] : Sums{-INFINITY, 0.f, 0.f});
   uint64_t key = 0;
   if (p.top > 0) {
-    // the waves' lists of up to 32 keys: two in a row of 64 lanes
-    constexpr int E = (WAVES + 1) / 2;
-    uint32_t khi[E], klo[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int w = 2 * e + (lane >> 5);
-      const uint2 k = w < WAVES && (lane & 31) < counts[w] ? lists[w][lane & 31] : make_uint2(0, 0);
-      khi[e] = k.y;
-      klo[e] = k.x;
+    int n = counts[0];
+    for (int w = 1; w < WAVES; ++w) {
+      const int own = counts[w];
+      for (int i = lane; i < own; i += 64) joined[n + i] = lists[w][i];
+      n += own;
     }
-    const uint32_t in = select_top(khi, klo, p.top);
-    // (list 0 has been read)
-    int at = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint64_t some = __ballot((in >> e) & 1);
-      if ((in >> e) & 1) list[at + below(some)] = make_uint2(klo[e], khi[e]);
-      at += count(some);
-    }
-    wave_fence();
-    if (lane < at) key = ((uint64_t)list[lane].y << 32) | list[lane].x;
+    for (int i = lane; i < counts[0]; i += 64) joined[i] = lists[0][i];
+    key = sort_list<E>(joined, n, p.top, lane);
   }
   if (p.parts == 1) return put_row(p, row, v, key, lane);
   const int64_t slot = (int64_t)row * p.parts + part;
@@ -346,8 +410,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobParams p) {
     if (k != 0) list[listed + below(some)] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
     listed += count(some);
   }
-  listed = cut_list(list, listed, p.top, lane);
-  put_row(p, row, v, lane < listed ? ((uint64_t)list[lane].y << 32) | list[lane].x : 0, lane);
+  put_row(p, row, v, p.top > 0 ? sort_list<LIST / 64>(list, listed, p.top, lane) : 0, lane);
 }
 
 // Threads of a workgroup and logits of a part (the whole row: one launch). skew: logits between an aligned
