@@ -412,9 +412,9 @@ int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_tensor* A, 
  * with the entropy of each row and its likeliest tokens (no counterpart in the reference):
  *   logprobs[r] = logits[r][tokens[r]] - lse[r], entropy[r] = lse[r] - sum_v p[r][v] logits[r][v]
  *   tokens [R] or [B, L] i64, any strides; one outside [0, V) gives 0
- *   logprobs [R] f32, entropy NULL or [R] f32, top_logprobs and top_tokens NULL or [R, top] f32 and i64
- *   (R = B * L), contiguous; top <= 32: the largest logits in descending order, equal ones by the lower
- *   token
+ *   logprobs f32 in the shape of tokens, entropy NULL or the same, top_logprobs and top_tokens NULL or
+ *   [..., top] f32 and i64, all contiguous; top <= 32: the largest logits in descending order, equal ones
+ *   by the lower token
  * A row with a NaN or +inf logit, or without one above -inf, gives NaN (and tokens 0, 1, ...); logits
  * beyond 2^127 in magnitude count as infinite. The workspace needs no particular contents.
  */

@@ -815,7 +815,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprobs: torch.T
                    entropy: torch.Tensor | None, top_logprobs: torch.Tensor | None,
                    top_tokens: torch.Tensor | None) -> None:
     """Log-probabilities of tokens [R] or [B, L] under logits [R, V] or [B, L, V], entropy and the
-    likeliest tokens, into the contiguous outputs [B * L] and [B * L, top]."""
+    likeliest tokens, into the contiguous outputs [...] and [..., top]."""
     host = _host or host_binding()
     if host:
         rc = host.token_logprobs(logits, tokens, logprobs, entropy, top_logprobs, top_tokens,
@@ -825,7 +825,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprobs: torch.T
     dev = _require_gpu(logits, tokens, logprobs, entropy, top_logprobs, top_tokens)
     stream = _stream(dev)
     need = int(lib().lq_token_logprobs_workspace(tokens.numel(), logits.shape[-1],
-                                                 0 if top_tokens is None else top_tokens.shape[1]))
+                                                 0 if top_tokens is None else top_tokens.shape[-1]))
     ws = _scratch.get(dev.index, stream, need) if need else None
     rc = lib().lq_token_logprobs(desc(logits), desc(tokens), desc(logprobs), desc(entropy),
                                  desc(top_logprobs), desc(top_tokens),

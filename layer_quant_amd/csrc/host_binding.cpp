@@ -456,11 +456,11 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   LQ_NOT_PLAIN(!t.add_all(a));
   const lq_tensor* const* p = t.ptr;
   LQ_NOT_PLAIN(p[0] == nullptr || p[0]->ndim < 2 || p[0]->ndim > 3 ||
-               (p[5] != nullptr && (p[5]->ndim != 2 || p[5]->shape[1] > INT32_MAX)));
+               (p[5] != nullptr && (p[5]->ndim != p[0]->ndim || p[5]->shape[p[0]->ndim - 1] > INT32_MAX)));
   const int nd = p[0]->ndim;
   const int64_t rows = (nd == 3 ? p[0]->shape[0] : 1) * p[0]->shape[nd - 2];
   const size_t need = entries.logprobs_workspace(rows, p[0]->shape[nd - 1],
-                                                 p[5] == nullptr ? 0 : (int)p[5]->shape[1]);
+                                                 p[5] == nullptr ? 0 : (int)p[5]->shape[nd - 1]);
   return launch_with(t.device, a[6], need, [&](void* ws, size_t bytes, void* s) {
     return entries.logprobs(p[0], p[1], p[2], p[3], p[4], p[5], ws, bytes, s);
   });

@@ -35,8 +35,10 @@ __device__ __forceinline__ bool finite(float x) {
   return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
 }
 
-template <int DP>
-__global__ __launch_bounds__(64 * NW) void prompt_attention_f32(PromptAttention p) {
+// VEC: fp32 k and v in 16-byte aligned rows of a multiple of 4 dims. Their tiles come in 16-byte loads, a
+// tile ahead.
+template <int DP, bool VEC>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f32(PromptAttention p) {
   __shared__ TileF32<DP> tile;
   const int hk = blockIdx.x % p.Hkv;
   Span sp;
@@ -79,13 +81,36 @@ __global__ __launch_bounds__(64 * NW) void prompt_attention_f32(PromptAttention 
   float m = -INFINITY, l = 0.f;
   const int64_t k_at = lead * p.k.s[0] + sp.begin * p.k.s[1] + hk * p.k.s[2];
   const int64_t v_at = lead * p.v.s[0] + sp.begin * p.v.s[1] + hk * p.v.s[2];
+  constexpr int LOADS = KT * DP / 4 / (64 * NW);  // 16-byte loads of a thread and tile
+  float4 kn[VEC ? LOADS : 1], vn[VEC ? LOADS : 1];
+  auto load_tile = [&](int kb) {
+#pragma unroll
+    for (int j = 0; j < (VEC ? LOADS : 0); ++j) {
+      const int i = j * 64 * NW + tid, key = i / (DP / 4), d = i % (DP / 4) * 4;
+      const bool in = kb + key < sp.len && d < p.D;
+      kn[j] = vn[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in) kn[j] = *(const float4*)((const float*)p.k.data + k_at + (int64_t)(kb + key) * p.k.s[1] + d);
+      if (in) vn[j] = *(const float4*)((const float*)p.v.data + v_at + (int64_t)(kb + key) * p.v.s[1] + d);
+    }
+  };
+  load_tile(0);
   const int pos_first = first / nrep;
   const int pos_last = min(first + NW * ROWS - 1, nrows - 1) / nrep;
   for (int kb = 0; kb <= pos_last; kb += KT) {
     const bool diagonal = kb + KT - 1 > pos_first;  // holds keys that some row must not see
     __syncthreads();
     int bad = 0;
-    for (int i = tid; i < KT * DP; i += 64 * NW) {
+    if (VEC) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int i = j * 64 * NW + tid, key = i / (DP / 4), d = i % (DP / 4) * 4;
+        *(float4*)&tile.k[key][d] = kn[j];
+        *(float4*)&tile.v[key][d] = vn[j];
+        bad |= !finite(vn[j].x) || !finite(vn[j].y) || !finite(vn[j].z) || !finite(vn[j].w);
+      }
+      if (kb + KT <= pos_last) load_tile(kb + KT);
+    }
+    for (int i = tid; i < (VEC ? 0 : KT * DP); i += 64 * NW) {
       const int key = i / DP, d = i % DP;
       float kv = 0.f, vv = 0.f;
       if (kb + key < sp.len && d < p.D) {
@@ -166,6 +191,14 @@ __global__ __launch_bounds__(64 * NW) void prompt_attention_f32(PromptAttention 
       if (d < p.D) store_float(p.out.data, p.out.dtype, out_at + d * p.out.s[3], o[b][i] * inv);
     }
   }
+}
+
+template <bool VEC>
+void launch_f32(const PromptAttention& p, dim3 grid, hipStream_t st) {
+  const dim3 block(64 * NW);
+  if (p.D <= 64) hipLaunchKernelGGL((prompt_attention_f32<64, VEC>), grid, block, 0, st, p);
+  else if (p.D <= 128) hipLaunchKernelGGL((prompt_attention_f32<128, VEC>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((prompt_attention_f32<256, VEC>), grid, block, 0, st, p);
 }
 
 }  // namespace
@@ -264,9 +297,14 @@ extern "C" int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const
     p.scale = scale == 0.f ? 1.f : fabsf(p.scale);
     return launch_prompt_attention_mfma(p, q->dtype, parts, st);
   }
-  const dim3 grid((unsigned)(parts * Hkv)), block(64 * NW);
-  if (D <= 64) hipLaunchKernelGGL(prompt_attention_f32<64>, grid, block, 0, st, p);
-  else if (D <= 128) hipLaunchKernelGGL(prompt_attention_f32<128>, grid, block, 0, st, p);
-  else hipLaunchKernelGGL(prompt_attention_f32<256>, grid, block, 0, st, p);
+  const dim3 grid((unsigned)(parts * Hkv));
+  bool in_rows = q->dtype == LQ_F32 && D % 4 == 0;
+  const lq_tensor* kv[2] = {k, v};
+  for (const lq_tensor* t : kv) {
+    in_rows = in_rows && t->stride[nd - 1] == 1 && ((uintptr_t)t->data & 15) == 0;
+    for (int i = 0; i < nd - 1; ++i) in_rows = in_rows && (t->shape[i] < 2 || t->stride[i] % 4 == 0);
+  }
+  if (in_rows) launch_f32<true>(p, grid, st);
+  else launch_f32<false>(p, grid, st);
   return check_launch("lq_prompt_attention");
 }

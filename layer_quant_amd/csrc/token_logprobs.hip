@@ -462,8 +462,8 @@ extern "C" int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* token
   const int nd = logits != nullptr && logits->ndim == 3 ? 3 : 2;
   if ((rc = check_tensor_or_empty(logits, "logits", nd, true)) != LQ_OK) return rc;
   if ((rc = check_tensor_or_empty(tokens, "tokens", nd - 1, false, LQ_I64)) != LQ_OK) return rc;
-  if ((rc = check_tensor_or_empty(logprobs, "logprobs", 1, false, LQ_F32)) != LQ_OK) return rc;
-  if (entropy != nullptr && (rc = check_tensor_or_empty(entropy, "entropy", 1, false, LQ_F32)) != LQ_OK) return rc;
+  if ((rc = check_tensor_or_empty(logprobs, "logprobs", nd - 1, false, LQ_F32)) != LQ_OK) return rc;
+  if (entropy != nullptr && (rc = check_tensor_or_empty(entropy, "entropy", nd - 1, false, LQ_F32)) != LQ_OK) return rc;
   if ((top_logprobs == nullptr) != (top_tokens == nullptr)) {
     return fail(LQ_ERR_INVALID_ARG, "top_logprobs and top_tokens: both or neither");
   }
@@ -476,17 +476,22 @@ extern "C" int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* token
   }
   int64_t top = 0;
   if (top_logprobs != nullptr) {
-    if ((rc = check_tensor_or_empty(top_logprobs, "top_logprobs", 2, false, LQ_F32)) != LQ_OK) return rc;
-    if ((rc = check_tensor_or_empty(top_tokens, "top_tokens", 2, false, LQ_I64)) != LQ_OK) return rc;
-    top = top_logprobs->shape[1];
+    if ((rc = check_tensor_or_empty(top_logprobs, "top_logprobs", nd, false, LQ_F32)) != LQ_OK) return rc;
+    if ((rc = check_tensor_or_empty(top_tokens, "top_tokens", nd, false, LQ_I64)) != LQ_OK) return rc;
+    top = top_logprobs->shape[nd - 1];
   }
   const lq_tensor* outs[4] = {logprobs, entropy, top_logprobs, top_tokens};
   for (const lq_tensor* t : outs) {
     if (t == nullptr) continue;
-    const bool flat = t->ndim == 1 ? t->stride[0] == 1 || rows < 2
-                                   : (t->stride[1] == 1 || top < 2) && (t->stride[0] == top || rows < 2);
-    if (t->shape[0] != rows || (t->ndim == 2 && t->shape[1] != top) || !flat) {
-      return fail(LQ_ERR_INVALID_ARG, "the outputs must be contiguous and have %lld rows", (long long)rows);
+    bool flat = true;
+    int64_t step = 1;
+    for (int i = t->ndim - 1; i >= 0; --i) {
+      const int64_t want = i < nd - 1 ? logits->shape[i] : top;
+      flat = flat && t->shape[i] == want && (want < 2 || rows < 1 || t->stride[i] == step);
+      step *= want;
+    }
+    if (!flat) {
+      return fail(LQ_ERR_INVALID_ARG, "the outputs must be contiguous and have a value for each row");
     }
   }
   if (rows == 0) return LQ_OK;

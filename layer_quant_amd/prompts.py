@@ -27,8 +27,10 @@ from . import _abi
 
 
 def _no_gradients(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the prompt operators have no backward: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the prompt operators have no backward: call them under torch.no_grad()")
 
 
 def _check_prompts(name: str, t: torch.Tensor, starts: torch.Tensor | None) -> None:
@@ -120,15 +122,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if top < 0:
         raise ValueError(f"top must not be negative, got {top}")
     _no_gradients(logits)
-    lead, rows = tuple(tokens.shape), tokens.numel()
-    device = logits.device
-    logprobs = torch.empty(rows, device=device, dtype=torch.float32)
-    entropy = torch.empty(rows, device=device, dtype=torch.float32)
+    lead, device = tokens.shape, logits.device
+    logprobs = torch.empty(lead, device=device, dtype=torch.float32)
+    entropy = torch.empty(lead, device=device, dtype=torch.float32)
     top_logprobs = top_tokens = None
     if top:
-        top_logprobs = torch.empty((rows, top), device=device, dtype=torch.float32)
-        top_tokens = torch.empty((rows, top), device=device, dtype=torch.int64)
+        top_logprobs = torch.empty((*lead, top), device=device, dtype=torch.float32)
+        top_tokens = torch.empty((*lead, top), device=device, dtype=torch.int64)
     _abi.token_logprobs(logits, tokens, logprobs, entropy, top_logprobs, top_tokens)
-    return TokenLogprobs(logprobs.view(lead), entropy.view(lead),
-                         None if top_logprobs is None else top_logprobs.view(*lead, top),
-                         None if top_tokens is None else top_tokens.view(*lead, top))
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)
