@@ -51,8 +51,40 @@ __device__ __forceinline__ float sums_of_four(const float (&v)[4], int lane) {
   return r;
 }
 
-template <int NPL, bool ADDS>
-__global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
+// Four values in a row as they lie in memory (8 bytes of 16-bit ones in x and y).
+template <int SIZE>
+__device__ __forceinline__ uint4 load_raw4(const void* base, int64_t at) {
+  if (SIZE == 4) return *(const uint4*)((const char*)base + at * 4);
+  const uint2 w = *(const uint2*)((const char*)base + at * 2);
+  return make_uint4(w.x, w.y, 0, 0);
+}
+template <int SIZE>
+__device__ __forceinline__ float4 values_of(uint4 w, int dtype) {
+  if (SIZE == 4) return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+  return make_float4(word_elem(w.x, 0, dtype), word_elem(w.x, 16, dtype), word_elem(w.y, 0, dtype),
+                     word_elem(w.y, 16, dtype));
+}
+template <int SIZE>
+__device__ __forceinline__ void store4(void* base, int dtype, int64_t at, float4 v) {
+  if (SIZE == 4) {
+    *(float4*)((char*)base + at * 4) = v;
+    return;
+  }
+  uint2 w;
+  if (dtype == LQ_BF16) {
+    w.x = float_to_bf16_bits(v.x) | ((uint32_t)float_to_bf16_bits(v.y) << 16);
+    w.y = float_to_bf16_bits(v.z) | ((uint32_t)float_to_bf16_bits(v.w) << 16);
+  } else {
+    w.x = __builtin_bit_cast(uint16_t, (_Float16)v.x) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v.y) << 16);
+    w.y = __builtin_bit_cast(uint16_t, (_Float16)v.z) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v.w) << 16);
+  }
+  *(uint2*)((char*)base + at * 2) = w;
+}
+
+// ADDS: find_segment's. SIZE: bytes of a value of x, B, C, z and out where four in a row are loaded at once,
+// a block of rows ahead, by WAVES waves; 0: any layout.
+template <int NPL, bool ADDS, int SIZE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void scan_rows_kernel(PromptScan p) {
   __shared__ RowTile<NPL> tile;
   const int h = blockIdx.x % p.H;
   const Segment seg = find_segment<ADDS>(p, blockIdx.x / p.H);
@@ -101,23 +133,57 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
   const int64_t b_at = lead * p.B.s[0] + g * p.B.s[2], c_at = lead * p.C.s[0] + g * p.C.s[2];
   const int64_t dt_at = lead * p.dt.s[0] + h * p.dt.s[2];
   float log_decay = 0.f;
+  // 16-byte chunks of a block: x, then B and C
+  constexpr int XC = 4 * WAVES, CHUNKS = TB * (XC + 8 * NPL), LOADS = CHUNKS / (64 * WAVES);
+  static_assert(SIZE == 0 || CHUNKS % (64 * WAVES) == 0, "every thread loads as many");
+  uint4 raw[SIZE == 0 ? 1 : LOADS];
+  auto load_block = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < (SIZE == 0 ? 0 : LOADS); ++j) {
+      const int i = j * 64 * WAVES + tid;
+      const bool is_x = i < TB * XC;
+      const int k = is_x ? i : i - TB * XC;
+      const int r = is_x ? k / XC : k / (8 * NPL), c = 4 * (is_x ? k % XC : k % (4 * NPL));
+      const bool is_b = is_x || k % (8 * NPL) < 4 * NPL;
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (t + r >= to || c >= (is_x ? width : p.N)) continue;
+      const int64_t row = row0 + t + r;
+      raw[j] = is_x ? load_raw4<SIZE>(p.x.data, x_at + row * p.x.s[1] + c)
+                    : load_raw4<SIZE>(is_b ? p.B.data : p.C.data,
+                                      is_b ? b_at + row * p.B.s[1] + c : c_at + row * p.C.s[1] + c);
+    }
+  };
+  load_block(from);
   for (int t = from; t < to; t += TB) {
     const int rows = min(TB, to - t);
     const int64_t row = row0 + t;
     __syncthreads();
-    for (int i = tid; i < rows * PB; i += blockDim.x) {
-      const int r = i / PB, c = i % PB;
-      tile.x[r][c] = c < width ? load_float(p.x.data, p.x.dtype, x_at + (row + r) * p.x.s[1] + c * p.x.s[3]) : 0.f;
-    }
-    for (int i = tid; i < rows * 16 * NPL; i += blockDim.x) {
-      const int r = i / (16 * NPL), n = i % (16 * NPL);
-      float b = 0.f, c = 0.f;
-      if (n < p.N) {
-        b = load_float(p.B.data, p.B.dtype, b_at + (row + r) * p.B.s[1] + n * p.B.s[3]);
-        c = load_float(p.C.data, p.C.dtype, c_at + (row + r) * p.C.s[1] + n * p.C.s[3]);
+    if (SIZE != 0) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int i = j * 64 * WAVES + tid;
+        const bool is_x = i < TB * XC;
+        const int k = is_x ? i : i - TB * XC;
+        const int r = is_x ? k / XC : k / (8 * NPL), c = 4 * (is_x ? k % XC : k % (4 * NPL));
+        float* to_row = is_x ? tile.x[r] : k % (8 * NPL) < 4 * NPL ? tile.b[r] : tile.c[r];
+        *(float4*)&to_row[c] = values_of<SIZE == 0 ? 4 : SIZE>(raw[j], p.x.dtype);
       }
-      tile.b[r][n] = b;
-      tile.c[r][n] = c;
+      load_block(t + TB);
+    } else {
+      for (int i = tid; i < rows * PB; i += blockDim.x) {
+        const int r = i / PB, c = i % PB;
+        tile.x[r][c] = c < width ? load_float(p.x.data, p.x.dtype, x_at + (row + r) * p.x.s[1] + c * p.x.s[3]) : 0.f;
+      }
+      for (int i = tid; i < rows * 16 * NPL; i += blockDim.x) {
+        const int r = i / (16 * NPL), n = i % (16 * NPL);
+        float b = 0.f, c = 0.f;
+        if (n < p.N) {
+          b = load_float(p.B.data, p.B.dtype, b_at + (row + r) * p.B.s[1] + n * p.B.s[3]);
+          c = load_float(p.C.data, p.C.dtype, c_at + (row + r) * p.C.s[1] + n * p.C.s[3]);
+        }
+        tile.b[r][n] = b;
+        tile.c[r][n] = c;
+      }
     }
     if (tid < rows) {
       const float dt = scan_step(p, load_float(p.dt.data, p.dt.dtype, dt_at + (row + tid) * p.dt.s[1]), bias);
@@ -152,7 +218,23 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(PromptScan p) {
     }
     if (!ADDS) {
       __syncthreads();
-      for (int i = tid; i < rows * PB; i += blockDim.x) {
+      for (int i = tid; i < (SIZE == 0 ? 0 : rows * XC); i += 64 * WAVES) {
+        const int r = i / XC, c = 4 * (i % XC);
+        if (c >= width) continue;
+        const float4 x4 = *(const float4*)&tile.x[r][c];
+        float4 y4 = *(const float4*)&tile.y[r][c];
+        y4 = make_float4(fmaf(D, x4.x, y4.x), fmaf(D, x4.y, y4.y), fmaf(D, x4.z, y4.z), fmaf(D, x4.w, y4.w));
+        if (p.z.data != nullptr) {
+          const float4 z4 = values_of<SIZE == 0 ? 4 : SIZE>(
+              load_raw4<SIZE == 0 ? 4 : SIZE>(p.z.data, z_at + (row + r) * p.z.s[1] + c), p.x.dtype);
+          y4.x *= scan_silu(z4.x);
+          y4.y *= scan_silu(z4.y);
+          y4.z *= scan_silu(z4.z);
+          y4.w *= scan_silu(z4.w);
+        }
+        store4<SIZE == 0 ? 4 : SIZE>(p.out.data, p.x.dtype, out_at + (row + r) * p.out.s[1] + c, y4);
+      }
+      for (int i = tid; i < (SIZE == 0 ? rows * PB : 0); i += blockDim.x) {
         const int r = i / PB, c = i % PB;
         if (c >= width) continue;
         float y = fmaf(D, tile.x[r][c], tile.y[r][c]);
@@ -256,14 +338,16 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
   }
 }
 
-constexpr int MIN_SEGMENT = 256;
-
-// Rows of a segment: as many as give about four workgroups per CU, a multiple of 64 and 256 at least
-// (a shorter one costs more in carried states than it wins).
-int64_t plan_segment(int64_t rows, int64_t heads) {
+// Rows of a segment, a multiple of 64: as many as give about four workgroups per CU (of the rows kernel; two
+// of the matrix kernel). Eight prompts or more fill the GPU with the matrix kernel's workgroups by themselves
+// unless their lengths differ much: twice as many rows then (24 prompts up to 700 rows of 128 heads: 134
+// -> 117 us; the rows kernel, 16 up to 900, would go from 574 to 791). A segment costs a part of the work
+// again and two launches, so that it has at least 256 rows (200 rows in two segments of 128 37 us, in one
+// 24), or 64 where the heads give few workgroups (8000 rows of 8 heads: 184 us with 256, 77 with 64).
+int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) {
   const int64_t want = (rows * heads + 4 * device_cus() - 1) / (4 * device_cus());
-  const int64_t seg = (want + 63) / 64 * 64;
-  return seg < MIN_SEGMENT ? MIN_SEGMENT : seg;
+  const int64_t seg = (matrix && prompts >= 8 ? 2 * want : want) + 63;
+  return max(seg / 64 * 64, matrix || heads >= 64 ? (int64_t)256 : (int64_t)64);
 }
 
 // Slots, at most: a prompt has a segment more than its rows fill, or, as one of several segments has more
@@ -276,12 +360,34 @@ int64_t slots_of(int64_t prompts, int64_t rows, int64_t segment, bool packed) {
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+template <bool ADDS, int SIZE, int WAVES>
+void launch_rows_of(const PromptScan& p, dim3 grid, hipStream_t st) {
+  const dim3 block(SIZE == 0 ? 64 * min(4, (p.P + 15) / 16) : 64 * WAVES);
+  if (p.N <= 64) hipLaunchKernelGGL((scan_rows_kernel<4, ADDS, SIZE, WAVES>), grid, block, 0, st, p);
+  else if (p.N <= 128) hipLaunchKernelGGL((scan_rows_kernel<8, ADDS, SIZE, WAVES>), grid, block, 0, st, p);
+  else if constexpr (SIZE == 0) hipLaunchKernelGGL((scan_rows_kernel<16, ADDS, 0, 4>), grid, block, 0, st, p);
+}
+
+// size: bytes of a value where all rows can be loaded four values at a time and N <= 128, else 0
 template <bool ADDS>
-void launch_rows(const PromptScan& p, dim3 grid, hipStream_t st) {
-  const dim3 block(64 * min(4, (p.P + 15) / 16));
-  if (p.N <= 64) hipLaunchKernelGGL((scan_rows_kernel<4, ADDS>), grid, block, 0, st, p);
-  else if (p.N <= 128) hipLaunchKernelGGL((scan_rows_kernel<8, ADDS>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((scan_rows_kernel<16, ADDS>), grid, block, 0, st, p);
+void launch_rows(const PromptScan& p, int size, dim3 grid, hipStream_t st) {
+  if (size == 4 && p.P <= 16) launch_rows_of<ADDS, 4, 1>(p, grid, st);
+  else if (size == 4) launch_rows_of<ADDS, 4, 4>(p, grid, st);
+  else if (size == 2 && p.P <= 16) launch_rows_of<ADDS, 2, 1>(p, grid, st);
+  else if (size == 2) launch_rows_of<ADDS, 2, 4>(p, grid, st);
+  else launch_rows_of<ADDS, 0, 4>(p, grid, st);
+}
+
+// Values of x's type, four in a row at addresses that are multiples of their bytes.
+bool in_fours(const lq_tensor* t, int dtype) {
+  if (t == nullptr) return true;
+  const int nd = t->ndim, size = dtype_size(dtype);
+  if (t->dtype != dtype || t->stride[nd - 1] != 1 || t->shape[nd - 1] % 4 != 0) return false;
+  if (((uintptr_t)t->data & (4 * size - 1)) != 0) return false;
+  for (int i = 0; i < nd - 1; ++i) {
+    if (t->shape[i] > 1 && t->stride[i] % 4 != 0) return false;
+  }
+  return true;
 }
 
 }  // namespace
@@ -293,8 +399,8 @@ extern "C" size_t lq_prompt_scan_workspace(int dtype, int64_t prompts, int64_t r
                                            int64_t heads, int64_t head_dim, int64_t dstate) {
   if (prompts <= 0 || rows <= 0 || heads <= 0 || head_dim <= 0 || dstate <= 0) return 0;
   const int64_t total = packed ? rows : prompts * rows;
-  const int64_t slots = slots_of(prompts, rows, plan_segment(total, heads), packed != 0);
   const bool mfma = prompt_scan_mfma_geometry(dtype, heads, head_dim, dstate);
+  const int64_t slots = slots_of(prompts, rows, plan_segment(mfma, prompts, total, heads), packed != 0);
   return align256((size_t)(slots * heads * head_dim * dstate) * 4) + align256((size_t)(slots * heads) * 4) +
          (mfma ? prompt_scan_mfma_workspace(total, heads) : 0);
 }
@@ -360,7 +466,7 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
     return fail(LQ_ERR_UNSUPPORTED, "%lld rows of %lld prompts exceed the launch limits",
                 (long long)total, (long long)S);
   }
-  p.segment = (int)plan_segment(total, H);
+  p.segment = (int)plan_segment(prompt_scan_mfma_geometry(x->dtype, H, P, N), S, total, H);
   const int64_t slots = slots_of(S, rows, p.segment, nd == 3);
   const int64_t parts =
       nd == 4 ? batch * (rows == 0 ? 1 : (rows + p.segment - 1) / p.segment) : rows / p.segment + S + 2;
@@ -410,6 +516,9 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   if (!mfma && diag(LQ_DIAG_PROMPT_REQUIRE_MFMA)) {
     return fail(LQ_ERR_INVALID_ARG, "the call takes the general kernel");
   }
+  int size = dtype_size(x->dtype);
+  const lq_tensor* fours[5] = {x, B, C, z, out};
+  for (const lq_tensor* t : fours) size = in_fours(t, x->dtype) && N <= 128 ? size : 0;
   const unsigned blocks = (unsigned)((H * P * N + 255) / 256);
   if (mfma && total > 0) {
     launch_prompt_scan_steps(p, chunks, st);
@@ -417,14 +526,14 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   }
   if (slots > 0) {
     if (mfma) launch_prompt_scan_mfma(p, true, slots, st);
-    else launch_rows<true>(p, dim3((unsigned)(slots * H), (unsigned)pblocks), st);
+    else launch_rows<true>(p, size, dim3((unsigned)(slots * H), (unsigned)pblocks), st);
     if ((rc = check_launch("lq_prompt_scan (segments)")) != LQ_OK) return rc;
     hipLaunchKernelGGL(scan_carry_kernel, dim3((blocks + 3) / 4, (unsigned)slots), dim3(256), 0, st, p);
     if ((rc = check_launch("lq_prompt_scan (carry)")) != LQ_OK) return rc;
   }
   if (parts > 0) {
     if (mfma) launch_prompt_scan_mfma(p, false, parts, st);
-    else launch_rows<false>(p, dim3((unsigned)(parts * H), (unsigned)pblocks), st);
+    else launch_rows<false>(p, size, dim3((unsigned)(parts * H), (unsigned)pblocks), st);
     if ((rc = check_launch("lq_prompt_scan")) != LQ_OK) return rc;
   }
   return LQ_OK;

@@ -112,7 +112,7 @@ def test_scan_of_nothing():
     assert lib.lq_prompt_scan_workspace(bf, 1, 0, 1, 8, 64, 128) == 0
     assert lib.lq_prompt_scan_workspace(bf, 0, 5, 0, 8, 64, 128) == 0
     # prompts of one segment carry nothing
-    assert lib.lq_prompt_scan_workspace(f32, 4, 200, 0, 8, 64, 128) == 0
+    assert lib.lq_prompt_scan_workspace(f32, 4, 200, 0, 64, 64, 128) == 0
     assert lib.lq_prompt_scan_workspace(f32, 1, 16384, 1, 128, 64, 128) > 0
     assert lib.lq_prompt_scan_workspace(bf, 4, 200, 0, 8, 64, 128) == 4 * 200 * 8 * 16
 
