@@ -9,7 +9,7 @@ by HIP kernels for gfx950 behind the C ABI (include/layer_quant.h):
     _int4_prefill_attention_kernel  -> lq_int4_prefill_attention  (ia.py:114-251)
 
 The reference never calls its prefill kernel (the patched forward runs SDPA on unquantized K/V
-for q_len > 1, ia.py:693-714, and so does this module); _prefill_attention keeps its
+for q_len > 1, ia.py:693-714, and so does this module by default); _prefill_attention keeps its
 signature (ia.py:594-625) for callers that attend over the packed cache instead.
 """
 from __future__ import annotations
@@ -20,7 +20,7 @@ from types import MethodType
 
 import torch
 
-from . import _abi
+from . import _abi, prompts
 
 
 @dataclass
@@ -287,8 +287,9 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
                            past_key_value=None, output_attentions=False, use_cache=False,
                            cache_position=None):
     """Patched attention forward (ia.py:628-714): pack this step's K/V into the INT4 cache;
-    decode (q_len == 1) attends over the cache, prefill runs SDPA on the unquantized K/V. Over a cache
-    with a shared prefix (beam_decode.share_prompt) only decode steps behind the prefix are defined."""
+    decode (q_len == 1) attends over the cache, prefill runs SDPA on the unquantized K/V, or with
+    prompt_kernel, no mask and no gradients prompts.prompt_attention. Over a cache with a shared prefix
+    (beam_decode.share_prompt) only decode steps behind the prefix are defined."""
     if output_attentions or hidden_states.device.type != "cuda" or past_key_value is None:
         return self._int4_kv_original_forward(
             hidden_states=hidden_states, attention_mask=attention_mask,
@@ -350,6 +351,11 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
                            layer_cache.k_scale, layer_cache.v_scale, positions, group_size)
     layer_cache.length = max(layer_cache.length, required_len)
 
+    if attention_mask is None and self._int4_kv_prompt_kernel and not torch.is_grad_enabled():
+        attn = prompts.prompt_attention(query_states.transpose(1, 2), key_states.transpose(1, 2),
+                                        value_states.transpose(1, 2))
+        return self.o_proj(attn.reshape(bsz, q_len, self.hidden_size)), None, past_key_value
+
     key_full = self._int4_kv_repeat_kv(key_states, self.num_key_value_groups)
     value_full = self._int4_kv_repeat_kv(value_states, self.num_key_value_groups)
     causal_mask = None
@@ -366,11 +372,13 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
     return self.o_proj(attn), None, past_key_value
 
 
-def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64):
+def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64, *, prompt_kernel: bool = False):
     """Route every attention block's forward through the INT4 cache (ia.py:717-731).
 
     Idempotent per layer; records the original forward, the group size and the remote module's
-    repeat_kv on each patched mixer.
+    repeat_kv on each patched mixer. prompt_kernel (no reference counterpart): prompts without a mask,
+    with gradients off, attend by prompts.prompt_attention, which reads each KV head once for its query
+    heads, instead of SDPA on repeated K and V.
     """
     remote = __import__(model.__class__.__module__, fromlist=["repeat_kv"])
     repeat_kv = remote.repeat_kv
@@ -382,6 +390,7 @@ def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64):
             continue
         attn._int4_kv_original_forward = attn.forward
         attn._int4_kv_group_size = group_size
+        attn._int4_kv_prompt_kernel = prompt_kernel
         attn._int4_kv_repeat_kv = repeat_kv
         attn.forward = MethodType(_forward_fused_int4_kv, attn)
         attn._int4_kv_patched = True
