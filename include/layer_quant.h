@@ -378,7 +378,8 @@ int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, int count,
  *     front of starts[0] and behind starts[S] get zeros. Starts outside [0, T] count as 0 or T; prompts
  *     that are not in ascending order give unspecified values.
  *   a batch: starts NULL, q, out [B, L, Hq, D], k, v [B, L, Hkv, D], every batch row a prompt
- *   q, k, v and out of one dtype (f32, f16 or bf16), any strides; D <= 256
+ *   q, k, v and out of one dtype (f32, f16 or bf16), any strides; D <= 256. out may be q, and overlaps
+ *   neither k nor v nor itself.
  * Rows behind a query's own never reach its result, whatever they hold.
  */
 int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor* v,

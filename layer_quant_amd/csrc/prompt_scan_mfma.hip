@@ -98,9 +98,11 @@ __global__ __launch_bounds__(256) void scan_steps_kernel(PromptScan p) {
     const double A = (double)load_float(p.A.data, p.A.dtype, h * p.A.s[0]) * 1.4426950408889634;
     const float bias = p.bias.data == nullptr ? 0.f : load_float(p.bias.data, p.bias.dtype, h * p.bias.s[0]);
     const bool in = lane < have;
-    const float dt = in ? scan_step(p, tile[lane][j], bias) : 0.f;
-    // (a NaN step has a decay here, and its NaN in what it multiplies)
-    const double c = prefix_sum(in ? fmin(fmax(A * dt, -256.0), 256.0) : 0.0);
+    float dt = in ? scan_step(p, tile[lane][j], bias) : 0.f;
+    // a decay that is NaN counts as one here, and has its NaN in what the step multiplies
+    const double lg = A * dt;
+    if (in && lg != lg) dt = __builtin_nanf("");
+    const double c = prefix_sum(in ? fmin(fmax(lg, -256.0), 256.0) : 0.0);
     const uint64_t u = __builtin_bit_cast(uint64_t, c);
     const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, 63);
     const uint32_t up = __builtin_amdgcn_readlane((uint32_t)(u >> 32), 63);
@@ -546,8 +548,9 @@ bool prompt_scan_mfma_fits(const lq_tensor* x, const lq_tensor* B, const lq_tens
   const lq_tensor* by_chunk[5] = {x, B, C, z, out};
   for (const lq_tensor* t : by_chunk) {
     if (t == nullptr) continue;
+    // (a single row's too: the rows past it have to be past the descriptors)
     const int64_t s = t->stride[nd - 3];
-    if (t->shape[nd - 3] > 1 && (s < t->shape[nd - 1] || s > (1 << 22))) return false;
+    if (s < t->shape[nd - 1] || s > (1 << 22)) return false;
   }
   return true;
 }

@@ -288,7 +288,7 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
                            cache_position=None):
     """Patched attention forward (ia.py:628-714): pack this step's K/V into the INT4 cache;
     decode (q_len == 1) attends over the cache, prefill runs SDPA on the unquantized K/V, or with
-    prompt_kernel, no mask and no gradients prompts.prompt_attention. Over a cache with a shared prefix
+    prompt_kernel, no mask, gradients or dropout prompts.prompt_attention. Over a cache with a shared prefix
     (beam_decode.share_prompt) only decode steps behind the prefix are defined."""
     if output_attentions or hidden_states.device.type != "cuda" or past_key_value is None:
         return self._int4_kv_original_forward(
@@ -351,7 +351,8 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
                            layer_cache.k_scale, layer_cache.v_scale, positions, group_size)
     layer_cache.length = max(layer_cache.length, required_len)
 
-    if attention_mask is None and self._int4_kv_prompt_kernel and not torch.is_grad_enabled():
+    if attention_mask is None and self._int4_kv_prompt_kernel and not torch.is_grad_enabled() \
+            and not (self.training and self.attention_dropout):
         attn = prompts.prompt_attention(query_states.transpose(1, 2), key_states.transpose(1, 2),
                                         value_states.transpose(1, 2))
         return self.o_proj(attn.reshape(bsz, q_len, self.hidden_size)), None, past_key_value
@@ -377,7 +378,7 @@ def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64, *, prompt_ke
 
     Idempotent per layer; records the original forward, the group size and the remote module's
     repeat_kv on each patched mixer. prompt_kernel (no reference counterpart): prompts without a mask,
-    with gradients off, attend by prompts.prompt_attention, which reads each KV head once for its query
+    with gradients and dropout off, attend by prompts.prompt_attention, which reads each KV head once for its query
     heads, instead of SDPA on repeated K and V.
     """
     remote = __import__(model.__class__.__module__, fromlist=["repeat_kv"])

@@ -51,7 +51,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     """Causal attention of whole prompts: query [T, Hq, D], key and value [T, Hkv, D] with `starts`, or
     [B, L, heads, D] without, in fp32, fp16 or bf16 with any strides; Hq a multiple of Hkv, D <= 256.
     Row t of a prompt attends to the prompt's rows up to t; scale is 1 / sqrt(D) unless given.
-    -> query's shape and dtype, in `out` where given.
+    -> query's shape and dtype, in `out` where given (which may be query, and overlaps no key or value).
 
     Scores, softmax and sums are fp32 (16-bit inputs: the weights are rounded to that type before
     they multiply the values). What stands behind a row in its prompt never reaches its result, be it NaN.

@@ -163,6 +163,50 @@ def test_attention_scale_and_large_scores(gpu):
     check_attention(gpu, (q * 30).contiguous(), k, v, starts, "large scores", scale=1.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_attention_small_values(gpu, dtype):
+    """Values, and products of scores, below the type's smallest normal number."""
+    q, k, v = attention_inputs(gpu, 70, 4, 2, 128, dtype, seed=12)
+    least = torch.finfo(dtype).tiny
+    starts = starts_of([70], gpu)
+    got = prompts.prompt_attention(q, (k.float() * least).to(dtype), (v.float() * least / 4).to(dtype), starts,
+                                   scale=1.0)
+    want, weight, score = ref.attention(q, (k.float() * least).to(dtype), (v.float() * least / 4).to(dtype),
+                                        [0, 70], 1.0)
+    within(got, want, ref.attention_bound(want, weight, score, dtype, 128), f"{dtype}")
+
+
+def test_attention_in_place(gpu):
+    q, k, v = attention_inputs(gpu, 300, 4, 2, 128, BF, seed=13)
+    starts = starts_of([200, 100], gpu)
+    want = prompts.prompt_attention(q, k, v, starts)
+    assert torch.equal(prompts.prompt_attention(q, k, v, starts, out=q), want)
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows 128 KiB apart and more: the same as rows one behind another."""
+    rows, apart = 40000, 65536
+    far = torch.empty(rows * apart, device=gpu, dtype=BF)
+    gen = torch.Generator(device=gpu).manual_seed(14)
+    tight = torch.randn(rows, 1, 384, device=gpu, generator=gen).to(BF)
+    wide = far.as_strided((rows, 1, 384), (apart, 384, 1))
+    wide.copy_(tight)
+    starts = torch.tensor([0, 7, rows], device=gpu)
+    split = lambda t: t.split(128, 2)  # noqa: E731
+    assert torch.equal(prompts.prompt_attention(*split(wide), starts),
+                       prompts.prompt_attention(*split(tight), starts))
+    x = lambda t: t.as_strided((rows, 2, 64), (t.stride(0), 64, 1), t.storage_offset())  # noqa: E731
+    dt, A = torch.randn(rows, 2, device=gpu, generator=gen), -torch.rand(2, device=gpu, generator=gen)
+    got = [prompts.prompt_scan(x(t), dt, A, *split(t)[1:], starts, dt_softplus=True) for t in (wide, tight)]
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    logits = torch.randn(20, 131072, device=gpu, generator=gen).to(BF)
+    spread = far.as_strided((20, 131072), (1 << 27, 1))
+    spread.copy_(logits)
+    tokens = torch.arange(20, device=gpu)
+    for a, b in zip(prompts.token_logprobs(spread, tokens, 4), prompts.token_logprobs(logits, tokens, 4)):
+        assert torch.equal(a, b)
+
+
 def test_attention_out_of_range_starts(gpu):
     """Starts past the rows count as the last row: nothing outside is read or written."""
     q, k, v = attention_inputs(gpu, 60, 4, 2, 128, BF, seed=6)
@@ -339,6 +383,67 @@ def test_scan_large_and_small_steps(gpu):
     for k in ("x", "B", "C"):
         t[k] = t[k].to(BF)
     check_scan(gpu, t, starts_of([200], gpu), "bf16")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_scan_starts_out_of_order(gpu, dtype):
+    """Starts that do not ascend give no defined values, and read and write nothing outside."""
+    t = scan_inputs(gpu, 1500, 4, 64, 128, 1, dtype, seed=16)
+    for s in ([0, 1500, 0, 1500, 0, 1500], [1500, 0], [-5, 3000, 7, -1, 1500], [900, 900, 100, 1500]):
+        starts = torch.tensor(s, device=gpu)
+        y, st = prompts.prompt_scan(t["x"], t["dt"], t["A"], t["B"], t["C"], starts, dt_softplus=True)
+        prompts.prompt_attention(t["x"], t["x"], t["x"], starts)
+        torch.cuda.synchronize()
+        assert y.shape == t["x"].shape and st.shape[0] == len(s) - 1
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_scan_growing_and_nan_decays(gpu, dtype):
+    """A > 0 (states that grow), A = 0, and NaN in A: that head's rows and state alone."""
+    t = scan_inputs(gpu, 90, 4, 64, 128, 1, dtype, seed=17)
+    t["A"] = torch.tensor([0.5, 0.0, math.nan, -1.0], device=gpu)
+    y, st = prompts.prompt_scan(t["x"], t["dt"], t["A"], t["B"], t["C"], starts_of([90], gpu),
+                                dt_bias=t["dt_bias"], dt_softplus=True)
+    assert torch.isnan(y[:, 2]).all() and torch.isnan(st[0, 2]).all()
+    good = [0, 1, 3]
+    pick = dict(t, x=t["x"][:, good], dt=t["dt"][:, good], A=t["A"][good], dt_bias=t["dt_bias"][good])
+    want, ws, wy, size = ref.scan(pick["x"], pick["dt"], pick["A"], t["B"], t["C"], [0, 90],
+                                  dt_bias=pick["dt_bias"], dt_softplus=True)
+    by, bs = scan_bounds(want, ws, wy, size, dtype, F32, 90)
+    within(y[:, good], want, by, "y")
+    within(st[:, good], ws, bs, "states")
+
+
+def test_scan_single_row_strides(gpu):
+    """A batch of single rows whose row strides say nothing (a transposed view of one row)."""
+    t = scan_inputs(gpu, 3, 8, 64, 128, 2, BF, seed=18)
+    y, st = prompts.prompt_scan(t["x"], t["dt"], t["A"], t["B"], t["C"], starts_of([1, 1, 1], gpu))
+    odd = {k: t[k].as_strided((3, 1, *t[k].shape[1:]), (t[k].stride(0), 0, *t[k].stride()[1:]))
+           for k in ("x", "dt", "B", "C")}
+    y1, st1 = prompts.prompt_scan(odd["x"], odd["dt"], t["A"], odd["B"], odd["C"])
+    want, ws, wy, size = ref.scan(t["x"], t["dt"], t["A"], t["B"], t["C"], [0, 1, 2, 3])
+    by, bs = scan_bounds(want, ws, wy, size, BF, F32, 3)
+    for a, b in ((y, st), (y1[:, 0], st1)):
+        within(a, want, by, "y")
+        within(b, ws, bs, "states")
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_scan_kernels_by_layout(gpu, dtype, diag):
+    """bf16 with 64 x 128 states, 16-byte aligned, takes the matrix kernel, anything else the rows one."""
+    from layer_quant_amd import _abi
+
+    t = scan_inputs(gpu, 400, 8, 64, 128, 2, dtype, seed=19)
+    starts = starts_of([300, 100], gpu)
+    diag.set("LQ_PROMPT_REQUIRE_MFMA")
+    if dtype == BF:
+        check_scan(gpu, t, starts, "matrix")
+    else:
+        with pytest.raises(_abi.LQError, match="general kernel"):
+            check_scan(gpu, t, starts, "rows")
+    diag.clear("LQ_PROMPT_REQUIRE_MFMA")
+    diag.set("LQ_PROMPT_FORCE_GENERIC")
+    check_scan(gpu, t, starts, "rows")
 
 
 def test_scan_agrees_with_single_tokens(gpu):
