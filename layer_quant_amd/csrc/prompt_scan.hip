@@ -339,15 +339,19 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
 }
 
 // Rows of a segment, a multiple of 64: as many as give about four workgroups per CU (of the rows kernel; two
-// of the matrix kernel). Eight prompts or more fill the GPU with the matrix kernel's workgroups by themselves
-// unless their lengths differ much: twice as many rows then (24 prompts up to 700 rows of 128 heads: 134
-// -> 117 us; the rows kernel, 16 up to 900, would go from 574 to 791). A segment costs a part of the work
-// again and two launches, so that it has at least 256 rows (200 rows in two segments of 128 37 us, in one
-// 24), or 64 where the heads give few workgroups (8000 rows of 8 heads: 184 us with 256, 77 with 64).
+// of the matrix kernel). Segments cost a part of the work again and two launches.
+// Matrix kernel: at least 256 rows, and prompts of up to 1024 rows, as far as their mean says, stay whole (4
+// prompts of 512 rows and 128 heads: 71 us in two segments each, 41 whole; one of 2000 rows: 107 us in two
+// of 1024, 73 in eight of 256). Eight prompts or more fill the GPU by themselves unless their lengths differ
+// much: twice as many rows then (24 prompts up to 700 rows: 134 -> 117 us; with the rows kernel, 16 up to 900
+// would go from 574 to 791).
+// Rows kernel: at least 256, or 64 where the heads give few workgroups (8000 rows of 8 heads: 184 us with
+// 256, 77 with 64).
 int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) {
   const int64_t want = (rows * heads + 4 * device_cus() - 1) / (4 * device_cus());
-  const int64_t seg = (matrix && prompts >= 8 ? 2 * want : want) + 63;
-  return max(seg / 64 * 64, matrix || heads >= 64 ? (int64_t)256 : (int64_t)64);
+  if (!matrix) return max((want + 63) / 64 * 64, heads >= 64 ? (int64_t)256 : (int64_t)64);
+  const int64_t seg = (prompts >= 8 ? 2 * want : want) + 63;
+  return max(seg / 64 * 64, rows <= 1024 * prompts ? (int64_t)1024 : (int64_t)256);
 }
 
 // Slots, at most: a prompt has a segment more than its rows fill, or, as one of several segments has more

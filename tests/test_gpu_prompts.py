@@ -320,6 +320,17 @@ def test_scan_segments(gpu, dtype):
     assert (y[:first] == 0).all() and (y[first + sum(lengths):] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_scan_many_segments(gpu, dtype):
+    """One long prompt in ten segments and more, the state in place, and without states before it."""
+    t = scan_inputs(gpu, 2600, 4, 64, 128, 1, dtype, seed=20)
+    t["A"] *= 0.02
+    starts = starts_of([2600], gpu)
+    state = torch.randn(1, 4, 64, 128, device=gpu, generator=torch.Generator(device=gpu).manual_seed(21))
+    check_scan(gpu, t, starts, "in place", initial=state, states=state, first_states=state.clone())
+    check_scan(gpu, t, starts, "bf16 states", states=torch.empty(1, 4, 64, 128, device=gpu, dtype=BF))
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 def test_scan_strides_and_options(gpu, dtype):
     """Views of one tensor as the convolution leaves them, a batch, fp32 steps, limits, no softplus."""
