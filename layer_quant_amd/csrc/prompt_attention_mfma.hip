@@ -22,6 +22,12 @@
 // Masked keys of a row have p = 0, which a value of inf or NaN would turn into NaN. Results that are not
 // finite are rare, so it is they that are looked for: a workgroup with one runs its rows again, and then
 // hands such values to the rows that see them and takes them out of the tile.
+//
+// What it measured (MI355X, 32 query / 8 KV heads of 128, us per call): one prompt of 16384 rows 1976-2057,
+// 1.07-1.11 PFLOP/s, where the library's large bf16 product reaches 1.14; 24 fp16 prompts up to 700 rows 31.6;
+// one of 333 rows 11.7. Bound by issue: per tile and wave 32 matrix instructions of 32 cycles and the softmax's VALU
+// instructions; the short ones by latency, up to 11 tiles in a row behind the span search and cold
+// instructions. prompt_attention_f32 in its first form, one value per load, took 57 ms, 518 and 131.
 #include "matrix16.h"
 #include "prompt_attention.h"
 

@@ -15,7 +15,9 @@
 // scan_rows_kernel walks the rows one by one with the state in registers, fp32 throughout: the kernel of
 // fp32 and fp16 inputs and of every geometry that the matrix kernel does not take. A thread holds 4 p x
 // (N / 16) n of the state: per row it reads N / 8 + 4 values from LDS for N / 2 fused multiply-adds with
-// the state's decay, and four sums over 16 lanes give y.
+// the state's decay, and four sums over 16 lanes give y. Three VALU instructions per state value and row are its floor.
+// Three fp32 prompts up to 1001 rows (2438 in all) of 128 heads x 64 x 128: 548 us (203-213 for what the
+// segments add, 28 to carry, 352-374 for the segments, where those instructions are 195).
 #include "prompt_scan.h"
 
 namespace lq {

@@ -80,8 +80,11 @@ def prompt_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Ten
     Any strides; x, B and C of one dtype, the rest fp32, fp16 or bf16; N <= 256.
 
     The states behind the prompts go to `states`, of any float dtype (the cache's own tensor, and the
-    same as initial_states to go on in place), or to a new fp32 tensor; a prompt without rows hands its
-    initial state on.
+    same as initial_states to go on in place; they overlap in no other way), or to a new fp32 tensor; a
+    prompt without rows hands its initial state on.
+
+    What stands behind a row in its prompt never reaches it. An x of inf or NaN leaves every y and state
+    that it reaches not finite, inf or NaN (the sign of an infinity is not followed through the products).
     """
     _check_prompts("x", x, starts)
     _no_gradients(x, dt, A, B, C, D, z, dt_bias, initial_states)

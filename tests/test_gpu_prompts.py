@@ -397,6 +397,17 @@ def test_scan_large_and_small_steps(gpu):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_no_prompts_at_all(gpu, dtype):
+    """One start, no prompt: every row is of none."""
+    starts = torch.tensor([5], device=gpu)
+    t = scan_inputs(gpu, 3000, 8, 64, 128, 1, dtype)
+    y, st = prompts.prompt_scan(t["x"], t["dt"], t["A"], t["B"], t["C"], starts)
+    assert st.shape == (0, 8, 64, 128) and y.shape == t["x"].shape and not y.any()
+    q, k, v = attention_inputs(gpu, 3000, 4, 2, 64, dtype)
+    assert not prompts.prompt_attention(q, k, v, starts).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_scan_starts_out_of_order(gpu, dtype):
     """Starts that do not ascend give no defined values, and read and write nothing outside."""
     t = scan_inputs(gpu, 1500, 4, 64, 128, 1, dtype, seed=16)
