@@ -26,6 +26,7 @@ namespace {
 constexpr int TB = 16;       // rows per staged block
 constexpr int PB = 64;       // p of a workgroup (16 per wave)
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr double MAX_SCALE = 40;  // a scaled state's, in powers of two
 
 template <int NPL>
 struct alignas(16) RowTile {
@@ -33,8 +34,24 @@ struct alignas(16) RowTile {
   float y[TB][PB];
   float b[TB][16 * NPL];
   float c[TB][16 * NPL];
-  float dt[TB], decay[TB];
+  float dt[TB], decay[TB];  // scaled: dt_s 2^(e - c_s), 2^(c_s - e); else dt_s, A dt_s log2(e)
+  float keep, log_decay;    // 2^e, e
+  int scaled;
 };
+
+// v + the value CTRL's shift away within 16 lanes (0 from outside them).
+template <int CTRL>
+__device__ __forceinline__ double plus_shifted(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+  return v + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+__device__ __forceinline__ float exp2_of(double v) {
+  const double whole = __builtin_rint(v);
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f((float)(v - whole)), (int)whole);
+}
 
 // v's sum over 16 lanes; lane (bit 3, bit 2) of each 16 ends with that of v[2 bit3 + bit2].
 __device__ __forceinline__ float sums_of_four(const float (&v)[4], int lane) {
@@ -126,7 +143,8 @@ __global__ __launch_bounds__(64 * WAVES) void scan_rows_kernel(PromptScan p) {
       st[i][j] = v;
     }
   }
-  const float A = load_float(p.A.data, p.A.dtype, h * p.A.s[0]) * LOG2E;
+  const float A_h = load_float(p.A.data, p.A.dtype, h * p.A.s[0]), A = A_h * LOG2E;
+  const double A64 = (double)A_h * 1.4426950408889634;
   const float bias = p.bias.data == nullptr ? 0.f : load_float(p.bias.data, p.bias.dtype, h * p.bias.s[0]);
   const float D = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, h * p.D.s[0]);
   const int g = h / p.ratio;
@@ -187,15 +205,68 @@ __global__ __launch_bounds__(64 * WAVES) void scan_rows_kernel(PromptScan p) {
         tile.c[r][n] = c;
       }
     }
-    if (tid < rows) {
-      const float dt = scan_step(p, load_float(p.dt.data, p.dt.dtype, dt_at + (row + tid) * p.dt.s[1]), bias);
-      tile.dt[tid] = dt;
-      tile.decay[tid] = A * dt;
+    if (tid < 64) {
+      const bool in = tid < rows;
+      float dt = 0.f;
+      if (in) dt = scan_step(p, load_float(p.dt.data, p.dt.dtype, dt_at + (row + tid) * p.dt.s[1]), bias);
+      const float lg = in ? A * dt : 0.f;
+      double c = in ? A64 * dt : 0.0;
+      c = plus_shifted<0x111>(c);  // row_shr 1, 2, 4, 8
+      c = plus_shifted<0x112>(c);
+      c = plus_shifted<0x114>(c);
+      c = plus_shifted<0x118>(c);
+      const uint64_t u = __builtin_bit_cast(uint64_t, c);
+      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, TB - 1);
+      const uint32_t up = __builtin_amdgcn_readlane((uint32_t)(u >> 32), TB - 1);
+      const double e = __builtin_bit_cast(double, ((uint64_t)up << 32) | lo);
+      const bool scaled = __all(!in || lg <= 0.f) && e >= -MAX_SCALE;
+      if (in) {
+        tile.dt[tid] = scaled ? dt * exp2_of(e - c) : dt;
+        tile.decay[tid] = scaled ? exp2_of(c - e) : lg;
+      }
+      if (tid == 0) {
+        tile.scaled = scaled;
+        tile.keep = scaled ? exp2_of(e) : 1.f;
+        tile.log_decay = (float)e;
+      }
     }
     __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-      const float lg = tile.decay[r], a = __builtin_amdgcn_exp2f(lg), dt = tile.dt[r];
-      log_decay += lg;
+    log_decay += tile.log_decay;
+    if (tile.scaled) {
+      const float keep = tile.keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) st[i][j] *= keep;
+      }
+      for (int r = 0; r < rows; ++r) {
+        const float dt = tile.dt[r];
+        const float4 x4 = *(const float4*)&tile.x[r][p0];
+        const float dx[4] = {dt * x4.x, dt * x4.y, dt * x4.z, dt * x4.w};
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NPL; j += 4) {
+          const float4 b4 = *(const float4*)&tile.b[r][16 * j + 4 * nl];
+          float4 c4 = b4;
+          if (!ADDS) c4 = *(const float4*)&tile.c[r][16 * j + 4 * nl];
+          const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              st[i][j + k] = fmaf(dx[i], b[k], st[i][j + k]);
+              if (!ADDS) y[i] = fmaf(st[i][j + k], c[k], y[i]);
+            }
+          }
+        }
+        if (!ADDS) {
+          const float sum = sums_of_four(y, lane) * tile.decay[r];
+          if ((lane & 3) == 0) tile.y[r][p0 + ((lane >> 2) & 3)] = sum;
+        }
+      }
+    }
+    for (int r = tile.scaled ? rows : 0; r < rows; ++r) {
+      const float a = __builtin_amdgcn_exp2f(tile.decay[r]), dt = tile.dt[r];
       const float4 x4 = *(const float4*)&tile.x[r][p0];
       const float dx[4] = {dt * x4.x, dt * x4.y, dt * x4.z, dt * x4.w};
       float y[4] = {0.f, 0.f, 0.f, 0.f};
