@@ -103,7 +103,7 @@ __device__ __forceinline__ void store4(void* base, int dtype, int64_t at, float4
 // ADDS: find_segment's. SIZE: bytes of a value of x, B, C, z and out where four in a row are loaded at once,
 // a block of rows ahead, by WAVES waves; 0: any layout.
 template <int NPL, bool ADDS, int SIZE, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void scan_rows_kernel(PromptScan p) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void scan_rows_kernel(PromptScan p) {
   __shared__ RowTile<NPL> tile;
   const int h = blockIdx.x % p.H;
   const Segment seg = find_segment<ADDS>(p, blockIdx.x / p.H);
@@ -239,6 +239,7 @@ __global__ __launch_bounds__(64 * WAVES) void scan_rows_kernel(PromptScan p) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j) st[i][j] *= keep;
       }
+#pragma unroll 1
       for (int r = 0; r < rows; ++r) {
         const float dt = tile.dt[r];
         const float4 x4 = *(const float4*)&tile.x[r][p0];
@@ -265,6 +266,7 @@ __global__ __launch_bounds__(64 * WAVES) void scan_rows_kernel(PromptScan p) {
         }
       }
     }
+#pragma unroll 1
     for (int r = tile.scaled ? rows : 0; r < rows; ++r) {
       const float a = __builtin_amdgcn_exp2f(tile.decay[r]), dt = tile.dt[r];
       const float4 x4 = *(const float4*)&tile.x[r][p0];
@@ -421,8 +423,8 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
 // Rows kernel: at least 256, or 64 where the heads give few workgroups (8000 rows of 8 heads: 184 us with
 // 256, 77 with 64).
 int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) {
-  const int64_t want = (rows * heads + 4 * device_cus() - 1) / (4 * device_cus());
-  if (!matrix) return max((want + 63) / 64 * 64, heads >= 64 ? (int64_t)256 : (int64_t)64);
+  const int64_t many = (matrix ? 4 : 8) * device_cus(), want = (rows * heads + many - 1) / many;
+  if (!matrix) return max((want + 63) / 64 * 64, heads >= 64 ? (int64_t)192 : (int64_t)64);
   const int64_t seg = (prompts >= 8 ? 2 * want : want) + 63;
   return max(seg / 64 * 64, rows <= 1024 * prompts ? (int64_t)1024 : (int64_t)256);
 }
