@@ -34,9 +34,10 @@ struct alignas(16) RowTile {
   float y[TB][PB];
   float b[TB][16 * NPL];
   float c[TB][16 * NPL];
-  float dt[TB], decay[TB];  // scaled: dt_s 2^(e - c_s), 2^(c_s - e); else dt_s, A dt_s log2(e)
-  float keep, log_decay;    // 2^e, e
-  int scaled;
+  // of 64 rows, four blocks
+  float dt[64], decay[64];                // scaled: dt_s 2^(e - c_s), 2^(c_s - e); else dt_s, A dt_s log2(e)
+  float keep[64 / TB], log_decay[64 / TB];  // 2^e, e
+  int scaled[64 / TB];
 };
 
 // v + the value CTRL's shift away within 16 lanes (0 from outside them).
@@ -205,8 +206,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
         tile.c[r][n] = c;
       }
     }
-    if (tid < 64) {
-      const bool in = tid < rows;
+    const int block = (t - from) / TB % (64 / TB);
+    if (block == 0 && tid < 64) {
+      const bool in = t + tid < to;
       float dt = 0.f;
       if (in) dt = scan_step(p, load_float(p.dt.data, p.dt.dtype, dt_at + (row + tid) * p.dt.s[1]), bias);
       const float lg = in ? A * dt : 0.f;
@@ -215,25 +217,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
       c = plus_shifted<0x112>(c);
       c = plus_shifted<0x114>(c);
       c = plus_shifted<0x118>(c);
-      const uint64_t u = __builtin_bit_cast(uint64_t, c);
-      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, TB - 1);
-      const uint32_t up = __builtin_amdgcn_readlane((uint32_t)(u >> 32), TB - 1);
-      const double e = __builtin_bit_cast(double, ((uint64_t)up << 32) | lo);
-      const bool scaled = __all(!in || lg <= 0.f) && e >= -MAX_SCALE;
-      if (in) {
-        tile.dt[tid] = scaled ? dt * exp2_of(e - c) : dt;
-        tile.decay[tid] = scaled ? exp2_of(c - e) : lg;
-      }
-      if (tid == 0) {
-        tile.scaled = scaled;
-        tile.keep = scaled ? exp2_of(e) : 1.f;
-        tile.log_decay = (float)e;
+      const double e = __shfl(c, lane | (TB - 1), 64);
+      const uint64_t falls = __ballot(lg <= 0.f) >> (lane & ~(TB - 1));
+      const bool scaled = (falls & 0xffff) == 0xffff && e >= -MAX_SCALE;
+      tile.dt[tid] = scaled ? dt * exp2_of(e - c) : dt;
+      tile.decay[tid] = scaled ? exp2_of(c - e) : lg;
+      if ((tid & (TB - 1)) == 0) {
+        tile.scaled[tid / TB] = scaled;
+        tile.keep[tid / TB] = scaled ? exp2_of(e) : 1.f;
+        tile.log_decay[tid / TB] = (float)e;
       }
     }
     __syncthreads();
-    log_decay += tile.log_decay;
-    if (tile.scaled) {
-      const float keep = tile.keep;
+    log_decay += tile.log_decay[block];
+    const bool scaled = tile.scaled[block];
+    const float *dts = &tile.dt[block * TB], *decays = &tile.decay[block * TB];
+    if (scaled) {
+      const float keep = tile.keep[block];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
       }
 #pragma unroll 1
       for (int r = 0; r < rows; ++r) {
-        const float dt = tile.dt[r];
+        const float dt = dts[r];
         const float4 x4 = *(const float4*)&tile.x[r][p0];
         const float dx[4] = {dt * x4.x, dt * x4.y, dt * x4.z, dt * x4.w};
         float y[4] = {0.f, 0.f, 0.f, 0.f};
@@ -261,14 +261,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
           }
         }
         if (!ADDS) {
-          const float sum = sums_of_four(y, lane) * tile.decay[r];
+          const float sum = sums_of_four(y, lane) * decays[r];
           if ((lane & 3) == 0) tile.y[r][p0 + ((lane >> 2) & 3)] = sum;
         }
       }
     }
 #pragma unroll 1
-    for (int r = tile.scaled ? rows : 0; r < rows; ++r) {
-      const float a = __builtin_amdgcn_exp2f(tile.decay[r]), dt = tile.dt[r];
+    for (int r = scaled ? rows : 0; r < rows; ++r) {
+      const float a = __builtin_amdgcn_exp2f(decays[r]), dt = dts[r];
       const float4 x4 = *(const float4*)&tile.x[r][p0];
       const float dx[4] = {dt * x4.x, dt * x4.y, dt * x4.z, dt * x4.w};
       float y[4] = {0.f, 0.f, 0.f, 0.f};
