@@ -18,6 +18,7 @@
 // the state's decay, and four sums over 16 lanes give y. Three VALU instructions per state value and row are its floor.
 // Three fp32 prompts up to 1001 rows (2438 in all) of 128 heads x 64 x 128: 548 us (203-213 for what the
 // segments add, 28 to carry, 352-374 for the segments, where those instructions are 195).
+#include "matrix16.h"
 #include "prompt_scan.h"
 
 namespace lq {
@@ -76,6 +77,12 @@ template <int SIZE>
 __device__ __forceinline__ uint4 load_raw4(const void* base, int64_t at) {
   if (SIZE == 4) return *(const uint4*)((const char*)base + at * 4);
   const uint2 w = *(const uint2*)((const char*)base + at * 2);
+  return make_uint4(w.x, w.y, 0, 0);
+}
+template <int SIZE>
+__device__ __forceinline__ uint4 buffer_load4(__amdgpu_buffer_rsrc_t rows, uint32_t offset) {
+  if (SIZE == 4) return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
+  const uint2 w = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0));
   return make_uint4(w.x, w.y, 0, 0);
 }
 template <int SIZE>
@@ -154,24 +161,29 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
   const int64_t b_at = lead * p.B.s[0] + g * p.B.s[2], c_at = lead * p.C.s[0] + g * p.C.s[2];
   const int64_t dt_at = lead * p.dt.s[0] + h * p.dt.s[2];
   float log_decay = 0.f;
-  // 16-byte chunks of a block: x, then B and C
-  constexpr int XC = 4 * WAVES, CHUNKS = TB * (XC + 8 * NPL), LOADS = CHUNKS / (64 * WAVES);
-  static_assert(SIZE == 0 || CHUNKS % (64 * WAVES) == 0, "every thread loads as many");
-  uint4 raw[SIZE == 0 ? 1 : LOADS];
+  // A block of x, B and C in chunks of four values: a thread has one chunk of x, and of B and of C those in
+  // its column (BR rows apart). Rows past the segment are past the descriptors and read as zero, columns
+  // past the row's values are sent there.
+  constexpr int XC = 4 * WAVES, BC = 4 * NPL, BR = 64 * WAVES / BC, BL = SIZE == 0 ? 0 : TB / BR;
+  static_assert(TB * XC == 64 * WAVES && (SIZE == 0 || BR * BL == TB), "every thread loads as many");
+  constexpr uint32_t OUTSIDE = 0x7fffff00;
+  const int xr = tid / XC, xc = 4 * (tid % XC), br = tid / BC, bc = 4 * (tid % BC);
+  const int xs = (int)p.x.s[1] * SIZE, bs = (int)p.B.s[1] * SIZE, cs = (int)p.C.s[1] * SIZE;
+  const uint32_t x_off = xc < width ? xr * xs + xc * SIZE : OUTSIDE;
+  const uint32_t b_off = bc < p.N ? br * bs + bc * SIZE : OUTSIDE, c_off = bc < p.N ? br * cs + bc * SIZE : OUTSIDE;
+  uint4 raw_x, raw_b[BL + 1], raw_c[BL + 1];
   auto load_block = [&](int t) {
+    if (SIZE == 0) return;
+    const int last = min(TB, to - t) - 1;
+    const int64_t row = row0 + t;
+    const auto xd = buffer_of((const char*)p.x.data + (x_at + row * p.x.s[1]) * SIZE, last < 0 ? 0 : last * xs + width * SIZE);
+    const auto bd = buffer_of((const char*)p.B.data + (b_at + row * p.B.s[1]) * SIZE, last < 0 ? 0 : last * bs + p.N * SIZE);
+    const auto cd = buffer_of((const char*)p.C.data + (c_at + row * p.C.s[1]) * SIZE, last < 0 ? 0 : last * cs + p.N * SIZE);
+    raw_x = buffer_load4<SIZE>(xd, x_off);
 #pragma unroll
-    for (int j = 0; j < (SIZE == 0 ? 0 : LOADS); ++j) {
-      const int i = j * 64 * WAVES + tid;
-      const bool is_x = i < TB * XC;
-      const int k = is_x ? i : i - TB * XC;
-      const int r = is_x ? k / XC : k / (8 * NPL), c = 4 * (is_x ? k % XC : k % (4 * NPL));
-      const bool is_b = is_x || k % (8 * NPL) < 4 * NPL;
-      raw[j] = make_uint4(0, 0, 0, 0);
-      if (t + r >= to || c >= (is_x ? width : p.N)) continue;
-      const int64_t row = row0 + t + r;
-      raw[j] = is_x ? load_raw4<SIZE>(p.x.data, x_at + row * p.x.s[1] + c)
-                    : load_raw4<SIZE>(is_b ? p.B.data : p.C.data,
-                                      is_b ? b_at + row * p.B.s[1] + c : c_at + row * p.C.s[1] + c);
+    for (int j = 0; j < BL; ++j) {
+      raw_b[j] = buffer_load4<SIZE>(bd, b_off + j * BR * bs);
+      if (!ADDS) raw_c[j] = buffer_load4<SIZE>(cd, c_off + j * BR * cs);
     }
   };
   load_block(from);
@@ -180,14 +192,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
     const int64_t row = row0 + t;
     __syncthreads();
     if (SIZE != 0) {
+      *(float4*)&tile.x[xr][xc] = values_of<SIZE == 0 ? 4 : SIZE>(raw_x, p.x.dtype);
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        const int i = j * 64 * WAVES + tid;
-        const bool is_x = i < TB * XC;
-        const int k = is_x ? i : i - TB * XC;
-        const int r = is_x ? k / XC : k / (8 * NPL), c = 4 * (is_x ? k % XC : k % (4 * NPL));
-        float* to_row = is_x ? tile.x[r] : k % (8 * NPL) < 4 * NPL ? tile.b[r] : tile.c[r];
-        *(float4*)&to_row[c] = values_of<SIZE == 0 ? 4 : SIZE>(raw[j], p.x.dtype);
+      for (int j = 0; j < BL; ++j) {
+        *(float4*)&tile.b[br + j * BR][bc] = values_of<SIZE == 0 ? 4 : SIZE>(raw_b[j], p.x.dtype);
+        if (!ADDS) *(float4*)&tile.c[br + j * BR][bc] = values_of<SIZE == 0 ? 4 : SIZE>(raw_c[j], p.x.dtype);
       }
       load_block(t + TB);
     } else {
@@ -275,14 +284,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NPL <= 8 ? 4 : 1) void sc
 #pragma unroll
       for (int j = 0; j < NPL; j += 4) {
         const float4 b4 = *(const float4*)&tile.b[r][16 * j + 4 * nl];
-        const float4 c4 = *(const float4*)&tile.c[r][16 * j + 4 * nl];
+        float4 c4 = b4;
+        if (!ADDS) c4 = *(const float4*)&tile.c[r][16 * j + 4 * nl];
         const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             st[i][j + e] = fmaf(st[i][j + e], a, dx[i] * b[e]);
-            y[i] = fmaf(st[i][j + e], c[e], y[i]);
+            if (!ADDS) y[i] = fmaf(st[i][j + e], c[e], y[i]);
           }
         }
       }
@@ -466,7 +476,9 @@ bool in_fours(const lq_tensor* t, int dtype) {
   for (int i = 0; i < nd - 1; ++i) {
     if (t->shape[i] > 1 && t->stride[i] % 4 != 0) return false;
   }
-  return true;
+  // a block's rows within 31 bits of bytes (a single row's too: the rows past it have to be past the end)
+  const int64_t s = t->stride[nd - 3];
+  return s >= t->shape[nd - 1] && s <= (1 << 22);
 }
 
 }  // namespace
