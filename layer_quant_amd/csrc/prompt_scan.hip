@@ -14,10 +14,21 @@
 //
 // scan_rows_kernel walks the rows one by one with the state in registers, fp32 throughout: the kernel of
 // fp32 and fp16 inputs and of every geometry that the matrix kernel does not take. A thread holds 4 p x
-// (N / 16) n of the state: per row it reads N / 8 + 4 values from LDS for N / 2 fused multiply-adds with
-// the state's decay, and four sums over 16 lanes give y. Three VALU instructions per state value and row are its floor.
-// Three fp32 prompts up to 1001 rows (2438 in all) of 128 heads x 64 x 128: 548 us (203-213 for what the
-// segments add, 28 to carry, 352-374 for the segments, where those instructions are 195).
+// (N / 16) n of the state: per row it reads N / 8 + 4 values from LDS, and four sums over 16 lanes give y.
+// Blocks of 16 rows are staged in LDS, loaded a block ahead. Within a block, with c the running sum of A dt
+// log2(e) and e its end, the state is held as 2^(e - c) S, so that
+//   2^(e - c_t) S_t = 2^(e - c_t-1) S_t-1 + 2^(e - c_t) dt_t x_t B_t^T,   y_t = 2^(c_t - e) (2^(e - c_t) S_t) C_t
+// takes two multiply-adds per value of the state instead of three, and one where y is not wanted. Only values
+// that are smaller than they would be stand in registers, by 2^-40 at most: blocks that decay further, or
+// grow, or have a NaN, take the steps as they are. c is summed in 64 bits, for the reason that
+// prompt_scan_mfma.hip gives.
+// Three fp32 prompts up to 1001 rows (2438 in all) of 128 heads x 64 x 128: 352 us (107-113 for what the
+// segments add, 33 to carry, 248-268 for the segments, where 85 VALU instructions per row and wave, 64 of them
+// these multiply-adds, are 173 at 2.4 GHz; the rest is the blocks' staging, barriers and silu, and latency at
+// four waves per SIMD). With a state not scaled, loads at addresses of their own and less of the GPU's
+// workgroups it was 548. Without effect or worse: z loaded ahead (350), two rows unrolled (358), five
+// workgroups per CU (350, and 620 with spills), all loads of a segment's first state at once (401 against
+// 393, with spills).
 #include "matrix16.h"
 #include "prompt_scan.h"
 
@@ -423,15 +434,15 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
   }
 }
 
-// Rows of a segment, a multiple of 64: as many as give about four workgroups per CU (of the rows kernel; two
-// of the matrix kernel). Segments cost a part of the work again and two launches.
-// Matrix kernel: at least 256 rows, and prompts of up to 1024 rows, as far as their mean says, stay whole (4
-// prompts of 512 rows and 128 heads: 71 us in two segments each, 41 whole; one of 2000 rows: 107 us in two
-// of 1024, 73 in eight of 256). Eight prompts or more fill the GPU by themselves unless their lengths differ
-// much: twice as many rows then (24 prompts up to 700 rows: 134 -> 117 us; with the rows kernel, 16 up to 900
-// would go from 574 to 791).
-// Rows kernel: at least 256, or 64 where the heads give few workgroups (8000 rows of 8 heads: 184 us with
-// 256, 77 with 64).
+// Rows of a segment, a multiple of 64. Segments cost a part of the work again and two launches.
+// Matrix kernel: as many as give two workgroups per CU (a workgroup has two heads), but at least 256 rows, and
+// prompts of up to 1024 rows, as far as their mean says, stay whole (4 prompts of 512 rows and 128 heads: 71 us
+// in two segments each, 41 whole; one of 2000 rows: 107 us in two of 1024, 73 in eight of 256). Eight prompts
+// or more fill the GPU by themselves unless their lengths differ much: twice as many rows then (24 prompts up
+// to 700 rows: 134 -> 117 us).
+// Rows kernel: as many as give eight workgroups per CU, of which it has four at a time (half as many
+// workgroups: three fp32 prompts up to 1001 rows 429 us against 394, one of 4000 fp16 rows 757 against 652);
+// at least 192 rows, or 64 where the heads give few workgroups (8000 rows of 8 heads: 145 us with 192, 75 with 64).
 int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) {
   const int64_t many = (matrix ? 4 : 8) * device_cus(), want = (rows * heads + many - 1) / many;
   if (!matrix) return max((want + 63) / 64 * 64, heads >= 64 ? (int64_t)192 : (int64_t)64);

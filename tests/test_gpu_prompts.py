@@ -407,6 +407,23 @@ def test_no_prompts_at_all(gpu, dtype):
     assert not prompts.prompt_attention(q, k, v, starts).any()
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("size", [1e-3, 1.0, 30.0])
+def test_scan_decays_of_a_block(gpu, dtype, size):
+    """Sixteen rows that decay by little, by almost 2^-40, by little more, by 2^-400, that grow, and whose steps
+    are negative: the state is scaled within some of them and not in others."""
+    h = 6
+    t = scan_inputs(gpu, 150, h, 64, 128, 1, dtype, seed=11, dt_dtype=F32)
+    t["x"] *= size
+    t["dt"] = torch.ones(150, h, device=gpu) / 8
+    per_row = torch.tensor([0.01, 39.9 / 16, 40.1 / 16, 25.0, -0.02, 2.0], device=gpu)
+    t["A"] = -per_row * 8 * math.log(2)
+    t["dt"][20:22, 5] *= -1
+    t["dt"][60:, 1] *= 1.01
+    check_scan(gpu, t, starts_of([150], gpu), f"{dtype} {size}", use=("D",), softplus=False,
+               limit=(-math.inf, math.inf))
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_scan_starts_out_of_order(gpu, dtype):
     """Starts that do not ascend give no defined values, and read and write nothing outside."""
