@@ -445,7 +445,10 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
 // at least 192 rows, or 64 where the heads give few workgroups (8000 rows of 8 heads: 145 us with 192, 75 with 64).
 int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) {
   const int64_t many = (matrix ? 4 : 8) * device_cus(), want = (rows * heads + many - 1) / many;
-  if (!matrix) return max((want + 63) / 64 * 64, heads >= 64 ? (int64_t)192 : (int64_t)64);
+  if (!matrix) {
+    const int64_t least = heads < 64 ? 64 : rows <= 256 * prompts ? 256 : 192;
+    return max((want + 63) / 64 * 64, least);
+  }
   const int64_t seg = (prompts >= 8 ? 2 * want : want) + 63;
   return max(seg / 64 * 64, rows <= 1024 * prompts ? (int64_t)1024 : (int64_t)256);
 }
