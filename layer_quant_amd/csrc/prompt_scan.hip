@@ -442,11 +442,17 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
 // to 700 rows: 134 -> 117 us).
 // Rows kernel: as many as give eight workgroups per CU, of which it has four at a time (half as many
 // workgroups: three fp32 prompts up to 1001 rows 429 us against 394, one of 4000 fp16 rows 757 against 652);
-// at least 192 rows, or 64 where the heads give few workgroups (8000 rows of 8 heads: 145 us with 192, 75 with 64).
+// at least 192 rows, or 256 where prompts have no more, as their mean says (4 of 200 rows, 64 heads: 137 us in two
+// segments each, 84 whole, 89 in four), or 64 where the heads give few workgroups (8000 rows of 8 heads: 145 us
+// with 192, 75 with 64) and for few prompts whose segments of 64 rows the GPU takes at once, or nearly, and
+// that either leave CUs without work or have more than 256 rows (128 heads: one of 200 fp32 rows 83 -> 61, of
+// 500 fp16 rows 154 -> 102, two of 300 fp32 rows 132 -> 109; one of 128 rows stays whole, 56 against 59).
 int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) {
   const int64_t many = (matrix ? 4 : 8) * device_cus(), want = (rows * heads + many - 1) / many;
   if (!matrix) {
-    const int64_t least = heads < 64 ? 64 : rows <= 256 * prompts ? 256 : 192;
+    const bool few = rows > 128 * prompts && rows * heads <= (int64_t)64 * 5 * device_cus() &&
+                     (prompts * heads < device_cus() || rows > 256 * prompts);
+    const int64_t least = heads < 64 || few ? 64 : rows <= 256 * prompts ? 256 : 192;
     return max((want + 63) / 64 * 64, least);
   }
   const int64_t seg = (prompts >= 8 ? 2 * want : want) + 63;

@@ -424,6 +424,15 @@ def test_scan_decays_of_a_block(gpu, dtype, size):
                limit=(-math.inf, math.inf))
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("lengths", [[200], [258], [0, 150, 129], [300, 1, 290], [256], [700]], ids=str)
+def test_scan_few_short_prompts(gpu, dtype, lengths):
+    """Many heads and few rows: whole prompts, or segments of 64 rows."""
+    t = scan_inputs(gpu, sum(lengths), 128, 4, 16, 2, dtype, seed=12)
+    first = torch.randn(len(lengths), 128, 4, 16, device=gpu)
+    check_scan(gpu, t, starts_of(lengths, gpu), f"{lengths}", use=("D", "dt_bias", "z"), initial=first)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_scan_starts_out_of_order(gpu, dtype):
     """Starts that do not ascend give no defined values, and read and write nothing outside."""
