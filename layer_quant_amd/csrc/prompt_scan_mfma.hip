@@ -19,7 +19,7 @@
 //   phase 1  S C^T (16 products) with C's operands shared by the mixing scores B C^T, of which three waves
 //            make one 32 x 32 block each (the fourth lies above the diagonal) for both heads and leave M in
 //            LDS as bf16
-//   phase 2  Y += M x + D x (6 and 4 products), stores, S' (16 or 32 products)
+//   phase 2  Y += M x + D x (6 and 4 products), stores, S' (32 products)
 // B lies in two LDS buffers; x goes to registers at once, and C and the decays are read in phase 1 alone, so
 // that one buffer each does, refilled from then on: 79 KB per workgroup, two of them per CU.
 //
@@ -32,8 +32,9 @@
 // in other orders (no difference); the last block's heads shared out to two waves (297).
 //
 // Roundings: M, D and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result); w x, which a
-// state keeps, to the sum of two bf16 values (2^-16) where the states leave in fp32 and to one (2^-8, less
-// than they lose then) where they leave in 16 bits. Everything else is fp32.
+// state keeps, to the sum of two bf16 values (2^-16), at 16 products more per wave and chunk. With one value a
+// state that leaves in bf16 was 1.4 to 1.5 times as far off as its own rounding makes it (287 us for 16384 rows).
+// Everything else is fp32.
 //
 // Rows behind a row in its chunk have M = 0 there, which an x of inf or NaN would turn into NaN. Such a value
 // stays in the state, so that it is enough to look at the state behind a segment: one that is not finite has
@@ -159,9 +160,8 @@ __device__ __forceinline__ void store8(char* at, int dtype, const float (&v)[8])
 
 __device__ __forceinline__ int size_of(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
 
-// A segment of two heads; whether it has to run again, with CAREFUL. ADDS: find_segment's. LO: w x as the
-// sum of two bf16 values.
-template <bool ADDS, bool LO, bool CAREFUL>
+// A segment of two heads; whether it has to run again, with CAREFUL. ADDS: find_segment's.
+template <bool ADDS, bool CAREFUL>
 __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& seg, int pair, int tid,
                                             ChunkLds& lds) {
   const Span& sp = seg.span;
@@ -453,15 +453,13 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
         const float b = w[2 * e + 1] * __uint_as_float(xa[i][e] & 0xffff0000u);
         const uint32_t ab = pack2<true>(a, b);
         top[e] = ab;
-        if (LO) lower[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
+        lower[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], top, st[b]);
-      if (LO) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], lower, st[b]);
-      }
+      for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], lower, st[b]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < 4; ++b) bc[b] = next[b];
@@ -496,7 +494,7 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
   return false;
 }
 
-template <bool ADDS, bool LO>
+template <bool ADDS>
 __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
   __shared__ ChunkLds lds;
   // the workgroups of a group's heads on one XCD (blocks go round the eight), as they read the same B and C
@@ -515,14 +513,14 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
     }
     return;
   }
-  if (!run_segment<ADDS, LO, false>(p, seg, pair, threadIdx.x, lds)) return;
+  if (!run_segment<ADDS, false>(p, seg, pair, threadIdx.x, lds)) return;
   // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
   // for the second one, through the loop.
   Segment again = seg;
   int tid = threadIdx.x, same = pair;
   asm volatile("" : "+s"(again.span.index), "+s"(again.span.begin), "+s"(again.span.part), "+s"(again.slot));
   asm volatile("" : "+v"(tid), "+s"(same));
-  run_segment<ADDS, LO, true>(p, again, same, tid, lds);
+  run_segment<ADDS, true>(p, again, same, tid, lds);
 }
 
 // Values in a row, every row 16-byte aligned.
@@ -572,11 +570,8 @@ void launch_prompt_scan_steps(const PromptScan& p, int64_t chunks, hipStream_t s
 
 void launch_prompt_scan_mfma(const PromptScan& p, bool adds, int64_t parts, hipStream_t st) {
   const dim3 grid((unsigned)(parts * (p.H / HEADS))), block(256);
-  const bool lo = p.states.data != nullptr && p.states.dtype == LQ_F32;
-  if (adds && lo) hipLaunchKernelGGL((scan_chunks_kernel<true, true>), grid, block, 0, st, p);
-  else if (adds) hipLaunchKernelGGL((scan_chunks_kernel<true, false>), grid, block, 0, st, p);
-  else if (lo) hipLaunchKernelGGL((scan_chunks_kernel<false, true>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((scan_chunks_kernel<false, false>), grid, block, 0, st, p);
+  if (adds) hipLaunchKernelGGL(scan_chunks_kernel<true>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(scan_chunks_kernel<false>, grid, block, 0, st, p);
 }
 
 }  // namespace lq

@@ -250,15 +250,14 @@ def scan_inputs(gpu, rows, h, p, n, g, dtype, seed=0, dt_dtype=None):
 
 def scan_bounds(y, s, wy, ws, dtype, state_dtype, rows):
     """bf16 products: the mixing weights and the state in front of a chunk are rounded to bf16 (half a
-    step, 2^-8 of the terms' sum); the state's own terms to two bf16 numbers (2^-16) where it leaves in
-    fp32, and to one where it leaves in 16 bits (2^-8, in y as well: 2^-7 there). fp32 sums, decays
+    step, 2^-8 of the terms' sum); the state's own terms to two bf16 numbers (2^-16). fp32 sums, decays
     and steps: less than 2^-21 of the terms' sum per 64 rows, and 2^-18 for logarithms and exponentials
     of decays (a decay exp(-u) is off by u 2^-22 of itself at most, u exp(-u) < 1 where it counts). A result below the type's
     smallest normal number is rounded to a multiple of tiny * eps."""
     half = torch.finfo(dtype).eps / 2
     fp32 = 2.0 ** -18 + (rows / 64 + 1) * 2.0 ** -21
     put = 0.0 if state_dtype == F32 else torch.finfo(state_dtype).eps / 2
-    own = fp32 if dtype != BF else (2.0 ** -16 if state_dtype == F32 else 2.0 ** -8) + fp32
+    own = fp32 if dtype != BF else 2.0 ** -16 + fp32
     mix = fp32 if dtype != BF else 2.0 ** -8 + own
     step = lambda t: torch.finfo(t).tiny * torch.finfo(t).eps  # noqa: E731
     return (half * y.abs() + mix * wy + step(dtype) / 2 + 1e-30,
