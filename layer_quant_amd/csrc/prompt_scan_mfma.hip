@@ -19,22 +19,24 @@
 //   phase 1  S C^T (16 products) with C's operands shared by the mixing scores B C^T, of which three waves
 //            make one 32 x 32 block each (the fourth lies above the diagonal) for both heads and leave M in
 //            LDS as bf16
-//   phase 2  Y += M x + D x (6 and 4 products), stores, S' (32 products)
+//   phase 2  Y += M x + D x (6 and 4 products), stores, S' (32 or 48 products)
 // B lies in two LDS buffers; x goes to registers at once, and C and the decays are read in phase 1 alone, so
 // that one buffer each does, refilled from then on: 79 KB per workgroup, two of them per CU.
 //
-// What it measured (MI355X, 128 heads, 8 groups, us): one prompt of 16384 rows 287 (steps 16, what the segments
-// add 81-87, carry 14, the segments 175-217), 24 prompts up to 700 rows 117 (8 + 4 + 5 + 103), one of 200 rows
-// 23.6 (5 + 19). A chunk takes a workgroup 3.2 us alone on its CU and 5 beside another one. Per wave and chunk 50
+// What it measured (MI355X, 128 heads, 8 groups, us): one prompt of 16384 rows 312 (steps 16, what the segments
+// add 92-114, carry 13, the segments 189-247), 24 prompts up to 700 rows with fp32 states 123 (8 + 4 + 5 + 107),
+// one of 200 rows 25.0 (5 + 20). With one value of w x a chunk took a workgroup 3.2 us alone on its CU and 5 beside
+// another one: per wave 50
 // matrix instructions (32 cycles) and 540 VALU ones (4), which add up, are two thirds of that; the rest is the
 // latency of LDS and of three barriers. Tried: one workgroup of eight waves and four heads with M in registers
 // and a single barrier (313 us: 66 and 681 instructions); loads further ahead into L2 (no gain); heads to XCDs
 // in other orders (no difference); the last block's heads shared out to two waves (297).
 //
-// Roundings: M, D and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result); w x, which a
-// state keeps, to the sum of two bf16 values (2^-16), at 16 products more per wave and chunk. With one value a
-// state that leaves in bf16 was 1.4 to 1.5 times as far off as its own rounding makes it (287 us for 16384 rows).
-// Everything else is fp32.
+// Roundings: M, D and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result). w x, which a
+// state keeps, to the sum of two bf16 values (2^-16) where the state leaves in 16 bits, and of three (its 24
+// bits) where it leaves in fp32: 700 rows' fp32 states are off by less than 5e-7 with three, 2e-6 with two (24
+// prompts 123 us, 117), and bf16 ones by 0.0017, their own rounding, with two, 0.0024 with one (16384 rows 312
+// us, 285). Everything else is fp32.
 //
 // Rows behind a row in its chunk have M = 0 there, which an x of inf or NaN would turn into NaN. Such a value
 // stays in the state, so that it is enough to look at the state behind a segment: one that is not finite has
@@ -160,8 +162,9 @@ __device__ __forceinline__ void store8(char* at, int dtype, const float (&v)[8])
 
 __device__ __forceinline__ int size_of(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
 
-// A segment of two heads; whether it has to run again, with CAREFUL. ADDS: find_segment's.
-template <bool ADDS, bool CAREFUL>
+// A segment of two heads; whether it has to run again, with CAREFUL. ADDS: find_segment's. TERMS: bf16
+// values that w x is the sum of.
+template <bool ADDS, int TERMS, bool CAREFUL>
 __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& seg, int pair, int tid,
                                             ChunkLds& lds) {
   const Span& sp = seg.span;
@@ -446,20 +449,27 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
         }
       }
       const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      words4_t top, lower;
+      words4_t top, lower, lowest;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float a = w[2 * e] * __uint_as_float(xa[i][e] << 16);
         const float b = w[2 * e + 1] * __uint_as_float(xa[i][e] & 0xffff0000u);
         const uint32_t ab = pack2<true>(a, b);
         top[e] = ab;
-        lower[e] = pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
+const float a1 = a - __uint_as_float(ab << 16), b1 = b - __uint_as_float(ab & 0xffff0000u);
+        const uint32_t ab1 = pack2<true>(a1, b1);
+        lower[e] = ab1;
+        if (TERMS == 3) lowest[e] = pack2<true>(a1 - __uint_as_float(ab1 << 16), b1 - __uint_as_float(ab1 & 0xffff0000u));
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], top, st[b]);
 #pragma unroll
       for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], lower, st[b]);
+      if (TERMS == 3) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) st[b] = mfma<true>(bc[b], lowest, st[b]);
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < 4; ++b) bc[b] = next[b];
@@ -494,7 +504,7 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
   return false;
 }
 
-template <bool ADDS>
+template <bool ADDS, int TERMS>
 __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
   __shared__ ChunkLds lds;
   // the workgroups of a group's heads on one XCD (blocks go round the eight), as they read the same B and C
@@ -513,14 +523,14 @@ __global__ __launch_bounds__(256, 2) void scan_chunks_kernel(PromptScan p) {
     }
     return;
   }
-  if (!run_segment<ADDS, false>(p, seg, pair, threadIdx.x, lds)) return;
+  if (!run_segment<ADDS, TERMS, false>(p, seg, pair, threadIdx.x, lds)) return;
   // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
   // for the second one, through the loop.
   Segment again = seg;
   int tid = threadIdx.x, same = pair;
   asm volatile("" : "+s"(again.span.index), "+s"(again.span.begin), "+s"(again.span.part), "+s"(again.slot));
   asm volatile("" : "+v"(tid), "+s"(same));
-  run_segment<ADDS, true>(p, again, same, tid, lds);
+  run_segment<ADDS, TERMS, true>(p, again, same, tid, lds);
 }
 
 // Values in a row, every row 16-byte aligned.
@@ -570,8 +580,11 @@ void launch_prompt_scan_steps(const PromptScan& p, int64_t chunks, hipStream_t s
 
 void launch_prompt_scan_mfma(const PromptScan& p, bool adds, int64_t parts, hipStream_t st) {
   const dim3 grid((unsigned)(parts * (p.H / HEADS))), block(256);
-  if (adds) hipLaunchKernelGGL(scan_chunks_kernel<true>, grid, block, 0, st, p);
-  else hipLaunchKernelGGL(scan_chunks_kernel<false>, grid, block, 0, st, p);
+  const bool three = p.states.data != nullptr && p.states.dtype == LQ_F32;
+  if (adds && three) hipLaunchKernelGGL((scan_chunks_kernel<true, 3>), grid, block, 0, st, p);
+  else if (adds) hipLaunchKernelGGL((scan_chunks_kernel<true, 2>), grid, block, 0, st, p);
+  else if (three) hipLaunchKernelGGL((scan_chunks_kernel<false, 3>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((scan_chunks_kernel<false, 2>), grid, block, 0, st, p);
 }
 
 }  // namespace lq

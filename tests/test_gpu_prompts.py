@@ -250,7 +250,8 @@ def scan_inputs(gpu, rows, h, p, n, g, dtype, seed=0, dt_dtype=None):
 
 def scan_bounds(y, s, wy, ws, dtype, state_dtype, rows):
     """bf16 products: the mixing weights and the state in front of a chunk are rounded to bf16 (half a
-    step, 2^-8 of the terms' sum); the state's own terms to two bf16 numbers (2^-16). fp32 sums, decays
+    step, 2^-8 of the terms' sum); the state's own terms to two bf16 numbers (2^-16) or
+    three. fp32 sums, decays
     and steps: less than 2^-21 of the terms' sum per 64 rows, and 2^-18 for logarithms and exponentials
     of decays (a decay exp(-u) is off by u 2^-22 of itself at most, u exp(-u) < 1 where it counts). A result below the type's
     smallest normal number is rounded to a multiple of tiny * eps."""
