@@ -24,7 +24,7 @@
 // that one buffer each does, refilled from then on: 79 KB per workgroup, two of them per CU.
 //
 // What it measured (MI355X, 128 heads, 8 groups, us): one prompt of 16384 rows 312 (steps 16, what the segments
-// add 92-114, carry 13, the segments 189-247), 24 prompts up to 700 rows with fp32 states 123 (8 + 4 + 5 + 107),
+// add 92-114, carry 13, the segments 189-247), 24 prompts up to 700 rows with fp32 states 123 (8 + 4 + 5 + 110-113),
 // one of 200 rows 25.0 (5 + 20). With one value of w x a chunk took a workgroup 3.2 us alone on its CU and 5 beside
 // another one: per wave 50
 // matrix instructions (32 cycles) and 540 VALU ones (4), which add up, are two thirds of that; the rest is the
