@@ -631,7 +631,7 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   const lq_tensor* fours[5] = {x, B, C, z, out};
   for (const lq_tensor* t : fours) size = in_fours(t, x->dtype) && N <= 128 ? size : 0;
   const unsigned blocks = (unsigned)((H * P * N + 255) / 256);
-  if (mfma && total > 0) {
+  if (mfma && chunks > 0) {  // (none where no prompt has a row)
     launch_prompt_scan_steps(p, chunks, st);
     if ((rc = check_launch("lq_prompt_scan (steps)")) != LQ_OK) return rc;
   }
