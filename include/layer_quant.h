@@ -380,7 +380,8 @@ int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, int count,
  *   a batch: starts NULL, q, out [B, L, Hq, D], k, v [B, L, Hkv, D], every batch row a prompt
  *   q, k, v and out of one dtype (f32, f16 or bf16), any strides; D <= 256. out may be q, and overlaps
  *   neither k nor v nor itself.
- * Rows behind a query's own never reach its result, whatever they hold.
+ * Rows behind a query's own never reach its result, whatever they hold. A value of inf that a row sees makes
+ * its result that infinity (NaN where its weight is below 2^-80), a NaN or infinities of both signs NaN.
  */
 int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor* v,
                         const lq_tensor* starts, const lq_tensor* out, float scale, void* stream);

@@ -19,6 +19,10 @@ struct PromptAttention {
 
 constexpr int PROMPT_ATTENTION_WAVES = 4;  // of a workgroup, 32 rows each
 
+// In a workgroup's second run the weights are this much smaller, so that no sum of 2^30 values, each weighed 2^8
+// at most, leaves fp32 where the result does not. What is a power of two rounds alike, down to weights of 2^-86.
+constexpr float PROMPT_ATTENTION_DOWN = 0x1p-40f;
+
 // The 16-bit kernel (prompt_attention_mfma.hip): whether the tensors are in its form, and its launch,
 // whose scale is positive.
 bool prompt_attention_mfma_fits(const lq_tensor* q, const lq_tensor* k, const lq_tensor* v,

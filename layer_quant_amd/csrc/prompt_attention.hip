@@ -16,6 +16,9 @@
 // S^T[key][row] = K Q^T: a lane then holds the scores of one row, its softmax needs one exchange with
 // the lane 32 away, and the register that holds p of a key is by itself the B operand of
 // O^T[dim][row] += V^T P^T.
+//
+// A workgroup with an infinity among its sums, which may be of large values alone, runs its rows again with
+// smaller weights (PROMPT_ATTENTION_DOWN).
 #include "prompt_attention.h"
 
 namespace lq {
@@ -37,19 +40,13 @@ __device__ __forceinline__ bool finite(float x) {
   return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
 }
 
+// A span's rows of a workgroup; whether they have to run again, DOWN.
 // VEC: fp32 k and v in 16-byte aligned rows of a multiple of 4 dims. Their tiles come in 16-byte loads, a
 // tile ahead.
-template <int DP, bool VEC>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f32(PromptAttention p) {
-  __shared__ TileF32<DP> tile;
-  const int hk = blockIdx.x % p.Hkv;
-  Span sp;
-  const int nrep = p.nrep;
-  const bool mine = find_span(
-      p.spans, blockIdx.x / p.Hkv,
-      [&](int len, bool) { return (len * nrep + NW * ROWS - 1) / (NW * ROWS); }, sp);
-  if (!mine) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, hi = lane >> 5;
+template <int DP, bool VEC, bool DOWN>
+__device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp, int hk, int tid,
+                                       TileF32<DP>& tile) {
+  const int nrep = p.nrep, lane = tid & 63, wave = tid >> 6, col = lane & 31, hi = lane >> 5;
   const int nrows = sp.len * nrep;
   // the last tile of a prompt has the most keys: it goes first
   const int tiles = (nrows + NW * ROWS - 1) / (NW * ROWS);
@@ -60,11 +57,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f
   const int64_t row = sp.begin + pos;
   const int64_t lead = p.spans.starts == nullptr ? sp.index : 0;
   const int64_t out_at = lead * p.out.s[0] + row * p.out.s[1] + head * p.out.s[2];
-  if (sp.gap) {
+  if (!DOWN && sp.gap) {
     if (r < nrows) {
       for (int d = hi; d < p.D; d += 2) store_float(p.out.data, p.out.dtype, out_at + d * p.out.s[3], 0.f);
     }
-    return;
+    return false;
   }
 
   // query values of dims 8 j + 4 hi .. + 3, in the order in which the K rows are read
@@ -164,14 +161,23 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f
     }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float base = top == -INFINITY ? 0.f : top;  // all keys so far at -inf: their p is 0
-    const float keep = __builtin_amdgcn_exp2f(m - base);
+    float keep = __builtin_amdgcn_exp2f(m - base);
     m = top;
     l *= keep;
+    if (__any(keep == 0.f)) {  // the infinities, this tile's among them, stay
+#pragma unroll
+      for (int i = 0; i < DP / 2; ++i) {
+        const float x = o[i >> 4][i & 15];
+        o[i >> 4][i & 15] = keep == 0.f && finite(x) ? 0.f : x;
+      }
+      keep = keep == 0.f ? 1.f : keep;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[i] = __builtin_amdgcn_exp2f(s[i] - base);
       l += s[i];
     }
+    if (DOWN) s *= PROMPT_ATTENTION_DOWN;
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
       o[b] *= keep;
@@ -182,17 +188,41 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f
       }
     }
   }
+  if (!DOWN) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 2; ++i) most = fmaxf(most, fabsf(o[i >> 4][i & 15]));
+    if (__syncthreads_or(most == INFINITY)) return true;
+  }
   l += __shfl_xor(l, 32, 64);
-  const float inv = 1.f / l;
-  if (r >= nrows) return;
+  const float inv = (DOWN ? 1.f / PROMPT_ATTENTION_DOWN : 1.f) / l;
+  if (r >= nrows) return false;
+  int dim = 4 * hi;
+  asm volatile("" : "+v"(dim));  // (else the addresses of all stores in registers, through the loop)
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int d = 32 * b + 8 * (i >> 2) + 4 * hi + (i & 3);
+      const int d = 32 * b + 8 * (i >> 2) + dim + (i & 3);
       if (d < p.D) store_float(p.out.data, p.out.dtype, out_at + d * p.out.s[3], o[b][i] * inv);
     }
   }
+  return false;
+}
+
+template <int DP, bool VEC>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f32(PromptAttention p) {
+  __shared__ TileF32<DP> tile;
+  int hk = blockIdx.x % p.Hkv, tid = threadIdx.x;
+  Span sp;
+  const bool mine = find_span(
+      p.spans, blockIdx.x / p.Hkv,
+      [&](int len, bool) { return (len * p.nrep + NW * ROWS - 1) / (NW * ROWS); }, sp);
+  if (!mine || !attend<DP, VEC, false>(p, sp, hk, tid, tile)) return;
+  // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
+  // for the second one, through the loop.
+  asm volatile("" : "+s"(sp.index), "+s"(sp.begin), "+s"(sp.len), "+s"(sp.part), "+s"(hk), "+v"(tid));
+  attend<DP, VEC, true>(p, sp, hk, tid, tile);
 }
 
 template <bool VEC>

@@ -21,7 +21,8 @@
 //
 // Masked keys of a row have p = 0, which a value of inf or NaN would turn into NaN. Results that are not
 // finite are rare, so it is they that are looked for: a workgroup with one runs its rows again, and then
-// hands such values to the rows that see them and takes them out of the tile.
+// hands such values to the rows that see them and takes them out of the tile. As unnormalised sums of values
+// next to bf16's largest can leave fp32, the weights are smaller then (PROMPT_ATTENTION_DOWN).
 //
 // What it measured (MI355X, 32 query / 8 KV heads of 128, us per call): one prompt of 16384 rows 1976-2057,
 // 1.07-1.11 PFLOP/s, where the library's large bf16 product reaches 1.14; 24 fp16 prompts up to 700 rows 31.6;
@@ -49,20 +50,17 @@ __device__ __forceinline__ int swizzle_v(int r) {
   return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
 }
 
-template <bool BF, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttention p) {
+template <int D>
+using Tiles = char[2][2][KT * 2 * D];  // [buffer][K, V]
+
+// A span's rows of a workgroup; whether they have to run again, with CAREFUL.
+template <bool BF, int D, int NW, bool CAREFUL>
+__device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp, int hk, int tid, Tiles<D>& tiles) {
   constexpr int ROW_BYTES = 2 * D, CH = D / 8, TILE = KT * ROW_BYTES;
   constexpr int PER_LOAD = 64 / CH;                 // rows of one load
   constexpr int LOADS = KT / PER_LOAD / NW;         // of K, and of V, per wave and tile
   static_assert(LOADS * PER_LOAD * NW == KT, "every wave loads as many rows");
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][TILE];  // [buffer][K, V]
-  const int hk = blockIdx.x % p.Hkv, nrep = p.nrep;
-  Span sp;
-  if (!find_span(p.spans, blockIdx.x / p.Hkv,
-                 [&](int len, bool) { return (len * nrep + NW * ROWS - 1) / (NW * ROWS); }, sp)) {
-    return;
-  }
-  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
+  const int nrep = p.nrep, lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nrows = sp.len * nrep, parts = (nrows + NW * ROWS - 1) / (NW * ROWS);
   // the last rows of a prompt have the most keys: they go first
@@ -71,12 +69,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
   const int pos = at / nrep, head = hk * nrep + at - pos * nrep;
   const int64_t lead = p.spans.starts == nullptr ? sp.index : 0, row = sp.begin + pos;
   uint16_t* out = (uint16_t*)p.out.data + lead * p.out.s[0] + row * p.out.s[1] + head * p.out.s[2];
-  if (sp.gap) {
+  if (!CAREFUL && sp.gap) {
     if (r < nrows) {
 #pragma unroll
       for (int i = 0; i < CH / 2; ++i) *(words4_t*)(out + 8 * (2 * i + hi)) = words4_t{0, 0, 0, 0};
     }
-    return;
+    return false;
   }
 
   words4_t q[D / 16];  // dims 16 i + 8 hi .. + 7
@@ -122,93 +120,100 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
   const int wave_first = __builtin_amdgcn_readfirstlane(min(first + wave * ROWS, nrows - 1) / nrep);
   const int wave_last = __builtin_amdgcn_readfirstlane(min(first + wave * ROWS + ROWS - 1, nrows - 1) / nrep);
   f32x16_t o[D / 32];
-  float m, l;
-  for (int careful = 0; careful < 2; ++careful) {
-    m = -INFINITY;
-    l = 0.f;
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = f32x16_t{};
-    load_tile(0, 0);
-    for (int kb = 0, buf = 0; kb <= pos_last; kb += KT, buf ^= 1) {
-      wait_loads<0>();
-      __syncthreads();
-      if (kb + KT <= pos_last) load_tile(kb + KT, buf ^ 1);
-      lds_t kt = (lds_t)&tiles[buf][0][0], vt = (lds_t)&tiles[buf][1][0];
-      if (careful && kb + KT - 1 > pos_first) {
-        uint16_t* v = (uint16_t*)&tiles[buf][1][0];
-        constexpr uint32_t INF = BF ? 0x7f80 : 0x7c00;
-        for (int key = 0; key < KT; ++key) {
-          if (kb + key > pos) continue;
+  for (int i = 0; i < D / 32; ++i) o[i] = f32x16_t{};
+  load_tile(0, 0);
+  for (int kb = 0, buf = 0; kb <= pos_last; kb += KT, buf ^= 1) {
+    wait_loads<0>();
+    __syncthreads();
+    if (kb + KT <= pos_last) load_tile(kb + KT, buf ^ 1);
+    lds_t kt = (lds_t)&tiles[buf][0][0], vt = (lds_t)&tiles[buf][1][0];
+    if (CAREFUL && kb + KT - 1 > pos_first) {
+      uint16_t* v = (uint16_t*)&tiles[buf][1][0];
+      constexpr uint32_t INF = BF ? 0x7f80 : 0x7c00;
+      for (int key = 0; key < KT; ++key) {
+        if (kb + key > pos) continue;
 #pragma unroll
-          for (int b = 0; b < D / 32; ++b) {
+        for (int b = 0; b < D / 32; ++b) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int d = 32 * b + 8 * (i >> 2) + 4 * hi + (i & 3);
-              const uint32_t x = v[key * D + 8 * ((d >> 3) ^ swizzle_v<D>(key)) + (d & 7)];
-              if ((x & INF) == INF) {
-                o[b][i] += BF ? bf16_bits_to_float(x) : (float)__builtin_bit_cast(_Float16, (uint16_t)x);
-              }
+          for (int i = 0; i < 16; ++i) {
+            const int d = 32 * b + 8 * (i >> 2) + 4 * hi + (i & 3);
+            const uint32_t x = v[key * D + 8 * ((d >> 3) ^ swizzle_v<D>(key)) + (d & 7)];
+            if ((x & INF) == INF) {
+              o[b][i] += BF ? bf16_bits_to_float(x) : (float)__builtin_bit_cast(_Float16, (uint16_t)x);
             }
           }
         }
-        __syncthreads();
-        for (int i = tid; i < KT * D; i += 64 * NW) {
-          if ((v[i] & INF) == INF) v[i] = 0;
-        }
-        __syncthreads();
       }
-      if (kb > wave_last) continue;
-      f32x16_t s[2] = {};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          s[b] = mfma<BF>(lds_read16(kt + (kaddr ^ (32 * i)) + b * 32 * ROW_BYTES), q[i], s[b]);
-        }
+      __syncthreads();
+      for (int i = tid; i < KT * D; i += 64 * NW) {
+        if ((v[i] & INF) == INF) v[i] = 0;
       }
-      if (kb + KT - 1 > wave_first) {
+      __syncthreads();
+    }
+    if (kb > wave_last) continue;
+    f32x16_t s[2] = {};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+    for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (kb + 32 * b + 8 * (i >> 2) + 4 * hi + (i & 3) > pos) s[b][i] = -INFINITY;
-          }
-        }
+      for (int b = 0; b < 2; ++b) {
+        s[b] = mfma<BF>(lds_read16(kt + (kaddr ^ (32 * i)) + b * 32 * ROW_BYTES), q[i], s[b]);
       }
-      float top = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any((top - m) * p.scale > LAZY || m == -INFINITY)) {
-        const float to = fmaxf(m, top);
-        // all keys so far at -inf: no weight yet, and none to rescale
-        const float keep = to == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - to) * p.scale);
-        m = to;
-        l *= keep;
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) o[b] *= keep;
-      }
-      const float base = m == -INFINITY ? 0.f : m * p.scale;
-      words4_t pk[4];
+    }
+    if (kb + KT - 1 > wave_first) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.scale, -base));
-          l += s[b][i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pk[2 * b + (i >> 2)][i & 3] = pack2<BF>(s[b][2 * i], s[b][2 * i + 1]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
-          lds_t from = vt + (vaddr ^ (64 * b)) + 16 * j * ROW_BYTES;
-          o[b] = mfma<BF>(lds_read_columns(from, from + 8 * ROW_BYTES), pk[j], o[b]);
+          if (kb + 32 * b + 8 * (i >> 2) + 4 * hi + (i & 3) > pos) s[b][i] = -INFINITY;
         }
       }
     }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any((top - m) * p.scale > LAZY || m == -INFINITY)) {
+      const float to = fmaxf(m, top);
+      // all keys so far at -inf: no weight yet
+      float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - to) * p.scale);
+      m = to;
+      l *= keep;
+      if (CAREFUL && __any(keep == 0.f)) {  // the infinities, this tile's among them, stay
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) {
+          const float x = o[i >> 4][i & 15];
+          o[i >> 4][i & 15] = keep == 0.f && x - x == 0.f ? 0.f : x;
+        }
+        keep = keep == 0.f ? 1.f : keep;
+      }
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) o[b] *= keep;
+    }
+    const float base = m == -INFINITY ? 0.f : m * p.scale;
+    words4_t pk[4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.scale, -base));
+        l += s[b][i];
+      }
+      if (BF && CAREFUL) s[b] *= PROMPT_ATTENTION_DOWN;  // (fp16 values are too small to need it)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pk[2 * b + (i >> 2)][i & 3] = pack2<BF>(s[b][2 * i], s[b][2 * i + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+        lds_t from = vt + (vaddr ^ (64 * b)) + 16 * j * ROW_BYTES;
+        o[b] = mfma<BF>(lds_read_columns(from, from + 8 * ROW_BYTES), pk[j], o[b]);
+      }
+    }
+  }
+  if (!CAREFUL) {
     // sum of the accumulators times 0: NaN if one is not finite
     float odd = 0.f;
 #pragma unroll
@@ -216,11 +221,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
 #pragma unroll
       for (int i = 0; i < 16; ++i) odd = fmaf(o[b][i], 0.f, odd);
     }
-    if (careful || !__syncthreads_or(odd != 0.f)) break;
+    if (__syncthreads_or(odd != 0.f)) return true;
   }
   l += __shfl_xor(l, 32, 64);
-  const float inv = 1.f / l;
-  if (r >= nrows) return;
+  const float inv = (BF && CAREFUL ? 1.f / PROMPT_ATTENTION_DOWN : 1.f) / l;
+  if (r >= nrows) return false;
 #pragma unroll
   for (int b = 0; b < D / 32; ++b) {
 #pragma unroll
@@ -234,6 +239,23 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_attention_mfma(PromptAttent
       *(words4_t*)(out + 32 * b + 16 * a + 8 * hi) = words4_t{x[0], y[0], x[1], y[1]};
     }
   }
+  return false;
+}
+
+template <bool BF, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prompt_attention_mfma(PromptAttention p) {
+  __shared__ __attribute__((aligned(1024))) Tiles<D> tiles;
+  int hk = blockIdx.x % p.Hkv, tid = threadIdx.x;
+  Span sp;
+  if (!find_span(p.spans, blockIdx.x / p.Hkv,
+                 [&](int len, bool) { return (len * p.nrep + NW * ROWS - 1) / (NW * ROWS); }, sp)) {
+    return;
+  }
+  if (!attend<BF, D, NW, false>(p, sp, hk, tid, tiles)) return;
+  // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
+  // for the second one, through the loop.
+  asm volatile("" : "+s"(sp.index), "+s"(sp.begin), "+s"(sp.len), "+s"(sp.part), "+s"(hk), "+v"(tid));
+  attend<BF, D, NW, true>(p, sp, hk, tid, tiles);
 }
 
 // A row's elements in a row, every row 16-byte aligned, 64 rows within 31 bits of bytes.

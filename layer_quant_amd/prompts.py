@@ -54,7 +54,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     -> query's shape and dtype, in `out` where given (which may be query, and overlaps no key or value).
 
     Scores, softmax and sums are fp32 (16-bit inputs: the weights are rounded to that type before
-    they multiply the values). What stands behind a row in its prompt never reaches its result, be it NaN.
+    they multiply the values). What stands behind a row in its prompt never reaches its result, be it NaN. A
+    value of inf or NaN that it sees does, as that infinity (NaN where its weight is below 2^-80) or as NaN.
     """
     _check_prompts("query", query, starts)
     _no_gradients(query, key, value)
