@@ -32,7 +32,8 @@
 // and a single barrier (313 us: 66 and 681 instructions); loads further ahead into L2 (no gain); heads to XCDs
 // in other orders (no difference); the last block's heads shared out to two waves (297).
 //
-// Roundings: M, D and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result). w x, which a
+// Roundings: M and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result), D to the sum of two
+// bf16 values (2^-17). w x, which a
 // state keeps, to the sum of two bf16 values (2^-16) where the state leaves in 16 bits, and of three (its 24
 // bits) where it leaves in fp32: 700 rows' fp32 states are off by less than 5e-7 with three, 2e-6 with two (24
 // prompts 123 us, 117), and bf16 ones by 0.0017, their own rounding, with two, 0.0024 with one (16384 rows 312
@@ -245,8 +246,11 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
     }
   };
 
+  // D as the sum of two bf16 values, each in both halves of a word
   const float D = p.D.data == nullptr ? 0.f : load_float(p.D.data, p.D.dtype, h * p.D.s[0]);
-  const uint32_t D16 = pack2<true>(D, 0.f);
+  const uint32_t D16 = pack2<true>(D, D);
+  const float rest = D - __uint_as_float(D16 << 16);
+  const uint32_t D16_rest = rest - rest == 0.f ? pack2<true>(rest, rest) : 0;  // (an infinite D has none)
   // operand addresses within the tiles; a product step exchanges chunks (^)
   const int sb = wave >= 2, tb = wave != 0;  // the mixing block of waves 0 to 2
   const int brow = 32 * sb + sigma(col);
@@ -386,14 +390,18 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
       asm volatile("" : "+v"(t));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        words4_t diagonal;  // D where s = t
+        words4_t diagonal, rest;  // D where s = t
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int s = 16 * i + 8 * hi + 2 * e;
-          diagonal[e] = t == s ? D16 : t == s + 1 ? D16 << 16 : 0;
+          const uint32_t here = t == s ? 0xffffu : t == s + 1 ? 0xffff0000u : 0;
+          diagonal[e] = here & D16;
+          rest[e] = here & D16_rest;
         }
         y[0] = mfma<true>(xa[i], diagonal, y[0]);
         y[1] = mfma<true>(xa[i + 2], diagonal, y[1]);
+        y[0] = mfma<true>(xa[i], rest, y[0]);
+        y[1] = mfma<true>(xa[i + 2], rest, y[1]);
         y[0] = mfma<true>(xa[i], lds_read16(mt + (m_at ^ (32 * i))), y[0]);
         y[1] = mfma<true>(xa[i], lds_read16(mt + 2048 + (m_at ^ (32 * i))), y[1]);
         y[1] = mfma<true>(xa[i + 2], lds_read16(mt + 4096 + (m_at ^ (32 * i))), y[1]);
