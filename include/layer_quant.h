@@ -392,7 +392,11 @@ int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor*
  *   dt = dt (+ dt_bias); dt = log(1 + e^dt) if dt_softplus; dt clamped to [dt_min, dt_max]
  *   S  = exp(A dt) S + dt x B^T     (S [P, N], from initial or zero)
  *   y  = S C (+ D x);  y *= z * sigmoid(z) when z is given
- * States in fp32; rounded where they are written.
+ * States and sums in fp32. bf16 x with P = 64, N = 128, H / G even and rows of 16 bytes (the matrix kernel):
+ * the factors of C are rounded to bf16, the state in front of each 64 rows and the weights of x within them
+ * (half a step of each term of y); what a row adds to the state is the sum of two bf16 values (off by 2^-16),
+ * or of three (2^-24) where states leave in fp32; D is the sum of two. Elsewhere y and states are rounded where
+ * they are written and nowhere else.
  *   packed: x, z, out [T, H, P], dt [T, H], B, C [T, G, N] (H % G == 0) and starts as for
  *     lq_prompt_attention; a batch: starts NULL, x [B, L, H, P] and so on
  *   A [H], D NULL or [H], dt_bias NULL or [H]; initial NULL or [S, H, P, N], states NULL or [S, H, P, N]

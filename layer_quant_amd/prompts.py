@@ -84,6 +84,11 @@ def prompt_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Ten
     same as initial_states to go on in place; they overlap in no other way), or to a new fp32 tensor; a
     prompt without rows hands its initial state on.
 
+    States and sums are fp32. bf16 prompts of heads of 64 and states of 128 run on matrix instructions: there
+    the state in front of each 64 rows and the weights of x within them are rounded to bf16 before they make y
+    (half a step of each term, beside y's own rounding), and what a row adds to the state is off by 2^-16 of
+    itself, or 2^-24 where `states` are fp32. The other prompts round what they return and nothing else.
+
     What stands behind a row in its prompt never reaches it. An x of inf or NaN leaves every y and state
     that it reaches not finite, inf or NaN (the sign of an infinity is not followed through the products).
     """
