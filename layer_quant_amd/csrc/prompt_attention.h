@@ -19,6 +19,15 @@ struct PromptAttention {
 
 constexpr int PROMPT_ATTENTION_WAVES = 4;  // of a workgroup, 32 rows each
 
+// The prompt and part of it (rows x query heads of a KV head) of workgroup t of a KV head.
+__device__ __forceinline__ bool find_part(const PromptAttention& p, int t, Span& out) {
+  constexpr int ROWS = 32 * PROMPT_ATTENTION_WAVES;
+  const int nrep = p.nrep;
+  return find_span<true>(
+      p.spans, t, [=](int len, bool) { return (len * nrep + ROWS - 1) / ROWS; },
+      [=](int begin, int i) { return begin * nrep / ROWS + i; }, out);
+}
+
 // In a workgroup's second run the weights are this much smaller, so that no sum of 2^30 values, each weighed 2^8
 // at most, leaves fp32 where the result does not. What is a power of two rounds alike, down to weights of 2^-86.
 constexpr float PROMPT_ATTENTION_DOWN = 0x1p-40f;

@@ -215,10 +215,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_attention_f
   __shared__ TileF32<DP> tile;
   int hk = blockIdx.x % p.Hkv, tid = threadIdx.x;
   Span sp;
-  const bool mine = find_span(
-      p.spans, blockIdx.x / p.Hkv,
-      [&](int len, bool) { return (len * p.nrep + NW * ROWS - 1) / (NW * ROWS); }, sp);
-  if (!mine || !attend<DP, VEC, false>(p, sp, hk, tid, tile)) return;
+  if (!find_part(p, blockIdx.x / p.Hkv, sp)) return;
+  if (!attend<DP, VEC, false>(p, sp, hk, tid, tile)) return;
   // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
   // for the second one, through the loop.
   asm volatile("" : "+s"(sp.index), "+s"(sp.begin), "+s"(sp.len), "+s"(sp.part), "+s"(hk), "+v"(tid));

@@ -247,10 +247,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prompt_attention_mfm
   __shared__ __attribute__((aligned(1024))) Tiles<D> tiles;
   int hk = blockIdx.x % p.Hkv, tid = threadIdx.x;
   Span sp;
-  if (!find_span(p.spans, blockIdx.x / p.Hkv,
-                 [&](int len, bool) { return (len * p.nrep + NW * ROWS - 1) / (NW * ROWS); }, sp)) {
-    return;
-  }
+  if (!find_part(p, blockIdx.x / p.Hkv, sp)) return;
   if (!attend<BF, D, NW, false>(p, sp, hk, tid, tiles)) return;
   // Again, from values hidden from the compiler: it would keep what the first run made of them in registers
   // for the second one, through the loop.

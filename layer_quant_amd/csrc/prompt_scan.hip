@@ -375,8 +375,10 @@ constexpr int AHEAD = 8;
 // blockIdx.y: slot; a prompt's first one carries all of its own. Four consecutive values per thread.
 __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
   Span sp;
-  const auto slots = [&](int len, bool gap) { return slots_of_span(p, len, gap); };
-  if (!find_span(p.spans, blockIdx.y, slots, sp) || sp.part != 0) return;
+  const bool mine = find_span<false>(
+      p.spans, blockIdx.y, [&](int len, bool gap) { return slots_of_span(p, len, gap); },
+      [&](int begin, int i) { return slot_of(p, begin, i); }, sp);
+  if (!mine || sp.part != 0) return;
   const int many = min(slots_of_span(p, sp.len, false), p.slots - (int)blockIdx.y);
   const int64_t size = (int64_t)p.H * p.P * p.N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= size) return;
@@ -457,6 +459,11 @@ int64_t plan_segment(bool matrix, int64_t prompts, int64_t rows, int64_t heads) 
   }
   const int64_t seg = (prompts >= 8 ? 2 * want : want) + 63;
   return max(seg / 64 * 64, rows <= 1024 * prompts ? (int64_t)1024 : (int64_t)256);
+}
+
+// Whether slot_of goes by the rows alone, as fewer slots are needed then.
+bool slots_by_rows(int64_t prompts, int64_t rows, int64_t segment) {
+  return 2 * rows / segment < rows / segment + prompts;
 }
 
 // Slots, at most: a prompt has a segment more than its rows fill, or, as one of several segments has more
@@ -615,6 +622,7 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   p.ratio = (int)(H / G);
   p.softplus = dt_softplus;
   p.slots = (int)slots;
+  p.slots_by_rows = slots_by_rows(S, rows, p.segment);
   p.dt_min = dt_min;
   p.dt_max = dt_max;
   p.slot_state = (float*)workspace;

@@ -91,8 +91,8 @@ __global__ __launch_bounds__(256) void scan_steps_kernel(PromptScan p) {
   __shared__ float tile[Q][STEP_HEADS + 1];
   const int blocks = (p.H + STEP_HEADS - 1) / STEP_HEADS, hb = blockIdx.x % blocks * STEP_HEADS;
   Span sp;
-  if (!find_span(p.spans, blockIdx.x / blocks, [&](int len, bool gap) { return gap ? 0 : (len + Q - 1) / Q; },
-                 sp)) {
+  if (!find_span<false>(p.spans, blockIdx.x / blocks, [](int len, bool) { return (len + Q - 1) / Q; },
+                        [](int begin, int i) { return begin / Q + i; }, sp)) {
     return;
   }
   const int64_t lead = p.spans.starts == nullptr ? sp.index : 0, row0 = sp.begin + sp.part * Q;

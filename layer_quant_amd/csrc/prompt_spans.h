@@ -2,8 +2,12 @@
 //
 // starts [S + 1] lies on the device, so the host knows the number of rows and of prompts and no length:
 // a launch has a workgroup for as many parts as such prompts can have at most, and each finds its own
-// from the starts, 64 prompts at a time. Rows in front of the first start and behind the last are spans
-// of their own (the first and the last one), so that every row belongs to one.
+// from the starts. Span i, of the rows b to e, begins at part floor(b / rows of a part) + i: a number that
+// grows by as many parts as the span can have, as floor(e / n) + 1 - floor(b / n) >= ceil((e - b) / n), and
+// that needs no other span's length. So a workgroup searches the starts, 64 at a time in a wave's lanes: one
+// round for up to 64 spans, four for 2^24. (A sum of the parts of all spans in front took a round per 64
+// spans in every workgroup.) Rows in front of the first start and behind the last are spans of their own
+// (the first and the last one), so that every row belongs to one.
 #pragma once
 
 #include "lq_common.h"
@@ -21,9 +25,8 @@ struct Span {
   int index;  // prompt, or batch row
   int begin;  // first row (0 in a batch)
   int len;
-  int part;    // the part of this span
-  int before;  // slots of the spans in front of this one
-  bool gap;    // rows of no prompt
+  int part;  // the part of this span
+  bool gap;  // rows of no prompt
 };
 
 // Starts are taken as they come, but never outside [0, rows].
@@ -34,19 +37,11 @@ __device__ __forceinline__ int span_bound(const Spans& s, int i) {
   return (int)(v < 0 ? 0 : v > s.rows ? s.rows : v);
 }
 
-__device__ __forceinline__ int wave_prefix_sum(int v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(v, o, 64);
-    if (lane >= o) v += up;
-  }
-  return v;
-}
-
-// The span and part behind t parts; false where there are not so many. parts(len, gap) gives a span's
-// number, slots(len, gap) another one that is summed. Every lane of a wave calls it with the same t.
-template <class F, class G>
-__device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, G&& slots, Span& out) {
+// The span and part of workgroup t; false where it has none. parts(len, gap): the parts of a span;
+// first(begin, i): the workgroup of its first one, i the span's number. GAPS: the rows of no prompt are spans,
+// too. Every lane of a wave calls it with the same t. Starts out of order give any span, and a part of it.
+template <bool GAPS, class F, class G>
+__device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, G&& first, Span& out) {
   if (s.starts == nullptr) {
     const int n = parts(s.rows, false);
     if (n == 0 || t >= n * s.S) return false;
@@ -54,44 +49,36 @@ __device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, G&& 
     out.part = t - out.index * n;
     out.begin = 0;
     out.len = s.rows;
-    out.before = out.index * slots(s.rows, false);
     out.gap = false;
     return true;
   }
-  const int lane = (int)(threadIdx.x & 63);
-  int run = 0, behind = 0;
-  for (int base = 0; base < s.S + 2; base += 64) {
-    const int i = base + lane;
-    int begin = 0, len = 0;
-    if (i < s.S + 2) {
-      begin = span_bound(s, i);
-      len = max(span_bound(s, i + 1) - begin, 0);
+  const int lane = (int)(threadIdx.x & 63), before = GAPS ? 0 : 1;
+  int at = 0, n = GAPS ? s.S + 2 : s.S;  // the span is one of n from `at` on
+  while (n > 0) {
+    const int step = (n + 63) >> 6, i = at + lane * step;
+    int begin = 0, end = 0;
+    bool reached = false;
+    if (lane * step < n) {
+      begin = span_bound(s, i + before);
+      end = span_bound(s, i + before + 1);
+      reached = first(begin, i) <= t;
     }
-    const bool gap = i == 0 || i >= s.S + 1;
-    const int n = parts(len, gap);
-    const int upto = wave_prefix_sum(n, lane);
-    const int own_slots = slots(len, gap), later = wave_prefix_sum(own_slots, lane);
-    const uint64_t have = __ballot(t < run + upto);
-    if (have != 0) {
-      const int l = __builtin_ctzll(have);
-      out.index = base + l - 1;
-      out.begin = __builtin_amdgcn_readlane(begin, l);
-      out.len = __builtin_amdgcn_readlane(len, l);
-      const int own = __builtin_amdgcn_readlane(n, l);
-      out.part = t - (run + __builtin_amdgcn_readlane(upto, l) - own);
-      out.gap = out.index < 0 || out.index >= s.S;
-      out.before = behind + __builtin_amdgcn_readlane(later, l) - __builtin_amdgcn_readlane(own_slots, l);
-      return true;
+    const uint64_t not_yet = ~__ballot(reached);
+    const int k = (not_yet == 0 ? 64 : __builtin_ctzll(not_yet)) - 1;
+    if (k < 0) return false;
+    at += k * step;
+    if (step > 1) {
+      n = min(step, n - k * step);
+      continue;
     }
-    run += __builtin_amdgcn_readlane(upto, 63);
-    behind += __builtin_amdgcn_readlane(later, 63);
+    out.index = at - 1 + before;
+    out.begin = __builtin_amdgcn_readlane(begin, k);
+    out.len = max(__builtin_amdgcn_readlane(end, k) - out.begin, 0);
+    out.part = t - first(out.begin, at);
+    out.gap = out.index < 0 || out.index >= s.S;
+    return out.part >= 0 && out.part < parts(out.len, out.gap);
   }
   return false;
-}
-
-template <class F>
-__device__ __forceinline__ bool find_span(const Spans& s, int t, F&& parts, Span& out) {
-  return find_span(s, t, parts, [](int, bool) { return 0; }, out);
 }
 
 // host: validates `starts` (NULL, or int32/int64 [S + 1]) against packed rows
