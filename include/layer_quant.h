@@ -379,7 +379,7 @@ int lq_reorder_beams(const lq_tensor* tensors, const int64_t* rows, int count,
  *     that are not in ascending order give unspecified values.
  *   a batch: starts NULL, q, out [B, L, Hq, D], k, v [B, L, Hkv, D], every batch row a prompt
  *   q, k, v and out of one dtype (f32, f16 or bf16), any strides; D <= 256. out may be q, and overlaps
- *   neither k nor v nor itself.
+ *   neither k nor v nor itself (refused; views that take turns in one tensor, as of fused rows, do not).
  * Rows behind a query's own never reach its result, whatever they hold. A value of inf that a row sees makes
  * its result that infinity (NaN where its weight is below 2^-80), a NaN or infinities of both signs NaN.
  */
@@ -400,9 +400,9 @@ int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor*
  *   packed: x, z, out [T, H, P], dt [T, H], B, C [T, G, N] (H % G == 0) and starts as for
  *     lq_prompt_attention; a batch: starts NULL, x [B, L, H, P] and so on
  *   A [H], D NULL or [H], dt_bias NULL or [H]; initial NULL or [S, H, P, N], states NULL or [S, H, P, N]
- *   (the state behind each prompt; an empty one's is its initial state). They may be one tensor; else no
- *   output may overlap an input. x, B and C of one dtype, the others of any float dtype; any strides.
- *   N <= 256. The workspace needs no particular contents; dtype is x's, `prompts` S and `rows` T (packed
+ *   (the state behind each prompt; an empty one's is its initial state). They may be one tensor; else an
+ *   output that overlaps an input, itself or the other one is refused. x, B and C of one dtype, the others of
+ *   any float dtype; any strides. N <= 256. The workspace needs no particular contents; dtype is x's, `prompts` S and `rows` T (packed
  *   1) or L (packed 0).
  */
 size_t lq_prompt_scan_workspace(int dtype, int64_t prompts, int64_t rows, int packed, int64_t heads,

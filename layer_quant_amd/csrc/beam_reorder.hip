@@ -184,23 +184,6 @@ int row_shape(const lq_tensor& t, int64_t rows, int64_t per_block, Item& item) {
   return LQ_OK;
 }
 
-// Whether two elements of t may share memory: by size, each stride has to reach past the extent of the
-// smaller ones.
-bool overlaps_itself(const lq_tensor& t) {
-  int order[4], dims = 0;
-  for (int d = 0; d < t.ndim; ++d) {
-    if (t.shape[d] > 1) order[dims++] = d;
-  }
-  std::sort(order, order + dims, [&](int a, int b) { return std::abs(t.stride[a]) < std::abs(t.stride[b]); });
-  int64_t extent = 1;
-  for (int i = 0; i < dims; ++i) {
-    const int64_t stride = std::abs(t.stride[order[i]]);
-    if (stride < extent) return true;
-    extent += (t.shape[order[i]] - 1) * stride;
-  }
-  return false;
-}
-
 // The bytes that t spans, from its first element's on.
 int64_t span_bytes(const lq_tensor& t) {
   int64_t last = 0;

@@ -64,6 +64,17 @@ inline int check_tensor_or_empty(const lq_tensor* t, const char* name, int ndim,
   return check_tensor(&with_data, name, ndim, float_dtype, exact_dtype);
 }
 
+// Whether two elements of t may share memory: by size, each stride has to reach past the extent of the
+// smaller ones.
+bool overlaps_itself(const lq_tensor& t);
+
+// Whether an element of a and one of b may share memory. Views of one tensor that take turns in it (q, k and
+// v of fused rows) do not; where the strides differ, memory between two elements counts as theirs.
+bool overlap(const lq_tensor& a, const lq_tensor& b);
+
+// Whether a and b are the same elements in the same places.
+bool same_elements(const lq_tensor& a, const lq_tensor& b);
+
 // Largest element offset reachable through a descriptor (for bounds reasoning on the host).
 int64_t max_offset(const lq_tensor* t);
 

@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "lq_common.h"
@@ -99,6 +100,76 @@ static uint32_t diag_from_env() {
 static std::atomic<uint32_t> g_diag{diag_from_env()};
 
 bool diag(uint32_t bit) { return (g_diag.load(std::memory_order_relaxed) & bit) != 0; }
+
+namespace {
+
+// A tensor's dimensions of more than one element, the largest stride first, in bytes and upwards.
+struct Extents {
+  int dims = 0;
+  int64_t shape[4], stride[4];
+  int64_t size;  // of an element
+  bool empty = false;
+  uintptr_t first;  // lowest address
+
+  explicit Extents(const lq_tensor& t) : size(dtype_size(t.dtype)), first((uintptr_t)t.data) {
+    for (int d = 0; d < t.ndim; ++d) {
+      empty = empty || t.shape[d] == 0;
+      if (t.shape[d] < 2) continue;
+      const int64_t s = t.stride[d] * size;
+      if (s < 0) first -= (uintptr_t)(-s * (t.shape[d] - 1));
+      int at = dims++;
+      for (; at > 0 && stride[at - 1] < std::abs(s); --at) stride[at] = stride[at - 1], shape[at] = shape[at - 1];
+      stride[at] = std::abs(s);
+      shape[at] = t.shape[d];
+    }
+  }
+  // bytes from the first to behind the last element of dimensions d ..
+  int64_t span(int d) const {
+    int64_t n = size;
+    for (; d < dims; ++d) n += (shape[d] - 1) * stride[d];
+    return n;
+  }
+};
+
+// Dimensions d .. of a and e .. of b, b's first byte `apart` bytes behind a's.
+bool meet(const Extents& a, int d, const Extents& b, int e, int64_t apart) {
+  const int64_t na = a.span(d), nb = b.span(e);
+  if (apart >= na || -apart >= nb) return false;
+  if (d == a.dims || e == b.dims || a.stride[d] != b.stride[e]) return true;
+  // a step that both take, and that reaches past what they hold within it: b's blocks lie `rest` behind a's,
+  // and reach into the next ones of a
+  const int64_t step = a.stride[d];
+  if (a.span(d + 1) > step || b.span(e + 1) > step) return true;
+  int64_t steps = apart / step, rest = apart - steps * step;
+  if (rest < 0) --steps, rest += step;
+  // a's block i and b's block j are (j - i + steps) step + rest apart
+  const auto have = [&](int64_t i_less_j) { return i_less_j > -b.shape[e] && i_less_j < a.shape[d]; };
+  return (have(steps) && meet(a, d + 1, b, e + 1, rest)) ||
+         (have(steps + 1) && meet(a, d + 1, b, e + 1, rest - step));
+}
+
+}  // namespace
+
+bool overlaps_itself(const lq_tensor& t) {
+  const Extents x(t);
+  for (int d = 0; d < x.dims && !x.empty; ++d) {
+    if (x.stride[d] < x.span(d + 1)) return true;
+  }
+  return false;
+}
+
+bool overlap(const lq_tensor& a, const lq_tensor& b) {
+  const Extents x(a), y(b);
+  return !x.empty && !y.empty && meet(x, 0, y, 0, (int64_t)(y.first - x.first));
+}
+
+bool same_elements(const lq_tensor& a, const lq_tensor& b) {
+  if (a.data != b.data || a.dtype != b.dtype || a.ndim != b.ndim) return false;
+  for (int d = 0; d < a.ndim; ++d) {
+    if (a.shape[d] != b.shape[d] || (a.shape[d] > 1 && a.stride[d] != b.stride[d])) return false;
+  }
+  return true;
+}
 
 int64_t max_offset(const lq_tensor* t) {
   int64_t off = 0;

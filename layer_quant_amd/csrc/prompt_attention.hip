@@ -297,6 +297,10 @@ extern "C" int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const
     return fail(LQ_ERR_UNSUPPORTED, "%lld rows of %lld heads exceed the launch limits",
                 (long long)rows, (long long)Hq);
   }
+  if (overlaps_itself(*out) || overlap(*out, *k) || overlap(*out, *v) ||
+      (overlap(*out, *q) && !same_elements(*out, *q)) || (starts != nullptr && overlap(*out, *starts))) {
+    return fail(LQ_ERR_INVALID_ARG, "out overlaps itself, k, v, starts, or q without being q");
+  }
   const lq_tensor* ts[4] = {q, k, v, out};
   View* vs[4] = {&p.q, &p.k, &p.v, &p.out};
   for (int i = 0; i < 4; ++i) {

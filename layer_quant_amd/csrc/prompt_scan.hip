@@ -603,6 +603,17 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   if (need > 0 && ((uintptr_t)workspace & 255) != 0) {
     return fail(LQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   }
+  const lq_tensor* inputs[10] = {x, dt, A, B, C, starts, D, z, dt_bias, initial};
+  for (int i = 0; i < 10; ++i) {
+    if (inputs[i] == nullptr) continue;
+    const bool in_place = i == 9 && states != nullptr && same_elements(*states, *initial);
+    if (overlap(*out, *inputs[i]) || (states != nullptr && !in_place && overlap(*states, *inputs[i]))) {
+      return fail(LQ_ERR_INVALID_ARG, "an output overlaps an input");
+    }
+  }
+  if (overlaps_itself(*out) || (states != nullptr && (overlaps_itself(*states) || overlap(*out, *states)))) {
+    return fail(LQ_ERR_INVALID_ARG, "the outputs overlap themselves or each other");
+  }
   const lq_tensor* ts[6] = {x, B, C, z, out, dt};
   View* vs[6] = {&p.x, &p.B, &p.C, &p.z, &p.out, &p.dt};
   for (int i = 0; i < 6; ++i) {
