@@ -351,8 +351,8 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
                            layer_cache.k_scale, layer_cache.v_scale, positions, group_size)
     layer_cache.length = max(layer_cache.length, required_len)
 
-    if attention_mask is None and self._int4_kv_prompt_kernel and not torch.is_grad_enabled() \
-            and not (self.training and self.attention_dropout):
+    if attention_mask is None and getattr(self, "_int4_kv_prompt_kernel", False) \
+            and not torch.is_grad_enabled() and not (self.training and self.attention_dropout):
         attn = prompts.prompt_attention(query_states.transpose(1, 2), key_states.transpose(1, 2),
                                         value_states.transpose(1, 2))
         return self.o_proj(attn.reshape(bsz, q_len, self.hidden_size)), None, past_key_value
