@@ -373,13 +373,15 @@ def _forward_fused_int4_kv(self, hidden_states, attention_mask=None, position_id
     return self.o_proj(attn), None, past_key_value
 
 
-def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64, *, prompt_kernel: bool = False):
+def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64, *,
+                                       prompt_kernel: bool | None = None):
     """Route every attention block's forward through the INT4 cache (ia.py:717-731).
 
     Idempotent per layer; records the original forward, the group size and the remote module's
-    repeat_kv on each patched mixer. prompt_kernel (no reference counterpart): prompts without a mask,
-    with gradients and dropout off, attend by prompts.prompt_attention, which reads each KV head once for its query
-    heads, instead of SDPA on repeated K and V.
+    repeat_kv on each patched mixer. prompt_kernel=True (no reference counterpart): prompts without a
+    mask, with gradients and dropout off, attend by prompts.prompt_attention, which reads each KV head once
+    for its query heads, instead of SDPA on repeated K and V. It can be switched on and off by patching again;
+    None leaves it as it is, off at first.
     """
     remote = __import__(model.__class__.__module__, fromlist=["repeat_kv"])
     repeat_kv = remote.repeat_kv
@@ -387,11 +389,14 @@ def patch_nemotron_h_attention_int4_kv(model, group_size: int = 64, *, prompt_ke
         if getattr(layer, "block_type", None) != "attention":
             continue
         attn = getattr(layer, "mixer", None)
-        if attn is None or getattr(attn, "_int4_kv_patched", False):
+        if attn is None:
+            continue
+        if prompt_kernel is not None:
+            attn._int4_kv_prompt_kernel = prompt_kernel
+        if getattr(attn, "_int4_kv_patched", False):
             continue
         attn._int4_kv_original_forward = attn.forward
         attn._int4_kv_group_size = group_size
-        attn._int4_kv_prompt_kernel = prompt_kernel
         attn._int4_kv_repeat_kv = repeat_kv
         attn.forward = MethodType(_forward_fused_int4_kv, attn)
         attn._int4_kv_patched = True

@@ -50,3 +50,17 @@ def test_a_model_patched_without_the_switch(gpu, model, calls):
         if hasattr(layer.mixer, "_int4_kv_prompt_kernel"):
             del layer.mixer._int4_kv_prompt_kernel
     assert torch.equal(logits_of(model, gpu), want) and calls[0] == 0
+
+
+def test_the_switch_of_a_patched_model(gpu, model, calls):
+    """Patching again with prompt_kernel switches it on and off, and without leaves it."""
+    layers = sum(layer.block_type == "attention" for layer in model.backbone.layers)
+    ia.patch_nemotron_h_attention_int4_kv(model, group_size=64)
+    plain = logits_of(model, gpu)
+    assert calls[0] == 0
+    for given, used in ((True, 1), (None, 1), (False, 0), (None, 0), (True, 1)):
+        calls[0] = 0
+        ia.patch_nemotron_h_attention_int4_kv(model, prompt_kernel=given)
+        got = logits_of(model, gpu)
+        assert calls[0] == used * layers, given
+        assert torch.equal(got, plain) if not used else (got - plain).norm() <= 2e-2 * plain.norm()
