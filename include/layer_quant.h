@@ -421,8 +421,8 @@ int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_tensor* A, 
  *   logprobs f32 in the shape of tokens, entropy NULL or the same, top_logprobs and top_tokens NULL or
  *   [..., top] f32 and i64, all contiguous; top <= 32: the largest logits in descending order, equal ones
  *   by the lower token
- * A row with a NaN or +inf logit, or without one above -inf, gives NaN (and tokens 0, 1, ...); logits
- * beyond 2^127 in magnitude count as infinite. The workspace needs no particular contents.
+ * A row with a NaN or +inf logit, or without one above -inf, gives NaN (and tokens 0, 1, ...). The
+ * workspace needs no particular contents.
  */
 size_t lq_token_logprobs_workspace(int64_t rows, int64_t vocab, int top);
 int lq_token_logprobs(const lq_tensor* logits, const lq_tensor* tokens, const lq_tensor* logprobs,

@@ -4,10 +4,11 @@
 //   lse = log sum_v exp(l_v),  logprob = l_token - lse,  entropy = lse - sum_v p_v l_v
 //
 // One pass over the logits. A thread takes 32 logits at a time, in 16-byte loads (rows that begin off that
-// alignment: from the aligned address in front of them), and keeps m = max l log2(e), s = sum 2^z and
-// t = sum 2^z z, z = l log2(e) - m, of its own: nothing is exchanged before the row's end. Every z is made
-// from the rounded m by one fused multiply-add, the given token's too, so that m's rounding falls out of
-// logprob and entropy. fp32 sums: a thread adds 8 terms in a row four times over, then the threads in a
+// alignment: from the aligned address in front of them), and keeps m = max l, s = sum 2^z and
+// t = sum 2^z z, z = l log2(e) - m log2(e), of its own: nothing is exchanged before the row's end. Every z is
+// made from the rounded m log2(e) by one fused multiply-add, the given token's too, so that its rounding falls
+// out of logprob and entropy. From |m| = 2^29 on, where that rounding would reach 32 and more, other logits are 32
+// or more below m: z is a power of two times l - m there, and their weights, right or not, 2^-64 at most. fp32 sums: a thread adds 8 terms in a row four times over, then the threads in a
 // tree.
 // The likeliest tokens: the k-th largest of a wave's 64 lane maxima is a limit that k logits reach, and the
 // largest of the waves' limits is the workgroup's. The logits that reach it are few (tens of 8192 random
@@ -43,6 +44,15 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 struct Sums {
   float m, s, t;
 };
+
+// z = l factor - base of a maximum m.
+struct Scale {
+  float factor, base;
+};
+__device__ __forceinline__ Scale scale_of(float m) {
+  const float factor = fabsf(m) < 0x1p29f ? LOG2E : fabsf(m) < 0x1p100f ? 2.f : 1.f;
+  return {factor, m == -INFINITY ? 0.f : m * factor};
+}
 
 struct LogprobParams {
   View logits;  // strides of (batch row, row, token)
@@ -207,9 +217,12 @@ __device__ __forceinline__ uint64_t sort_list(uint2* list, int n, int top, int l
   return ((uint64_t)sorted.y << 32) | sorted.x;
 }
 
-// Sums over another maximum: z' = z + m - to.
+// Sums over another maximum: z' = z + d. (Where a factor is not log2(e) another maximum is 32 or more
+// away, and what has it nothing beside the larger one.)
 __device__ __forceinline__ Sums moved(Sums v, float to) {
-  const float d = fmaxf(v.m - (to == -INFINITY ? 0.f : to), -200.f);
+  const Scale from = scale_of(v.m), next = scale_of(to);
+  const bool near = from.factor == LOG2E && next.factor == LOG2E;
+  const float d = v.m == to ? 0.f : near ? fmaxf(from.base - next.base, -200.f) : -200.f;
   const float w = __builtin_amdgcn_exp2f(d);
   return {to, w * v.s, w * fmaf(d, v.s, v.t)};
 }
@@ -227,16 +240,23 @@ __device__ __forceinline__ int64_t row_at(const LogprobParams& p, int row) {
 
 // A row's results from its sums and, in one wave's registers, its `top` largest keys (lane k: the k-th).
 __device__ __forceinline__ void put_row(const LogprobParams& p, int row, Sums v, uint64_t key, int lane) {
-  const float base = v.m == -INFINITY ? 0.f : v.m, log2s = __builtin_amdgcn_logf(v.s);
+  const Scale scale = scale_of(v.m);
+  const float log2s = __builtin_amdgcn_logf(v.s);
   const bool known = v.s > 0.f && v.s < INFINITY && v.m < INFINITY;
   const float nan = __builtin_nanf("");
+  const auto logprob_of = [&](float l) {
+    const float z = fmaf(l, scale.factor, -scale.base);
+    // (far below the maximum z can leave fp32 where l - m does not)
+    if (scale.factor != LOG2E || z < -0x1p100f) return (l - v.m) - log2s * LN2;
+    return (z - log2s) * LN2;
+  };
   if (lane == 0) {
     const int b = row / p.len;
     const int64_t token = ((const int64_t*)p.tokens.data)[b * p.tokens.s[0] + (row - b * p.len) * p.tokens.s[1]];
     float lp = 0.f;
     if (token >= 0 && token < p.V) {
       const float l = load_float(p.logits.data, p.logits.dtype, row_at(p, row) + token * p.logits.s[2]);
-      lp = known ? (fmaf(l, LOG2E, -base) - log2s) * LN2 : nan;
+      lp = known ? logprob_of(l) : nan;
     }
     p.logprobs[row] = lp;
     if (p.entropy != nullptr) p.entropy[row] = known ? LN2 * (log2s - v.t / v.s) : nan;
@@ -244,7 +264,7 @@ __device__ __forceinline__ void put_row(const LogprobParams& p, int row, Sums v,
   if (lane < p.top) {
     // (a row that is not known can hold logits that are not numbers, and its order is not one)
     const int64_t at = (int64_t)row * p.top + lane;
-    p.top_logprobs[at] = known ? (fmaf(logit_of((uint32_t)(key >> 32)), LOG2E, -base) - log2s) * LN2 : nan;
+    p.top_logprobs[at] = known ? logprob_of(logit_of((uint32_t)(key >> 32))) : nan;
     p.top_tokens[at] = known ? (int64_t)(0xffffffffu - (uint32_t)key) : lane;
   }
 }
@@ -321,12 +341,12 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobParams p) {
 #pragma unroll
     for (int i = 4; i < VPT; ++i) most[i & 3] = fmaxf(most[i & 3], x[i]);
     const float top_l = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-    v = moved(v, fmaxf(v.m, top_l * LOG2E));
-    const float m = v.m == -INFINITY ? 0.f : v.m;
+    v = moved(v, fmaxf(v.m, top_l));
+    const Scale scale = scale_of(v.m);
     float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const float z = fmaf(x[i], LOG2E, -m);
+      const float z = fmaf(x[i], scale.factor, -scale.base);
       const float e = __builtin_amdgcn_exp2f(z);  // NaN stays; 0 for -inf
       s[i & 3] += e;
       t[i & 3] = fmaf(e, fmaxf(z, -200.f), t[i & 3]);
