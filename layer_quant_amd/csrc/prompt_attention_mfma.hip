@@ -22,7 +22,8 @@
 // Masked keys of a row have p = 0, which a value of inf or NaN would turn into NaN. Results that are not
 // finite are rare, so it is they that are looked for: a workgroup with one runs its rows again, and then
 // hands such values to the rows that see them and takes them out of the tile. As unnormalised sums of values
-// next to bf16's largest can leave fp32, the weights are smaller then (PROMPT_ATTENTION_DOWN).
+// next to bf16's largest can leave fp32, the weights are smaller then (PROMPT_ATTENTION_DOWN). Weights that are
+// too large or all 0 because scores beyond 2^30 round c m by too much are made from s - m.
 //
 // What it measured (MI355X, 32 query / 8 KV heads of 128, us per call): one prompt of 16384 rows 1976-2057,
 // 1.07-1.11 PFLOP/s, where the library's large bf16 product reaches 1.14; 24 fp16 prompts up to 700 rows 31.6;
@@ -192,12 +193,15 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
       for (int b = 0; b < D / 32; ++b) o[b] *= keep;
     }
     const float base = m == -INFINITY ? 0.f : m * p.scale;
+    const bool far = fabsf(base) >= 0x1p24f;  // the rounding of base is no small factor of all weights
     words4_t pk[4];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.scale, -base));
+        float z = fmaf(s[b][i], p.scale, -base);
+        if (CAREFUL && far) z = (s[b][i] - m) * p.scale;
+        s[b][i] = __builtin_amdgcn_exp2f(z);
         l += s[b][i];
       }
       if (BF && CAREFUL) s[b] *= PROMPT_ATTENTION_DOWN;  // (fp16 values are too small to need it)
@@ -213,17 +217,17 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
       }
     }
   }
+  l += __shfl_xor(l, 32, 64);
   if (!CAREFUL) {
     // sum of the accumulators times 0: NaN if one is not finite
-    float odd = 0.f;
+    float odd = l * 0.f;
 #pragma unroll
     for (int b = 0; b < D / 32; ++b) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) odd = fmaf(o[b][i], 0.f, odd);
     }
-    if (__syncthreads_or(odd != 0.f)) return true;
+    if (__syncthreads_or(odd != 0.f || l == 0.f)) return true;
   }
-  l += __shfl_xor(l, 32, 64);
   const float inv = (BF && CAREFUL ? 1.f / PROMPT_ATTENTION_DOWN : 1.f) / l;
   if (r >= nrows) return false;
 #pragma unroll
