@@ -290,7 +290,8 @@ extern "C" int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const
     return fail(LQ_ERR_UNSUPPORTED, "head_dim %lld unsupported (<= %d)", (long long)D,
                 PROMPT_ATTENTION_MAX_D);
   }
-  if (!(scale - scale == 0.f)) return fail(LQ_ERR_INVALID_ARG, "scale must be finite");
+  const float scale2 = scale * 1.44269504088896340736f;  // of exponents of 2
+  if (!(scale2 - scale2 == 0.f)) return fail(LQ_ERR_INVALID_ARG, "scale must be finite, and so scale log2(e)");
   if (batch == 0 || rows == 0) return LQ_OK;
   const int64_t nrep = Hq / Hkv;
   if (rows * nrep > INT32_MAX / 2) {
@@ -311,7 +312,7 @@ extern "C" int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const
   p.Hkv = (int)Hkv;
   p.nrep = (int)nrep;
   p.D = (int)D;
-  p.scale = scale * 1.44269504088896340736f;
+  p.scale = scale2;
   // parts of 128 rows; packed prompts (and the rows of none in front and behind) have one more each
   const int64_t part = NW * ROWS;
   const int64_t parts = starts == nullptr ? batch * ((rows * nrep + part - 1) / part)
