@@ -403,7 +403,7 @@ int lq_prompt_attention(const lq_tensor* q, const lq_tensor* k, const lq_tensor*
  *   (the state behind each prompt; an empty one's is its initial state). They may be one tensor; else an
  *   output that overlaps an input, itself or the other one is refused. x, B and C of one dtype, the others of
  *   any float dtype; any strides. N <= 256. The workspace needs no particular contents; dtype is x's, `prompts` S and `rows` T (packed
- *   1) or L (packed 0).
+ *   1) or L (packed 0). Sizes that the call refuses need 0 bytes.
  */
 size_t lq_prompt_scan_workspace(int dtype, int64_t prompts, int64_t rows, int packed, int64_t heads,
                                 int64_t head_dim, int64_t dstate);

@@ -508,6 +508,13 @@ bool in_fours(const lq_tensor* t, int dtype) {
   return s >= t->shape[nd - 1] && s <= (1 << 22);
 }
 
+// Sizes that a call takes, the launch limits aside (no product leaves 64 bits).
+bool sizes_fit(int64_t prompts, int64_t rows, bool packed, int64_t heads, int64_t head_dim, int64_t dstate) {
+  constexpr int64_t MOST = INT32_MAX / 2;
+  return prompts <= 65535 && rows <= MOST && (packed || prompts * rows <= MOST) && dstate <= PROMPT_SCAN_MAX_N &&
+         head_dim <= 65535 && heads <= MOST && heads * head_dim <= MOST && heads * head_dim * dstate <= MOST;
+}
+
 }  // namespace
 }  // namespace lq
 
@@ -516,6 +523,7 @@ using namespace lq;
 extern "C" size_t lq_prompt_scan_workspace(int dtype, int64_t prompts, int64_t rows, int packed,
                                            int64_t heads, int64_t head_dim, int64_t dstate) {
   if (prompts <= 0 || rows <= 0 || heads <= 0 || head_dim <= 0 || dstate <= 0) return 0;
+  if (!sizes_fit(prompts, rows, packed != 0, heads, head_dim, dstate)) return 0;
   const int64_t total = packed ? rows : prompts * rows;
   const bool mfma = prompt_scan_mfma_geometry(dtype, heads, head_dim, dstate);
   const int64_t slots = slots_of(prompts, rows, plan_segment(mfma, prompts, total, heads), packed != 0);
@@ -580,7 +588,7 @@ extern "C" int lq_prompt_scan(const lq_tensor* x, const lq_tensor* dt, const lq_
   if (!(dt_min <= dt_max)) return fail(LQ_ERR_INVALID_ARG, "dt_limit %g .. %g", dt_min, dt_max);
   if (batch == 0 || (S == 0 && rows == 0)) return LQ_OK;
   const int64_t total = nd == 4 ? batch * rows : rows;
-  if (total > INT32_MAX / 2 || S > 65535 || H * P * N > INT32_MAX / 2) {
+  if (!sizes_fit(S, rows, nd == 3, H, P, N)) {
     return fail(LQ_ERR_UNSUPPORTED, "%lld rows of %lld prompts exceed the launch limits",
                 (long long)total, (long long)S);
   }

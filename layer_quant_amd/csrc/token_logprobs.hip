@@ -475,7 +475,7 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 using namespace lq;
 
 extern "C" size_t lq_token_logprobs_workspace(int64_t rows, int64_t vocab, int top) {
-  if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+  if (rows <= 0 || vocab <= 0 || top < 0 || top > MAX_TOP || vocab > INT32_MAX / 2) return 0;
   const Plan plan = plan_of(rows, vocab, MAX_SKEW);
   if (plan.parts == 1) return 0;
   const size_t parts = (size_t)rows * (size_t)plan.parts;
