@@ -172,11 +172,14 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
       }
       keep = keep == 0.f ? 1.f : keep;
     }
+    // (by itself: many small terms, each rounded beside a large l, would be off together)
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[i] = __builtin_amdgcn_exp2f(s[i] - base);
-      l += s[i];
+      sum += s[i];
     }
+    l += sum;
     if (DOWN) s *= PROMPT_ATTENTION_DOWN;
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {

@@ -195,6 +195,7 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
     const float base = m == -INFINITY ? 0.f : m * p.scale;
     const bool far = fabsf(base) >= 0x1p24f;  // the rounding of base is no small factor of all weights
     words4_t pk[4];
+    float sum = 0.f;  // (by itself: many small terms, each rounded beside a large l, would be off together)
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -202,12 +203,13 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
         float z = fmaf(s[b][i], p.scale, -base);
         if (CAREFUL && far) z = (s[b][i] - m) * p.scale;
         s[b][i] = __builtin_amdgcn_exp2f(z);
-        l += s[b][i];
+        sum += s[b][i];
       }
       if (BF && CAREFUL) s[b] *= PROMPT_ATTENTION_DOWN;  // (fp16 values are too small to need it)
 #pragma unroll
       for (int i = 0; i < 8; ++i) pk[2 * b + (i >> 2)][i & 3] = pack2<BF>(s[b][2 * i], s[b][2 * i + 1]);
     }
+    l += sum;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
