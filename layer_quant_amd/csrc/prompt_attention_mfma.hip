@@ -17,7 +17,9 @@
 //
 // The running maximum moves only when a score exceeds it by 2^LAZY: p <= 2^8 then, and the 64
 // accumulators are rescaled in a few tiles only. Weights are rounded to the inputs' type, their sum is
-// fp32 and of the unrounded ones: the rounding is half a step per weight, as if the values had it.
+// fp32 and of the unrounded ones: the rounding is half a step per weight, as if the values had it. fp16 ones are
+// raised by 2^7, so that this holds down to 2^-21 of the largest weight so far; below it they are off by 2^-32
+// of that one.
 //
 // Masked keys of a row have p = 0, which a value of inf or NaN would turn into NaN. Results that are not
 // finite are rare, so it is they that are looked for: a workgroup with one runs its rows again, and then
@@ -39,6 +41,7 @@ namespace {
 constexpr int KT = 64;    // keys per tile
 constexpr int ROWS = 32;  // rows per wave
 constexpr float LAZY = 8.f;
+constexpr float RAISE = 7.f;  // of fp16 weights' exponents: 2^(LAZY + RAISE) is in fp16
 
 // Chunks by which a tile row's chunks are exchanged. D = 128 (256-byte rows): 16 rows' equal chunks, and
 // 4 rows' runs of 4 chunks, lie in different banks. D = 64: two rows share 256 bytes.
@@ -192,8 +195,8 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
 #pragma unroll
       for (int b = 0; b < D / 32; ++b) o[b] *= keep;
     }
-    const float base = m == -INFINITY ? 0.f : m * p.scale;
-    const bool far = fabsf(base) >= 0x1p24f;  // the rounding of base is no small factor of all weights
+    const float rounded = m == -INFINITY ? 0.f : m * p.scale, base = BF ? rounded : rounded - RAISE;
+    const bool far = fabsf(rounded) >= 0x1p24f;  // its rounding is no small factor of all weights
     words4_t pk[4];
     float sum = 0.f;  // (by itself: many small terms, each rounded beside a large l, would be off together)
 #pragma unroll
@@ -201,7 +204,7 @@ __device__ __forceinline__ bool attend(const PromptAttention& p, const Span& sp,
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float z = fmaf(s[b][i], p.scale, -base);
-        if (CAREFUL && far) z = (s[b][i] - m) * p.scale;
+        if (CAREFUL && far) z = (s[b][i] - m) * p.scale + (BF ? 0.f : RAISE);
         s[b][i] = __builtin_amdgcn_exp2f(z);
         sum += s[b][i];
       }

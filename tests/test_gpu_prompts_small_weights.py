@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("below", [9.0, 11.5, 13.25, 14.25])
 def test_many_small_weights(gpu, dtype, d, below):
