@@ -39,15 +39,15 @@ void launch_prompt_scan_steps(const PromptScan& p, int64_t chunks, hipStream_t s
 void launch_prompt_scan_mfma(const PromptScan& p, bool adds, int64_t parts, hipStream_t st);
 
 // Segments of a prompt (an empty one has one, which hands its state on), and its slots: one for each of
-// several segments. Its first slot, where prompts are packed: floor(begin / segment) + its number, or with many
-// prompts of a segment or less, which need none, floor(2 begin / segment): 2 len / segment whole ones are
-// ceil(len / segment) or more where len > segment.
+// several segments. With many prompts the first slot of one (find_span's first_slot) is floor(begin / segment) +
+// its number, or with many of a segment or less, which need none, floor(2 begin / segment): 2 len / segment whole
+// ones are ceil(len / segment) or more where len > segment.
 __device__ __forceinline__ int segments_of(const PromptScan& p, int len, bool gap) {
   return max((len + p.segment - 1) / p.segment, gap ? 0 : 1);
 }
-__device__ __forceinline__ int slots_of_span(const PromptScan& p, int len, bool gap) {
-  const int n = segments_of(p, len, gap);
-  return gap || n < 2 ? 0 : n;
+__device__ __forceinline__ int slots_of_prompt(const PromptScan& p, int len) {
+  const int n = segments_of(p, len, false);
+  return n < 2 ? 0 : n;
 }
 __device__ __forceinline__ int slot_of(const PromptScan& p, int begin, int i) {
   return p.slots_by_rows ? 2 * begin / p.segment : begin / p.segment + i;
@@ -64,19 +64,20 @@ struct Segment {
 template <bool ADDS>
 __device__ __forceinline__ Segment find_segment(const PromptScan& p, int t) {
   Segment s;
+  const auto slots = [&](int len) { return slots_of_prompt(p, len); };
+  const auto first_slot = [&](int begin, int i) { return slot_of(p, begin, i); };
   if (ADDS) {
     s.valid = find_span<false>(
-        p.spans, t, [&](int len, bool gap) { return slots_of_span(p, len, gap); },
-        [&](int begin, int i) { return slot_of(p, begin, i); }, s.span);
+        p.spans, t, [&](int len, bool) { return slots(len); }, first_slot, slots, first_slot, s.span);
   } else {
     s.valid = find_span<true>(
         p.spans, t, [&](int len, bool gap) { return segments_of(p, len, gap); },
-        [&](int begin, int i) { return begin / p.segment + i; }, s.span);
+        [&](int begin, int i) { return begin / p.segment + i; }, slots, first_slot, s.span);
   }
   if (!s.valid || s.span.gap) return s;
   const int n = segments_of(p, s.span.len, false);
   s.several = n > 1;
-  s.slot = (p.spans.starts == nullptr ? s.span.index * n : slot_of(p, s.span.begin, s.span.index)) + s.span.part;
+  s.slot = s.span.slots + s.span.part;
   // the last one adds to nothing; starts out of order can ask for more slots than there are
   if (ADDS ? s.span.part == n - 1 || s.slot + 1 >= p.slots : s.several && s.slot >= p.slots) s.valid = false;
   return s;

@@ -376,10 +376,10 @@ constexpr int AHEAD = 8;
 __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
   Span sp;
   const bool mine = find_span<false>(
-      p.spans, blockIdx.y, [&](int len, bool gap) { return slots_of_span(p, len, gap); },
+      p.spans, blockIdx.y, [&](int len, bool) { return slots_of_prompt(p, len); },
       [&](int begin, int i) { return slot_of(p, begin, i); }, sp);
   if (!mine || sp.part != 0) return;
-  const int many = min(slots_of_span(p, sp.len, false), p.slots - (int)blockIdx.y);
+  const int many = min(slots_of_prompt(p, sp.len), p.slots - (int)blockIdx.y);
   const int64_t size = (int64_t)p.H * p.P * p.N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= size) return;
   float* state = p.slot_state + (int64_t)blockIdx.y * size + i;

@@ -27,9 +27,10 @@ def check_rows_by_length(got, call, lengths, starts):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("count", [1, 61, 62, 63, 64, 65, 126, 127, 129, 4000, 4094, 4095, 4097])
+@pytest.mark.parametrize("count", [1, 61, 62, 63, 64, 65, 126, 127, 129, 400, 509, 510, 511, 4000, 4094, 4095, 4097])
 def test_attention_of_many_prompts(gpu, dtype, count):
-    """As many spans as a wave's lanes, a power of them, and one more or less; empty prompts in runs."""
+    """As many spans as a wave's lanes, eight for each, a power of them, and one more or less; empty prompts in
+    runs."""
     rng = random.Random(count)
     lengths = [rng.choice([0, 0, 0, 1, 2, 33, 130 if count < 200 else 5]) for _ in range(count)]
     lengths[rng.randrange(count)] = 300
@@ -62,7 +63,7 @@ def test_attention_of_a_million_prompts(gpu):
 
 
 @pytest.mark.parametrize("geometry,dtype", [((2, 64, 128), BF), ((4, 16, 32), F16), ((4, 16, 32), F32)], ids=str)
-@pytest.mark.parametrize("many", [0, 3, 700])
+@pytest.mark.parametrize("many", [0, 3, 57, 58, 100, 505, 506, 700])
 def test_scan_segments_among_many_prompts(gpu, geometry, dtype, many):
     """Prompts of several segments among few and many others (their first segments' places go by the
     prompts' number, or by the rows alone), empty ones in runs, the states in place."""
