@@ -7,7 +7,7 @@
 // prompt_attention_f32: any float dtype and strides, head_dim <= 256, fp32 products and sums on
 // v_mfma_f32_32x32x2_f32. It is the kernel of fp32 inputs and of layouts that the 16-bit kernel
 // (prompt_attention_mfma.hip) does not take. Three fp32 prompts up to 1001 rows, 32 query and 8 KV heads:
-// 229 us, 73 TFLOP/s, half of the rate of a large fp32 library product (153). With loads one value at a time,
+// 231 us, 72 TFLOP/s, half of the rate of a large fp32 library product (153). With loads one value at a time,
 // waited for before each tile, it was 608.
 //
 // A prompt's rows of a KV head are its positions times the n_rep query heads, head by head within a

@@ -27,11 +27,13 @@
 // next to bf16's largest can leave fp32, the weights are smaller then (PROMPT_ATTENTION_DOWN). Weights that are
 // too large or all 0 because scores beyond 2^30 round c m by too much are made from s - m.
 //
-// What it measured (MI355X, 32 query / 8 KV heads of 128, us per call): one prompt of 16384 rows 1976-2057,
-// 1.07-1.11 PFLOP/s, where the library's large bf16 product reaches 1.14; 24 fp16 prompts up to 700 rows 31.6;
-// one of 333 rows 11.7. Bound by issue: per tile and wave 32 matrix instructions of 32 cycles and the softmax's VALU
-// instructions; the short ones by latency, up to 11 tiles in a row behind the span search and cold
-// instructions. prompt_attention_f32 in its first form, one value per load, took 57 ms, 518 and 131.
+// What it measured (MI355X, 32 query / 8 KV heads of 128, us per call): one prompt of 16384 rows 1995-2054,
+// 1.07-1.10 PFLOP/s, where the library's large bf16 product reaches 1.14; 24 fp16 prompts up to 700 rows 31.6;
+// one of 333 rows 11.5. Bound by issue: per tile and wave 32 matrix instructions of 32 cycles and the softmax's VALU
+// instructions; the short prompt by latency, six tiles in a row behind the span search and cold instructions; the
+// 24 by their order too: the one of 700 rows is the 20th, and its workgroups, of eleven tiles, begin late
+// (longest first 26.5 us where the given order takes 33-35, shortest first 33-35). prompt_attention_f32 in its
+// first form, one value per load, took 57 ms, 518 and 131.
 #include "matrix16.h"
 #include "prompt_attention.h"
 

@@ -22,8 +22,8 @@
 // that are smaller than they would be stand in registers, by 2^-40 at most: blocks that decay further, or
 // grow, or have a NaN, take the steps as they are. c is summed in 64 bits, for the reason that
 // prompt_scan_mfma.hip gives.
-// Three fp32 prompts up to 1001 rows (2438 in all) of 128 heads x 64 x 128: 352 us (107-113 for what the
-// segments add, 33 to carry, 248-268 for the segments, where 85 VALU instructions per row and wave, 64 of them
+// Three fp32 prompts up to 1001 rows (2438 in all) of 128 heads x 64 x 128: 350-372 us (101-113 for what
+// the segments add, 33 to carry, 234-268 for the segments, where 85 VALU instructions per row and wave, 64 of them
 // these multiply-adds, are 173 at 2.4 GHz; the rest is the blocks' staging, barriers and silu, and latency at
 // four waves per SIMD). With a state not scaled, loads at addresses of their own and less of the GPU's
 // workgroups it was 548. Without effect or worse: z loaded ahead (350), two rows unrolled (358), five
@@ -439,9 +439,9 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(PromptScan p) {
 // Rows of a segment, a multiple of 64. Segments cost a part of the work again and two launches.
 // Matrix kernel: as many as give two workgroups per CU (a workgroup has two heads), but at least 256 rows, and
 // prompts of up to 1024 rows, as far as their mean says, stay whole (4 prompts of 512 rows and 128 heads: 71 us
-// in two segments each, 41 whole; one of 2000 rows: 107 us in two of 1024, 73 in eight of 256). Eight prompts
-// or more fill the GPU by themselves unless their lengths differ much: twice as many rows then (24 prompts up
-// to 700 rows: 134 -> 117 us).
+// in two segments each, 41 whole; one of 2000 rows: 107 us in two of 1024, 73 in eight of 256, and 108 again with a
+// prompt of 40 rows beside it, as the lengths are not known here). Eight prompts or more fill the GPU by themselves:
+// twice as many rows then (24 prompts up to 700 rows: 134 -> 117 us).
 // Rows kernel: as many as give eight workgroups per CU, of which it has four at a time (half as many
 // workgroups: three fp32 prompts up to 1001 rows 429 us against 394, one of 4000 fp16 rows 757 against 652);
 // at least 192 rows, or 256 where prompts have no more, as their mean says (4 of 200 rows, 64 heads: 137 us in two

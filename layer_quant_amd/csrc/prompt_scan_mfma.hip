@@ -23,21 +23,22 @@
 // B lies in two LDS buffers; x goes to registers at once, and C and the decays are read in phase 1 alone, so
 // that one buffer each does, refilled from then on: 79 KB per workgroup, two of them per CU.
 //
-// What it measured (MI355X, 128 heads, 8 groups, us): one prompt of 16384 rows 312 (steps 16, what the segments
-// add 92-114, carry 13, the segments 189-247), 24 prompts up to 700 rows with fp32 states 123 (8 + 4 + 5 + 110-113),
-// one of 200 rows 25.0 (5 + 20). With one value of w x a chunk took a workgroup 3.2 us alone on its CU and 5 beside
-// another one: per wave 50
-// matrix instructions (32 cycles) and 540 VALU ones (4), which add up, are two thirds of that; the rest is the
-// latency of LDS and of three barriers. Tried: one workgroup of eight waves and four heads with M in registers
-// and a single barrier (313 us: 66 and 681 instructions); loads further ahead into L2 (no gain); heads to XCDs
-// in other orders (no difference); the last block's heads shared out to two waves (297).
+// What it measured (MI355X, 128 heads, 8 groups, us): one prompt of 16384 rows 318-328 (steps 15-18, what the
+// segments add 90-103, carry 13, the segments 203-229), 24 prompts up to 700 rows with fp32 states 124 (8 + 3-5 + 5 +
+// 110-112; longest first 105: the one of 700 rows is the 20th and begins late), one of 200 rows 25.3 (5 + 20). A chunk
+// takes a workgroup 3.3 us alone on its CU, 3.7 with fp32 states, and 6.3-7.2 beside another one: per wave 70 matrix
+// instructions (32 cycles) and 600 other VALU ones (4), which add up, are 1.9 us at 2.4 GHz; the rest is the latency
+// of LDS and of three barriers. Tried, with one value of w x (50 matrix instructions, 289 us): one workgroup of eight
+// waves and four heads with M in registers and a single barrier (313); loads further ahead into L2 (no gain); heads to
+// XCDs in other orders (no difference); the last block's heads shared out to two waves (297).
 //
 // Roundings: M and S to bf16 as operands (half a step, 2^-8, of each term of a bf16 result), D to the sum of two
-// bf16 values (2^-17). w x, which a
-// state keeps, to the sum of two bf16 values (2^-16) where the state leaves in 16 bits, and of three (its 24
+// bf16 values (2^-17). w x, which a state keeps, to the sum of two bf16 values (2^-16) where the state leaves in 16 bits, and of three (its 24
 // bits) where it leaves in fp32: 700 rows' fp32 states are off by less than 5e-7 with three, 2e-6 with two (24
 // prompts 123 us, 117), and bf16 ones by 0.0017, their own rounding, with two, 0.0024 with one (16384 rows 312
-// us, 285). Everything else is fp32.
+// us, 285). y is off by 0.0019-0.0022 of itself, of which its own rounding is 0.0017; with D as one bf16 value it
+// was 0.0023 (16384 rows 316 us, 325 with two; D's rest in M's diagonal instead of products of its own 328, 24
+// prompts 134 us against 124). Everything else is fp32.
 //
 // Rows behind a row in its chunk have M = 0 there, which an x of inf or NaN would turn into NaN. Such a value
 // stays in the state, so that it is enough to look at the state behind a segment: one that is not finite has
@@ -464,7 +465,7 @@ __device__ __forceinline__ bool run_segment(const PromptScan& p, const Segment& 
         const float b = w[2 * e + 1] * __uint_as_float(xa[i][e] & 0xffff0000u);
         const uint32_t ab = pack2<true>(a, b);
         top[e] = ab;
-const float a1 = a - __uint_as_float(ab << 16), b1 = b - __uint_as_float(ab & 0xffff0000u);
+        const float a1 = a - __uint_as_float(ab << 16), b1 = b - __uint_as_float(ab & 0xffff0000u);
         const uint32_t ab1 = pack2<true>(a1, b1);
         lower[e] = ab1;
         if (TERMS == 3) lowest[e] = pack2<true>(a1 - __uint_as_float(ab1 << 16), b1 - __uint_as_float(ab1 & 0xffff0000u));

@@ -8,8 +8,8 @@
 // t = sum 2^z z, z = l log2(e) - m log2(e), of its own: nothing is exchanged before the row's end. Every z is
 // made from the rounded m log2(e) by one fused multiply-add, the given token's too, so that its rounding falls
 // out of logprob and entropy. From |m| = 2^29 on, where that rounding would reach 32 and more, other logits are 32
-// or more below m: z is a power of two times l - m there, and their weights, right or not, 2^-64 at most. fp32 sums: a thread adds 8 terms in a row four times over, then the threads in a
-// tree.
+// or more below m: z is a power of two times l - m there, and their weights, right or not, are 2^-64 and less
+// of the largest one's. fp32 sums: a thread adds 8 terms in a row four times over, then the threads in a tree.
 // The likeliest tokens: the k-th largest of a wave's 64 lane maxima is a limit that k logits reach, and the
 // largest of the waves' limits is the workgroup's. The logits that reach it are few (tens of 8192 random
 // ones for k = 8) and go to the wave's list; a full list is cut to its k largest, by ballots, bit by bit from
@@ -21,10 +21,11 @@
 // a wave per row joins the parts, a second launch. One workgroup of 1024 threads over several sweeps instead of
 // the parts: 37 rows of 50257 fp32 logits 17.8 us against 16.5.
 //
-// What it measured (MI355X, us per call, kernel time in brackets): 2048 rows of 131072 bf16 logits 96 (93-98, 5.6
-// TB/s: a device copy's rate), with 8 or 32 tokens each 145; 64 rows, 8 tokens 15.5-16.0 (10.9-11.4 + 4.5-4.8);
-// 37 rows of 50257 fp32, 20 tokens 16.5 (10.5 + 6); one row of 32000, 5 tokens 12.2 (10.2; the host's part is
-// 12). The small ones are bound by the latency of their dependent steps: load, limit, list, order.
+// What it measured (MI355X, us per call, kernel time in brackets): 2048 rows of 131072 bf16 logits 97 (95-96, 5.5
+// TB/s: a device copy's rate), with 8 or 32 tokens each 147-150; 64 rows, 8 tokens 16.6 (11.2-11.7 + 5.0);
+// 37 rows of 50257 fp32, 20 tokens 17.1 (11-11.6 + 6.4); one row of 32000, 5 tokens 12.2 (10.7; the host's part is
+// 12). The small ones are bound by the latency of their dependent steps: load, limit, list, order. Rows whose limit
+// holds few logits back, 8 tokens each: all but ten masked 47 (64 rows) and 184 (2048), equal logits 66 and 1380.
 //
 // Order: the larger logit first, of equal ones (and of 0 and -0) the lower token. -inf logits have no
 // part in the sums. A row with a NaN or an infinity, or with -inf alone, has no distribution: NaN.
